@@ -396,6 +396,33 @@ int32_t _mlir_ciface_nova_hip_reduce_sum_f32(const NovaMemRef3D *x, NovaMemRef2D
 int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D *dst,
                                            int32_t src_dt);
 /* ------------------------------------------------------------------------
+ * Attention of packed sequences (MFMA).  No reference counterpart: the
+ * reference runs an attention as its two batch GEMMs.
+ *
+ * Sequence b is the query rows [q_offsets[b], q_offsets[b + 1]) and the key
+ * rows [k_offsets[b], k_offsets[b + 1]) of the packed operands; the offsets
+ * (device memory, i32, [sequences + 1]) do not decrease and lie inside the
+ * operands (each is cut to that range: whatever they hold, no access leaves
+ * an operand).  Lengths may differ and may be zero.
+ *   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G]) v[j, h / G],
+ *   G = heads / key heads; causal: query i of a sequence sees the keys
+ *   j <= i + (keys - queries), so that the last query sees the last key.
+ * A query that sees no key gives a zero row and lse -inf.
+ *   q, out : [query tokens, heads, D]; k, v : [key tokens, key heads, D];
+ *   dt NOVA_HIP_DT_BF16 or _F16; D a multiple of 8 up to 128; unit stride on
+ *   D, any order of the other dims, rows 16-byte aligned.
+ *   lse : [heads, query tokens] f32, log sum exp of the scaled scores, or
+ *   NULL.
+ * Scores, softmax and sums are f32; the weights are rounded to dt for the
+ * product with v.  Rows outside every sequence are left as they were.  No
+ * workspace: concurrent calls and captured graphs share nothing.
+ * ---------------------------------------------------------------------- */
+int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3D *k,
+                                        const NovaMemRef3D *v, const NovaMemRef1D *q_offsets,
+                                        const NovaMemRef1D *k_offsets, NovaMemRef3D *out,
+                                        NovaMemRef2D *lse, float scale, int32_t causal,
+                                        int32_t dt);
+/* ------------------------------------------------------------------------
  * Typed aliases for lowered modules (nova-compiler_amd/mlir/
  * NovaHipLowering.cpp).  An MLIR module declares each callee once, with one
  * type, so the generic entry points above get one name per operand dtype

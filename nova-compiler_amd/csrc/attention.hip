@@ -1,0 +1,212 @@
+// Attention of packed sequences, forward:  O = softmax(scale Q K^T) V per
+// sequence and head, lse = log sum exp of each row's scaled scores.
+//
+// One pass over the keys with the running maximum m and sum l of the softmax:
+// a row's accumulators are sums of exp2((s - m) c) v, c = scale log2 e, which
+// a larger m multiplies by exp2((m_old - m) c).  m follows the scores only
+// when one is more than 2^8 above it (the factor is exact either way, and
+// f32 sums and 16-bit weights have that much room), so most tiles multiply no
+// accumulator.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attention.h"
+
+namespace nova_hip {
+namespace attn {
+namespace {
+
+struct FwdArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t *o;
+  float *lse;  // [heads][Tq] with row stride slse, or null
+  const int *q_off, *k_off;
+  Rows sq, sk, sv, so;
+  int64_t slse;
+  int Tq, Tk, B, heads, group, D, tiles;  // group: query heads per key head
+  float c;                                // scale * log2(e)
+};
+
+constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
+constexpr float kSlack = 8.0f;  // m c may lag the largest score by this much
+
+// Workgroup id -> (head, tile): the hardware deals ids to the 8 XCDs in turn;
+// each XCD takes one run of the head-major order, so the heads that share
+// keys and values share an L2.
+__device__ __forceinline__ int xcd_run(int id, int total) {
+  const int per = total >> 3, rem = total & 7, x = id & 7;
+  return x * per + min(x, rem) + (id >> 3);
+}
+
+template <int DT, int DP, bool CAUSAL>
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a) {
+  constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
+  __shared__ __attribute__((aligned(1024))) char sk0[kTile];
+  __shared__ __attribute__((aligned(1024))) char sk1[kTile];
+  __shared__ __attribute__((aligned(1024))) char sv0[kTile];
+  __shared__ __attribute__((aligned(1024))) char sv1[kTile];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
+  const int head = w / a.tiles, tile = a.tiles - 1 - (w - head * a.tiles);
+  int b, row0;
+  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, row0)) return;
+  int qs, qe, ks, ke;
+  seq_rows(a.q_off, b, a.Tq, qs, qe);
+  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  const int Lq = qe - qs, Lk = ke - ks;
+  // Query i sees keys 0 .. i + Lk - Lq.
+  const int shift = Lk - Lq;
+  const int keys = CAUSAL ? min(Lk, max(0, row0 + kBM + shift)) : Lk;
+  const int nt = (keys + kBN - 1) / kBN;
+
+  const int q0 = row0 + 32 * wave, qn = min(32, Lq - q0);  // this wave's rows, maybe none
+  u32x4 qf[DP / 16];
+  load_cols<DP>(qf, a.q + (qs + q0) * a.sq.t + head * a.sq.h, a.sq.t, qn, a.D, lane);
+
+  const uint16_t *kp = a.k + ks * a.sk.t + (head / a.group) * a.sk.h;
+  const uint16_t *vp = a.v + ks * a.sv.t + (head / a.group) * a.sv.h;
+  TileLoad<kBN, CH, kWaves> lk, lv;
+  lk.init(a.sk.t, a.D);
+  lv.init(a.sv.t, a.D);
+
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+  float mc = -INFINITY, l = 0.0f;  // m c and this lane's share of the sum
+  const int last = q0 + (lane & 31) + shift;  // causal: the last key this lane's row sees
+
+  auto fetch = [&](int t, char *sk, char *sv) __attribute__((always_inline)) {
+    lk.load(kp + (int64_t)t * kBN * a.sk.t, a.sk.t, Lk - t * kBN, a.D, sk);
+    lv.load(vp + (int64_t)t * kBN * a.sv.t, a.sv.t, Lk - t * kBN, a.D, sv);
+  };
+  auto step = [&](int t, const char *sk, const char *sv) __attribute__((always_inline)) {
+    const int k0 = t * kBN;
+    if (qn <= 0 || (CAUSAL && k0 > q0 + qn - 1 + shift)) return;  // wave-uniform
+    f32x16 s[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i] = f32x16{};
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+        s[i] = mfma_32x32x16<DT>(read_row_frag(sk, row_frag<CH>(32 * i, kk, lane)), qf[kk], s[i]);
+    }
+    if (k0 + kBN > Lk || (CAUSAL && k0 + kBN - 1 > q0 + shift)) {
+      const int end = CAUSAL ? min(Lk, last + 1) : Lk;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[i][r] = -INFINITY;
+    }
+    float m = s[0][0];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = fmaxf(m, fmaxf(s[0][r], s[1][r]));
+    m = both_max(m) * a.c;
+    if (__ballot(m > mc + kSlack)) {
+      const float to = fmaxf(m, mc), f = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - to);
+      mc = to;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
+    }
+    const float mu = mc == -INFINITY ? 0.0f : mc;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.c, -mu));
+        l += s[i][r];
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        // The weights round to the operands' type for the product (the sum l
+        // takes them in f32): half a step of it, as much as the result's own.
+        const u32x4 pf = pack_frag<DT>(s[i], kk);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+          acc[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sv, 32 * i + 16 * kk, 32 * db, lane), pf,
+                                      acc[db]);
+      }
+  };
+  // One barrier per tile: behind it the tile just fetched is whole and the
+  // other stage has no reader left.
+  auto sync = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA has landed
+    __syncthreads();
+  };
+  if (nt > 0) fetch(0, sk0, sv0);
+  for (int t = 0; t < nt; t += 2) {
+    sync();
+    if (t + 1 < nt) fetch(t + 1, sk1, sv1);
+    step(t, sk0, sv0);
+    if (t + 1 >= nt) break;
+    sync();
+    if (t + 2 < nt) fetch(t + 2, sk0, sv0);
+    step(t + 1, sk1, sv1);
+  }
+  if (qn <= 0) return;
+  l = both_sum(l);
+  // A row that sees no key is zero, its lse -inf.
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  store_rows<DT, DP>(acc, inv, a.o + (qs + q0) * a.so.t + head * a.so.h, a.so.t, qn, a.D, lane);
+  if (a.lse && lane < qn)
+    a.lse[head * a.slse + qs + q0 + lane] = l == 0.0f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+}
+
+template <int DT, int DP>
+void launch_fwd(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {
+  if (causal)
+    hipLaunchKernelGGL((attention_fwd_kernel<DT, DP, true>), dim3(grid), dim3(64 * kWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((attention_fwd_kernel<DT, DP, false>), dim3(grid), dim3(64 * kWaves), 0, s, a);
+}
+template <int DT>
+void launch_fwd(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {
+  if (a.D <= 32) launch_fwd<DT, 32>(a, causal, grid, s);
+  else if (a.D <= 64) launch_fwd<DT, 64>(a, causal, grid, s);
+  else if (a.D <= 96) launch_fwd<DT, 96>(a, causal, grid, s);
+  else launch_fwd<DT, 128>(a, causal, grid, s);
+}
+
+}  // namespace
+}  // namespace attn
+
+int32_t launch_attention(const AttentionProblem &p, hipStream_t s) {
+  if (p.Tq == 0 || p.heads == 0 || p.D == 0 || p.B == 0) return NOVA_HIP_SUCCESS;
+  attn::FwdArgs a;
+  a.q = static_cast<const uint16_t *>(p.q.p);
+  a.k = static_cast<const uint16_t *>(p.k.p);
+  a.v = static_cast<const uint16_t *>(p.v.p);
+  a.o = static_cast<uint16_t *>(p.o.p);
+  a.lse = p.lse;
+  a.slse = p.slse;
+  a.q_off = p.q_off;
+  a.k_off = p.k_off;
+  a.sq = {p.q.st, p.q.sh};
+  a.sk = {p.k.st, p.k.sh};
+  a.sv = {p.v.st, p.v.sh};
+  a.so = {p.o.st, p.o.sh};
+  a.Tq = (int)p.Tq;
+  a.Tk = (int)p.Tk;
+  a.B = (int)p.B;
+  a.heads = (int)p.heads;
+  a.group = (int)(p.heads / p.kv_heads);
+  a.D = (int)p.D;
+  a.c = p.scale * attn::kLog2e;
+  // Whole tiles and, for each sequence, at most one that is not.
+  const int64_t tiles = std::min(p.Tq, p.Tq / attn::kBM + p.B);
+  if (tiles * p.heads > 0x7fffffff)
+    return fail(NOVA_HIP_ERANGE, "attention: %lld tiles of %lld heads exceed 2^31 - 1",
+                (long long)tiles, (long long)p.heads);
+  a.tiles = (int)tiles;
+  const unsigned grid = (unsigned)(tiles * p.heads);
+  if (p.dt == NOVA_HIP_DT_BF16) attn::launch_fwd<NOVA_HIP_DT_BF16>(a, p.causal, grid, s);
+  else attn::launch_fwd<NOVA_HIP_DT_F16>(a, p.causal, grid, s);
+  return check_hip(hipGetLastError(), "attention launch");
+}
+
+}  // namespace nova_hip

@@ -7,7 +7,9 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <memory>
 #include <unordered_map>
@@ -866,6 +868,127 @@ int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D
                              reinterpret_cast<int32_t *>(const_cast<char *>(data_of(dst))) +
                                  dst->offset,
                              src->sizes[0], current_stream());
+}
+
+// ---- attention --------------------------------------------------------------------
+namespace {
+constexpr int64_t kAttnMaxStride = 1 << 24;  // elements; 128 rows stay below 2^32 bytes
+
+// One operand [T, heads, D]: unit stride on D, rows of whole 16-byte chunks at
+// 16-byte aligned addresses.  A dim of extent 1 is never stepped.
+int32_t attn_operand(const NovaMemRef3D *d, const char *w, const char *what, bool out,
+                     AttentionOperand &o) {
+  if (!d) return fail(NOVA_HIP_EINVAL, "%s: null %s descriptor", w, what);
+  if (!nonneg_sizes(d, 3)) return fail(NOVA_HIP_ESHAPE, "%s: negative size", w);
+  const int64_t T = d->sizes[0], H = d->sizes[1], D = d->sizes[2];
+  o.st = T > 1 ? d->strides[0] : 0;
+  o.sh = H > 1 ? d->strides[1] : 0;
+  if (T > 0x7fffffff || H > 0xffff)
+    return fail(NOVA_HIP_ERANGE, "%s: %s has more than 2^31 - 1 tokens or 65535 heads", w, what);
+  if (T == 0 || H == 0 || D == 0) {
+    o.p = nullptr;
+    return NOVA_HIP_SUCCESS;
+  }
+  if (!d->aligned) return fail(NOVA_HIP_EINVAL, "%s: null %s data pointer", w, what);
+  if (D > 1 && d->strides[2] != 1)
+    return fail(NOVA_HIP_ESTRIDE, "%s: %s must have unit stride on the head dim", w, what);
+  if (o.st < 0 || o.sh < 0)
+    return fail(NOVA_HIP_ESTRIDE, "%s: negative strides are not addressed", w);
+  o.p = const_cast<char *>(data_of(d)) + d->offset * 2;
+  if (o.st % 8 || o.sh % 8 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s must start at 16-byte aligned addresses", w, what);
+  if (o.st > kAttnMaxStride)
+    return fail(NOVA_HIP_ERANGE, "%s: token stride of %s exceeds 2^24 elements", w, what);
+  if (out) {
+    const int64_t inner = std::min(T > 1 ? o.st : INT64_MAX, H > 1 ? o.sh : INT64_MAX);
+    const bool t_inner = T > 1 && (H <= 1 || o.st <= o.sh);
+    if ((T > 1 || H > 1) && inner < D) return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
+    if (T > 1 && H > 1 &&
+        (t_inner ? o.sh < (T - 1) * o.st + D : o.st < (H - 1) * o.sh + D))
+      return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
+  }
+  return NOVA_HIP_SUCCESS;
+}
+
+bool dense_i32(const NovaMemRef1D *d) { return d->sizes[0] <= 1 || d->strides[0] == 1; }
+
+// The checks attention and its backward share: q, k, v, offsets and lse.
+int32_t attn_common(const NovaMemRef3D *q, const NovaMemRef3D *k, const NovaMemRef3D *v,
+                    const NovaMemRef1D *q_off, const NovaMemRef1D *k_off, const NovaMemRef2D *lse,
+                    float scale, int32_t causal, int32_t dt, const char *w, AttentionProblem &p) {
+  int32_t rc;
+  if (!q_off || !k_off) return fail(NOVA_HIP_EINVAL, "%s: null offsets descriptor", w);
+  if (dt != NOVA_HIP_DT_BF16 && dt != NOVA_HIP_DT_F16)
+    return fail(NOVA_HIP_EDTYPE, "%s: dtype %d (bf16 and f16 are provided)", w, dt);
+  if (!(scale > 0.0f) || !(scale < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: scale must be positive and finite", w);
+  if (causal != 0 && causal != 1) return fail(NOVA_HIP_EINVAL, "%s: causal is %d", w, causal);
+  if ((rc = attn_operand(q, w, "q", false, p.q)) || (rc = attn_operand(k, w, "k", false, p.k)) ||
+      (rc = attn_operand(v, w, "v", false, p.v)))
+    return rc;
+  p.Tq = q->sizes[0];
+  p.heads = q->sizes[1];
+  p.D = q->sizes[2];
+  p.Tk = k->sizes[0];
+  p.kv_heads = k->sizes[1];
+  if (k->sizes[2] != p.D || v->sizes[0] != p.Tk || v->sizes[1] != p.kv_heads || v->sizes[2] != p.D)
+    return fail(NOVA_HIP_ESHAPE, "%s: q [%lld,%lld,%lld], k [%lld,%lld,%lld], v [%lld,%lld,%lld]", w,
+                (long long)p.Tq, (long long)p.heads, (long long)p.D, (long long)p.Tk,
+                (long long)p.kv_heads, (long long)k->sizes[2], (long long)v->sizes[0],
+                (long long)v->sizes[1], (long long)v->sizes[2]);
+  if (p.heads > 0 && (p.kv_heads == 0 || p.heads % p.kv_heads))
+    return fail(NOVA_HIP_ESHAPE, "%s: %lld query heads do not share %lld key heads evenly", w,
+                (long long)p.heads, (long long)p.kv_heads);
+  if (p.D % 8 || p.D > 128)
+    return fail(NOVA_HIP_ERANGE, "%s: head dim %lld is not a multiple of 8 up to 128", w,
+                (long long)p.D);
+  if (q_off->sizes[0] < 1 || q_off->sizes[0] != k_off->sizes[0])
+    return fail(NOVA_HIP_ESHAPE, "%s: offsets must both be [sequences + 1]", w);
+  if (!dense_i32(q_off) || !dense_i32(k_off))
+    return fail(NOVA_HIP_ESTRIDE, "%s: offsets must be dense", w);
+  if (!q_off->aligned || !k_off->aligned) return fail(NOVA_HIP_EINVAL, "%s: null offsets pointer", w);
+  p.B = q_off->sizes[0] - 1;
+  if (p.B > (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 sequences", w);
+  p.q_off = reinterpret_cast<const int32_t *>(data_of(q_off)) + q_off->offset;
+  p.k_off = reinterpret_cast<const int32_t *>(data_of(k_off)) + k_off->offset;
+  p.lse = nullptr;
+  p.slse = 0;
+  if (lse) {
+    if (lse->sizes[0] != p.heads || lse->sizes[1] != p.Tq)
+      return fail(NOVA_HIP_ESHAPE, "%s: lse must be [heads, query tokens]", w);
+    if ((p.Tq > 1 && lse->strides[1] != 1) || (p.heads > 1 && lse->strides[0] < p.Tq))
+      return fail(NOVA_HIP_ESTRIDE, "%s: lse rows must be dense and not overlap", w);
+    if (!lse->aligned && p.heads * p.Tq > 0)
+      return fail(NOVA_HIP_EINVAL, "%s: null lse pointer", w);
+    p.lse = reinterpret_cast<float *>(const_cast<char *>(data_of(lse))) + lse->offset;
+    p.slse = lse->strides[0];
+  }
+  p.scale = scale;
+  p.causal = causal != 0;
+  p.dt = dt;
+  return NOVA_HIP_SUCCESS;
+}
+
+int32_t same_shape(const NovaMemRef3D *a, const NovaMemRef3D *b, const char *w, const char *what) {
+  if (!a) return fail(NOVA_HIP_EINVAL, "%s: null %s descriptor", w, what);
+  for (int i = 0; i < 3; ++i)
+    if (a->sizes[i] != b->sizes[i]) return fail(NOVA_HIP_ESHAPE, "%s: shape of %s", w, what);
+  return NOVA_HIP_SUCCESS;
+}
+}  // namespace
+
+int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3D *k,
+                                        const NovaMemRef3D *v, const NovaMemRef1D *q_offsets,
+                                        const NovaMemRef1D *k_offsets, NovaMemRef3D *out,
+                                        NovaMemRef2D *lse, float scale, int32_t causal,
+                                        int32_t dt) {
+  clear_error();
+  const char *w = "attention";
+  AttentionProblem p;
+  int32_t rc = attn_common(q, k, v, q_offsets, k_offsets, lse, scale, causal, dt, w, p);
+  if (rc || (rc = same_shape(out, q, w, "out")) || (rc = attn_operand(out, w, "out", true, p.o)))
+    return rc;
+  return launch_attention(p, current_stream());
 }
 
 void nova_hip_set_stream(void *stream) { t_stream = static_cast<hipStream_t>(stream); }

@@ -122,6 +122,24 @@ int32_t launch_col_sum(const ColSumProblem &p, hipStream_t s);
 // groups index with 32-bit ints and run up to 2^20 past the extents).
 bool col_sum_in_range(int64_t rows, int64_t cols);
 
+// ---- attention (attention*.hip) ------------------------------------------------
+// One operand [tokens, heads, D] with unit stride on D; strides in elements.
+struct AttentionOperand {
+  void *p;
+  int64_t st, sh;  // token and head strides
+};
+struct AttentionProblem {
+  AttentionOperand q, k, v, o;
+  float *lse;  // [heads, Tq], row stride slse; may be null
+  int64_t slse;
+  const int32_t *q_off, *k_off;  // [B + 1] each
+  int64_t Tq, Tk, B, heads, kv_heads, D;
+  float scale;
+  bool causal;
+  int dt;
+};
+int32_t launch_attention(const AttentionProblem &p, hipStream_t s);
+
 // ---- program glue (glue.hip) -------------------------------------------------
 // c = a (op) b over a [4]-shaped index space; strides in elements, 0 on a
 // broadcast dimension.

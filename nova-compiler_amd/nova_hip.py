@@ -64,6 +64,7 @@ EXPORTS = (
     "_mlir_ciface_nova_hip_scatter_add_f32",
     "_mlir_ciface_nova_hip_reduce_sum_f32",
     "_mlir_ciface_nova_hip_index_to_i32",
+    "_mlir_ciface_nova_hip_attention",
     "nova_hip_set_stream",
     "nova_hip_get_stream",
     "nova_hip_synchronize",
@@ -159,6 +160,8 @@ def lib() -> ctypes.CDLL:
     L._mlir_ciface_nova_hip_scatter_add_f32.argtypes = [P, P, P, ctypes.c_int32]
     L._mlir_ciface_nova_hip_reduce_sum_f32.argtypes = [P, P]
     L._mlir_ciface_nova_hip_index_to_i32.argtypes = [P, P, ctypes.c_int32]
+    F, I = ctypes.c_float, ctypes.c_int32
+    L._mlir_ciface_nova_hip_attention.argtypes = [P, P, P, P, P, P, P, F, I, I]
     for name in EXPORTS:
         if name.startswith("_mlir_ciface_"):
             getattr(L, name).restype = ctypes.c_int32
@@ -541,3 +544,65 @@ def index_to_i32(idx, out=None):
     _bind_stream()
     check(lib()._mlir_ciface_nova_hip_index_to_i32(*[ref(v) for v in d], _index_dt(idx)))
     return out.reshape(idx.shape)
+
+
+# --------------------------------------------------------------------------
+# attention of packed sequences
+# --------------------------------------------------------------------------
+
+class _on_device:
+    """Makes the tensors' device the current one for a call, on its current
+    stream, and refuses tensors of different devices (descriptors carry none)."""
+
+    def __init__(self, *tensors):
+        dev = tensors[0].device
+        if dev.type != "cuda":
+            raise NovaHipError(1, f"tensors must be on the GPU, not on {dev}")
+        for t in tensors:
+            if t is not None and t.device != dev:
+                raise NovaHipError(1, f"tensors on {dev} and {t.device}")
+        self._ctx = None
+        torch = _torch()
+        if dev.index != torch.cuda.current_device():
+            self._ctx = torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        _bind_stream()
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+            _bind_stream()
+        return False
+
+
+def _want_dtype(dtype, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.dtype != dtype:
+            raise NovaHipError(4, f"{name} is {t.dtype}, not {dtype}")
+
+
+def attention(q, k, v, q_offsets, k_offsets, *, causal: bool = True, scale=None, out=None,
+              lse=None, want_lse: bool = True):
+    """Attention of packed sequences: q [tokens, heads, D], k and v [tokens,
+    key heads, D] (bf16 / f16), offsets [sequences + 1] i32 on the GPU.
+    ``causal`` aligns the last query with the last key; ``scale`` is
+    1 / sqrt(D) by default.  Returns (out, lse [heads, tokens] f32), lse None
+    with ``want_lse`` False; rows outside every sequence are not written."""
+    torch = _torch()
+    _want_dtype(q.dtype, k=k, v=v, out=out)
+    _want_dtype(torch.int32, q_offsets=q_offsets, k_offsets=k_offsets)
+    _want_dtype(torch.float32, lse=lse)
+    with _on_device(q, k, v, q_offsets, k_offsets, out, lse):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if lse is None and want_lse:
+            lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+        if scale is None:
+            scale = q.shape[2] ** -0.5
+        d = [memref_of(t) if t is not None else None
+             for t in (q, k, v, q_offsets, k_offsets, out, lse)]
+        check(lib()._mlir_ciface_nova_hip_attention(*[ref(x) for x in d], scale, int(causal), _dt(q)))
+    return out, lse

@@ -1,0 +1,176 @@
+"""Attention of packed sequences on the GPU against its definition in 64 bits.
+
+Tolerances, with u = finfo(dtype).eps / 2 and A = sum_j p_j |v_j| for an output
+row: the weights round once to dtype (u A, and in f16 2^-25 per weight below
+2^-14, as the largest is at least 1), the result once (u |o|).  Scores are f32
+sums of exact products; with D <= 128 unit-normal values they are off by less
+than 1e-5, which moves a weight by that much of itself: 4e-5 A covers them, the
+exponential, the sum and the division."""
+import math
+
+import pytest
+import torch
+
+import nova_hip as nh
+
+pytestmark = pytest.mark.gpu
+F64 = torch.float64
+BF, HF = torch.bfloat16, torch.float16
+
+
+def offsets(lens, dev, first=0):
+    o = [first]
+    for n in lens:
+        o.append(o[-1] + n)
+    return torch.tensor(o, dtype=torch.int32, device=dev)
+
+
+def make(dev, qlens, klens, H, G, D, dt, seed=0, layout="thd", pad=0):
+    """q, k, v: packed rows, `pad` rows of NaN behind the last sequence."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    Tq, Tk = sum(qlens), sum(klens)
+
+    def one(T, heads):
+        x = torch.randn(T + pad, heads, D, generator=g, device=dev).to(dt)
+        if pad:
+            x[T:] = float("nan")
+        if layout == "htd":
+            x = x.transpose(0, 1).contiguous().transpose(0, 1)
+        return x
+
+    if layout == "fused":
+        qkv = torch.randn(Tq + pad, H + 2 * G, D, generator=g, device=dev).to(dt)
+        if pad:
+            qkv[Tq:] = float("nan")
+        return qkv[:, :H], qkv[:, H:H + G], qkv[:, H + G:]
+    return one(Tq, H), one(Tk, G), one(Tk, G)
+
+
+def reference(q, k, v, qlens, klens, causal, scale):
+    """out, lse, sum p|v|, sum of visible |v|, all [.., heads] in 64 bits."""
+    Tq, H, D = q.shape
+    G = k.shape[1]
+    dev = q.device
+    out = torch.zeros(Tq, H, D, dtype=F64, device=dev)
+    amp, vis = torch.zeros_like(out), torch.zeros_like(out)
+    lse = torch.full((H, Tq), -math.inf, dtype=F64, device=dev)
+    a = c = 0
+    for n, m in zip(qlens, klens):
+        keep = torch.ones(n, m, dtype=torch.bool, device=dev)
+        if causal:
+            keep = keep.tril(m - n)
+        some = keep.any(1)
+        for h in range(H):
+            kh, vh = k[c:c + m, h * G // H].double(), v[c:c + m, h * G // H].double()
+            s = (torch.mm(q[a:a + n, h].double(), kh.t().contiguous()) * scale).masked_fill(~keep, -math.inf)
+            p = torch.where(some[:, None], torch.softmax(s, 1), torch.zeros_like(s)) if m else s
+            # A masked weight takes no part, whatever stands in v.
+            clean = torch.nan_to_num(vh, 0.0, 0.0, 0.0)
+            out[a:a + n, h] = torch.mm(p, clean)
+            amp[a:a + n, h] = torch.mm(p, clean.abs())
+            vis[a:a + n, h] = torch.mm(keep.double(), clean.abs())
+            lse[h, a:a + n] = torch.logsumexp(s, 1) if m else -math.inf
+        a, c = a + n, c + m
+    return out, lse, amp, vis
+
+
+def check(out, lse, q, k, v, qlens, klens, causal, scale, what=""):
+    want, wlse, amp, vis = reference(q, k, v, qlens, klens, causal, scale)
+    T = sum(qlens)
+    u = torch.finfo(q.dtype).eps / 2
+    tol = u * (amp + want.abs()) * 1.01 + 4e-5 * amp + (2.0 ** -25 * vis if q.dtype == HF else 0.0)
+    tol = tol + torch.finfo(q.dtype).smallest_normal * torch.finfo(q.dtype).eps  # subnormal results
+    err = (out.double() - want).abs()[:T]
+    assert not torch.isnan(err).any(), what
+    worst = (err - tol[:T]).max().item() if err.numel() else 0.0
+    assert worst <= 0, (what, worst, err.max().item())
+    if lse is not None:
+        empty = torch.isinf(wlse[:, :T])
+        assert torch.equal(torch.isinf(lse[:, :T]), empty), what
+        d = (lse[:, :T].double() - wlse[:, :T]).masked_fill(empty, 0.0).abs()
+        assert d.numel() == 0 or d.max().item() <= 4e-5, (what, d.max().item())
+
+
+def run(dev, qlens, klens, H, G, D, dt, causal, layout="thd", seed=0, scale=None, pad=0):
+    q, k, v = make(dev, qlens, klens, H, G, D, dt, seed, layout, pad)
+    scale = D ** -0.5 if scale is None else scale
+    out = torch.full(q.shape, 7.0, dtype=dt, device=dev)
+    lse = torch.full((H, q.shape[0]), 7.0, device=dev)
+    nh.attention(q, k, v, offsets(qlens, dev), offsets(klens, dev), causal=causal, scale=scale,
+                 out=out, lse=lse)
+    T = sum(qlens)
+    assert (out[T:] == 7.0).all() and (lse[:, T:] == 7.0).all()  # rows behind the last sequence
+    check(out, lse, q, k, v, qlens, klens, causal, scale, (qlens, klens, H, G, D, dt, causal, layout))
+    return out
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 80, 96, 120, 128])
+def test_head_dims(cuda, dt, causal, D):
+    run(cuda, [197, 33], [197, 33], 4, 2, D, dt, causal)
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 1000])
+@pytest.mark.parametrize("causal", [False, True])
+def test_lengths(cuda, n, causal):
+    run(cuda, [n], [n], 2, 1, 64, BF, causal)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("qlens,klens", [
+    ([5, 0, 130, 1], [77, 3, 130, 200]),    # more keys than queries, an empty query part
+    ([40, 3, 0], [0, 70, 0]),               # no keys; nothing at all
+    ([200, 64], [70, 1]),                   # causal: the first queries see no key
+    ([1] * 70 + [65] + [0] * 70 + [2], [64] * 70 + [65] + [0] * 70 + [1]),
+])
+def test_uneven_and_empty_sequences(cuda, qlens, klens, D):
+    for causal in (False, True):
+        run(cuda, qlens, klens, 4, 2, D, BF, causal, pad=3)
+
+
+@pytest.mark.parametrize("layout", ["thd", "htd", "fused"])
+@pytest.mark.parametrize("H,G", [(1, 1), (8, 1), (6, 6), (9, 3), (32, 8)])
+def test_layouts_and_shared_heads(cuda, layout, H, G):
+    run(cuda, [150, 70, 3], [150, 70, 3], H, G, 64, HF, True, layout, pad=5 if layout != "fused" else 0)
+
+
+@pytest.mark.parametrize("scale", [1e-3, 0.125, 1.0])
+def test_scales(cuda, scale):
+    # Scores of scale 1 reach +-40: the running maximum moves and the sums are
+    # rescaled.  |s| <= 64 carries 64 * 128 * 2^-24 of rounding at most, but the
+    # f32 sum's is far below its bound; 4e-5 still holds as 2^-24 * 64 * 8.
+    run(cuda, [300], [300], 2, 2, 64, BF, True, scale=scale)
+
+
+def test_growing_scores_move_the_maximum(cuda):
+    """Keys ordered so that each tile's scores are far above the last one's."""
+    n, D = 512, 64
+    q = torch.ones(n, 1, D, device=cuda, dtype=BF)
+    k = (torch.arange(n, device=cuda)[:, None, None] / 8.0 * torch.ones(1, 1, D, device=cuda)).to(BF)
+    v = torch.randn(n, 1, D, device=cuda).to(BF)
+    for flip in (False, True):
+        kk = k.flip(0).contiguous() if flip else k
+        out, lse = nh.attention(q, kk, v, offsets([n], cuda), offsets([n], cuda), causal=False,
+                                scale=0.125)
+        # Scores are exact multiples of 1/8 up to 2^9; lse rounds at 2^-15 there.
+        want, wlse, amp, _ = reference(q, kk, v, [n], [n], False, 0.125)
+        u = 2.0 ** -8
+        assert ((out.double() - want).abs() <= u * (amp + want.abs()) * 1.01 + 4e-4 * amp).all()
+        assert ((lse.double() - wlse).abs() <= 2.0 ** -13).all()
+
+
+def test_rows_of_other_sequences_do_not_leak(cuda):
+    """A sequence between two that hold NaN and infinity."""
+    lens = [37, 70, 50]
+    q, k, v = make(cuda, lens, lens, 2, 2, 64, BF)
+    for t in (q, k, v):
+        t[:37] = float("nan")
+        t[107:] = float("inf")
+    out, lse = nh.attention(q, k, v, offsets(lens, cuda), offsets(lens, cuda), causal=False)
+    sl = slice(37, 107)
+    check(out[sl], lse[:, sl], q[sl], k[sl], v[sl], [70], [70], False, 0.125)
+
+
+def test_long_sequence(cuda):
+    run(cuda, [2500], [4001], 2, 1, 128, BF, True)
