@@ -422,6 +422,86 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
                                         const NovaMemRef1D *k_offsets, NovaMemRef3D *out,
                                         NovaMemRef2D *lse, float scale, int32_t causal,
                                         int32_t dt);
+/* The gradients of _mlir_ciface_nova_hip_attention's result with respect to
+ * q, k and v, from its operands, its result `out` and its `lse`:
+ *   P = exp(scale S - lse), dS = P o (grad_out V^T - rowsum(grad_out o out)),
+ *   dv = P^T grad_out, dq = scale dS k, dk = scale dS^T q,
+ * dk and dv summed over the query heads that share a key head.  Shapes and
+ * strides as for the forward (grad_out, out, dq as q; dk, dv as k); lse
+ * [heads, query tokens]; scratch : at least 2 * heads * query tokens f32,
+ * dense, used by this call only.  P and dS are rounded to dt for the
+ * products, sums are f32 in a fixed order (no atomics: the same bits on every
+ * run).  A query that sees no key has gradient zero and adds none; rows
+ * outside every sequence are left as they were. */
+int32_t _mlir_ciface_nova_hip_attention_backward(
+    const NovaMemRef3D *grad_out, const NovaMemRef3D *q, const NovaMemRef3D *k,
+    const NovaMemRef3D *v, const NovaMemRef3D *out, const NovaMemRef2D *lse,
+    const NovaMemRef1D *q_offsets, const NovaMemRef1D *k_offsets, NovaMemRef3D *dq,
+    NovaMemRef3D *dk, NovaMemRef3D *dv, NovaMemRef1D *scratch, float scale, int32_t causal,
+    int32_t dt);
+/* Attention of one query per sequence over a padded cache (single-token
+ * serving): out[b, h] = softmax(scale q[b, h] . k[b, :lengths[b]]) v.
+ *   q, out : [sequences, heads, D]; k, v : [sequences, cache rows, key heads,
+ *   D], unit stride on D, any order of the other dims, rows 16-byte aligned;
+ *   lengths : [sequences] i32 in device memory, each cut to [0, cache rows];
+ *   rows behind a length are not read.  lse : [sequences, heads] f32 or NULL.
+ *   scratch : nova_hip_attention_decode_scratch() f32, dense and 8-byte aligned,
+ *   used by this call only (NULL when that is 0).
+ * A length of 0 gives a zero row and lse -inf.  Types and roundings as for
+ * _mlir_ciface_nova_hip_attention. */
+int32_t _mlir_ciface_nova_hip_attention_decode(const NovaMemRef3D *q, const NovaMemRef4D *k,
+                                               const NovaMemRef4D *v, const NovaMemRef1D *lengths,
+                                               NovaMemRef3D *out, NovaMemRef2D *lse,
+                                               NovaMemRef1D *scratch, float scale, int32_t dt);
+/* Floats of scratch the call above needs on sizes it accepts. */
+int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int64_t heads,
+                                          int64_t kv_heads, int64_t D);
+/* ------------------------------------------------------------------------
+ * Losses over token log-probabilities (HBM bound), beside nova.sce.  No
+ * reference counterpart.  For all three:
+ *   logits, grad : [R, C] of dt NOVA_HIP_DT_F32, _BF16 or _F16; any row
+ *   stride; grad must not overlap logits; labels : [R] i32.
+ * A row with a negative label (a prompt token, padding) takes no part: its
+ * logits are not read, its log-probability is 0 and its gradient row zero.  A
+ * label of C or more makes the row's results NaN.  Row results and sums are
+ * f32, sums over rows are taken in 64 bits in a fixed order.  No workspace.
+ * ---------------------------------------------------------------------- */
+/* logp[r] = logits[r, labels[r]] - lse[r], lse = log sum exp of the row (or
+ * NULL; 0 in rows without a label). */
+int32_t _mlir_ciface_nova_hip_token_logp(const NovaMemRef2D *logits, const NovaMemRef1D *labels,
+                                         NovaMemRef1D *logp, NovaMemRef1D *lse, int32_t dt);
+/* The clipped policy loss with a KL term.  With logp as above and, per row,
+ *   ratio = exp(logp - old_logp),
+ *   l = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (exp(ref_logp - logp) - (ref_logp - logp) - 1):
+ *   row_loss = weight l, loss[0] = sum of row_loss, and grad (or NULL) =
+ *   grad_scale * d loss / d logits in the same pass over the logits.
+ * Where both sides of the min are equal the gradient is the first's.
+ *   old_logp, ref_logp, advantage (A), weight, logp, row_loss : [R] f32;
+ *   ref_logp may be NULL when kl_coef is 0.  A row with weight 0 takes no
+ *   part either.  weight carries the mean a caller wants (1 / valid tokens,
+ *   1 / (sequences length), ...); grad_scale is a loss scale. */
+int32_t _mlir_ciface_nova_hip_policy_loss(
+    const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *old_logp,
+    const NovaMemRef1D *ref_logp, const NovaMemRef1D *advantage, const NovaMemRef1D *weight,
+    NovaMemRef1D *loss, NovaMemRef1D *logp, NovaMemRef1D *row_loss, NovaMemRef2D *grad,
+    float clip_low, float clip_high, float kl_coef, float grad_scale, int32_t dt);
+/* The paired preference loss.  Sequence s is the rows [offsets[s],
+ * offsets[s + 1]) (i32 in device memory, not decreasing, each cut to [0, R]),
+ * 2p the chosen and 2p + 1 the rejected one of pair p; seq_logp[s] = sum of its
+ * rows' logp; with
+ *   h = beta ((seq_logp - ref_logp)[2p] - (seq_logp - ref_logp)[2p + 1]):
+ *   pair_loss[p] = -(1 - smoothing) log sigmoid(h) - smoothing log sigmoid(-h),
+ *   loss[0] = mean of pair_loss, grad (or NULL) = grad_scale d loss / d logits,
+ * zero in rows outside every sequence.
+ *   offsets : [2 pairs + 1]; ref_logp, seq_logp : [2 pairs] f32; pair_loss :
+ *   [pairs] f32; token : [3, R] f32, written with the rows' logp, lse and slope
+ *   grad_scale * d loss / d logp. */
+int32_t _mlir_ciface_nova_hip_preference_loss(
+    const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *offsets,
+    const NovaMemRef1D *ref_logp, NovaMemRef1D *loss, NovaMemRef1D *seq_logp,
+    NovaMemRef1D *pair_loss, NovaMemRef2D *token, NovaMemRef2D *grad, float beta, float smoothing,
+    float grad_scale, int32_t dt);
 /* ------------------------------------------------------------------------
  * Typed aliases for lowered modules (nova-compiler_amd/mlir/
  * NovaHipLowering.cpp).  An MLIR module declares each callee once, with one

@@ -1,0 +1,396 @@
+// Backward of attention over packed sequences (attention.hip), from the
+// forward's result and log-sum-exp:  P = exp(scale S - lse),
+//   dV = P^T dO,  dP = dO V^T,  dS = P o (dP - delta),  delta = rowsum(dO o O),
+//   dQ = scale dS K,  dK = scale dS^T Q.
+//
+// Two kernels, each recomputing P and dP for itself, so that every sum is
+// made by one workgroup in a fixed order: no atomics, no partial sums in
+// memory, the same bits on every run, and the gradients of keys shared by a
+// group of query heads are summed over the group inside the workgroup.  That
+// is seven products where five are the least.  attention_dq_kernel holds 32
+// queries per wave and streams keys and values; it also writes the rows' two
+// constants (lse in base 2, delta), which attention_dkv_kernel, behind it on
+// the stream, reads while it holds keys and values and streams Q and dO.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "attention.h"
+
+namespace nova_hip {
+namespace attn {
+namespace {
+
+struct BwdArgs {
+  const uint16_t *q, *k, *v, *o, *go;
+  const float *lse;
+  uint16_t *dq, *dk, *dv;
+  float *rows;  // [2][heads][Tq]: lse log2 e, delta
+  const int *q_off, *k_off;
+  Rows sq, sk, sv, so, sgo, sdq, sdk, sdv;
+  int64_t slse;
+  int Tq, Tk, B, heads, group, D, tiles;
+  float c, scale;
+};
+
+constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
+
+// f16 weights take a factor 2^8 in the product for dV (they are at most 1, and
+// in long rows most lie under 2^-14, where f16 has fewer bits), taken back at
+// the store; bf16 has f32's exponents and needs none.
+template <int DT>
+constexpr float kWeightLog2 = DT == NOVA_HIP_DT_F16 ? 8.0f : 0.0f;
+
+__device__ __forceinline__ int xcd_run(int id, int total) {
+  const int per = total >> 3, rem = total & 7, x = id & 7;
+  return x * per + min(x, rem) + (id >> 3);
+}
+
+// sum over d of a row's products, the row held as load_cols gives it.
+template <int DT, int DP>
+__device__ __forceinline__ float row_dot(const u32x4 (&x)[DP / 16], const u32x4 (&y)[DP / 16]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == NOVA_HIP_DT_BF16) {
+        s = __builtin_fmaf(__uint_as_float(x[i][j] << 16), __uint_as_float(y[i][j] << 16), s);
+        s = __builtin_fmaf(__uint_as_float(x[i][j] & 0xffff0000u),
+                           __uint_as_float(y[i][j] & 0xffff0000u), s);
+      } else {
+        const auto a = __builtin_bit_cast(gemm::f16x2v, (uint32_t)x[i][j]);
+        const auto b = __builtin_bit_cast(gemm::f16x2v, (uint32_t)y[i][j]);
+        s = __builtin_fmaf((float)a[0], (float)b[0], s);
+        s = __builtin_fmaf((float)a[1], (float)b[1], s);
+      }
+    }
+  return both_sum(s);
+}
+
+template <int DT, int DP, bool CAUSAL>
+__global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a) {
+  constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
+  __shared__ __attribute__((aligned(1024))) char sk0[kTile];
+  __shared__ __attribute__((aligned(1024))) char sk1[kTile];
+  __shared__ __attribute__((aligned(1024))) char sv0[kTile];
+  __shared__ __attribute__((aligned(1024))) char sv1[kTile];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
+  const int head = w / a.tiles, tile = a.tiles - 1 - (w - head * a.tiles);
+  int b, row0;
+  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, row0)) return;
+  int qs, qe, ks, ke;
+  seq_rows(a.q_off, b, a.Tq, qs, qe);
+  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  const int Lq = qe - qs, Lk = ke - ks, shift = Lk - Lq;
+  const int keys = CAUSAL ? min(Lk, max(0, row0 + kBM + shift)) : Lk;
+  const int nt = (keys + kBN - 1) / kBN;
+
+  const int q0 = row0 + 32 * wave, qn = min(32, Lq - q0);
+  u32x4 qf[DP / 16], gf[DP / 16];
+  load_cols<DP>(qf, a.q + (qs + q0) * a.sq.t + head * a.sq.h, a.sq.t, qn, a.D, lane);
+  load_cols<DP>(gf, a.go + (qs + q0) * a.sgo.t + head * a.sgo.h, a.sgo.t, qn, a.D, lane);
+  float nl = 0.0f, delta;
+  {
+    u32x4 of[DP / 16];
+    load_cols<DP>(of, a.o + (qs + q0) * a.so.t + head * a.so.h, a.so.t, qn, a.D, lane);
+    delta = row_dot<DT, DP>(gf, of);
+  }
+  const int64_t at = (int64_t)head * a.Tq + qs + q0 + (lane & 31);
+  if ((lane & 31) < qn) {
+    const float lse = a.lse[head * a.slse + qs + q0 + (lane & 31)];
+    // A row without keys (lse -inf): every weight is masked below.
+    nl = lse == -INFINITY ? 0.0f : lse * kLog2e;
+    if (lane < 32) {
+      a.rows[at] = nl - kWeightLog2<DT>;
+      a.rows[(int64_t)a.heads * a.Tq + at] = delta;
+    }
+  }
+
+  const uint16_t *kp = a.k + ks * a.sk.t + (head / a.group) * a.sk.h;
+  const uint16_t *vp = a.v + ks * a.sv.t + (head / a.group) * a.sv.h;
+  TileLoad<kBN, CH, kWaves> lk, lv;
+  lk.init(a.sk.t, a.D);
+  lv.init(a.sv.t, a.D);
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+  const int last = q0 + (lane & 31) + shift;
+
+  auto fetch = [&](int t, char *sk, char *sv) __attribute__((always_inline)) {
+    lk.load(kp + (int64_t)t * kBN * a.sk.t, a.sk.t, Lk - t * kBN, a.D, sk);
+    lv.load(vp + (int64_t)t * kBN * a.sv.t, a.sv.t, Lk - t * kBN, a.D, sv);
+  };
+  auto step = [&](int t, const char *sk, const char *sv) __attribute__((always_inline)) {
+    const int k0 = t * kBN;
+    if (qn <= 0 || (CAUSAL && k0 > q0 + qn - 1 + shift)) return;
+    const bool edge = k0 + kBN > Lk || (CAUSAL && k0 + kBN - 1 > q0 + shift);
+    const int end = CAUSAL ? min(Lk, last + 1) : Lk;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        s = mfma_32x32x16<DT>(read_row_frag(sk, row_frag<CH>(32 * i, kk, lane)), qf[kk], s);
+        dp = mfma_32x32x16<DT>(read_row_frag(sv, row_frag<CH>(32 * i, kk, lane)), gf[kk], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl)) * (dp[r] - delta);
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[r] = 0.0f;
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const u32x4 sf = pack_frag<DT>(s, kk);  // dS rounds to the operands' type
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+          acc[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sk, 32 * i + 16 * kk, 32 * db, lane), sf,
+                                      acc[db]);
+      }
+    }
+  };
+  auto sync = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+  };
+  if (nt > 0) fetch(0, sk0, sv0);
+  for (int t = 0; t < nt; t += 2) {
+    sync();
+    if (t + 1 < nt) fetch(t + 1, sk1, sv1);
+    step(t, sk0, sv0);
+    if (t + 1 >= nt) break;
+    sync();
+    if (t + 2 < nt) fetch(t + 2, sk0, sv0);
+    step(t + 1, sk1, sv1);
+  }
+  if (qn <= 0) return;
+  store_rows<DT, DP>(acc, a.scale, a.dq + (qs + q0) * a.sdq.t + head * a.sdq.h, a.sdq.t, qn, a.D,
+                     lane);
+}
+
+// Keys [32 WK of them] x all query heads of the group and all their queries.
+// WK waves share the keys, 4 / WK the queries of a tile; the latter's sums
+// are added in wave order at the end.
+template <int DT, int DP, bool CAUSAL, int WK>
+__global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_kernel(BwdArgs a) {
+  constexpr int WQ = kWaves / WK, kKeys = 32 * WK;
+  constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
+  __shared__ __attribute__((aligned(1024))) char sq0[kTile];
+  __shared__ __attribute__((aligned(1024))) char sq1[kTile];
+  __shared__ __attribute__((aligned(1024))) char sg0[kTile];
+  __shared__ __attribute__((aligned(1024))) char sg1[kTile];
+  __shared__ __attribute__((aligned(1024))) float sc0[2 * kBN];  // the tile's row constants
+  __shared__ __attribute__((aligned(1024))) float sc1[2 * kBN];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = wave % WK, wq = wave / WK;
+  const int kv_heads = a.heads / a.group;
+  const int w = xcd_run(blockIdx.x, a.tiles * kv_heads);
+  const int kh = w / a.tiles, tile = w - kh * a.tiles;
+  int b, row0;
+  if (!find_tile(a.k_off, a.B, a.Tk, kKeys, tile, b, row0)) return;
+  int qs, qe, ks, ke;
+  seq_rows(a.q_off, b, a.Tq, qs, qe);
+  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  const int Lq = qe - qs, Lk = ke - ks, shift = Lk - Lq;
+  // Causal: key j is seen by the queries j - shift and on.
+  const int first = CAUSAL ? min(Lq, max(0, row0 - shift)) : 0;
+  const int nt = (Lq - first + kBN - 1) / kBN, total = nt * a.group;
+
+  const int k0 = row0 + 32 * wk, kn = min(32, Lk - k0);
+  u32x4 kf[DP / 16], vf[DP / 16];
+  load_cols<DP>(kf, a.k + (ks + k0) * a.sk.t + kh * a.sk.h, a.sk.t, kn, a.D, lane);
+  load_cols<DP>(vf, a.v + (ks + k0) * a.sv.t + kh * a.sv.h, a.sv.t, kn, a.D, lane);
+  TileLoad<kBN, CH, kWaves> lq, lg;
+  lq.init(a.sq.t, a.D);
+  lg.init(a.sgo.t, a.D);
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
+
+  auto fetch = [&](int u, char *sq, char *sg, float *sc) __attribute__((always_inline)) {
+    const int g = u / nt, q0 = first + (u - g * nt) * kBN, head = kh * a.group + g;
+    const int n = Lq - q0;
+    lq.load(a.q + (int64_t)(qs + q0) * a.sq.t + head * a.sq.h, a.sq.t, n, a.D, sq);
+    lg.load(a.go + (int64_t)(qs + q0) * a.sgo.t + head * a.sgo.h, a.sgo.t, n, a.D, sg);
+    // Rows behind the sequence read zero: with q and dO zero there too, they
+    // add nothing.
+    if (wave < 2) {
+      const float *p = a.rows + ((int64_t)wave * a.heads + head) * a.Tq + qs + q0;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<float *>(p), (short)0, min(n, kBN) * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(sc + kBN * wave), 4, lane * 4, 0, 0,
+                                               0);
+    }
+  };
+  auto step = [&](int u, const char *sq, const char *sg, const float *sc)
+      __attribute__((always_inline)) {
+    const int q0 = first + (u % nt) * kBN;
+    if (kn <= 0) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i % WQ != wq) continue;
+      if (CAUSAL && q0 + 32 * i + 31 + shift < k0) continue;  // no query of these sees these keys
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        s = mfma_32x32x16<DT>(read_row_frag(sq, row_frag<CH>(32 * i, kk, lane)), kf[kk], s);
+        dp = mfma_32x32x16<DT>(read_row_frag(sg, row_frag<CH>(32 * i, kk, lane)), vf[kk], dp);
+      }
+      constexpr float kDown = DT == NOVA_HIP_DT_F16 ? 1.0f / 256.0f : 1.0f;
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int row = 32 * i + 8 * r4 + 4 * (lane >> 5);
+        const gemm::f32x4 nl = *reinterpret_cast<const gemm::f32x4 *>(sc + row);
+        const gemm::f32x4 de = *reinterpret_cast<const gemm::f32x4 *>(sc + kBN + row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * r4 + e;
+          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl[e]));
+          dp[r] = s[r] * ((dp[r] - de[e]) * kDown);
+        }
+      }
+      if (CAUSAL && q0 + 32 * i + shift < k0 + 31) {
+        const int from = k0 + (lane & 31) - shift - q0 - 32 * i - 4 * (lane >> 5);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + (r & 3) < from) s[r] = dp[r] = 0.0f;
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        // Weights and dS round to the operands' type for these products.
+        const u32x4 pf = pack_frag<DT>(s, kk), sf = pack_frag<DT>(dp, kk);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+          dv[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sg, 32 * i + 16 * kk, 32 * db, lane), pf,
+                                     dv[db]);
+          dk[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sq, 32 * i + 16 * kk, 32 * db, lane), sf,
+                                     dk[db]);
+        }
+      }
+    }
+  };
+  auto sync = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __syncthreads();
+  };
+  if (total > 0) fetch(0, sq0, sg0, sc0);
+  for (int u = 0; u < total; u += 2) {
+    sync();
+    if (u + 1 < total) fetch(u + 1, sq1, sg1, sc1);
+    step(u, sq0, sg0, sc0);
+    if (u + 1 >= total) break;
+    sync();
+    if (u + 2 < total) fetch(u + 2, sq0, sg0, sc0);
+    step(u + 1, sq1, sg1, sc1);
+  }
+  if constexpr (WQ == 2) {
+    // The second wave of each key block hands its sums over through LDS, 32
+    // columns of d at a time (one 32 x 32 block of f32 per pair of waves).
+    float *box = reinterpret_cast<float *>(wk ? sq1 : sq0);
+    static_assert(WK == 2 && kTile >= 64 * 16 * 4, "one block per box");
+#pragma unroll
+    for (int j = 0; j < 2 * (DP / 32); ++j) {
+      f32x16 &x = j < DP / 32 ? dk[j % (DP / 32)] : dv[j % (DP / 32)];
+      __syncthreads();
+      if (wq == 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[64 * r + lane] = x[r];
+      }
+      __syncthreads();
+      if (wq == 0) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] += box[64 * r + lane];
+      }
+    }
+    if (wq == 1) return;
+  }
+  if (kn <= 0) return;
+  store_rows<DT, DP>(dk, a.scale, a.dk + (ks + k0) * a.sdk.t + kh * a.sdk.h, a.sdk.t, kn, a.D,
+                     lane);
+  store_rows<DT, DP>(dv, DT == NOVA_HIP_DT_F16 ? 1.0f / 256.0f : 1.0f,
+                     a.dv + (ks + k0) * a.sdv.t + kh * a.sdv.h, a.sdv.t, kn, a.D, lane);
+}
+
+constexpr int kWK = 4;  // key blocks of a workgroup
+
+template <int DT, int DP, bool CAUSAL>
+int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s) {
+  if (q_tiles > 0) {
+    a.tiles = (int)q_tiles;
+    hipLaunchKernelGGL((attention_dq_kernel<DT, DP, CAUSAL>), dim3((unsigned)(q_tiles * a.heads)),
+                       dim3(64 * kWaves), 0, s, a);
+    const int32_t rc = check_hip(hipGetLastError(), "attention_backward launch");
+    if (rc) return rc;
+  }
+  if (k_tiles > 0) {
+    a.tiles = (int)k_tiles;
+    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL, kWK>),
+                       dim3((unsigned)(k_tiles * (a.heads / a.group))), dim3(64 * kWaves), 0, s, a);
+  }
+  return check_hip(hipGetLastError(), "attention_backward launch");
+}
+template <int DT, int DP>
+int32_t launch_bwd_c(const BwdArgs &a, bool causal, int64_t qt, int64_t kt, hipStream_t s) {
+  return causal ? launch_bwd_t<DT, DP, true>(a, qt, kt, s) : launch_bwd_t<DT, DP, false>(a, qt, kt, s);
+}
+template <int DT>
+int32_t launch_bwd(const BwdArgs &a, bool causal, int64_t qt, int64_t kt, hipStream_t s) {
+  if (a.D <= 32) return launch_bwd_c<DT, 32>(a, causal, qt, kt, s);
+  if (a.D <= 64) return launch_bwd_c<DT, 64>(a, causal, qt, kt, s);
+  if (a.D <= 96) return launch_bwd_c<DT, 96>(a, causal, qt, kt, s);
+  return launch_bwd_c<DT, 128>(a, causal, qt, kt, s);
+}
+
+}  // namespace
+}  // namespace attn
+
+int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t s) {
+  if (p.f.heads == 0 || p.f.D == 0 || p.f.B == 0) return NOVA_HIP_SUCCESS;
+  attn::BwdArgs a;
+  a.q = static_cast<const uint16_t *>(p.f.q.p);
+  a.k = static_cast<const uint16_t *>(p.f.k.p);
+  a.v = static_cast<const uint16_t *>(p.f.v.p);
+  a.o = static_cast<const uint16_t *>(p.f.o.p);
+  a.go = static_cast<const uint16_t *>(p.go.p);
+  a.dq = static_cast<uint16_t *>(p.dq.p);
+  a.dk = static_cast<uint16_t *>(p.dk.p);
+  a.dv = static_cast<uint16_t *>(p.dv.p);
+  a.lse = p.f.lse;
+  a.slse = p.f.slse;
+  a.rows = p.rows;
+  a.q_off = p.f.q_off;
+  a.k_off = p.f.k_off;
+  a.sq = {p.f.q.st, p.f.q.sh};
+  a.sk = {p.f.k.st, p.f.k.sh};
+  a.sv = {p.f.v.st, p.f.v.sh};
+  a.so = {p.f.o.st, p.f.o.sh};
+  a.sgo = {p.go.st, p.go.sh};
+  a.sdq = {p.dq.st, p.dq.sh};
+  a.sdk = {p.dk.st, p.dk.sh};
+  a.sdv = {p.dv.st, p.dv.sh};
+  a.Tq = (int)p.f.Tq;
+  a.Tk = (int)p.f.Tk;
+  a.B = (int)p.f.B;
+  a.heads = (int)p.f.heads;
+  a.group = (int)(p.f.heads / p.f.kv_heads);
+  a.D = (int)p.f.D;
+  a.tiles = 0;
+  a.c = p.f.scale * attn::kLog2e;
+  a.scale = p.f.scale;
+  // Whole tiles and, for each sequence, at most one that is not.
+  const int64_t qt = std::min(p.f.Tq, p.f.Tq / attn::kBM + p.f.B);
+  const int64_t kt = std::min(p.f.Tk, p.f.Tk / (32 * attn::kWK) + p.f.B);
+  if (std::max(qt * p.f.heads, kt * p.f.kv_heads) > 0x7fffffff)
+    return fail(NOVA_HIP_ERANGE, "attention_backward: more than 2^31 - 1 tiles");
+  return p.f.dt == NOVA_HIP_DT_BF16
+             ? attn::launch_bwd<NOVA_HIP_DT_BF16>(a, p.f.causal, qt, kt, s)
+             : attn::launch_bwd<NOVA_HIP_DT_F16>(a, p.f.causal, qt, kt, s);
+}
+
+}  // namespace nova_hip

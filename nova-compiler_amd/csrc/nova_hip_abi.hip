@@ -872,19 +872,21 @@ int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D
 
 // ---- attention --------------------------------------------------------------------
 namespace {
-constexpr int64_t kAttnMaxStride = 1 << 24;  // elements; 128 rows stay below 2^32 bytes
+constexpr int64_t kAttnMaxStride = 1 << 24;  // elements; 64 rows stay below 2^31 bytes
 
 // One operand [T, heads, D]: unit stride on D, rows of whole 16-byte chunks at
-// 16-byte aligned addresses.  A dim of extent 1 is never stepped.
+// 16-byte aligned addresses.  A dim of extent 1 may have any stride: it gets
+// the row's own length, so that the rows a tile holds behind the last one lie
+// outside the operand, where loads return zero.
 int32_t attn_operand(const NovaMemRef3D *d, const char *w, const char *what, bool out,
                      AttentionOperand &o) {
   if (!d) return fail(NOVA_HIP_EINVAL, "%s: null %s descriptor", w, what);
   if (!nonneg_sizes(d, 3)) return fail(NOVA_HIP_ESHAPE, "%s: negative size", w);
   const int64_t T = d->sizes[0], H = d->sizes[1], D = d->sizes[2];
-  o.st = T > 1 ? d->strides[0] : 0;
+  o.st = T > 1 ? d->strides[0] : (D + 7) / 8 * 8;
   o.sh = H > 1 ? d->strides[1] : 0;
-  if (T > 0x7fffffff || H > 0xffff)
-    return fail(NOVA_HIP_ERANGE, "%s: %s has more than 2^31 - 1 tokens or 65535 heads", w, what);
+  if (T > 0x7fffffff - (1 << 20) || H > 0xffff)
+    return fail(NOVA_HIP_ERANGE, "%s: %s has more than 2^31 - 2^20 tokens or 65535 heads", w, what);
   if (T == 0 || H == 0 || D == 0) {
     o.p = nullptr;
     return NOVA_HIP_SUCCESS;
@@ -892,20 +894,17 @@ int32_t attn_operand(const NovaMemRef3D *d, const char *w, const char *what, boo
   if (!d->aligned) return fail(NOVA_HIP_EINVAL, "%s: null %s data pointer", w, what);
   if (D > 1 && d->strides[2] != 1)
     return fail(NOVA_HIP_ESTRIDE, "%s: %s must have unit stride on the head dim", w, what);
-  if (o.st < 0 || o.sh < 0)
-    return fail(NOVA_HIP_ESTRIDE, "%s: negative strides are not addressed", w);
+  if ((T > 1 && o.st < D) || o.sh < 0)
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
   o.p = const_cast<char *>(data_of(d)) + d->offset * 2;
   if (o.st % 8 || o.sh % 8 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
     return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s must start at 16-byte aligned addresses", w, what);
   if (o.st > kAttnMaxStride)
     return fail(NOVA_HIP_ERANGE, "%s: token stride of %s exceeds 2^24 elements", w, what);
-  if (out) {
-    const int64_t inner = std::min(T > 1 ? o.st : INT64_MAX, H > 1 ? o.sh : INT64_MAX);
-    const bool t_inner = T > 1 && (H <= 1 || o.st <= o.sh);
-    if ((T > 1 || H > 1) && inner < D) return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
-    if (T > 1 && H > 1 &&
-        (t_inner ? o.sh < (T - 1) * o.st + D : o.st < (H - 1) * o.sh + D))
-      return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
+  if (out && H > 1) {
+    const bool apart = o.sh >= D && (T <= 1 || (o.st <= o.sh ? o.sh >= (T - 1) * o.st + D
+                                                             : o.st >= (H - 1) * o.sh + D));
+    if (!apart) return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
   }
   return NOVA_HIP_SUCCESS;
 }
@@ -989,6 +988,288 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
   if (rc || (rc = same_shape(out, q, w, "out")) || (rc = attn_operand(out, w, "out", true, p.o)))
     return rc;
   return launch_attention(p, current_stream());
+}
+
+int32_t _mlir_ciface_nova_hip_attention_backward(
+    const NovaMemRef3D *grad_out, const NovaMemRef3D *q, const NovaMemRef3D *k,
+    const NovaMemRef3D *v, const NovaMemRef3D *out, const NovaMemRef2D *lse,
+    const NovaMemRef1D *q_offsets, const NovaMemRef1D *k_offsets, NovaMemRef3D *dq,
+    NovaMemRef3D *dk, NovaMemRef3D *dv, NovaMemRef1D *scratch, float scale, int32_t causal,
+    int32_t dt) {
+  clear_error();
+  const char *w = "attention_backward";
+  if (!lse) return fail(NOVA_HIP_EINVAL, "%s: null lse descriptor", w);
+  AttentionBackwardProblem p;
+  int32_t rc = attn_common(q, k, v, q_offsets, k_offsets, lse, scale, causal, dt, w, p.f);
+  if (rc || (rc = same_shape(out, q, w, "out")) || (rc = same_shape(grad_out, q, w, "grad_out")) ||
+      (rc = same_shape(dq, q, w, "dq")) || (rc = same_shape(dk, k, w, "dk")) ||
+      (rc = same_shape(dv, k, w, "dv")) || (rc = attn_operand(out, w, "out", false, p.f.o)) ||
+      (rc = attn_operand(grad_out, w, "grad_out", false, p.go)) ||
+      (rc = attn_operand(dq, w, "dq", true, p.dq)) || (rc = attn_operand(dk, w, "dk", true, p.dk)) ||
+      (rc = attn_operand(dv, w, "dv", true, p.dv)))
+    return rc;
+  if (!scratch) return fail(NOVA_HIP_EINVAL, "%s: null scratch descriptor", w);
+  if ((rc = dense1(scratch, w, "scratch"))) return rc;
+  if (scratch->sizes[0] < 2 * p.f.heads * p.f.Tq)
+    return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, 2 heads tokens = %lld are needed", w,
+                (long long)scratch->sizes[0], (long long)(2 * p.f.heads * p.f.Tq));
+  p.rows = out_f32(scratch);
+  return launch_attention_backward(p, current_stream());
+}
+
+int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int64_t heads,
+                                          int64_t kv_heads, int64_t D) {
+  if (sequences <= 0 || cache <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0) return 0;
+  if (sequences > 0xffff || cache > 0x7fffffff || heads > 0xffff || kv_heads > heads || D > 128)
+    return 0;  // the call itself refuses these
+  const int64_t chunk = attention_decode_chunk(sequences, cache, kv_heads);
+  const int64_t splits = (cache + chunk - 1) / chunk;
+  return splits <= 1 ? 0 : sequences * heads * splits * (D + 2);
+}
+
+int32_t _mlir_ciface_nova_hip_attention_decode(const NovaMemRef3D *q, const NovaMemRef4D *k,
+                                               const NovaMemRef4D *v, const NovaMemRef1D *lengths,
+                                               NovaMemRef3D *out, NovaMemRef2D *lse,
+                                               NovaMemRef1D *scratch, float scale, int32_t dt) {
+  clear_error();
+  const char *w = "attention_decode";
+  if (!q || !k || !v || !lengths || !out) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if (dt != NOVA_HIP_DT_BF16 && dt != NOVA_HIP_DT_F16)
+    return fail(NOVA_HIP_EDTYPE, "%s: dtype %d (bf16 and f16 are provided)", w, dt);
+  if (!(scale > 0.0f) || !(scale < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: scale must be positive and finite", w);
+  if (!nonneg_sizes(q, 3) || !nonneg_sizes(k, 4) || !nonneg_sizes(v, 4) || !nonneg_sizes(out, 3) ||
+      !nonneg_sizes(lengths, 1))
+    return fail(NOVA_HIP_ESHAPE, "%s: negative size", w);
+  AttentionDecodeProblem p;
+  p.B = q->sizes[0];
+  p.heads = q->sizes[1];
+  p.D = q->sizes[2];
+  p.S = k->sizes[1];
+  p.kv_heads = k->sizes[2];
+  for (int i = 0; i < 4; ++i)
+    if (k->sizes[i] != v->sizes[i]) return fail(NOVA_HIP_ESHAPE, "%s: shapes of k and v differ", w);
+  if (k->sizes[0] != p.B || k->sizes[3] != p.D || lengths->sizes[0] != p.B)
+    return fail(NOVA_HIP_ESHAPE, "%s: q [%lld,%lld,%lld], k [%lld,%lld,%lld,%lld], lengths [%lld]", w,
+                (long long)p.B, (long long)p.heads, (long long)p.D, (long long)k->sizes[0],
+                (long long)p.S, (long long)p.kv_heads, (long long)k->sizes[3],
+                (long long)lengths->sizes[0]);
+  int32_t rc = same_shape(out, q, w, "out");
+  if (rc) return rc;
+  if (p.heads > 0 && (p.kv_heads == 0 || p.heads % p.kv_heads))
+    return fail(NOVA_HIP_ESHAPE, "%s: %lld query heads do not share %lld key heads evenly", w,
+                (long long)p.heads, (long long)p.kv_heads);
+  if (p.D % 8 || p.D > 128)
+    return fail(NOVA_HIP_ERANGE, "%s: head dim %lld is not a multiple of 8 up to 128", w,
+                (long long)p.D);
+  if (p.B > 0xffff || p.heads > 0xffff || p.S > 0x7fffffff - (1 << 20))
+    return fail(NOVA_HIP_ERANGE, "%s: more than 65535 sequences or heads, or 2^31 - 2^20 rows", w);
+  if (!dense_i32(lengths)) return fail(NOVA_HIP_ESTRIDE, "%s: lengths must be dense", w);
+  if (lse && (lse->sizes[0] != p.B || lse->sizes[1] != p.heads))
+    return fail(NOVA_HIP_ESHAPE, "%s: lse must be [sequences, heads]", w);
+  if (p.B == 0 || p.heads == 0 || p.D == 0) return NOVA_HIP_SUCCESS;
+  if (!q->aligned || !out->aligned || !lengths->aligned || (lse && !lse->aligned) ||
+      (p.S > 0 && (!k->aligned || !v->aligned)))
+    return fail(NOVA_HIP_EINVAL, "%s: null data pointer", w);
+  // A dim of extent 1 may have any stride (see attn_operand).
+  auto stride = [&](int64_t size, int64_t s) { return size > 1 ? s : p.D; };
+  p.sqb = stride(p.B, q->strides[0]);
+  p.sqh = stride(p.heads, q->strides[1]);
+  p.sob = stride(p.B, out->strides[0]);
+  p.soh = stride(p.heads, out->strides[1]);
+  p.skb = stride(p.B, k->strides[0]);
+  p.skt = stride(p.S, k->strides[1]);
+  p.skh = stride(p.kv_heads, k->strides[2]);
+  p.svb = stride(p.B, v->strides[0]);
+  p.svt = stride(p.S, v->strides[1]);
+  p.svh = stride(p.kv_heads, v->strides[2]);
+  p.q = data_of(q) + q->offset * 2;
+  p.k = data_of(k) + k->offset * 2;
+  p.v = data_of(v) + v->offset * 2;
+  p.o = const_cast<char *>(data_of(out)) + out->offset * 2;
+  if (p.D > 1 && (q->strides[2] != 1 || out->strides[2] != 1 ||
+                  (p.S > 0 && (k->strides[3] != 1 || v->strides[3] != 1))))
+    return fail(NOVA_HIP_ESTRIDE, "%s: operands must have unit stride on the head dim", w);
+  if (p.S == 0) {  // no rows to address
+    p.k = p.v = nullptr;
+    p.skb = p.skt = p.skh = p.svb = p.svt = p.svh = p.D;
+  }
+  if (p.sqb < 0 || p.skb < 0 || p.svb < 0 || p.skh < 0 || p.svh < 0 ||
+      (p.heads > 1 && (p.sqh < p.D || p.soh < p.D)) ||
+      (p.S > 1 && (p.skt < p.D || p.svt < p.D)))
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows overlap", w);
+  if (p.B > 1 && p.sob < p.D) return fail(NOVA_HIP_ESTRIDE, "%s: rows of out overlap", w);
+  if (p.B > 1 && p.heads > 1 &&
+      (p.soh <= p.sob ? p.sob < (p.heads - 1) * p.soh + p.D : p.soh < (p.B - 1) * p.sob + p.D))
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows of out overlap", w);
+  const int64_t any = p.sqb | p.sqh | p.sob | p.soh | p.skb | p.skt | p.skh | p.svb | p.svt | p.svh;
+  if (any % 8 || ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) |
+                   reinterpret_cast<uintptr_t>(p.v) | reinterpret_cast<uintptr_t>(p.o)) & 15u))
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows must start at 16-byte aligned addresses", w);
+  if (p.sqh > kAttnMaxStride || p.skt > kAttnMaxStride || p.svt > kAttnMaxStride)
+    return fail(NOVA_HIP_ERANGE, "%s: a row stride exceeds 2^24 elements", w);
+  p.lens = reinterpret_cast<const int32_t *>(data_of(lengths)) + lengths->offset;
+  p.lse = nullptr;
+  p.slse = 0;
+  if (lse) {
+    if ((p.heads > 1 && lse->strides[1] != 1) || (p.B > 1 && lse->strides[0] < p.heads))
+      return fail(NOVA_HIP_ESTRIDE, "%s: lse rows must be dense and not overlap", w);
+    p.lse = out_f32(lse);
+    p.slse = lse->strides[0];
+  }
+  p.partial = nullptr;
+  const int64_t need =
+      nova_hip_attention_decode_scratch(p.B, p.S, p.heads, p.kv_heads, p.D);
+  if (need > 0) {
+    if (!scratch) return fail(NOVA_HIP_EINVAL, "%s: null scratch descriptor", w);
+    if ((rc = dense1(scratch, w, "scratch"))) return rc;
+    if (scratch->sizes[0] < need)
+      return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, %lld are needed", w,
+                  (long long)scratch->sizes[0], (long long)need);
+    p.partial = out_f32(scratch);
+    if (reinterpret_cast<uintptr_t>(p.partial) & 7u)
+      return fail(NOVA_HIP_ESTRIDE, "%s: scratch must be 8-byte aligned", w);
+  }
+  p.scale = scale;
+  p.dt = dt;
+  return launch_attention_decode(p, current_stream());
+}
+
+// ---- losses over token log-probabilities ---------------------------------------------
+namespace {
+// logits [R, C], labels [R] and the optional gradient, shared by the three losses.
+int32_t token_common(const NovaMemRef2D *logits, const NovaMemRef1D *labels, NovaMemRef2D *grad,
+                     int32_t dt, const char *w, TokenLossProblem &p) {
+  if (!logits || !labels) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if (dt != NOVA_HIP_DT_F32 && dt != NOVA_HIP_DT_BF16 && dt != NOVA_HIP_DT_F16)
+    return fail(NOVA_HIP_EDTYPE, "%s: dtype %d (f32, bf16 and f16 are provided)", w, dt);
+  p.rows = logits->sizes[0];
+  p.C = logits->sizes[1];
+  if (p.rows < 0 || p.C < 0) return fail(NOVA_HIP_ESHAPE, "%s: negative size", w);
+  if (p.C == 0) return fail(NOVA_HIP_ESHAPE, "%s: zero classes", w);
+  if (labels->sizes[0] != p.rows) return fail(NOVA_HIP_ESHAPE, "%s: labels size != rows", w);
+  if (grad && (grad->sizes[0] != p.rows || grad->sizes[1] != p.C))
+    return fail(NOVA_HIP_ESHAPE, "%s: grad shape differs from logits", w);
+  if ((p.C > 1 && (logits->strides[1] != 1 || (grad && grad->strides[1] != 1))) ||
+      (p.rows > 1 && labels->strides[0] != 1))
+    return fail(NOVA_HIP_ESTRIDE, "%s: last dim must be contiguous", w);
+  if (p.rows > 1 && (logits->strides[0] < p.C || (grad && grad->strides[0] < p.C)))
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows overlap", w);
+  if (p.rows > 0 && (!logits->aligned || !labels->aligned || (grad && !grad->aligned)))
+    return fail(NOVA_HIP_EINVAL, "%s: null data pointer", w);
+  const int sz = dtype_size(dt);
+  p.logits = data_of(logits) + logits->offset * sz;
+  p.grad = grad ? const_cast<char *>(data_of(grad)) + grad->offset * sz : nullptr;
+  p.labels = reinterpret_cast<const int32_t *>(data_of(labels)) + labels->offset;
+  p.sx = logits->strides[0];
+  p.sg = grad ? grad->strides[0] : 0;
+  p.dt = dt;
+  return NOVA_HIP_SUCCESS;
+}
+
+// A dense f32 vector of n values.
+int32_t vector_f32(const NovaMemRef1D *d, int64_t n, const char *w, const char *what) {
+  int32_t rc = dense1(d, w, what);
+  if (rc) return rc;
+  if (d->sizes[0] != n)
+    return fail(NOVA_HIP_ESHAPE, "%s: %s has %lld values, not %lld", w, what,
+                (long long)d->sizes[0], (long long)n);
+  return NOVA_HIP_SUCCESS;
+}
+}  // namespace
+
+int32_t _mlir_ciface_nova_hip_token_logp(const NovaMemRef2D *logits, const NovaMemRef1D *labels,
+                                         NovaMemRef1D *logp, NovaMemRef1D *lse, int32_t dt) {
+  clear_error();
+  const char *w = "token_logp";
+  TokenLossProblem p;
+  int32_t rc = token_common(logits, labels, nullptr, dt, w, p);
+  if (rc || (rc = vector_f32(logp, p.rows, w, "logp")) ||
+      (lse && (rc = vector_f32(lse, p.rows, w, "lse"))))
+    return rc;
+  return launch_token_logp(p, out_f32(logp), lse ? out_f32(lse) : nullptr, current_stream());
+}
+
+int32_t _mlir_ciface_nova_hip_policy_loss(
+    const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *old_logp,
+    const NovaMemRef1D *ref_logp, const NovaMemRef1D *advantage, const NovaMemRef1D *weight,
+    NovaMemRef1D *loss, NovaMemRef1D *logp, NovaMemRef1D *row_loss, NovaMemRef2D *grad,
+    float clip_low, float clip_high, float kl_coef, float grad_scale, int32_t dt) {
+  clear_error();
+  const char *w = "policy_loss";
+  PolicyProblem p;
+  int32_t rc = token_common(logits, labels, grad, dt, w, p.t);
+  const int64_t R = p.t.rows;
+  if (rc || (rc = vector_f32(old_logp, R, w, "old_logp")) ||
+      (ref_logp && (rc = vector_f32(ref_logp, R, w, "ref_logp"))) ||
+      (rc = vector_f32(advantage, R, w, "advantage")) || (rc = vector_f32(weight, R, w, "weight")) ||
+      (rc = vector_f32(loss, 1, w, "loss")) || (rc = vector_f32(logp, R, w, "logp")) ||
+      (rc = vector_f32(row_loss, R, w, "row_loss")))
+    return rc;
+  if (!(clip_low >= 0.0f && clip_low <= 1.0f) || !(clip_high >= 0.0f && clip_high < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: clip_low must be in [0, 1], clip_high finite and >= 0", w);
+  if (!std::isfinite(kl_coef) || !std::isfinite(grad_scale))
+    return fail(NOVA_HIP_EINVAL, "%s: kl_coef and grad_scale must be finite", w);
+  if (!ref_logp && kl_coef != 0.0f)
+    return fail(NOVA_HIP_EINVAL, "%s: the KL term needs ref_logp", w);
+  p.old_logp = in_f32(old_logp);
+  p.ref_logp = ref_logp && kl_coef != 0.0f ? in_f32(ref_logp) : nullptr;
+  p.advantage = in_f32(advantage);
+  p.weight = in_f32(weight);
+  p.loss = out_f32(loss);
+  p.logp = out_f32(logp);
+  p.row_loss = out_f32(row_loss);
+  p.clip_low = clip_low;
+  p.clip_high = clip_high;
+  p.kl_coef = kl_coef;
+  p.grad_scale = grad_scale;
+  return launch_policy_loss(p, current_stream());
+}
+
+int32_t _mlir_ciface_nova_hip_preference_loss(
+    const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *offsets,
+    const NovaMemRef1D *ref_logp, NovaMemRef1D *loss, NovaMemRef1D *seq_logp,
+    NovaMemRef1D *pair_loss, NovaMemRef2D *token, NovaMemRef2D *grad, float beta, float smoothing,
+    float grad_scale, int32_t dt) {
+  clear_error();
+  const char *w = "preference_loss";
+  PreferenceProblem p;
+  int32_t rc = token_common(logits, labels, grad, dt, w, p.t);
+  if (rc) return rc;
+  if (!offsets || !token) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  const int64_t n = offsets->sizes[0] - 1;  // sequences
+  if (n < 2 || n % 2)
+    return fail(NOVA_HIP_ESHAPE, "%s: offsets must be [2 pairs + 1], at least one pair", w);
+  p.pairs = n / 2;
+  if (p.pairs > (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 pairs", w);
+  if (!dense_i32(offsets)) return fail(NOVA_HIP_ESTRIDE, "%s: offsets must be dense", w);
+  if (!offsets->aligned) return fail(NOVA_HIP_EINVAL, "%s: null offsets pointer", w);
+  if ((rc = vector_f32(ref_logp, n, w, "ref_logp")) || (rc = vector_f32(loss, 1, w, "loss")) ||
+      (rc = vector_f32(seq_logp, n, w, "seq_logp")) ||
+      (rc = vector_f32(pair_loss, p.pairs, w, "pair_loss")))
+    return rc;
+  const int64_t R = p.t.rows;
+  if (token->sizes[0] != 3 || token->sizes[1] != R)
+    return fail(NOVA_HIP_ESHAPE, "%s: token must be [3, rows]", w);
+  if ((R > 1 && token->strides[1] != 1) || token->strides[0] < R)
+    return fail(NOVA_HIP_ESTRIDE, "%s: token rows must be dense and not overlap", w);
+  if (R > 0 && !token->aligned) return fail(NOVA_HIP_EINVAL, "%s: null token pointer", w);
+  if (!(beta > 0.0f && beta < INFINITY) || !(smoothing >= 0.0f && smoothing <= 1.0f) ||
+      !std::isfinite(grad_scale))
+    return fail(NOVA_HIP_EINVAL,
+                "%s: beta must be positive, smoothing in [0, 1], grad_scale finite", w);
+  p.offsets = reinterpret_cast<const int32_t *>(data_of(offsets)) + offsets->offset;
+  p.ref_logp = in_f32(ref_logp);
+  p.loss = out_f32(loss);
+  p.seq_logp = out_f32(seq_logp);
+  p.pair_loss = out_f32(pair_loss);
+  p.logp = out_f32(token);
+  p.lse = p.logp + token->strides[0];
+  p.slope = p.lse + token->strides[0];
+  p.beta = beta;
+  p.smoothing = smoothing;
+  p.grad_scale = grad_scale;
+  return launch_preference_loss(p, current_stream());
 }
 
 void nova_hip_set_stream(void *stream) { t_stream = static_cast<hipStream_t>(stream); }

@@ -140,6 +140,59 @@ struct AttentionProblem {
 };
 int32_t launch_attention(const AttentionProblem &p, hipStream_t s);
 
+struct AttentionBackwardProblem {
+  AttentionProblem f;  // the forward's operands, result and lse
+  AttentionOperand go, dq, dk, dv;
+  float *rows;  // scratch, [2][heads][Tq]
+};
+int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t s);
+
+struct AttentionDecodeProblem {
+  const void *q, *k, *v;
+  void *o;
+  float *lse;      // [B, heads], row stride slse; may be null
+  float *partial;  // scratch of attention_decode_scratch() floats
+  const int32_t *lens;
+  int64_t B, S, heads, kv_heads, D;
+  int64_t sqb, sqh, sob, soh, slse;            // strides (elements)
+  int64_t skb, skt, skh, svb, svt, svh;
+  float scale;
+  int dt;
+};
+// Keys of one split of a cache of S rows.
+int64_t attention_decode_chunk(int64_t B, int64_t S, int64_t kv_heads);
+int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s);
+
+// ---- losses over token log-probabilities (losses.hip) --------------------------
+struct TokenLossProblem {
+  const void *logits;
+  void *grad;  // may be null
+  const int32_t *labels;
+  int64_t rows, C;
+  int64_t sx, sg;  // row strides (elements)
+  int dt;
+};
+int32_t launch_token_logp(const TokenLossProblem &p, float *logp, float *lse, hipStream_t s);
+
+struct PolicyProblem {
+  TokenLossProblem t;
+  const float *old_logp, *ref_logp, *advantage, *weight;  // ref_logp may be null
+  float *loss, *logp, *row_loss;
+  float clip_low, clip_high, kl_coef, grad_scale;
+};
+int32_t launch_policy_loss(const PolicyProblem &p, hipStream_t s);
+
+struct PreferenceProblem {
+  TokenLossProblem t;
+  const int32_t *offsets;  // [2 pairs + 1]
+  const float *ref_logp;   // [2 pairs]
+  int64_t pairs;
+  float *loss, *seq_logp, *pair_loss;
+  float *logp, *lse, *slope;  // [rows] each
+  float beta, smoothing, grad_scale;
+};
+int32_t launch_preference_loss(const PreferenceProblem &p, hipStream_t s);
+
 // ---- program glue (glue.hip) -------------------------------------------------
 // c = a (op) b over a [4]-shaped index space; strides in elements, 0 on a
 // broadcast dimension.

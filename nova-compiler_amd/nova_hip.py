@@ -65,6 +65,12 @@ EXPORTS = (
     "_mlir_ciface_nova_hip_reduce_sum_f32",
     "_mlir_ciface_nova_hip_index_to_i32",
     "_mlir_ciface_nova_hip_attention",
+    "_mlir_ciface_nova_hip_attention_backward",
+    "_mlir_ciface_nova_hip_attention_decode",
+    "nova_hip_attention_decode_scratch",
+    "_mlir_ciface_nova_hip_token_logp",
+    "_mlir_ciface_nova_hip_policy_loss",
+    "_mlir_ciface_nova_hip_preference_loss",
     "nova_hip_set_stream",
     "nova_hip_get_stream",
     "nova_hip_synchronize",
@@ -161,7 +167,14 @@ def lib() -> ctypes.CDLL:
     L._mlir_ciface_nova_hip_reduce_sum_f32.argtypes = [P, P]
     L._mlir_ciface_nova_hip_index_to_i32.argtypes = [P, P, ctypes.c_int32]
     F, I = ctypes.c_float, ctypes.c_int32
-    L._mlir_ciface_nova_hip_attention.argtypes = [P, P, P, P, P, P, P, F, I, I]
+    L._mlir_ciface_nova_hip_attention.argtypes = [P] * 7 + [F, I, I]
+    L._mlir_ciface_nova_hip_attention_backward.argtypes = [P] * 12 + [F, I, I]
+    L._mlir_ciface_nova_hip_attention_decode.argtypes = [P] * 7 + [F, I]
+    L.nova_hip_attention_decode_scratch.argtypes = [ctypes.c_int64] * 5
+    L.nova_hip_attention_decode_scratch.restype = ctypes.c_int64
+    L._mlir_ciface_nova_hip_token_logp.argtypes = [P] * 4 + [I]
+    L._mlir_ciface_nova_hip_policy_loss.argtypes = [P] * 10 + [F] * 4 + [I]
+    L._mlir_ciface_nova_hip_preference_loss.argtypes = [P] * 9 + [F] * 3 + [I]
     for name in EXPORTS:
         if name.startswith("_mlir_ciface_"):
             getattr(L, name).restype = ctypes.c_int32
@@ -606,3 +619,130 @@ def attention(q, k, v, q_offsets, k_offsets, *, causal: bool = True, scale=None,
              for t in (q, k, v, q_offsets, k_offsets, out, lse)]
         check(lib()._mlir_ciface_nova_hip_attention(*[ref(x) for x in d], scale, int(causal), _dt(q)))
     return out, lse
+
+
+def attention_backward(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, causal: bool = True,
+                       scale=None, dq=None, dk=None, dv=None):
+    """Gradients of ``attention``'s result, from its ``out`` and ``lse``:
+    returns (dq, dk, dv) in the operands' dtype."""
+    torch = _torch()
+    _want_dtype(q.dtype, grad_out=grad_out, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
+    _want_dtype(torch.int32, q_offsets=q_offsets, k_offsets=k_offsets)
+    _want_dtype(torch.float32, lse=lse)
+    with _on_device(q, grad_out, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv):
+        if dq is None:
+            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if dk is None:
+            dk = torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        if dv is None:
+            dv = torch.empty(k.shape, dtype=k.dtype, device=q.device)
+        scratch = torch.empty(2 * q.shape[0] * q.shape[1], dtype=torch.float32, device=q.device)
+        if scale is None:
+            scale = q.shape[2] ** -0.5
+        d = [memref_of(t) for t in (grad_out, q, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv,
+                                    scratch)]
+        check(lib()._mlir_ciface_nova_hip_attention_backward(*[ref(x) for x in d], scale,
+                                                             int(causal), _dt(q)))
+    return dq, dk, dv
+
+
+def attention_decode(q, k, v, lengths, *, scale=None, out=None, lse=None):
+    """Attention of one query per sequence over a padded cache: q [sequences,
+    heads, D], k and v [sequences, cache rows, key heads, D] (any order of the
+    first three dims in memory), lengths [sequences] i32.  Returns out;
+    ``lse`` [sequences, heads] f32 is written when given."""
+    torch = _torch()
+    _want_dtype(q.dtype, k=k, v=v, out=out)
+    _want_dtype(torch.int32, lengths=lengths)
+    _want_dtype(torch.float32, lse=lse)
+    with _on_device(q, k, v, lengths, out, lse):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if scale is None:
+            scale = q.shape[2] ** -0.5
+        need = lib().nova_hip_attention_decode_scratch(q.shape[0], k.shape[1], q.shape[1], k.shape[2],
+                                                       q.shape[2])
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+        d = [memref_of(t) if t is not None else None for t in (q, k, v, lengths, out, lse, scratch)]
+        check(lib()._mlir_ciface_nova_hip_attention_decode(*[ref(x) for x in d], scale, _dt(q)))
+    return out
+
+
+# --------------------------------------------------------------------------
+# losses over token log-probabilities
+# --------------------------------------------------------------------------
+
+def token_logp(logits, labels, *, logp=None, lse=None):
+    """The log-probability of each row's label [rows] f32 (0 where the label is
+    negative); ``lse`` [rows] f32 is written when given."""
+    torch = _torch()
+    _want_dtype(torch.int32, labels=labels)
+    _want_dtype(torch.float32, logp=logp, lse=lse)
+    with _on_device(logits, labels, logp, lse):
+        if logp is None:
+            logp = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        d = [memref_of(t) if t is not None else None for t in (logits, labels, logp, lse)]
+        check(lib()._mlir_ciface_nova_hip_token_logp(*[ref(x) for x in d], _dt(logits)))
+    return logp
+
+
+def policy_loss(logits, labels, old_logp, advantage, weight, *, ref_logp=None, clip=(0.2, 0.2),
+                kl_coef: float = 0.0, grad_scale: float = 1.0, loss=None, logp=None, grad=None,
+                row_loss=None, want_grad: bool = True):
+    """The clipped policy loss over tokens, weighted by ``weight``, with a KL
+    term to ``ref_logp``: returns (loss[1], logp [rows], grad), grad None
+    with ``want_grad`` False.  ``clip`` is (low, high): the ratio is clamped to
+    [1 - low, 1 + high].  Rows with a negative label or weight 0 take no part."""
+    torch = _torch()
+    _want_dtype(torch.int32, labels=labels)
+    _want_dtype(torch.float32, old_logp=old_logp, advantage=advantage, weight=weight,
+                ref_logp=ref_logp, loss=loss, logp=logp, row_loss=row_loss)
+    _want_dtype(logits.dtype, grad=grad)
+    with _on_device(logits, labels, old_logp, advantage, weight, ref_logp, loss, logp, row_loss, grad):
+        rows, dev = logits.shape[0], logits.device
+        if loss is None:
+            loss = torch.empty(1, dtype=torch.float32, device=dev)
+        if logp is None:
+            logp = torch.empty(rows, dtype=torch.float32, device=dev)
+        if row_loss is None:
+            row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
+        if grad is None and want_grad:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        d = [memref_of(t) if t is not None else None
+             for t in (logits, labels, old_logp, ref_logp, advantage, weight, loss, logp, row_loss,
+                       grad)]
+        check(lib()._mlir_ciface_nova_hip_policy_loss(*[ref(x) for x in d], clip[0], clip[1], kl_coef,
+                                                      grad_scale, _dt(logits)))
+    return loss, logp, grad
+
+
+def preference_loss(logits, labels, offsets, ref_logp, *, beta: float = 0.1, smoothing: float = 0.0,
+                    grad_scale: float = 1.0, loss=None, seq_logp=None, pair_loss=None, token=None,
+                    grad=None, want_grad: bool = True):
+    """The paired preference loss over packed sequences, pair p being sequences
+    2p (chosen) and 2p + 1 (rejected) of ``offsets`` [2 pairs + 1] i32:
+    returns (loss[1], seq_logp [2 pairs], grad), grad None with ``want_grad``
+    False.  ``pair_loss`` [pairs] and ``token`` [3, rows] (logp, lse, slope) are
+    written when given."""
+    torch = _torch()
+    _want_dtype(torch.int32, labels=labels, offsets=offsets)
+    _want_dtype(torch.float32, ref_logp=ref_logp, loss=loss, seq_logp=seq_logp,
+                pair_loss=pair_loss, token=token)
+    _want_dtype(logits.dtype, grad=grad)
+    with _on_device(logits, labels, offsets, ref_logp, loss, seq_logp, pair_loss, token, grad):
+        rows, seqs, dev = logits.shape[0], max(offsets.numel() - 1, 0), logits.device
+        if loss is None:
+            loss = torch.empty(1, dtype=torch.float32, device=dev)
+        if seq_logp is None:
+            seq_logp = torch.empty(seqs, dtype=torch.float32, device=dev)
+        if pair_loss is None:
+            pair_loss = torch.empty(seqs // 2, dtype=torch.float32, device=dev)
+        if token is None:
+            token = torch.empty((3, rows), dtype=torch.float32, device=dev)
+        if grad is None and want_grad:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        d = [memref_of(t) if t is not None else None
+             for t in (logits, labels, offsets, ref_logp, loss, seq_logp, pair_loss, token, grad)]
+        check(lib()._mlir_ciface_nova_hip_preference_loss(*[ref(x) for x in d], beta, smoothing,
+                                                          grad_scale, _dt(logits)))
+    return loss, seq_logp, grad

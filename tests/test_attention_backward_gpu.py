@@ -1,0 +1,154 @@
+"""attention_backward on the GPU against its formula in 64 bits, and against
+differences of the forward.
+
+Tolerances, u = finfo(dtype).eps / 2.  P and dS round once to dtype for the
+products and each gradient once at the end: u times the sums of absolute
+products, and u |result|.  f32 scores and dP are sums of exact products; scores
+below 64 and D <= 128 keep P within 4e-5 of itself, dP and delta within 1e-5 of
+their absolute sums.  In f16 a dS under 2^-14 rounds by 2^-25 at most."""
+import math
+
+import pytest
+import torch
+
+import nova_hip as nh
+from test_attention_gpu import BF, F64, HF, make, offsets
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(go, q, k, v, o, lse, qlens, klens, causal, scale):
+    """(dq, dk, dv) and, for each, the bound of its error without u |result|."""
+    H, G, dev = q.shape[1], k.shape[1], q.device
+    u = torch.finfo(q.dtype).eps / 2
+    tiny = 2.0 ** -25 if q.dtype == HF else 0.0
+    res = [torch.zeros(t.shape, dtype=F64, device=dev) for t in (q, k, k)]
+    tol = [torch.zeros_like(r) for r in res]
+    a = c = 0
+    for n, m in zip(qlens, klens):
+        keep = torch.ones(n, m, dtype=torch.bool, device=dev)
+        if causal:
+            keep = keep.tril(m - n)
+        for h in range(H if n and m else 0):
+            g = h * G // H
+            Q, GO, O = (t[a:a + n, h].double() for t in (q, go, o))
+            K, V = k[c:c + m, g].double(), v[c:c + m, g].double()
+            s = torch.mm(Q, K.t().contiguous()) * scale
+            p = torch.where(keep, torch.exp(s - lse[h, a:a + n].double()[:, None]), torch.zeros_like(s))
+            dp = torch.mm(GO, V.t().contiguous())
+            ds = p * (dp - (GO * O).sum(1)[:, None])
+            slack = p * (torch.mm(GO.abs(), V.t().abs().contiguous()) + (GO * O).abs().sum(1)[:, None])
+            ds_err = (u * 1.01 + 4e-5) * ds.abs() + 1e-5 * slack + tiny * keep
+            p_err = (u * 1.01 + 4e-5) * p + (tiny / 256) * keep
+            sl, kl = slice(a, a + n), slice(c, c + m)
+            res[0][sl, h] = torch.mm(ds, K) * scale
+            tol[0][sl, h] = torch.mm(ds_err, K.abs()) * scale
+            res[1][kl, g] += torch.mm(ds.t().contiguous(), Q) * scale
+            tol[1][kl, g] += torch.mm(ds_err.t().contiguous(), Q.abs()) * scale
+            res[2][kl, g] += torch.mm(p.t().contiguous(), GO)
+            tol[2][kl, g] += torch.mm(p_err.t().contiguous(), GO.abs())
+        a, c = a + n, c + m
+    return res, tol
+
+
+def run(dev, qlens, klens, H, G, D, dt, causal, layout="thd", seed=0, pad=0):
+    q, k, v = make(dev, qlens, klens, H, G, D, dt, seed, layout, pad)
+    g = torch.Generator(device=dev).manual_seed(seed + 1)
+    go = torch.randn(q.shape, generator=g, device=dev).to(dt)
+    Tq, Tk = sum(qlens), sum(klens)
+    go[Tq:] = float("nan")
+    if layout == "htd":
+        go = go.transpose(0, 1).contiguous().transpose(0, 1)
+    scale = D ** -0.5
+    qo, ko = offsets(qlens, dev), offsets(klens, dev)
+    o, lse = nh.attention(q, k, v, qo, ko, causal=causal)
+    grads = [torch.full(t.shape, 7.0, dtype=dt, device=dev) for t in (q, k, v)]
+    nh.attention_backward(go, q, k, v, o, lse, qo, ko, causal=causal, dq=grads[0], dk=grads[1],
+                          dv=grads[2])
+    want, tol = reference(go, q, k, v, o, lse, qlens, klens, causal, scale)
+    u = torch.finfo(dt).eps / 2
+    for name, got, w, t, T in zip(("dq", "dk", "dv"), grads, want, tol, (Tq, Tk, Tk)):
+        assert (got[T:] == 7.0).all(), name  # rows behind the last sequence
+        err = (got.double() - w).abs()[:T]
+        assert not torch.isnan(err).any(), name
+        bound = t[:T] * 1.01 + u * w[:T].abs() * 1.01 + 2.0 ** -25 * (dt == HF) + 1e-30
+        worst = (err - bound).max().item() if err.numel() else 0.0
+        assert worst <= 0, (name, worst, err.max().item(), qlens, klens, H, G, D, dt, causal, layout)
+    return q, k, v, go, grads
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 80, 96, 128])
+def test_head_dims(cuda, dt, causal, D):
+    run(cuda, [197, 33], [197, 33], 4, 2, D, dt, causal)
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 33, 63, 64, 65, 127, 129, 257, 600])
+@pytest.mark.parametrize("causal", [False, True])
+def test_lengths(cuda, n, causal):
+    run(cuda, [n], [n], 2, 1, 64, BF, causal)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("qlens,klens", [
+    ([5, 0, 130, 1], [77, 3, 130, 200]),
+    ([40, 3, 0], [0, 70, 0]),
+    ([200, 64], [70, 1]),
+    ([1] * 70 + [65] + [0] * 70 + [2], [64] * 70 + [65] + [0] * 70 + [1]),
+])
+def test_uneven_and_empty_sequences(cuda, qlens, klens, D):
+    for causal in (False, True):
+        run(cuda, qlens, klens, 4, 2, D, BF, causal, pad=3)
+
+
+@pytest.mark.parametrize("layout", ["thd", "htd", "fused"])
+@pytest.mark.parametrize("H,G", [(1, 1), (8, 1), (9, 3), (32, 8)])
+def test_layouts_and_shared_heads(cuda, layout, H, G):
+    run(cuda, [150, 70, 3], [150, 70, 3], H, G, 64, HF, True, layout, pad=5 if layout != "fused" else 0)
+
+
+def test_long_sequence(cuda):
+    run(cuda, [2500], [4001], 2, 1, 128, BF, True)
+    run(cuda, [4001], [4001], 1, 1, 64, HF, False)
+
+
+def test_same_bits_on_every_run(cuda):
+    first = run(cuda, [300, 200], [300, 200], 8, 2, 128, BF, True)[4]
+    for _ in range(3):
+        again = run(cuda, [300, 200], [300, 200], 8, 2, 128, BF, True)[4]
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_against_differences_of_the_forward(cuda):
+    """d loss / d x along a random direction by central differences of the
+    64-bit forward, loss = sum(out * grad_out).  The step's error is of order
+    h^2; the gradients' own roundings, independent from element to element, give
+    u |x'| |direction| each, within six standard deviations."""
+    lens, H, G, D = [50, 21], 4, 2, 64
+    q, k, v, go, grads = run(cuda, lens, lens, H, G, D, BF, True)
+
+    def loss(q, k, v):
+        total, a = 0.0, 0
+        for n in lens:
+            keep = torch.ones(n, n, dtype=torch.bool, device=cuda).tril()
+            for h in range(H):
+                s = torch.mm(q[a:a + n, h], k[a:a + n, h * G // H].t().contiguous()) * D ** -0.5
+                p = torch.softmax(s.masked_fill(~keep, -math.inf), 1)
+                total = total + (torch.mm(p, v[a:a + n, h * G // H]) * go[a:a + n, h].double()).sum()
+            a += n
+        return total
+
+    x = [t.double() for t in (q, k, v)]
+    gen = torch.Generator(device=cuda).manual_seed(9)
+    for i in range(3):
+        d = torch.randn(x[i].shape, generator=gen, device=cuda, dtype=F64)
+        step = 1e-4
+        hi, lo = list(x), list(x)
+        hi[i], lo[i] = x[i] + step * d, x[i] - step * d
+        numeric = ((loss(*hi) - loss(*lo)) / (2 * step)).item()
+        ours = (grads[i].double() * d).sum().item()
+        u = 2.0 ** -8
+        # Rounded weights and dS: their sums err by at most the same again.
+        noise = 6 * 2 * u * ((grads[i].double() * d) ** 2).sum().sqrt().item() + 6 * u * d.norm().item()
+        assert abs(ours - numeric) <= noise + 1e-6 * abs(numeric), (i, ours, numeric, noise)
