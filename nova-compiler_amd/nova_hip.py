@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Tuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -560,41 +561,53 @@ def index_to_i32(idx, out=None):
 
 
 # --------------------------------------------------------------------------
-# attention of packed sequences
+# attention of packed sequences, losses over token log-probabilities
 # --------------------------------------------------------------------------
+# These calls are made once per layer and token, where their smallest take the
+# GPU less than 10 us, so the wrappers below spend little: a descriptor is one
+# packed struct, and the current stream is read without a Stream object.
 
-class _on_device:
-    """Makes the tensors' device the current one for a call, on its current
-    stream, and refuses tensors of different devices (descriptors carry none)."""
-
-    def __init__(self, *tensors):
-        dev = tensors[0].device
-        if dev.type != "cuda":
-            raise NovaHipError(1, f"tensors must be on the GPU, not on {dev}")
-        for t in tensors:
-            if t is not None and t.device != dev:
-                raise NovaHipError(1, f"tensors on {dev} and {t.device}")
-        self._ctx = None
-        torch = _torch()
-        if dev.index != torch.cuda.current_device():
-            self._ctx = torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
-        _bind_stream()
-
-    def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
-            _bind_stream()
-        return False
+_PACK = {r: struct.Struct("PPq" + "q" * (2 * r)) for r in (1, 2, 3, 4)}
 
 
-def _want_dtype(dtype, **tensors) -> None:
+def _desc(t, rank: int, name: str):
+    """Descriptor of a tensor of the given rank, as bytes (None passes NULL)."""
+    if t is None:
+        return None
+    shape = t.shape
+    if len(shape) != rank:
+        raise NovaHipError(2, f"{name} has {len(shape)} dims, not {rank}")
+    p = t.data_ptr()
+    return _PACK[rank].pack(p, p, 0, *shape, *t.stride())
+
+
+def _check_dtype(dtype, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.dtype != dtype:
+        if t is not None and t.dtype is not dtype:
             raise NovaHipError(4, f"{name} is {t.dtype}, not {dtype}")
+
+
+def _launch(entry: str, tensors, *args) -> None:
+    """Calls an entry point on the tensors' device and its current stream;
+    refuses tensors of different devices, which descriptors do not show."""
+    torch = _torch()
+    dev = tensors[0].get_device()
+    if dev < 0:
+        raise NovaHipError(1, "tensors must be on the GPU")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise NovaHipError(1, f"tensors on devices {dev} and {t.get_device()}")
+    L = lib()
+    if dev == torch.cuda.current_device():
+        L.nova_hip_set_stream(torch._C._cuda_getCurrentRawStream(dev))
+        rc = getattr(L, entry)(*args)
+    else:
+        with torch.cuda.device(dev):
+            L.nova_hip_set_stream(torch._C._cuda_getCurrentRawStream(dev))
+            rc = getattr(L, entry)(*args)
+        _bind_stream()
+    if rc:
+        check(rc)
 
 
 def attention(q, k, v, q_offsets, k_offsets, *, causal: bool = True, scale=None, out=None,
@@ -605,19 +618,22 @@ def attention(q, k, v, q_offsets, k_offsets, *, causal: bool = True, scale=None,
     1 / sqrt(D) by default.  Returns (out, lse [heads, tokens] f32), lse None
     with ``want_lse`` False; rows outside every sequence are not written."""
     torch = _torch()
-    _want_dtype(q.dtype, k=k, v=v, out=out)
-    _want_dtype(torch.int32, q_offsets=q_offsets, k_offsets=k_offsets)
-    _want_dtype(torch.float32, lse=lse)
-    with _on_device(q, k, v, q_offsets, k_offsets, out, lse):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if lse is None and want_lse:
-            lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-        if scale is None:
-            scale = q.shape[2] ** -0.5
-        d = [memref_of(t) if t is not None else None
-             for t in (q, k, v, q_offsets, k_offsets, out, lse)]
-        check(lib()._mlir_ciface_nova_hip_attention(*[ref(x) for x in d], scale, int(causal), _dt(q)))
+    f32, i32 = torch.float32, torch.int32
+    _check_dtype(q.dtype, k=k, v=v, out=out)
+    _check_dtype(i32, q_offsets=q_offsets, k_offsets=k_offsets)
+    dq = _desc(q, 3, "q")
+    T, H, D = q.shape
+    if out is None:
+        out = q.new_empty((T, H, D))
+    if lse is None:
+        if want_lse:
+            lse = q.new_empty((H, T), dtype=f32)
+    else:
+        _check_dtype(f32, lse=lse)
+    _launch("_mlir_ciface_nova_hip_attention", (q, k, v, q_offsets, k_offsets, out, lse), dq,
+            _desc(k, 3, "k"), _desc(v, 3, "v"), _desc(q_offsets, 1, "q_offsets"),
+            _desc(k_offsets, 1, "k_offsets"), _desc(out, 3, "out"), _desc(lse, 2, "lse"),
+            D ** -0.5 if scale is None else scale, 1 if causal else 0, _dt(q))
     return out, lse
 
 
@@ -626,23 +642,25 @@ def attention_backward(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, cau
     """Gradients of ``attention``'s result, from its ``out`` and ``lse``:
     returns (dq, dk, dv) in the operands' dtype."""
     torch = _torch()
-    _want_dtype(q.dtype, grad_out=grad_out, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
-    _want_dtype(torch.int32, q_offsets=q_offsets, k_offsets=k_offsets)
-    _want_dtype(torch.float32, lse=lse)
-    with _on_device(q, grad_out, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv):
-        if dq is None:
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if dk is None:
-            dk = torch.empty(k.shape, dtype=k.dtype, device=q.device)
-        if dv is None:
-            dv = torch.empty(k.shape, dtype=k.dtype, device=q.device)
-        scratch = torch.empty(2 * q.shape[0] * q.shape[1], dtype=torch.float32, device=q.device)
-        if scale is None:
-            scale = q.shape[2] ** -0.5
-        d = [memref_of(t) for t in (grad_out, q, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv,
-                                    scratch)]
-        check(lib()._mlir_ciface_nova_hip_attention_backward(*[ref(x) for x in d], scale,
-                                                             int(causal), _dt(q)))
+    f32, i32 = torch.float32, torch.int32
+    _check_dtype(q.dtype, grad_out=grad_out, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
+    _check_dtype(i32, q_offsets=q_offsets, k_offsets=k_offsets)
+    _check_dtype(f32, lse=lse)
+    desc_q, desc_k = _desc(q, 3, "q"), _desc(k, 3, "k")
+    T, H, D = q.shape
+    if dq is None:
+        dq = q.new_empty((T, H, D))
+    if dk is None:
+        dk = k.new_empty(tuple(k.shape))
+    if dv is None:
+        dv = k.new_empty(tuple(k.shape))
+    scratch = q.new_empty(2 * H * T, dtype=f32)
+    _launch("_mlir_ciface_nova_hip_attention_backward",
+            (q, grad_out, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv),
+            _desc(grad_out, 3, "grad_out"), desc_q, desc_k, _desc(v, 3, "v"), _desc(out, 3, "out"),
+            _desc(lse, 2, "lse"), _desc(q_offsets, 1, "q_offsets"), _desc(k_offsets, 1, "k_offsets"),
+            _desc(dq, 3, "dq"), _desc(dk, 3, "dk"), _desc(dv, 3, "dv"), _desc(scratch, 1, "scratch"),
+            D ** -0.5 if scale is None else scale, 1 if causal else 0, _dt(q))
     return dq, dk, dv
 
 
@@ -652,37 +670,32 @@ def attention_decode(q, k, v, lengths, *, scale=None, out=None, lse=None):
     first three dims in memory), lengths [sequences] i32.  Returns out;
     ``lse`` [sequences, heads] f32 is written when given."""
     torch = _torch()
-    _want_dtype(q.dtype, k=k, v=v, out=out)
-    _want_dtype(torch.int32, lengths=lengths)
-    _want_dtype(torch.float32, lse=lse)
-    with _on_device(q, k, v, lengths, out, lse):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if scale is None:
-            scale = q.shape[2] ** -0.5
-        need = lib().nova_hip_attention_decode_scratch(q.shape[0], k.shape[1], q.shape[1], k.shape[2],
-                                                       q.shape[2])
-        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
-        d = [memref_of(t) if t is not None else None for t in (q, k, v, lengths, out, lse, scratch)]
-        check(lib()._mlir_ciface_nova_hip_attention_decode(*[ref(x) for x in d], scale, _dt(q)))
+    _check_dtype(q.dtype, k=k, v=v, out=out)
+    _check_dtype(torch.int32, lengths=lengths)
+    _check_dtype(torch.float32, lse=lse)
+    dq, dk = _desc(q, 3, "q"), _desc(k, 4, "k")
+    B, H, D = q.shape
+    if out is None:
+        out = q.new_empty((B, H, D))
+    need = lib().nova_hip_attention_decode_scratch(B, k.shape[1], H, k.shape[2], D)
+    scratch = q.new_empty(need, dtype=torch.float32) if need else None
+    _launch("_mlir_ciface_nova_hip_attention_decode", (q, k, v, lengths, out, lse), dq, dk,
+            _desc(v, 4, "v"), _desc(lengths, 1, "lengths"), _desc(out, 3, "out"), _desc(lse, 2, "lse"),
+            _desc(scratch, 1, "scratch"), D ** -0.5 if scale is None else scale, _dt(q))
     return out
 
-
-# --------------------------------------------------------------------------
-# losses over token log-probabilities
-# --------------------------------------------------------------------------
 
 def token_logp(logits, labels, *, logp=None, lse=None):
     """The log-probability of each row's label [rows] f32 (0 where the label is
     negative); ``lse`` [rows] f32 is written when given."""
     torch = _torch()
-    _want_dtype(torch.int32, labels=labels)
-    _want_dtype(torch.float32, logp=logp, lse=lse)
-    with _on_device(logits, labels, logp, lse):
-        if logp is None:
-            logp = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        d = [memref_of(t) if t is not None else None for t in (logits, labels, logp, lse)]
-        check(lib()._mlir_ciface_nova_hip_token_logp(*[ref(x) for x in d], _dt(logits)))
+    _check_dtype(torch.int32, labels=labels)
+    _check_dtype(torch.float32, logp=logp, lse=lse)
+    d = _desc(logits, 2, "logits")
+    if logp is None:
+        logp = logits.new_empty(logits.shape[0], dtype=torch.float32)
+    _launch("_mlir_ciface_nova_hip_token_logp", (logits, labels, logp, lse), d,
+            _desc(labels, 1, "labels"), _desc(logp, 1, "logp"), _desc(lse, 1, "lse"), _dt(logits))
     return logp
 
 
@@ -694,25 +707,27 @@ def policy_loss(logits, labels, old_logp, advantage, weight, *, ref_logp=None, c
     with ``want_grad`` False.  ``clip`` is (low, high): the ratio is clamped to
     [1 - low, 1 + high].  Rows with a negative label or weight 0 take no part."""
     torch = _torch()
-    _want_dtype(torch.int32, labels=labels)
-    _want_dtype(torch.float32, old_logp=old_logp, advantage=advantage, weight=weight,
-                ref_logp=ref_logp, loss=loss, logp=logp, row_loss=row_loss)
-    _want_dtype(logits.dtype, grad=grad)
-    with _on_device(logits, labels, old_logp, advantage, weight, ref_logp, loss, logp, row_loss, grad):
-        rows, dev = logits.shape[0], logits.device
-        if loss is None:
-            loss = torch.empty(1, dtype=torch.float32, device=dev)
-        if logp is None:
-            logp = torch.empty(rows, dtype=torch.float32, device=dev)
-        if row_loss is None:
-            row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
-        if grad is None and want_grad:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        d = [memref_of(t) if t is not None else None
-             for t in (logits, labels, old_logp, ref_logp, advantage, weight, loss, logp, row_loss,
-                       grad)]
-        check(lib()._mlir_ciface_nova_hip_policy_loss(*[ref(x) for x in d], clip[0], clip[1], kl_coef,
-                                                      grad_scale, _dt(logits)))
+    f32 = torch.float32
+    _check_dtype(torch.int32, labels=labels)
+    _check_dtype(f32, old_logp=old_logp, advantage=advantage, weight=weight, ref_logp=ref_logp,
+                 loss=loss, logp=logp, row_loss=row_loss)
+    _check_dtype(logits.dtype, grad=grad)
+    d = _desc(logits, 2, "logits")
+    rows, classes = logits.shape
+    if loss is None:
+        loss = logits.new_empty(1, dtype=f32)
+    if logp is None:
+        logp = logits.new_empty(rows, dtype=f32)
+    if row_loss is None:
+        row_loss = logits.new_empty(rows, dtype=f32)
+    if grad is None and want_grad:
+        grad = logits.new_empty((rows, classes))
+    _launch("_mlir_ciface_nova_hip_policy_loss",
+            (logits, labels, old_logp, advantage, weight, ref_logp, loss, logp, row_loss, grad), d,
+            _desc(labels, 1, "labels"), _desc(old_logp, 1, "old_logp"), _desc(ref_logp, 1, "ref_logp"),
+            _desc(advantage, 1, "advantage"), _desc(weight, 1, "weight"), _desc(loss, 1, "loss"),
+            _desc(logp, 1, "logp"), _desc(row_loss, 1, "row_loss"), _desc(grad, 2, "grad"),
+            clip[0], clip[1], kl_coef, grad_scale, _dt(logits))
     return loss, logp, grad
 
 
@@ -725,24 +740,27 @@ def preference_loss(logits, labels, offsets, ref_logp, *, beta: float = 0.1, smo
     False.  ``pair_loss`` [pairs] and ``token`` [3, rows] (logp, lse, slope) are
     written when given."""
     torch = _torch()
-    _want_dtype(torch.int32, labels=labels, offsets=offsets)
-    _want_dtype(torch.float32, ref_logp=ref_logp, loss=loss, seq_logp=seq_logp,
-                pair_loss=pair_loss, token=token)
-    _want_dtype(logits.dtype, grad=grad)
-    with _on_device(logits, labels, offsets, ref_logp, loss, seq_logp, pair_loss, token, grad):
-        rows, seqs, dev = logits.shape[0], max(offsets.numel() - 1, 0), logits.device
-        if loss is None:
-            loss = torch.empty(1, dtype=torch.float32, device=dev)
-        if seq_logp is None:
-            seq_logp = torch.empty(seqs, dtype=torch.float32, device=dev)
-        if pair_loss is None:
-            pair_loss = torch.empty(seqs // 2, dtype=torch.float32, device=dev)
-        if token is None:
-            token = torch.empty((3, rows), dtype=torch.float32, device=dev)
-        if grad is None and want_grad:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        d = [memref_of(t) if t is not None else None
-             for t in (logits, labels, offsets, ref_logp, loss, seq_logp, pair_loss, token, grad)]
-        check(lib()._mlir_ciface_nova_hip_preference_loss(*[ref(x) for x in d], beta, smoothing,
-                                                          grad_scale, _dt(logits)))
+    f32 = torch.float32
+    _check_dtype(torch.int32, labels=labels, offsets=offsets)
+    _check_dtype(f32, ref_logp=ref_logp, loss=loss, seq_logp=seq_logp, pair_loss=pair_loss,
+                 token=token)
+    _check_dtype(logits.dtype, grad=grad)
+    d, do = _desc(logits, 2, "logits"), _desc(offsets, 1, "offsets")
+    rows, classes = logits.shape
+    seqs = max(offsets.shape[0] - 1, 0)
+    if loss is None:
+        loss = logits.new_empty(1, dtype=f32)
+    if seq_logp is None:
+        seq_logp = logits.new_empty(seqs, dtype=f32)
+    if pair_loss is None:
+        pair_loss = logits.new_empty(seqs // 2, dtype=f32)
+    if token is None:
+        token = logits.new_empty((3, rows), dtype=f32)
+    if grad is None and want_grad:
+        grad = logits.new_empty((rows, classes))
+    _launch("_mlir_ciface_nova_hip_preference_loss",
+            (logits, labels, offsets, ref_logp, loss, seq_logp, pair_loss, token, grad), d,
+            _desc(labels, 1, "labels"), do, _desc(ref_logp, 1, "ref_logp"), _desc(loss, 1, "loss"),
+            _desc(seq_logp, 1, "seq_logp"), _desc(pair_loss, 1, "pair_loss"),
+            _desc(token, 2, "token"), _desc(grad, 2, "grad"), beta, smoothing, grad_scale, _dt(logits))
     return loss, seq_logp, grad
