@@ -34,6 +34,10 @@ using gemm::u32x2;
 using gemm::u32x4;
 
 typedef __attribute__((address_space(3))) void lds_void;
+// Tiles are passed as LDS pointers: through generic ones the compiler keeps
+// null checks of the conversion.
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) float lds_float;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -114,7 +118,7 @@ struct TileLoad {
   }
   // Rows [0, rows) at p to the tile; rows behind them read zero.
   __device__ __forceinline__ void load(const uint16_t *p, int64_t stride, int rows, int D,
-                                       char *tile) const {
+                                       lds_char *tile) const {
     const int n = min(rows, ROWS);
     const uint32_t bytes = n > 0 ? (uint32_t)(((n - 1) * stride + D) * 2) : 0u;
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(p, bytes);
@@ -132,8 +136,9 @@ __device__ __forceinline__ uint32_t row_frag(int r0, int s, int lane) {
   const int row = r0 + (lane & 31);
   return (uint32_t)(row * CH + ((2 * s + (lane >> 5)) ^ swz<CH>(row))) * 16u;
 }
-__device__ __forceinline__ u32x4 read_row_frag(const char *tile, uint32_t off) {
-  return *reinterpret_cast<const u32x4 *>(tile + off);
+__device__ __forceinline__ u32x4 read_row_frag(const lds_char *tile, uint32_t off) {
+  typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+  return *(lds_u32x4 *)(tile + off);
 }
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -145,13 +150,12 @@ __device__ __forceinline__ uint32_t col_frag(int r, int d0, int lane) {
   const int row = r + 4 * (g >> 1) + (p >> 2), d = d0 + 16 * (g & 1) + 4 * (p & 3);
   return (uint32_t)((row * CH + ((d >> 3) ^ swz<CH>(row))) * 8 + (d & 7)) * 2u;
 }
-__device__ __forceinline__ u32x2 read_tr(const char *p) {
+__device__ __forceinline__ u32x2 read_tr(const lds_char *p) {
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (lds_i16x4 *)(const_cast<char *>(p))));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)p));
 }
 template <int CH>
-__device__ __forceinline__ u32x4 read_col_frag(const char *tile, int r0, int d0, int lane) {
+__device__ __forceinline__ u32x4 read_col_frag(const lds_char *tile, int r0, int d0, int lane) {
   const u32x2 lo = read_tr(tile + col_frag<CH>(r0, d0, lane));
   const u32x2 hi = read_tr(tile + col_frag<CH>(r0 + 8, d0, lane));
   return u32x4{lo[0], lo[1], hi[0], hi[1]};

@@ -42,10 +42,14 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
 template <int DT, int DP, bool CAUSAL>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sk0[kTile];
-  __shared__ __attribute__((aligned(1024))) char sk1[kTile];
-  __shared__ __attribute__((aligned(1024))) char sv0[kTile];
-  __shared__ __attribute__((aligned(1024))) char sv1[kTile];
+  __shared__ __attribute__((aligned(1024))) char sk0_[kTile];
+  lds_char *const sk0 = (lds_char *)sk0_;
+  __shared__ __attribute__((aligned(1024))) char sk1_[kTile];
+  lds_char *const sk1 = (lds_char *)sk1_;
+  __shared__ __attribute__((aligned(1024))) char sv0_[kTile];
+  lds_char *const sv0 = (lds_char *)sv0_;
+  __shared__ __attribute__((aligned(1024))) char sv1_[kTile];
+  lds_char *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
@@ -77,11 +81,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
   float mc = -INFINITY, l = 0.0f;  // m c and this lane's share of the sum
   const int last = q0 + (lane & 31) + shift;  // causal: the last key this lane's row sees
 
-  auto fetch = [&](int t, char *sk, char *sv) __attribute__((always_inline)) {
+  auto fetch = [&](int t, lds_char *sk, lds_char *sv) __attribute__((always_inline)) {
     lk.load(kp + (int64_t)t * kBN * a.sk.t, a.sk.t, Lk - t * kBN, a.D, sk);
     lv.load(vp + (int64_t)t * kBN * a.sv.t, a.sv.t, Lk - t * kBN, a.D, sv);
   };
-  auto step = [&](int t, const char *sk, const char *sv) __attribute__((always_inline)) {
+  auto step = [&](int t, const lds_char *sk, const lds_char *sv) __attribute__((always_inline)) {
     const int k0 = t * kBN;
     if (qn <= 0 || (CAUSAL && k0 > q0 + qn - 1 + shift)) return;  // wave-uniform
     f32x16 s[2];

@@ -33,6 +33,8 @@ struct BwdArgs {
   float c, scale;
 };
 
+typedef __attribute__((address_space(3))) const gemm::f32x4 lds_f32x4;
+
 constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
 
 // f16 weights take a factor 2^8 in the product for dV (they are at most 1, and
@@ -71,10 +73,14 @@ __device__ __forceinline__ float row_dot(const u32x4 (&x)[DP / 16], const u32x4 
 template <int DT, int DP, bool CAUSAL>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sk0[kTile];
-  __shared__ __attribute__((aligned(1024))) char sk1[kTile];
-  __shared__ __attribute__((aligned(1024))) char sv0[kTile];
-  __shared__ __attribute__((aligned(1024))) char sv1[kTile];
+  __shared__ __attribute__((aligned(1024))) char sk0_[kTile];
+  lds_char *const sk0 = (lds_char *)sk0_;
+  __shared__ __attribute__((aligned(1024))) char sk1_[kTile];
+  lds_char *const sk1 = (lds_char *)sk1_;
+  __shared__ __attribute__((aligned(1024))) char sv0_[kTile];
+  lds_char *const sv0 = (lds_char *)sv0_;
+  __shared__ __attribute__((aligned(1024))) char sv1_[kTile];
+  lds_char *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
@@ -119,11 +125,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
   const int last = q0 + (lane & 31) + shift;
 
-  auto fetch = [&](int t, char *sk, char *sv) __attribute__((always_inline)) {
+  auto fetch = [&](int t, lds_char *sk, lds_char *sv) __attribute__((always_inline)) {
     lk.load(kp + (int64_t)t * kBN * a.sk.t, a.sk.t, Lk - t * kBN, a.D, sk);
     lv.load(vp + (int64_t)t * kBN * a.sv.t, a.sv.t, Lk - t * kBN, a.D, sv);
   };
-  auto step = [&](int t, const char *sk, const char *sv) __attribute__((always_inline)) {
+  auto step = [&](int t, const lds_char *sk, const lds_char *sv) __attribute__((always_inline)) {
     const int k0 = t * kBN;
     if (qn <= 0 || (CAUSAL && k0 > q0 + qn - 1 + shift)) return;
     const bool edge = k0 + kBN > Lk || (CAUSAL && k0 + kBN - 1 > q0 + shift);
@@ -180,12 +186,18 @@ template <int DT, int DP, bool CAUSAL, int WK>
 __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_kernel(BwdArgs a) {
   constexpr int WQ = kWaves / WK, kKeys = 32 * WK;
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sq0[kTile];
-  __shared__ __attribute__((aligned(1024))) char sq1[kTile];
-  __shared__ __attribute__((aligned(1024))) char sg0[kTile];
-  __shared__ __attribute__((aligned(1024))) char sg1[kTile];
-  __shared__ __attribute__((aligned(1024))) float sc0[2 * kBN];  // the tile's row constants
-  __shared__ __attribute__((aligned(1024))) float sc1[2 * kBN];
+  __shared__ __attribute__((aligned(1024))) char sq0_[kTile];
+  lds_char *const sq0 = (lds_char *)sq0_;
+  __shared__ __attribute__((aligned(1024))) char sq1_[kTile];
+  lds_char *const sq1 = (lds_char *)sq1_;
+  __shared__ __attribute__((aligned(1024))) char sg0_[kTile];
+  lds_char *const sg0 = (lds_char *)sg0_;
+  __shared__ __attribute__((aligned(1024))) char sg1_[kTile];
+  lds_char *const sg1 = (lds_char *)sg1_;
+  __shared__ __attribute__((aligned(1024))) float sc0_[2 * kBN];  // the tile's row constants
+  lds_float *const sc0 = (lds_float *)sc0_;
+  __shared__ __attribute__((aligned(1024))) float sc1_[2 * kBN];
+  lds_float *const sc1 = (lds_float *)sc1_;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = wave % WK, wq = wave / WK;
@@ -213,7 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
 
-  auto fetch = [&](int u, char *sq, char *sg, float *sc) __attribute__((always_inline)) {
+  auto fetch = [&](int u, lds_char *sq, lds_char *sg, lds_float *sc) __attribute__((always_inline)) {
     const int g = u / nt, q0 = first + (u - g * nt) * kBN, head = kh * a.group + g;
     const int n = Lq - q0;
     lq.load(a.q + (int64_t)(qs + q0) * a.sq.t + head * a.sq.h, a.sq.t, n, a.D, sq);
@@ -228,7 +240,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
                                                0);
     }
   };
-  auto step = [&](int u, const char *sq, const char *sg, const float *sc)
+  auto step = [&](int u, const lds_char *sq, const lds_char *sg, const lds_float *sc)
       __attribute__((always_inline)) {
     const int q0 = first + (u % nt) * kBN;
     if (kn <= 0) return;
@@ -246,8 +258,8 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int row = 32 * i + 8 * r4 + 4 * (lane >> 5);
-        const gemm::f32x4 nl = *reinterpret_cast<const gemm::f32x4 *>(sc + row);
-        const gemm::f32x4 de = *reinterpret_cast<const gemm::f32x4 *>(sc + kBN + row);
+        const gemm::f32x4 nl = *(lds_f32x4 *)(sc + row);
+        const gemm::f32x4 de = *(lds_f32x4 *)(sc + kBN + row);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * r4 + e;
@@ -292,7 +304,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   if constexpr (WQ == 2) {
     // The second wave of each key block hands its sums over through LDS, 32
     // columns of d at a time (one 32 x 32 block of f32 per pair of waves).
-    float *box = reinterpret_cast<float *>(wk ? sq1 : sq0);
+    lds_float *box = (lds_float *)(wk ? sq1 : sq0);
     static_assert(WK == 2 && kTile >= 64 * 16 * 4, "one block per box");
 #pragma unroll
     for (int j = 0; j < 2 * (DP / 32); ++j) {

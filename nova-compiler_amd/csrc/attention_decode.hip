@@ -2,17 +2,22 @@
 // single tokens.  Bound by HBM: keys and values are read once, for all query
 // heads of their group together (the group's heads are the MFMA's columns).
 //
-// A cache of S rows is cut into splits of `chunk` keys; a workgroup takes one
-// split of one sequence and key head, its waves alternate over blocks of 32
-// keys, each with a two-stage ring of its own in LDS filled by DMA (no
-// barrier until the end), and the waves' sums are joined through LDS.  With
-// more than one split the joined sums go to the caller's scratch and
-// attention_join_kernel adds them in split order.
+// A cache of S rows is cut into splits of `chunk` keys; a workgroup of one wave
+// takes one split of one sequence and key head, 32 keys at a time through a
+// two-stage ring in LDS filled by DMA, without a barrier.  (Two waves sharing a
+// split joined their sums through LDS and took 2% longer.)  With more than
+// one split the sums go to the caller's scratch, and attention_join_kernel adds
+// them in a fixed order.
+//
+// Measured: 32 sequences of 1500 to 8192 rows, 597 MB of keys and values, in
+// 100 us (5.8 TB/s); 8 of 131072 in 685 us (6.3 TB/s).  Without the products
+// (the DMA alone) it takes the same: the loads are the time.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "attention.h"
+#include "wave.h"
 
 namespace nova_hip {
 namespace attn {
@@ -30,59 +35,68 @@ struct DecodeArgs {
   float c;
 };
 
-constexpr int kWaves = 2, kBN = 32;
+constexpr int kBN = 32;
 
 template <int DT, int DP>
-__global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64) void attention_decode_kernel(DecodeArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sk0[kWaves * kTile];
-  __shared__ __attribute__((aligned(1024))) char sk1[kWaves * kTile];
-  __shared__ __attribute__((aligned(1024))) char sv0[kWaves * kTile];
-  __shared__ __attribute__((aligned(1024))) char sv1[kWaves * kTile];
-  __shared__ float sm[kWaves][32], sl[kWaves][32];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = blockIdx.z, split = blockIdx.x;
+  __shared__ __attribute__((aligned(1024))) char sk0_[kTile];
+  lds_char *const sk0 = (lds_char *)sk0_;
+  __shared__ __attribute__((aligned(1024))) char sk1_[kTile];
+  lds_char *const sk1 = (lds_char *)sk1_;
+  __shared__ __attribute__((aligned(1024))) char sv0_[kTile];
+  lds_char *const sv0 = (lds_char *)sv0_;
+  __shared__ __attribute__((aligned(1024))) char sv1_[kTile];
+  lds_char *const sv1 = (lds_char *)sv1_;
+  const int lane = threadIdx.x;
+  const int b = blockIdx.y, split = blockIdx.z;
   const int blocks = (a.group + 31) / 32;  // of 32 query heads
-  const int kh = blockIdx.y / blocks, h0 = kh * a.group + 32 * (blockIdx.y - kh * blocks);
+  const int kh = blockIdx.x / blocks, h0 = kh * a.group + 32 * (blockIdx.x - kh * blocks);
   const int hn = min(32, (kh + 1) * a.group - h0);
   const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
   const int from = split * a.chunk, to = min(len, from + a.chunk);
   if (from >= len && split > 0) return;  // nothing here; the join does not read it
 
-  u32x4 qf[DP / 16];
-  load_cols<DP>(qf, a.q + b * a.sqb + h0 * a.sqh, a.sqh, hn, a.D, lane);
   const uint16_t *kp = a.k + b * a.skb + kh * a.skh, *vp = a.v + b * a.svb + kh * a.svh;
 
   // A wave's own loads: 64 lanes cover 64 / CH rows at a time.
   constexpr int kN = kBN * CH / 64, kStep = 64 / CH;
   const int row = lane / CH;
-  auto fetch = [&](int t, char *sk, char *sv) __attribute__((always_inline)) {
+  auto fetch = [&](int t, lds_char *sk, lds_char *sv) __attribute__((always_inline)) {
     const int k0 = from + t * kBN, n = min(to - k0, kBN);
     const __amdgpu_buffer_rsrc_t rk = make_rsrc(
         kp + (int64_t)k0 * a.skt, n > 0 ? (uint32_t)(((n - 1) * a.skt + a.D) * 2) : 0u);
     const __amdgpu_buffer_rsrc_t rv = make_rsrc(
         vp + (int64_t)k0 * a.svt, n > 0 ? (uint32_t)(((n - 1) * a.svt + a.D) * 2) : 0u);
+    // Read once by the whole chip: the nontemporal hint (1 in aux bit 1) keeps
+    // them from pushing each other through the L2s (32 sequences of 1500 to
+    // 8192 rows: 122 -> 105 us; 8 of 131072: 757 -> 688 us).
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int r = i * kStep + row, c = (lane & (CH - 1)) ^ swz<CH>(r);
-      const uint32_t ok = c * 8 < a.D ? (uint32_t)(r * a.skt + c * 8) * 2u : kOOB;
-      const uint32_t ov = c * 8 < a.D ? (uint32_t)(r * a.svt + c * 8) * 2u : kOOB;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(sk + wave * kTile + i * 1024), 16,
-                                               ok, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(sv + wave * kTile + i * 1024), 16,
-                                               ov, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rk, (lds_void *)(sk + i * 1024), 16,
+          c * 8 < a.D ? (uint32_t)(r * a.skt + c * 8) * 2u : kOOB, 0, 0, 2);
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int r = i * kStep + row, c = (lane & (CH - 1)) ^ swz<CH>(r);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rv, (lds_void *)(sv + i * 1024), 16,
+          c * 8 < a.D ? (uint32_t)(r * a.svt + c * 8) * 2u : kOOB, 0, 0, 2);
     }
   };
+  const int nb = (max(to - from, 0) + kBN - 1) / kBN;
+  if (nb > 0) fetch(0, sk0, sv0);
+  u32x4 qf[DP / 16];
+  load_cols<DP>(qf, a.q + b * a.sqb + h0 * a.sqh, a.sqh, hn, a.D, lane);
 
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
   float mc = -INFINITY, l = 0.0f;
-  auto step = [&](int t, const char *sk, const char *sv) __attribute__((always_inline)) {
+  auto step = [&](int t, const lds_char *sk, const lds_char *sv) __attribute__((always_inline)) {
     const int k0 = from + t * kBN;
-    sk += wave * kTile;
-    sv += wave * kTile;
     f32x16 s = {};
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk)
@@ -117,10 +131,8 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(DecodeArg
         acc[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sv, 16 * kk, 32 * db, lane), pf, acc[db]);
     }
   };
-  // This wave's blocks are wave, wave + kWaves, ...; a stage is refilled when
-  // the reads of it have returned.
+  // A stage is refilled when the reads of it have returned.
   constexpr int kInFlight = 2 * kN;  // DMA instructions of one stage
-  const int nb = (max(to - from, 0) + kBN - 1) / kBN;
   auto landed = [&](bool more) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     if (more) __builtin_amdgcn_s_waitcnt(0x0F70 | (kInFlight & 15) | ((kInFlight >> 4) << 14));
@@ -132,61 +144,29 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(DecodeArg
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (wave < nb) fetch(wave, sk0, sv0);
-  for (int t = wave; t < nb; t += 2 * kWaves) {
-    const bool two = t + kWaves < nb;
+  for (int t = 0; t < nb; t += 2) {
+    const bool two = t + 1 < nb;
     drained();
-    if (two) fetch(t + kWaves, sk1, sv1);
+    if (two) fetch(t + 1, sk1, sv1);
     landed(two);
     step(t, sk0, sv0);
     if (!two) break;
-    const bool three = t + 2 * kWaves < nb;
+    const bool three = t + 2 < nb;
     drained();
-    if (three) fetch(t + 2 * kWaves, sk0, sv0);
+    if (three) fetch(t + 2, sk0, sv0);
     landed(three);
-    step(t + kWaves, sk1, sv1);
+    step(t + 1, sk1, sv1);
   }
 
-  // Join the waves: to the largest of their maxima, then in wave order.
   l = both_sum(l);
-  if (lane < 32) {
-    sm[wave][lane] = mc;
-    sl[wave][lane] = l;
-  }
-  __syncthreads();  // also: every wave is done with its ring
-  const int col = lane & 31;
-  float mx = sm[0][col], sum = 0.0f;
-#pragma unroll
-  for (int i = 1; i < kWaves; ++i) mx = fmaxf(mx, sm[i][col]);
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i)
-    sum += sm[i][col] == -INFINITY ? 0.0f : sl[i][col] * __builtin_amdgcn_exp2f(sm[i][col] - mx);
-  const float f = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - mx);
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
-  float *box = reinterpret_cast<float *>(sk0);
-  static_assert(kWaves == 2 && kWaves * kTile >= 64 * 16 * 4, "one block of the second wave");
-#pragma unroll
-  for (int db = 0; db < DP / 32; ++db) {
-    if (db) __syncthreads();
-    if (wave == 1) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) box[64 * r + lane] = acc[db][r];
-    }
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[db][r] += box[64 * r + lane];
-    }
-  }
-  if (wave == 1) return;
   if (a.splits == 1) {
-    store_rows<DT, DP>(acc, sum == 0.0f ? 0.0f : 1.0f / sum, a.o + b * a.sob + h0 * a.soh, a.soh, hn,
+    store_rows<DT, DP>(acc, l == 0.0f ? 0.0f : 1.0f / l, a.o + b * a.sob + h0 * a.soh, a.soh, hn,
                        a.D, lane);
     if (a.lse && lane < hn)
-      a.lse[b * a.slse + h0 + lane] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
+      a.lse[b * a.slse + h0 + lane] = l == 0.0f ? -INFINITY : (mc + __log2f(l)) * kLn2;
     return;
   }
+  const int col = lane & 31;
   if (col >= hn) return;
   float *p = a.partial + (((int64_t)b * a.heads + h0 + col) * a.splits + split) * (a.D + 2);
 #pragma unroll
@@ -196,25 +176,29 @@ __global__ __launch_bounds__(64 * kWaves) void attention_decode_kernel(DecodeArg
       const int d = 32 * db + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
       if (d < a.D) *reinterpret_cast<float2 *>(p + d) = float2{acc[db][r], acc[db][r + 1]};
     }
-  if (lane < 32) *reinterpret_cast<float2 *>(p + a.D) = float2{mx, sum};
+  if (lane < 32) *reinterpret_cast<float2 *>(p + a.D) = float2{mc, l};
 }
 
-// One wave per (sequence, head): the splits' sums to their largest maximum,
-// added in split order.
+// One workgroup per (sequence, head): the splits' sums to their largest
+// maximum, added in split order within each wave's quarter (splits w, w + 4,
+// ...), then the four quarters in order.
 template <int DT>
-__global__ __launch_bounds__(64) void attention_join_kernel(DecodeArgs a) {
-  const int lane = threadIdx.x, h = blockIdx.x, b = blockIdx.y;
+__global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a) {
+  __shared__ float smax[4], ssum[4], sx[4][128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = blockIdx.x, b = blockIdx.y;
   const int len = min(max(a.lens[b], 0), a.S);
   const int n = max(1, (len + a.chunk - 1) / a.chunk);
   const float *p = a.partial + ((int64_t)b * a.heads + h) * a.splits * (a.D + 2);
   float mx = -INFINITY;
-  for (int i = lane; i < n; i += 64) mx = fmaxf(mx, p[(int64_t)i * (a.D + 2) + a.D]);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
+  for (int i = threadIdx.x; i < n; i += 256) mx = fmaxf(mx, p[(int64_t)i * (a.D + 2) + a.D]);
+  mx = wave_max(mx);
+  if (lane == 0) smax[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
   float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
   const int d = 2 * lane;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+#pragma unroll 8
+  for (int i = wave; i < n; i += 4) {
     const float *r = p + (int64_t)i * (a.D + 2);
     const float2 ml = *reinterpret_cast<const float2 *>(r + a.D);
     const float2 v = *reinterpret_cast<const float2 *>(r + min(d, a.D - 2));
@@ -223,6 +207,14 @@ __global__ __launch_bounds__(64) void attention_join_kernel(DecodeArgs a) {
     x0 = __builtin_fmaf(v.x, f, x0);
     x1 = __builtin_fmaf(v.y, f, x1);
   }
+  sx[wave][d] = x0;
+  sx[wave][d + 1] = x1;
+  if (lane == 0) ssum[wave] = sum;
+  __syncthreads();
+  if (wave) return;
+  sum = (ssum[0] + ssum[1]) + (ssum[2] + ssum[3]);
+  x0 = (sx[0][d] + sx[1][d]) + (sx[2][d] + sx[3][d]);
+  x1 = (sx[0][d + 1] + sx[1][d + 1]) + (sx[2][d + 1] + sx[3][d + 1]);
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (d < a.D)
     *reinterpret_cast<uint32_t *>(a.o + b * a.sob + h * a.soh + d) = pack<DT>(x0 * inv, x1 * inv);
@@ -232,7 +224,7 @@ __global__ __launch_bounds__(64) void attention_join_kernel(DecodeArgs a) {
 
 template <int DT, int DP>
 void launch_decode_t(const DecodeArgs &a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((attention_decode_kernel<DT, DP>), grid, dim3(64 * kWaves), 0, s, a);
+  hipLaunchKernelGGL((attention_decode_kernel<DT, DP>), grid, dim3(64), 0, s, a);
 }
 template <int DT>
 int32_t launch_decode(const DecodeArgs &a, dim3 grid, hipStream_t s) {
@@ -242,18 +234,26 @@ int32_t launch_decode(const DecodeArgs &a, dim3 grid, hipStream_t s) {
   else launch_decode_t<DT, 128>(a, grid, s);
   const int32_t rc = check_hip(hipGetLastError(), "attention_decode launch");
   if (rc || a.splits == 1) return rc;
-  hipLaunchKernelGGL(attention_join_kernel<DT>, dim3((unsigned)a.heads, grid.z), dim3(64), 0, s, a);
+  hipLaunchKernelGGL(attention_join_kernel<DT>, dim3((unsigned)a.heads, grid.y), dim3(256), 0, s, a);
   return check_hip(hipGetLastError(), "attention_decode join launch");
 }
 
 }  // namespace
 }  // namespace attn
 
-// Keys per split, a multiple of 64 (a block for each wave): about 2048 splits
-// in all, eight per CU, if the cache is full.
+// Keys per split, a multiple of 64.  A wave per split, 1024 of them resident
+// (four per CU by LDS): short splits for parallelism while the cache is
+// small, at most 512 keys while there are fewer than eight rounds of them (long
+// ones leave a ragged batch's last round idle), longer beyond.  Measured at 64
+// / 128 / 256 / 512 / 1024 keys, heads 32 and 8 of 128, us:
+//   1 x 8192 rows                13.9 / 13.8 / 17.6 / 27.6 / 45.5
+//   8 x 8192                     69.2 / 57.7 / 51.5 / 48.5 / 50.8
+//   32 x 1500 .. 8192 of 8192     151 /  128 /  114 /  103 /  116
+//   8 x 131072                   1007 /  878 /  797 /  755 /  685
 int64_t attention_decode_chunk(int64_t B, int64_t S, int64_t kv_heads) {
   const int64_t all = B * S * kv_heads;
-  return std::max<int64_t>(64, std::min<int64_t>((all / 2048 + 63) / 64 * 64, (S + 63) / 64 * 64));
+  const int64_t keys = std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
+  return std::max<int64_t>(64, (keys + 63) / 64 * 64);
 }
 
 int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s) {
@@ -279,7 +279,11 @@ int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s) 
   a.chunk = (int)chunk;
   a.splits = (int)std::max<int64_t>(1, (p.S + chunk - 1) / chunk);
   a.c = p.scale * attn::kLog2e;
-  const dim3 grid((unsigned)a.splits, (unsigned)(p.kv_heads * ((a.group + 31) / 32)), (unsigned)p.B);
+  // Splits outermost: sequences shorter than the cache leave the last splits
+  // empty, and with splits innermost a power of two of them put every first
+  // split on the same XCD (32 sequences of 300 rows in a cache of 8192, splits
+  // of 512: 90 us, 16 with the order below).
+  const dim3 grid((unsigned)(p.kv_heads * ((a.group + 31) / 32)), (unsigned)p.B, (unsigned)a.splits);
   return p.dt == NOVA_HIP_DT_BF16 ? attn::launch_decode<NOVA_HIP_DT_BF16>(a, grid, s)
                                   : attn::launch_decode<NOVA_HIP_DT_F16>(a, grid, s);
 }
