@@ -428,8 +428,8 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
  *   dv = P^T grad_out, dq = scale dS k, dk = scale dS^T q,
  * dk and dv summed over the query heads that share a key head.  Shapes and
  * strides as for the forward (grad_out, out, dq as q; dk, dv as k); lse
- * [heads, query tokens]; scratch : at least 2 * heads * query tokens f32,
- * dense, used by this call only.  P and dS are rounded to dt for the
+ * [heads, query tokens]; scratch : at least
+ * nova_hip_attention_backward_scratch() f32, dense, used by this call only.  P and dS are rounded to dt for the
  * products, sums are f32 in a fixed order (no atomics: the same bits on every
  * run).  A query that sees no key has gradient zero and adds none; rows
  * outside every sequence are left as they were. */
@@ -439,6 +439,10 @@ int32_t _mlir_ciface_nova_hip_attention_backward(
     const NovaMemRef1D *q_offsets, const NovaMemRef1D *k_offsets, NovaMemRef3D *dq,
     NovaMemRef3D *dk, NovaMemRef3D *dv, NovaMemRef1D *scratch, float scale, int32_t causal,
     int32_t dt);
+/* Floats of scratch the call above needs on sizes it accepts. */
+int64_t nova_hip_attention_backward_scratch(int64_t q_tokens, int64_t k_tokens, int64_t sequences,
+                                            int64_t heads, int64_t kv_heads, int64_t D,
+                                            int32_t causal);
 /* Attention of one query per sequence over a padded cache (single-token
  * serving): out[b, h] = softmax(scale q[b, h] . k[b, :lengths[b]]) v.
  *   q, out : [sequences, heads, D]; k, v : [sequences, cache rows, key heads,

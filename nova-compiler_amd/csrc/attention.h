@@ -57,37 +57,63 @@ __device__ __forceinline__ int swz(int row) {
   else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// The sequence of tile t when each sequence takes ceil(rows / BM) tiles, and
-// the first row of that tile in it: false when t lies behind the last tile.
-// off[0 .. B] are the sequences' first rows; whatever they hold, every
-// sequence is cut to rows inside [0, T).  Wave-uniform; every wave searches
-// for itself, 64 sequences at a time.
+__device__ __forceinline__ int wave_sum_int(int v) {
+#define NOVA_DPP_ADD(c) v += __builtin_amdgcn_mov_dpp(v, c, 0xF, 0xF, false)
+  NOVA_DPP_ADD(0xB1);   // quad_perm [1,0,3,2]
+  NOVA_DPP_ADD(0x4E);   // quad_perm [2,3,0,1]
+  NOVA_DPP_ADD(0x141);  // row_half_mirror
+  NOVA_DPP_ADD(0x140);  // row_mirror
+#undef NOVA_DPP_ADD
+  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) +
+         (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+
+// Tile t of the sequences' tiles of BM rows, off[0 .. B] being the sequences'
+// first rows (whatever they hold, every sequence is cut to rows inside [0, T)),
+// in the order of falling index within the sequence: the last tiles of the
+// longest sequences first.  That is the order of falling work of causal
+// attention (or of rising index counted from the end, for keys), so that what
+// runs last is short.  Gives the sequence, the tile's index in it and the
+// sequence's tiles; false when t lies behind the last tile.
+// Wave-uniform; every wave searches for itself: with S(l) = sum over sequences
+// of max(0, tiles - l), the tiles of index l and above, it finds the largest
+// l with S(l) > t, bit by bit.
 __device__ __forceinline__ bool find_tile(const int *off, int B, int T, int BM, int t, int &seq,
-                                          int &row0) {
+                                          int &index, int &tiles) {
   const int lane = threadIdx.x & 63;
-  int before = 0;  // tiles of the sequences before this group of 64
+  auto tiles_of = [&](int b) __attribute__((always_inline)) {
+    if (b >= B) return 0;
+    const int s = min(max(off[b], 0), T), e = min(max(off[b + 1], 0), T);
+    return e > s ? (e - s + BM - 1) / BM : 0;
+  };
+  const int n0 = tiles_of(lane);  // the first 64 sequences stay in registers
+  auto above = [&](int l) __attribute__((always_inline)) {
+    int v = max(0, n0 - l);
+    for (int b0 = 64; b0 < B; b0 += 64) v += max(0, tiles_of(b0 + lane) - l);
+    return wave_sum_int(v);
+  };
+  if (above(0) <= t) return false;
+  int level = 0;
+  // No sequence has 2^k tiles once S(2^k) is 0.
+  int bit = 1;
+  while (bit < (1 << 26) && above(bit) > t) bit <<= 1;
+  for (bit >>= 1; bit > 0; bit >>= 1)
+    if (above(level + bit) > t) level += bit;
+  int k = t - above(level + 1);  // among the sequences with a tile of that index
   for (int b0 = 0; b0 < B; b0 += 64) {
-    const int b = b0 + lane;
-    int n = 0;
-    if (b < B) {
-      const int s = min(max(off[b], 0), T), e = min(max(off[b + 1], 0), T);
-      n = e > s ? (e - s + BM - 1) / BM : 0;
-    }
-    int incl = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int v = __shfl_up(incl, d);
-      if (lane >= d) incl += v;
-    }
-    const uint64_t hit = __ballot(before + incl > t);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int first = before + __builtin_amdgcn_readlane(incl - n, l);
+    const int n = b0 ? tiles_of(b0 + lane) : n0;
+    const uint64_t has = __ballot(n > level);
+    const int count = __builtin_popcountll(has);
+    if (k < count) {
+      const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+      const int l = __builtin_ctzll(__ballot(n > level && rank == k));
       seq = __builtin_amdgcn_readfirstlane(b0 + l);
-      row0 = __builtin_amdgcn_readfirstlane((t - first) * BM);
+      index = __builtin_amdgcn_readfirstlane(level);
+      tiles = __builtin_amdgcn_readlane(n, l);
       return true;
     }
-    before += __builtin_amdgcn_readlane(incl, 63);
+    k -= count;
   }
   return false;
 }
@@ -120,7 +146,7 @@ struct TileLoad {
   __device__ __forceinline__ void load(const uint16_t *p, int64_t stride, int rows, int D,
                                        lds_char *tile) const {
     const int n = min(rows, ROWS);
-    const uint32_t bytes = n > 0 ? (uint32_t)(((n - 1) * stride + D) * 2) : 0u;
+    const uint32_t bytes = n > 0 ? ((uint32_t)(n - 1) * (uint32_t)stride + D) * 2u : 0u;
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(p, bytes);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
@@ -160,6 +186,11 @@ __device__ __forceinline__ u32x4 read_col_frag(const lds_char *tile, int r0, int
   const u32x2 hi = read_tr(tile + col_frag<CH>(r0 + 8, d0, lane));
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
+
+// Inside a wave-uniform branch around masks: an empty statement with a side
+// effect keeps the compiler from turning the branch into selects, which every
+// tile would pay for.
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
 template <int DT>
 __device__ __forceinline__ uint32_t pack(float a, float b) {

@@ -53,9 +53,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
-  const int head = w / a.tiles, tile = a.tiles - 1 - (w - head * a.tiles);
-  int b, row0;
-  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, row0)) return;
+  const int head = w / a.tiles;
+  int b, index, n;
+  if (!find_tile(a.q_off, a.B, a.Tq, kBM, w - head * a.tiles, b, index, n)) return;
+  const int row0 = index * kBM;
   int qs, qe, ks, ke;
   seq_rows(a.q_off, b, a.Tq, qs, qe);
   seq_rows(a.k_off, b, a.Tk, ks, ke);
@@ -88,6 +89,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
   auto step = [&](int t, const lds_char *sk, const lds_char *sv) __attribute__((always_inline)) {
     const int k0 = t * kBN;
     if (qn <= 0 || (CAUSAL && k0 > q0 + qn - 1 + shift)) return;  // wave-uniform
+    __builtin_amdgcn_iglp_opt(0);  // a product, an LDS read, a product, ...: 2% at D = 128
     f32x16 s[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -97,6 +99,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
         s[i] = mfma_32x32x16<DT>(read_row_frag(sk, row_frag<CH>(32 * i, kk, lane)), qf[kk], s[i]);
     }
     if (k0 + kBN > Lk || (CAUSAL && k0 + kBN - 1 > q0 + shift)) {
+      keep_branch();
       const int end = CAUSAL ? min(Lk, last + 1) : Lk;
 #pragma unroll
       for (int i = 0; i < 2; ++i)

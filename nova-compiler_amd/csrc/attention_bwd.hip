@@ -25,17 +25,22 @@ struct BwdArgs {
   const uint16_t *q, *k, *v, *o, *go;
   const float *lse;
   uint16_t *dq, *dk, *dv;
-  float *rows;  // [2][heads][Tq]: lse log2 e, delta
+  float *rows;  // [2][heads][Tq]: lse log2 e, -delta
+  float *partial;  // [key heads][tiles][splits][wave][dK, dV][DP / 2][lane] (splits > 1)
   const int *q_off, *k_off;
   Rows sq, sk, sv, so, sgo, sdq, sdk, sdv;
   int64_t slse;
-  int Tq, Tk, B, heads, group, D, tiles;
+  int Tq, Tk, B, heads, group, D, tiles, splits;
   float c, scale;
 };
 
 typedef __attribute__((address_space(3))) const gemm::f32x4 lds_f32x4;
 
 constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
+
+// Floats of one wave's dK and dV.
+template <int DP>
+constexpr int64_t kPartial = DP * 64;
 
 // f16 weights take a factor 2^8 in the product for dV (they are at most 1, and
 // in long rows most lie under 2^-14, where f16 has fewer bits), taken back at
@@ -84,9 +89,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
-  const int head = w / a.tiles, tile = a.tiles - 1 - (w - head * a.tiles);
-  int b, row0;
-  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, row0)) return;
+  const int head = w / a.tiles;
+  int b, index, n;
+  if (!find_tile(a.q_off, a.B, a.Tq, kBM, w - head * a.tiles, b, index, n)) return;
+  const int row0 = index * kBM;
   int qs, qe, ks, ke;
   seq_rows(a.q_off, b, a.Tq, qs, qe);
   seq_rows(a.k_off, b, a.Tk, ks, ke);
@@ -111,7 +117,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
     nl = lse == -INFINITY ? 0.0f : lse * kLog2e;
     if (lane < 32) {
       a.rows[at] = nl - kWeightLog2<DT>;
-      a.rows[(int64_t)a.heads * a.Tq + at] = delta;
+      a.rows[(int64_t)a.heads * a.Tq + at] = -delta;
     }
   }
 
@@ -146,6 +152,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
       for (int r = 0; r < 16; ++r)
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl)) * (dp[r] - delta);
       if (edge) {
+        keep_branch();
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (k0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[r] = 0.0f;
@@ -179,12 +186,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
                      lane);
 }
 
-// Keys [32 WK of them] x all query heads of the group and all their queries.
-// WK waves share the keys, 4 / WK the queries of a tile; the latter's sums
-// are added in wave order at the end.
-template <int DT, int DP, bool CAUSAL, int WK>
+// 128 keys, 32 to a wave, x the queries that see them in every query head of the
+// group: `total` tiles of 64 queries, or, where tiles of keys alone are too few
+// or too uneven for the chip, one of `splits` runs of them; the runs' sums
+// then go to scratch and attention_dkv_join_kernel adds them in order.
+//
+// At D = 128 the keys, the values and the two gradients of a wave's 32 keys
+// take 192 registers, so one wave runs per SIMD (two at D <= 64).  What then
+// bounds it is the issue of one wave: of 4400 cycles per tile of 64 queries
+// 2048 are the products, 2400 go by issuing instructions (counters).  Hence
+// few of them: masked tiles in a loop of their own, the heads' and tiles'
+// pointers advanced and not computed, dP's sum started from -delta.
+template <int DT, int DP, bool CAUSAL>
 __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_kernel(BwdArgs a) {
-  constexpr int WQ = kWaves / WK, kKeys = 32 * WK;
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
   __shared__ __attribute__((aligned(1024))) char sq0_[kTile];
   lds_char *const sq0 = (lds_char *)sq0_;
@@ -200,12 +214,14 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   lds_float *const sc1 = (lds_float *)sc1_;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wk = wave % WK, wq = wave / WK;
   const int kv_heads = a.heads / a.group;
-  const int w = xcd_run(blockIdx.x, a.tiles * kv_heads);
-  const int kh = w / a.tiles, tile = w - kh * a.tiles;
-  int b, row0;
-  if (!find_tile(a.k_off, a.B, a.Tk, kKeys, tile, b, row0)) return;
+  const int unit = xcd_run(blockIdx.x, a.tiles * kv_heads * a.splits);
+  const int w = unit / a.splits, split = unit - w * a.splits;  // (key head, tile)
+  const int kh = w / a.tiles;
+  int b, index, n;
+  if (!find_tile(a.k_off, a.B, a.Tk, kBM, w - kh * a.tiles, b, index, n)) return;
+  // Causal: the first keys have the most queries.
+  const int row0 = (n - 1 - index) * kBM;
   int qs, qe, ks, ke;
   seq_rows(a.q_off, b, a.Tq, qs, qe);
   seq_rows(a.k_off, b, a.Tk, ks, ke);
@@ -213,11 +229,18 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   // Causal: key j is seen by the queries j - shift and on.
   const int first = CAUSAL ? min(Lq, max(0, row0 - shift)) : 0;
   const int nt = (Lq - first + kBN - 1) / kBN, total = nt * a.group;
+  // The first `nm` of a head's tiles of queries hold some that do not see all of
+  // the keys.  Every head's come first, the others behind them, in a loop of
+  // its own without masks.
+  const int nm = CAUSAL ? min(nt, max(0, (row0 + kBM - shift - first + kBN - 2) / kBN)) : 0;
+  const int masked = nm * a.group;
+  const int from = (int)((int64_t)total * split / a.splits);
+  const int to = (int)((int64_t)total * (split + 1) / a.splits);
 
-  const int k0 = row0 + 32 * wk, kn = min(32, Lk - k0);
+  const int k0 = row0 + 32 * wave, kn = min(32, Lk - k0);
   u32x4 kf[DP / 16], vf[DP / 16];
-  load_cols<DP>(kf, a.k + (ks + k0) * a.sk.t + kh * a.sk.h, a.sk.t, kn, a.D, lane);
-  load_cols<DP>(vf, a.v + (ks + k0) * a.sv.t + kh * a.sv.h, a.sv.t, kn, a.D, lane);
+  load_cols<DP>(kf, a.k + (int64_t)(ks + k0) * a.sk.t + kh * a.sk.h, a.sk.t, kn, a.D, lane);
+  load_cols<DP>(vf, a.v + (int64_t)(ks + k0) * a.sv.t + kh * a.sv.h, a.sv.t, kn, a.D, lane);
   TileLoad<kBN, CH, kWaves> lq, lg;
   lq.init(a.sq.t, a.D);
   lg.init(a.sgo.t, a.D);
@@ -225,111 +248,152 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
 
-  auto fetch = [&](int u, lds_char *sq, lds_char *sg, lds_float *sc) __attribute__((always_inline)) {
-    const int g = u / nt, q0 = first + (u - g * nt) * kBN, head = kh * a.group + g;
-    const int n = Lq - q0;
-    lq.load(a.q + (int64_t)(qs + q0) * a.sq.t + head * a.sq.h, a.sq.t, n, a.D, sq);
-    lg.load(a.go + (int64_t)(qs + q0) * a.sgo.t + head * a.sgo.h, a.sgo.t, n, a.D, sg);
-    // Rows behind the sequence read zero: with q and dO zero there too, they
-    // add nothing.
-    if (wave < 2) {
-      const float *p = a.rows + ((int64_t)wave * a.heads + head) * a.Tq + qs + q0;
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<float *>(p), (short)0, min(n, kBN) * 4, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(sc + kBN * wave), 4, lane * 4, 0, 0,
-                                               0);
-    }
-  };
-  auto step = [&](int u, const lds_char *sq, const lds_char *sg, const lds_float *sc)
-      __attribute__((always_inline)) {
-    const int q0 = first + (u % nt) * kBN;
-    if (kn <= 0) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (i % WQ != wq) continue;
-      if (CAUSAL && q0 + 32 * i + 31 + shift < k0) continue;  // no query of these sees these keys
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        s = mfma_32x32x16<DT>(read_row_frag(sq, row_frag<CH>(32 * i, kk, lane)), kf[kk], s);
-        dp = mfma_32x32x16<DT>(read_row_frag(sg, row_frag<CH>(32 * i, kk, lane)), vf[kk], dp);
+  // Tiles [lo, hi) of the part of each head's tiles [j0, j1).
+  auto run = [&](auto mask, int lo, int hi, int j0, int j1) __attribute__((always_inline)) {
+    constexpr bool kMask = decltype(mask)::value;
+    if (lo >= hi) return;
+    // The next tile to fetch, and (masked) the next to compute: head of the
+    // group and tile.
+    int fg = lo / (j1 - j0), fj = j0 + lo - fg * (j1 - j0), cj = fj;
+    auto fetch = [&](lds_char *sq, lds_char *sg, lds_float *sc) __attribute__((always_inline)) {
+      const int q0 = first + fj * kBN, head = kh * a.group + fg, left = Lq - q0;
+      lq.load(a.q + (int64_t)(qs + q0) * a.sq.t + head * a.sq.h, a.sq.t, left, a.D, sq);
+      lg.load(a.go + (int64_t)(qs + q0) * a.sgo.t + head * a.sgo.h, a.sgo.t, left, a.D, sg);
+      // Rows behind the sequence read zero: with q and dO zero there too, they
+      // add nothing.
+      if (wave < 2) {
+        const float *p = a.rows + ((int64_t)wave * a.heads + head) * a.Tq + qs + q0;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<float *>(p), (short)0, min(left, kBN) * 4, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(sc + kBN * wave), 4, lane * 4, 0,
+                                                 0, 0);
       }
+      if (++fj == j1) {
+        fj = j0;
+        ++fg;
+      }
+    };
+    auto step = [&](const lds_char *sq, const lds_char *sg, const lds_float *sc)
+        __attribute__((always_inline)) {
       constexpr float kDown = DT == NOVA_HIP_DT_F16 ? 1.0f / 256.0f : 1.0f;
+      const int q0 = first + cj * kBN;
+      if (kMask && ++cj == j1) cj = j0;
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        const int row = 32 * i + 8 * r4 + 4 * (lane >> 5);
-        const gemm::f32x4 nl = *(lds_f32x4 *)(sc + row);
-        const gemm::f32x4 de = *(lds_f32x4 *)(sc + kBN + row);
+      for (int i = 0; i < 2; ++i) {
+        if (kMask && q0 + 32 * i + 31 + shift < k0) continue;  // none of these sees these keys
+        if (i) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_iglp_opt(0);  // a product, an LDS read, a product, ...
+        f32x16 s = {}, dp;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * r4 + e;
-          s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl[e]));
-          dp[r] = s[r] * ((dp[r] - de[e]) * kDown);
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const gemm::f32x4 de = *(lds_f32x4 *)(sc + kBN + 32 * i + 8 * r4 + 4 * (lane >> 5));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[4 * r4 + e] = de[e];
+        }
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          s = mfma_32x32x16<DT>(read_row_frag(sq, row_frag<CH>(32 * i, kk, lane)), kf[kk], s);
+          dp = mfma_32x32x16<DT>(read_row_frag(sg, row_frag<CH>(32 * i, kk, lane)), vf[kk], dp);
+        }
+        // Rows of this block from which on the lane's key is seen.
+        const int seen = kMask ? k0 + (lane & 31) - shift - q0 - 32 * i - 4 * (lane >> 5) : 0;
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const gemm::f32x4 nl = *(lds_f32x4 *)(sc + 32 * i + 8 * r4 + 4 * (lane >> 5));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * r4 + e;
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl[e]));
+            dp[r] = s[r] * (DT == NOVA_HIP_DT_F16 ? dp[r] * kDown : dp[r]);
+            if constexpr (kMask)
+              if (8 * (r >> 2) + (r & 3) < seen) s[r] = dp[r] = 0.0f;
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          // Weights and dS round to the operands' type for these products.
+          const u32x4 pf = pack_frag<DT>(s, kk), sf = pack_frag<DT>(dp, kk);
+#pragma unroll
+          for (int db = 0; db < DP / 32; ++db) {
+            dv[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sg, 32 * i + 16 * kk, 32 * db, lane), pf,
+                                       dv[db]);
+            dk[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sq, 32 * i + 16 * kk, 32 * db, lane), sf,
+                                       dk[db]);
+          }
         }
       }
-      if (CAUSAL && q0 + 32 * i + shift < k0 + 31) {
-        const int from = k0 + (lane & 31) - shift - q0 - 32 * i - 4 * (lane >> 5);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (8 * (r >> 2) + (r & 3) < from) s[r] = dp[r] = 0.0f;
-      }
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        // Weights and dS round to the operands' type for these products.
-        const u32x4 pf = pack_frag<DT>(s, kk), sf = pack_frag<DT>(dp, kk);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-          dv[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sg, 32 * i + 16 * kk, 32 * db, lane), pf,
-                                     dv[db]);
-          dk[db] = mfma_32x32x16<DT>(read_col_frag<CH>(sq, 32 * i + 16 * kk, 32 * db, lane), sf,
-                                     dk[db]);
-        }
-      }
-    }
-  };
-  auto sync = [&]() __attribute__((always_inline)) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-    __syncthreads();
-  };
-  if (total > 0) fetch(0, sq0, sg0, sc0);
-  for (int u = 0; u < total; u += 2) {
-    sync();
-    if (u + 1 < total) fetch(u + 1, sq1, sg1, sc1);
-    step(u, sq0, sg0, sc0);
-    if (u + 1 >= total) break;
-    sync();
-    if (u + 2 < total) fetch(u + 2, sq0, sg0, sc0);
-    step(u + 1, sq1, sg1, sc1);
-  }
-  if constexpr (WQ == 2) {
-    // The second wave of each key block hands its sums over through LDS, 32
-    // columns of d at a time (one 32 x 32 block of f32 per pair of waves).
-    lds_float *box = (lds_float *)(wk ? sq1 : sq0);
-    static_assert(WK == 2 && kTile >= 64 * 16 * 4, "one block per box");
-#pragma unroll
-    for (int j = 0; j < 2 * (DP / 32); ++j) {
-      f32x16 &x = j < DP / 32 ? dk[j % (DP / 32)] : dv[j % (DP / 32)];
+    };
+    auto sync = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
-      if (wq == 1) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) box[64 * r + lane] = x[r];
-      }
-      __syncthreads();
-      if (wq == 0) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] += box[64 * r + lane];
-      }
+    };
+    fetch(sq0, sg0, sc0);
+    for (int u = lo; u < hi; u += 2) {
+      sync();
+      if (u + 1 < hi) fetch(sq1, sg1, sc1);
+      step(sq0, sg0, sc0);
+      if (u + 1 >= hi) break;
+      sync();
+      if (u + 2 < hi) fetch(sq0, sg0, sc0);
+      step(sq1, sg1, sc1);
     }
-    if (wq == 1) return;
-  }
+    __syncthreads();  // stage 0 has no reader left
+  };
+  if constexpr (CAUSAL) run(std::true_type(), from, min(to, masked), 0, nm);
+  run(std::false_type(), max(from - masked, 0), to - masked, nm, nt);
   if (kn <= 0) return;
-  store_rows<DT, DP>(dk, a.scale, a.dk + (ks + k0) * a.sdk.t + kh * a.sdk.h, a.sdk.t, kn, a.D,
-                     lane);
+  if (a.splits > 1) {
+    float *p = a.partial + ((int64_t)unit * kWaves + wave) * kPartial<DP> + lane;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[(16 * i + r) * 64] = dk[i][r];
+        p[(DP / 2 + 16 * i + r) * 64] = dv[i][r];
+      }
+    return;
+  }
+  store_rows<DT, DP>(dk, a.scale, a.dk + (int64_t)(ks + k0) * a.sdk.t + kh * a.sdk.h, a.sdk.t, kn,
+                     a.D, lane);
   store_rows<DT, DP>(dv, DT == NOVA_HIP_DT_F16 ? 1.0f / 256.0f : 1.0f,
-                     a.dv + (ks + k0) * a.sdv.t + kh * a.sdv.h, a.sdv.t, kn, a.D, lane);
+                     a.dv + (int64_t)(ks + k0) * a.sdv.t + kh * a.sdv.h, a.sdv.t, kn, a.D, lane);
 }
 
-constexpr int kWK = 4;  // key blocks of a workgroup
+// The sums of a tile of keys from those of its splits, in split order.
+template <int DT, int DP>
+__global__ __launch_bounds__(64 * kWaves) void attention_dkv_join_kernel(BwdArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = blockIdx.x, kh = w / a.tiles;
+  int b, index, n, ks, ke;
+  if (!find_tile(a.k_off, a.B, a.Tk, kBM, w - kh * a.tiles, b, index, n)) return;
+  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  const int k0 = (n - 1 - index) * kBM + 32 * wave, kn = min(32, ke - ks - k0);
+  if (kn <= 0) return;
+  f32x16 x[DP / 32];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const float *p = a.partial + ((int64_t)w * a.splits * kWaves + wave) * kPartial<DP> +
+                     half * (DP / 2 * 64) + lane;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[i][r] = p[(16 * i + r) * 64];
+    for (int s = 1; s < a.splits; ++s) {
+      p += (int64_t)kWaves * kPartial<DP>;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[i][r] += p[(16 * i + r) * 64];
+    }
+    if (half == 0)
+      store_rows<DT, DP>(x, a.scale, a.dk + (ks + k0) * a.sdk.t + kh * a.sdk.h, a.sdk.t, kn, a.D,
+                         lane);
+    else
+      store_rows<DT, DP>(x, DT == NOVA_HIP_DT_F16 ? 1.0f / 256.0f : 1.0f,
+                         a.dv + (ks + k0) * a.sdv.t + kh * a.sdv.h, a.sdv.t, kn, a.D, lane);
+  }
+}
 
 template <int DT, int DP, bool CAUSAL>
 int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s) {
@@ -342,8 +406,14 @@ int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s)
   }
   if (k_tiles > 0) {
     a.tiles = (int)k_tiles;
-    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL, kWK>),
-                       dim3((unsigned)(k_tiles * (a.heads / a.group))), dim3(64 * kWaves), 0, s, a);
+    const unsigned grid = (unsigned)(k_tiles * (a.heads / a.group));
+    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL>), dim3(grid * a.splits),
+                       dim3(64 * kWaves), 0, s, a);
+    if (a.splits > 1) {
+      const int32_t rc = check_hip(hipGetLastError(), "attention_backward launch");
+      if (rc) return rc;
+      hipLaunchKernelGGL((attention_dkv_join_kernel<DT, DP>), dim3(grid), dim3(64 * kWaves), 0, s, a);
+    }
   }
   return check_hip(hipGetLastError(), "attention_backward launch");
 }
@@ -362,6 +432,37 @@ int32_t launch_bwd(const BwdArgs &a, bool causal, int64_t qt, int64_t kt, hipStr
 }  // namespace
 }  // namespace attn
 
+namespace {
+int64_t padded_dim(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+// Tiles of BM rows: whole ones and, for each sequence, at most one that is not.
+int64_t tile_bound(int64_t T, int64_t B) { return std::min(T, T / attn::kBM + B); }
+
+// Runs of queries that a tile of keys is split into: as many as fill the chip
+// (256 workgroups at once, 512 at D <= 64), with four tiles of queries to a run
+// at least, by the mean length; and two for causal sequences of four rounds or
+// fewer, whose first tiles take twice the mean, where the products (of mean
+// length x group queries per key) outweigh writing and reading the sums.
+// Measured without / with two: packed causal sequences of 1 to 4096 tokens, 32
+// heads in groups of four of 128, 506 / 446 + 35 us; 8 x 1024 of 6 heads of 64
+// 36.8 / 33.5 + 14.5.
+int64_t dkv_splits(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
+                   bool causal) {
+  if (B == 0 || kv_heads == 0 || Tk == 0) return 1;
+  const int64_t units = tile_bound(Tk, B) * kv_heads, slots = D <= 64 ? 512 : 256;
+  const int64_t group = heads / kv_heads, queries = Tq / B * group;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(8, queries / (4 * attn::kBN)));
+  if (units < slots) return std::min(most, slots / units);
+  return causal && units < 4 * slots && queries >= 2048 ? 2 : 1;
+}
+}  // namespace
+
+int64_t attention_backward_scratch(int64_t Tq, int64_t Tk, int64_t B, int64_t heads,
+                                   int64_t kv_heads, int64_t D, bool causal) {
+  const int64_t rows = 2 * heads * Tq, splits = dkv_splits(Tq, Tk, B, heads, kv_heads, D, causal);
+  if (splits <= 1) return rows;
+  return rows + tile_bound(Tk, B) * kv_heads * splits * attn::kWaves * 64 * padded_dim(D);
+}
+
 int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t s) {
   if (p.f.heads == 0 || p.f.D == 0 || p.f.B == 0) return NOVA_HIP_SUCCESS;
   attn::BwdArgs a;
@@ -375,7 +476,8 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   a.dv = static_cast<uint16_t *>(p.dv.p);
   a.lse = p.f.lse;
   a.slse = p.f.slse;
-  a.rows = p.rows;
+  a.rows = p.scratch;
+  a.partial = p.scratch + 2 * p.f.heads * p.f.Tq;
   a.q_off = p.f.q_off;
   a.k_off = p.f.k_off;
   a.sq = {p.f.q.st, p.f.q.sh};
@@ -395,10 +497,9 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   a.tiles = 0;
   a.c = p.f.scale * attn::kLog2e;
   a.scale = p.f.scale;
-  // Whole tiles and, for each sequence, at most one that is not.
-  const int64_t qt = std::min(p.f.Tq, p.f.Tq / attn::kBM + p.f.B);
-  const int64_t kt = std::min(p.f.Tk, p.f.Tk / (32 * attn::kWK) + p.f.B);
-  if (std::max(qt * p.f.heads, kt * p.f.kv_heads) > 0x7fffffff)
+  a.splits = (int)dkv_splits(p.f.Tq, p.f.Tk, p.f.B, p.f.heads, p.f.kv_heads, p.f.D, p.f.causal);
+  const int64_t qt = tile_bound(p.f.Tq, p.f.B), kt = tile_bound(p.f.Tk, p.f.B);
+  if (std::max(qt * p.f.heads, kt * p.f.kv_heads * a.splits) > 0x7fffffff)
     return fail(NOVA_HIP_ERANGE, "attention_backward: more than 2^31 - 1 tiles");
   return p.f.dt == NOVA_HIP_DT_BF16
              ? attn::launch_bwd<NOVA_HIP_DT_BF16>(a, p.f.causal, qt, kt, s)

@@ -102,6 +102,7 @@ __global__ __launch_bounds__(64) void attention_decode_kernel(DecodeArgs a) {
     for (int kk = 0; kk < DP / 16; ++kk)
       s = mfma_32x32x16<DT>(read_row_frag(sk, row_frag<CH>(0, kk, lane)), qf[kk], s);
     if (k0 + kBN > to) {
+      keep_branch();
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= to) s[r] = -INFINITY;

@@ -872,7 +872,7 @@ int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D
 
 // ---- attention --------------------------------------------------------------------
 namespace {
-constexpr int64_t kAttnMaxStride = 1 << 24;  // elements; 64 rows stay below 2^31 bytes
+constexpr int64_t kAttnMaxStride = 1 << 23;  // elements; 128 rows stay below 2^31 bytes
 
 // One operand [T, heads, D]: unit stride on D, rows of whole 16-byte chunks at
 // 16-byte aligned addresses.  A dim of extent 1 may have any stride: it gets
@@ -900,7 +900,7 @@ int32_t attn_operand(const NovaMemRef3D *d, const char *w, const char *what, boo
   if (o.st % 8 || o.sh % 8 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
     return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s must start at 16-byte aligned addresses", w, what);
   if (o.st > kAttnMaxStride)
-    return fail(NOVA_HIP_ERANGE, "%s: token stride of %s exceeds 2^24 elements", w, what);
+    return fail(NOVA_HIP_ERANGE, "%s: token stride of %s exceeds 2^23 elements", w, what);
   if (out && H > 1) {
     const bool apart = o.sh >= D && (T <= 1 || (o.st <= o.sh ? o.sh >= (T - 1) * o.st + D
                                                              : o.st >= (H - 1) * o.sh + D));
@@ -990,6 +990,16 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
   return launch_attention(p, current_stream());
 }
 
+int64_t nova_hip_attention_backward_scratch(int64_t q_tokens, int64_t k_tokens, int64_t sequences,
+                                            int64_t heads, int64_t kv_heads, int64_t D,
+                                            int32_t causal) {
+  if (q_tokens < 0 || k_tokens < 0 || sequences < 0 || heads <= 0 || kv_heads <= 0 || D <= 0 ||
+      q_tokens > 0x7fffffff || k_tokens > 0x7fffffff || sequences > (1 << 24) || heads > 0xffff ||
+      kv_heads > heads || D > 128)
+    return 0;  // the call itself refuses these, or has nothing to do
+  return attention_backward_scratch(q_tokens, k_tokens, sequences, heads, kv_heads, D, causal != 0);
+}
+
 int32_t _mlir_ciface_nova_hip_attention_backward(
     const NovaMemRef3D *grad_out, const NovaMemRef3D *q, const NovaMemRef3D *k,
     const NovaMemRef3D *v, const NovaMemRef3D *out, const NovaMemRef2D *lse,
@@ -1010,10 +1020,12 @@ int32_t _mlir_ciface_nova_hip_attention_backward(
     return rc;
   if (!scratch) return fail(NOVA_HIP_EINVAL, "%s: null scratch descriptor", w);
   if ((rc = dense1(scratch, w, "scratch"))) return rc;
-  if (scratch->sizes[0] < 2 * p.f.heads * p.f.Tq)
-    return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, 2 heads tokens = %lld are needed", w,
-                (long long)scratch->sizes[0], (long long)(2 * p.f.heads * p.f.Tq));
-  p.rows = out_f32(scratch);
+  const int64_t need = nova_hip_attention_backward_scratch(p.f.Tq, p.f.Tk, p.f.B, p.f.heads,
+                                                           p.f.kv_heads, p.f.D, causal);
+  if (scratch->sizes[0] < need)
+    return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, %lld are needed", w,
+                (long long)scratch->sizes[0], (long long)need);
+  p.scratch = out_f32(scratch);
   return launch_attention_backward(p, current_stream());
 }
 
@@ -1107,7 +1119,7 @@ int32_t _mlir_ciface_nova_hip_attention_decode(const NovaMemRef3D *q, const Nova
                    reinterpret_cast<uintptr_t>(p.v) | reinterpret_cast<uintptr_t>(p.o)) & 15u))
     return fail(NOVA_HIP_ESTRIDE, "%s: rows must start at 16-byte aligned addresses", w);
   if (p.sqh > kAttnMaxStride || p.skt > kAttnMaxStride || p.svt > kAttnMaxStride)
-    return fail(NOVA_HIP_ERANGE, "%s: a row stride exceeds 2^24 elements", w);
+    return fail(NOVA_HIP_ERANGE, "%s: a row stride exceeds 2^23 elements", w);
   p.lens = reinterpret_cast<const int32_t *>(data_of(lengths)) + lengths->offset;
   p.lse = nullptr;
   p.slse = 0;

@@ -143,8 +143,10 @@ int32_t launch_attention(const AttentionProblem &p, hipStream_t s);
 struct AttentionBackwardProblem {
   AttentionProblem f;  // the forward's operands, result and lse
   AttentionOperand go, dq, dk, dv;
-  float *rows;  // scratch, [2][heads][Tq]
+  float *scratch;  // of attention_backward_scratch() floats
 };
+int64_t attention_backward_scratch(int64_t Tq, int64_t Tk, int64_t B, int64_t heads,
+                                   int64_t kv_heads, int64_t D, bool causal);
 int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t s);
 
 struct AttentionDecodeProblem {

@@ -68,6 +68,7 @@ EXPORTS = (
     "_mlir_ciface_nova_hip_attention",
     "_mlir_ciface_nova_hip_attention_backward",
     "_mlir_ciface_nova_hip_attention_decode",
+    "nova_hip_attention_backward_scratch",
     "nova_hip_attention_decode_scratch",
     "_mlir_ciface_nova_hip_token_logp",
     "_mlir_ciface_nova_hip_policy_loss",
@@ -171,6 +172,8 @@ def lib() -> ctypes.CDLL:
     L._mlir_ciface_nova_hip_attention.argtypes = [P] * 7 + [F, I, I]
     L._mlir_ciface_nova_hip_attention_backward.argtypes = [P] * 12 + [F, I, I]
     L._mlir_ciface_nova_hip_attention_decode.argtypes = [P] * 7 + [F, I]
+    L.nova_hip_attention_backward_scratch.argtypes = [ctypes.c_int64] * 6 + [I]
+    L.nova_hip_attention_backward_scratch.restype = ctypes.c_int64
     L.nova_hip_attention_decode_scratch.argtypes = [ctypes.c_int64] * 5
     L.nova_hip_attention_decode_scratch.restype = ctypes.c_int64
     L._mlir_ciface_nova_hip_token_logp.argtypes = [P] * 4 + [I]
@@ -654,7 +657,9 @@ def attention_backward(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, cau
         dk = k.new_empty(tuple(k.shape))
     if dv is None:
         dv = k.new_empty(tuple(k.shape))
-    scratch = q.new_empty(2 * H * T, dtype=f32)
+    need = lib().nova_hip_attention_backward_scratch(T, k.shape[0], max(q_offsets.numel() - 1, 0), H,
+                                                     k.shape[1], D, 1 if causal else 0)
+    scratch = q.new_empty(need, dtype=f32)
     _launch("_mlir_ciface_nova_hip_attention_backward",
             (q, grad_out, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv),
             _desc(grad_out, 3, "grad_out"), desc_q, desc_k, _desc(v, 3, "v"), _desc(out, 3, "out"),
