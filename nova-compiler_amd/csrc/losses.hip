@@ -27,7 +27,8 @@ using gemm::u32x4;
 
 constexpr float kL2e = 1.4426950408889634f;
 
-enum Mode { kLogp, kPolicy };
+// kPairs: kLogp ahead of a second pass over the logits.
+enum Mode { kLogp, kPairs, kPolicy };
 
 struct RowArgs {
   const void *logits;
@@ -54,6 +55,13 @@ struct Chunk {
     if constexpr (DT == NOVA_HIP_DT_F32)
       return __builtin_nontemporal_load(reinterpret_cast<const u32x4_at4 *>(p));
     else return __builtin_nontemporal_load(reinterpret_cast<const u32x4_at2 *>(p));
+  }
+  // With KEEP the line stays in the caches for a second pass.
+  template <bool KEEP>
+  static __device__ __forceinline__ u32x4 load_as(const T *p) {
+    if constexpr (!KEEP) return load(p);
+    else if constexpr (DT == NOVA_HIP_DT_F32) return *reinterpret_cast<const u32x4_at4 *>(p);
+    else return *reinterpret_cast<const u32x4_at2 *>(p);
   }
   static __device__ __forceinline__ void store(T *p, u32x4 v) {
     if constexpr (DT == NOVA_HIP_DT_F32)
@@ -147,7 +155,7 @@ __device__ __forceinline__ void policy_row(const RowArgs &a, int row, float lp, 
 
 // TH threads per row, NC chunks per thread; TH == 64: four rows a workgroup.
 template <int DT, int TH, int NC, int MODE>
-__global__ __launch_bounds__(TH == 64 ? 256 : TH, TH == 512 ? 4 : 1) void logp_row_kernel(RowArgs a) {
+__global__ __launch_bounds__(TH == 64 ? 256 : TH, TH >= 512 ? 4 : 1) void logp_row_kernel(RowArgs a) {
   typedef Chunk<DT> X;
   typedef typename X::T T;
   __shared__ float red[TH > 64 ? TH / 64 : 1];
@@ -177,7 +185,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH == 512 ? 4 : 1) void logp_r
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = tid + TH * i;
-    v[i] = c < nc ? X::load(x + c * X::kE) : X::none();  // -inf: no part of the sum
+    v[i] = c < nc ? X::template load_as<MODE == kPairs>(x + c * X::kE) : X::none();  // -inf: no part of the sum
   }
   float xt = -INFINITY;  // this thread's value behind the last chunk
   if (tid < tail) xt = X::widen(x[nc * X::kE + tid]);
@@ -203,7 +211,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH == 512 ? 4 : 1) void logp_r
   s = group_reduce<TH, false>(s, red);
   const float ls = logf(s), lse = mm + ls;
   const float lp = (xy - mm) - ls;
-  if constexpr (MODE == kLogp) {
+  if constexpr (MODE != kPolicy) {
     if (tid == 0) {
       if (a.logp) a.logp[row] = lp;
       if (a.lse) a.lse[row] = lse;
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
   if (xt != xt) s = xt;
 #pragma unroll 4
   for (int c = tid; c < nc; c += TH) {
-    const u32x4 v = X::load(x + (int64_t)c * X::kE);
+    const u32x4 v = X::template load_as<MODE != kLogp>(x + (int64_t)c * X::kE);
     float t = X::at(v, 0);
 #pragma unroll
     for (int e = 1; e < X::kE; ++e) t = fmaxf(t, X::at(v, e));
@@ -286,7 +294,7 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
   s = group_reduce<TH, false>(s, red);
   const float ls = logf(s), lse = mm + ls;
   const float lp = (xy - mm) - ls;
-  if constexpr (MODE == kLogp) {
+  if constexpr (MODE != kPolicy) {
     if (tid == 0) {
       if (a.logp) a.logp[row] = lp;
       if (a.lse) a.lse[row] = lse;
@@ -319,19 +327,23 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
   }
 }
 
-// out[0] = sum of v[0 .. n) * scale, in 64 bits: each thread its own stride,
-// then the threads in order of a fixed tree.
-__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *v, int n, double scale,
-                                                        float *out) {
-  __shared__ double part[1024];
+// out[0] = sum of v[0 .. n) * scale by TH threads, in 64 bits: each its own
+// stride, then the threads in the order of a fixed tree.
+template <int TH>
+__device__ __forceinline__ void sum_losses(const float *v, int n, double scale, float *out) {
+  __shared__ double part[TH];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) s += (double)v[i];
+  for (int i = threadIdx.x; i < n; i += TH) s += (double)v[i];
   part[threadIdx.x] = s;
-  for (int d = 512; d > 0; d >>= 1) {
+  for (int d = TH / 2; d > 0; d >>= 1) {
     __syncthreads();
     if (threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
   }
   if (threadIdx.x == 0) out[0] = (float)(part[0] * scale);
+}
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float *v, int n, double scale,
+                                                        float *out) {
+  sum_losses<1024>(v, n, scale, out);
 }
 
 struct PairArgs {
@@ -386,15 +398,21 @@ struct GradArgs {
   const int32_t *labels;
   const float *lse, *slope;
   int64_t sx, sg;
-  int rows, C;
+  int rows, C, pairs;
+  const float *pair_loss;
+  float *loss;
 };
 
-// grad[row] = slope (onehot(label) - exp(x - lse)).
+// grad[row] = slope (onehot(label) - exp(x - lse)), from the last row to the
+// first.  The first workgroup also sums the pairs' losses (a launch of its own
+// would take longer than a small call's other kernels).
 template <int DT, int TH>
 __global__ __launch_bounds__(TH == 64 ? 256 : TH) void logits_grad_kernel(GradArgs a) {
   typedef Chunk<DT> X;
   typedef typename X::T T;
   const int tid = TH == 64 ? threadIdx.x & 63 : threadIdx.x;
+  if (blockIdx.x == 0)
+    sum_losses<TH == 64 ? 256 : TH>(a.pair_loss, a.pairs, 1.0 / (double)a.pairs, a.loss);
   const int r = TH == 64 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (r >= a.rows) return;
   const int row = a.rows - 1 - r;
@@ -412,7 +430,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH) void logits_grad_kernel(GradAr
   for (int c = tid; c < nc; c += TH) {
     u32x4 o = {0, 0, 0, 0};
     if (!none) {
-      const u32x4 v = X::load(x + (int64_t)c * X::kE);
+      const u32x4 v = X::template load_as<true>(x + (int64_t)c * X::kE);
       o = X::make([&](int e) { return value(X::at(v, e), (int64_t)c * X::kE + e); });
     }
     X::store(g + (int64_t)c * X::kE, o);
@@ -434,13 +452,19 @@ void launch_rows_t(const RowArgs &a, hipStream_t s) {
   };
   using std::integral_constant;
 #define NOVA_ROWS(TH, NC) go(integral_constant<int, TH>(), integral_constant<int, NC>())
+  // With a gradient to write, few wide workgroups per CU serve HBM better (1024
+  // threads at 8192 x 50304 f32, 8192 x 50304 bf16, 4096 x 32000 f32: 526, 270
+  // and 172 us; 512 threads: 554, 278 and 178); to read alone, narrower ones
+  // (8192 x 50304 bf16 97 us, 105 with 1024; 4096 x 32000 bf16 29 and 36).
   if (chunks <= 64 * 4) NOVA_ROWS(64, 4);
   else if (chunks <= 256 * 4) NOVA_ROWS(256, 4);
-  else if (chunks <= 256 * 8) NOVA_ROWS(256, 8);
+  else if (chunks <= 512 * 4) NOVA_ROWS(512, 4);
   else if (chunks <= 512 * 8) NOVA_ROWS(512, 8);
-  else if (chunks <= 512 * 13) NOVA_ROWS(512, 13);
-  else if (chunks <= 512 * 16) NOVA_ROWS(512, 16);
-  else if (chunks <= 512 * 25) NOVA_ROWS(512, 25);
+  else if (chunks <= 1024 * 8) {
+    if constexpr (MODE == kPolicy) NOVA_ROWS(1024, 8);
+    else if (chunks <= 512 * 13) NOVA_ROWS(512, 13);
+    else NOVA_ROWS(512, 16);
+  } else if (chunks <= 1024 * 13) NOVA_ROWS(1024, 13);
   else hipLaunchKernelGGL((logp_long_kernel<DT, MODE>), dim3(g), dim3(512), 0, s, a);
 #undef NOVA_ROWS
 }
@@ -523,17 +547,19 @@ int32_t launch_preference_loss(const PreferenceProblem &p, hipStream_t s) {
   a.logp = p.logp;
   a.lse = p.lse;
   a.slope = p.slope;
-  if (p.t.rows > 0 && (rc = launch_rows<kLogp>(a, p.t.dt, "preference_loss launch", s))) return rc;
+  const bool grad = p.t.grad && p.t.rows > 0;
+  if (p.t.rows > 0 && (rc = grad ? launch_rows<kPairs>(a, p.t.dt, "preference_loss launch", s)
+                                 : launch_rows<kLogp>(a, p.t.dt, "preference_loss launch", s)))
+    return rc;
   const PairArgs b = {p.logp, p.slope, p.offsets, p.ref_logp, p.seq_logp, p.pair_loss,
                       (int)p.t.rows, (int)p.pairs, p.beta, p.smoothing, p.grad_scale};
   hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)p.pairs), dim3(256), 0, s, b);
-  if ((rc = check_hip(hipGetLastError(), "preference_loss pair launch")) ||
-      (rc = launch_loss_sum(p.pair_loss, p.pairs, 1.0 / (double)p.pairs, p.loss,
-                            "preference_loss sum launch", s)))
-    return rc;
-  if (!p.t.grad || p.t.rows == 0) return NOVA_HIP_SUCCESS;
+  if ((rc = check_hip(hipGetLastError(), "preference_loss pair launch"))) return rc;
+  if (!grad)
+    return launch_loss_sum(p.pair_loss, p.pairs, 1.0 / (double)p.pairs, p.loss,
+                           "preference_loss sum launch", s);
   const GradArgs g = {p.t.logits, p.t.grad, p.t.labels, p.lse, p.slope, p.t.sx, p.t.sg,
-                      (int)p.t.rows, (int)p.t.C};
+                      (int)p.t.rows, (int)p.t.C, (int)p.pairs, p.pair_loss, p.loss};
   if (p.t.dt == NOVA_HIP_DT_F32) launch_grad_t<NOVA_HIP_DT_F32>(g, s);
   else if (p.t.dt == NOVA_HIP_DT_BF16) launch_grad_t<NOVA_HIP_DT_BF16>(g, s);
   else launch_grad_t<NOVA_HIP_DT_F16>(g, s);
