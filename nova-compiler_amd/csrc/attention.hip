@@ -31,14 +31,6 @@ struct FwdArgs {
 constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
 constexpr float kSlack = 8.0f;  // m c may lag the largest score by this much
 
-// Workgroup id -> (head, tile): the hardware deals ids to the 8 XCDs in turn;
-// each XCD takes one run of the head-major order, so the heads that share
-// keys and values share an L2.
-__device__ __forceinline__ int xcd_run(int id, int total) {
-  const int per = total >> 3, rem = total & 7, x = id & 7;
-  return x * per + min(x, rem) + (id >> 3);
-}
-
 template <int DT, int DP, bool CAUSAL>
 __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
@@ -52,10 +44,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
   lds_char *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
-  const int head = w / a.tiles;
+  int head, tile;
+  unit_of(blockIdx.x, a.heads, a.tiles, CAUSAL, head, tile);
   int b, index, n;
-  if (!find_tile(a.q_off, a.B, a.Tq, kBM, w - head * a.tiles, b, index, n)) return;
+  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, index, n)) return;
   const int row0 = index * kBM;
   int qs, qe, ks, ke;
   seq_rows(a.q_off, b, a.Tq, qs, qe);

@@ -48,11 +48,6 @@ constexpr int64_t kPartial = DP * 64;
 template <int DT>
 constexpr float kWeightLog2 = DT == NOVA_HIP_DT_F16 ? 8.0f : 0.0f;
 
-__device__ __forceinline__ int xcd_run(int id, int total) {
-  const int per = total >> 3, rem = total & 7, x = id & 7;
-  return x * per + min(x, rem) + (id >> 3);
-}
-
 // sum over d of a row's products, the row held as load_cols gives it.
 template <int DT, int DP>
 __device__ __forceinline__ float row_dot(const u32x4 (&x)[DP / 16], const u32x4 (&y)[DP / 16]) {
@@ -88,10 +83,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
   lds_char *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int w = xcd_run(blockIdx.x, a.tiles * a.heads);
-  const int head = w / a.tiles;
+  int head, tile;
+  unit_of(blockIdx.x, a.heads, a.tiles, CAUSAL, head, tile);
   int b, index, n;
-  if (!find_tile(a.q_off, a.B, a.Tq, kBM, w - head * a.tiles, b, index, n)) return;
+  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, index, n)) return;
   const int row0 = index * kBM;
   int qs, qe, ks, ke;
   seq_rows(a.q_off, b, a.Tq, qs, qe);
@@ -215,11 +210,12 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kv_heads = a.heads / a.group;
-  const int unit = xcd_run(blockIdx.x, a.tiles * kv_heads * a.splits);
-  const int w = unit / a.splits, split = unit - w * a.splits;  // (key head, tile)
-  const int kh = w / a.tiles;
+  int kh, tile;
+  unit_of(blockIdx.x, kv_heads, a.tiles * a.splits, CAUSAL, kh, tile);
+  const int split = tile % a.splits, unit = kh * a.tiles * a.splits + tile;
+  tile /= a.splits;
   int b, index, n;
-  if (!find_tile(a.k_off, a.B, a.Tk, kBM, w - kh * a.tiles, b, index, n)) return;
+  if (!find_tile(a.k_off, a.B, a.Tk, kBM, tile, b, index, n)) return;
   // Causal: the first keys have the most queries.
   const int row0 = (n - 1 - index) * kBM;
   int qs, qe, ks, ke;
