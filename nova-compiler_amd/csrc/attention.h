@@ -57,25 +57,29 @@ __device__ __forceinline__ int swz(int row) {
   else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// Workgroup id -> (head, tile).  The hardware deals ids to the 8 XCDs in turn,
-// and each XCD takes one run of the heads, so that the workgroups that read the
-// same keys share an L2.  Within a run heads follow one another, or, where
-// tiles differ in work (causal) and the runs are whole, all heads' largest tiles
-// come first: with heads in turn the last head's largest tiles start late and
-// run alone (forward, 32 heads of 128: 8192 tokens 566 -> 535 us, packed 1 to
-// 4096 tokens 235 -> 213; the heads' own keys, 570 -> 540, still fit).
+// Workgroup id -> (head, tile).  The hardware deals ids to the 8 XCDs in turn.
+// Equal tiles: each XCD takes one run of the heads' tiles, head after head, so
+// that the workgroups that read the same keys share an L2.  Tiles of falling
+// work (causal): every head's first tile, then every head's second, the heads
+// still divided over the XCDs where they divide evenly; with heads in turn the
+// last one's largest tiles start late and run alone.  Forward / backward, us,
+// heads in turn against this: 8192 tokens of 32 heads of 128 566 / 1817 against
+// 535 / 1786, of 12 heads 288 / 1096 against 228 / 712.
 __device__ __forceinline__ void unit_of(int id, int heads, int tiles, bool causal, int &head,
                                         int &tile) {
   const int x = id & 7, r = id >> 3;
-  if (causal && heads % 8 == 0) {
-    const int mine = heads >> 3;
-    tile = r / mine;
-    head = x * mine + r - tile * mine;
-  } else {
+  if (!causal) {
     const int total = heads * tiles, per = total >> 3, rem = total & 7;
     const int w = x * per + min(x, rem) + r;
     head = w / tiles;
     tile = w - head * tiles;
+  } else if (heads % 8 == 0) {
+    const int mine = heads >> 3;
+    tile = r / mine;
+    head = x * mine + r - tile * mine;
+  } else {
+    tile = id / heads;
+    head = id - tile * heads;
   }
 }
 
