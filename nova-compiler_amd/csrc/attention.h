@@ -94,25 +94,42 @@ __device__ __forceinline__ int wave_sum_int(int v) {
          (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
 }
 
+// A tile's place: its index among its sequence's tiles, their number, and the
+// sequence's rows in the operand that is tiled and in the other one.
+struct Tile {
+  int index, tiles, s, e, os, oe;
+};
+
 // Tile t of the sequences' tiles of BM rows, off[0 .. B] being the sequences'
-// first rows (whatever they hold, every sequence is cut to rows inside [0, T)),
-// in the order of falling index within the sequence: the last tiles of the
-// longest sequences first.  That is the order of falling work of causal
-// attention (or of rising index counted from the end, for keys), so that what
-// runs last is short.  Gives the sequence, the tile's index in it and the
-// sequence's tiles; false when t lies behind the last tile.
+// first rows and other[0 .. B] those of the other operand (whatever they hold,
+// every sequence is cut to rows inside [0, T) and [0, To)), in the order of
+// falling index within the sequence: the last tiles of the longest sequences
+// first.  That is the order of falling work of causal attention (or of rising
+// index counted from the end, for keys), so that what runs last is short.
+// False when t lies behind the last tile.
 // Wave-uniform; every wave searches for itself: with S(l) = sum over sequences
 // of max(0, tiles - l), the tiles of index l and above, it finds the largest
-// l with S(l) > t, bit by bit.
-__device__ __forceinline__ bool find_tile(const int *off, int B, int T, int BM, int t, int &seq,
-                                          int &index, int &tiles) {
+// l with S(l) > t, bit by bit.  The first 64 sequences' rows are loaded together
+// and stay in registers: a call of few sequences waits for one load.
+__device__ __forceinline__ bool find_tile(const int *off, const int *other, int B, int T, int To,
+                                          int BM, int t, Tile &tile) {
   const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](int b) __attribute__((always_inline)) {
-    if (b >= B) return 0;
-    const int s = min(max(off[b], 0), T), e = min(max(off[b + 1], 0), T);
-    return e > s ? (e - s + BM - 1) / BM : 0;
+  auto rows_of = [&](const int *o, int n, int b, int &s, int &e) __attribute__((always_inline)) {
+    s = e = 0;
+    if (b < B) {
+      s = min(max(o[b], 0), n);
+      e = max(s, min(max(o[b + 1], 0), n));
+    }
   };
-  const int n0 = tiles_of(lane);  // the first 64 sequences stay in registers
+  auto tiles_of = [&](int b) __attribute__((always_inline)) {
+    int s, e;
+    rows_of(off, T, b, s, e);
+    return (e - s + BM - 1) / BM;
+  };
+  int s0, e0, os0, oe0;
+  rows_of(off, T, lane, s0, e0);
+  rows_of(other, To, lane, os0, oe0);
+  const int n0 = (e0 - s0 + BM - 1) / BM;
   auto above = [&](int l) __attribute__((always_inline)) {
     int v = max(0, n0 - l);
     for (int b0 = 64; b0 < B; b0 += 64) v += max(0, tiles_of(b0 + lane) - l);
@@ -127,28 +144,28 @@ __device__ __forceinline__ bool find_tile(const int *off, int B, int T, int BM, 
     if (above(level + bit) > t) level += bit;
   int k = t - above(level + 1);  // among the sequences with a tile of that index
   for (int b0 = 0; b0 < B; b0 += 64) {
-    const int n = b0 ? tiles_of(b0 + lane) : n0;
+    if (b0) {
+      rows_of(off, T, b0 + lane, s0, e0);
+      rows_of(other, To, b0 + lane, os0, oe0);
+    }
+    const int n = (e0 - s0 + BM - 1) / BM;
     const uint64_t has = __ballot(n > level);
     const int count = __builtin_popcountll(has);
     if (k < count) {
       const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
       const int l = __builtin_ctzll(__ballot(n > level && rank == k));
-      seq = __builtin_amdgcn_readfirstlane(b0 + l);
-      index = __builtin_amdgcn_readfirstlane(level);
-      tiles = __builtin_amdgcn_readlane(n, l);
+      tile.index = __builtin_amdgcn_readfirstlane(level);
+      tile.tiles = __builtin_amdgcn_readlane(n, l);
+      tile.s = __builtin_amdgcn_readlane(s0, l);
+      tile.e = __builtin_amdgcn_readlane(e0, l);
+      tile.os = __builtin_amdgcn_readlane(os0, l);
+      tile.oe = __builtin_amdgcn_readlane(oe0, l);
       return true;
     }
     k -= count;
   }
   return false;
-}
-
-// Rows [s, e) of sequence b, cut to [0, T).
-__device__ __forceinline__ void seq_rows(const int *off, int b, int T, int &s, int &e) {
-  s = __builtin_amdgcn_readfirstlane(min(max(off[b], 0), T));
-  e = __builtin_amdgcn_readfirstlane(min(max(off[b + 1], 0), T));
-  if (e < s) e = s;
 }
 
 // Loads of one LDS tile of ROWS rows by NW waves: per thread, the byte offset

@@ -46,12 +46,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int head, tile;
   unit_of(blockIdx.x, a.heads, a.tiles, CAUSAL, head, tile);
-  int b, index, n;
-  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, index, n)) return;
-  const int row0 = index * kBM;
-  int qs, qe, ks, ke;
-  seq_rows(a.q_off, b, a.Tq, qs, qe);
-  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  Tile at;
+  if (!find_tile(a.q_off, a.k_off, a.B, a.Tq, a.Tk, kBM, tile, at)) return;
+  const int row0 = at.index * kBM, qs = at.s, qe = at.e, ks = at.os, ke = at.oe;
   const int Lq = qe - qs, Lk = ke - ks;
   // Query i sees keys 0 .. i + Lk - Lq.
   const int shift = Lk - Lq;

@@ -85,12 +85,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int head, tile;
   unit_of(blockIdx.x, a.heads, a.tiles, CAUSAL, head, tile);
-  int b, index, n;
-  if (!find_tile(a.q_off, a.B, a.Tq, kBM, tile, b, index, n)) return;
-  const int row0 = index * kBM;
-  int qs, qe, ks, ke;
-  seq_rows(a.q_off, b, a.Tq, qs, qe);
-  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  Tile place;
+  if (!find_tile(a.q_off, a.k_off, a.B, a.Tq, a.Tk, kBM, tile, place)) return;
+  const int row0 = place.index * kBM, qs = place.s, qe = place.e, ks = place.os, ke = place.oe;
   const int Lq = qe - qs, Lk = ke - ks, shift = Lk - Lq;
   const int keys = CAUSAL ? min(Lk, max(0, row0 + kBM + shift)) : Lk;
   const int nt = (keys + kBN - 1) / kBN;
@@ -214,13 +211,11 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   unit_of(blockIdx.x, kv_heads, a.tiles * a.splits, CAUSAL, kh, tile);
   const int split = tile % a.splits, unit = kh * a.tiles * a.splits + tile;
   tile /= a.splits;
-  int b, index, n;
-  if (!find_tile(a.k_off, a.B, a.Tk, kBM, tile, b, index, n)) return;
+  Tile place;
+  if (!find_tile(a.k_off, a.q_off, a.B, a.Tk, a.Tq, kBM, tile, place)) return;
   // Causal: the first keys have the most queries.
-  const int row0 = (n - 1 - index) * kBM;
-  int qs, qe, ks, ke;
-  seq_rows(a.q_off, b, a.Tq, qs, qe);
-  seq_rows(a.k_off, b, a.Tk, ks, ke);
+  const int row0 = (place.tiles - 1 - place.index) * kBM;
+  const int qs = place.os, qe = place.oe, ks = place.s, ke = place.e;
   const int Lq = qe - qs, Lk = ke - ks, shift = Lk - Lq;
   // Causal: key j is seen by the queries j - shift and on.
   const int first = CAUSAL ? min(Lq, max(0, row0 - shift)) : 0;
@@ -361,10 +356,10 @@ __global__ __launch_bounds__(64 * kWaves) void attention_dkv_join_kernel(BwdArgs
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = blockIdx.x, kh = w / a.tiles;
-  int b, index, n, ks, ke;
-  if (!find_tile(a.k_off, a.B, a.Tk, kBM, w - kh * a.tiles, b, index, n)) return;
-  seq_rows(a.k_off, b, a.Tk, ks, ke);
-  const int k0 = (n - 1 - index) * kBM + 32 * wave, kn = min(32, ke - ks - k0);
+  Tile place;
+  if (!find_tile(a.k_off, a.q_off, a.B, a.Tk, a.Tq, kBM, w - kh * a.tiles, place)) return;
+  const int ks = place.s, ke = place.e;
+  const int k0 = (place.tiles - 1 - place.index) * kBM + 32 * wave, kn = min(32, ke - ks - k0);
   if (kn <= 0) return;
   f32x16 x[DP / 32];
 #pragma unroll

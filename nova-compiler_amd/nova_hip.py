@@ -567,47 +567,41 @@ def index_to_i32(idx, out=None):
 # attention of packed sequences, losses over token log-probabilities
 # --------------------------------------------------------------------------
 # These calls are made once per layer and token, where their smallest take the
-# GPU less than 10 us, so the wrappers below spend little: a descriptor is one
-# packed struct, and the current stream is read without a Stream object.
+# GPU less than 10 us, so the wrappers spend little: one pass over a tensor
+# checks and packs its descriptor, and the current stream is read without a
+# Stream object.
 
-_PACK = {r: struct.Struct("PPq" + "q" * (2 * r)) for r in (1, 2, 3, 4)}
+_PACK = {r: struct.Struct("PPq" + "q" * (2 * r)).pack for r in (1, 2, 3, 4)}
 
 
-def _desc(t, rank: int, name: str):
-    """Descriptor of a tensor of the given rank, as bytes (None passes NULL)."""
+def _desc(t, rank: int, dtype, dev: int, name: str):
+    """Descriptor, as bytes, of a tensor that must have this rank, dtype and
+    device (None passes NULL)."""
     if t is None:
         return None
+    if t.dtype is not dtype:
+        raise NovaHipError(4, f"{name} is {t.dtype}, not {dtype}")
+    if t.get_device() != dev:
+        raise NovaHipError(1, f"{name} is on another device than the first operand")
     shape = t.shape
     if len(shape) != rank:
         raise NovaHipError(2, f"{name} has {len(shape)} dims, not {rank}")
     p = t.data_ptr()
-    return _PACK[rank].pack(p, p, 0, *shape, *t.stride())
+    return _PACK[rank](p, p, 0, *shape, *t.stride())
 
 
-def _check_dtype(dtype, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.dtype is not dtype:
-            raise NovaHipError(4, f"{name} is {t.dtype}, not {dtype}")
-
-
-def _launch(entry: str, tensors, *args) -> None:
-    """Calls an entry point on the tensors' device and its current stream;
-    refuses tensors of different devices, which descriptors do not show."""
+def _launch(entry, dev: int, *args) -> None:
+    """Calls an entry point on that device and its current stream."""
     torch = _torch()
-    dev = tensors[0].get_device()
     if dev < 0:
         raise NovaHipError(1, "tensors must be on the GPU")
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise NovaHipError(1, f"tensors on devices {dev} and {t.get_device()}")
-    L = lib()
     if dev == torch.cuda.current_device():
-        L.nova_hip_set_stream(torch._C._cuda_getCurrentRawStream(dev))
-        rc = getattr(L, entry)(*args)
+        _lib.nova_hip_set_stream(torch._C._cuda_getCurrentRawStream(dev))
+        rc = entry(*args)
     else:
         with torch.cuda.device(dev):
-            L.nova_hip_set_stream(torch._C._cuda_getCurrentRawStream(dev))
-            rc = getattr(L, entry)(*args)
+            _lib.nova_hip_set_stream(torch._C._cuda_getCurrentRawStream(dev))
+            rc = entry(*args)
         _bind_stream()
     if rc:
         check(rc)
@@ -621,22 +615,17 @@ def attention(q, k, v, q_offsets, k_offsets, *, causal: bool = True, scale=None,
     1 / sqrt(D) by default.  Returns (out, lse [heads, tokens] f32), lse None
     with ``want_lse`` False; rows outside every sequence are not written."""
     torch = _torch()
-    f32, i32 = torch.float32, torch.int32
-    _check_dtype(q.dtype, k=k, v=v, out=out)
-    _check_dtype(i32, q_offsets=q_offsets, k_offsets=k_offsets)
-    dq = _desc(q, 3, "q")
+    f32, i32, dt, dev = torch.float32, torch.int32, q.dtype, q.get_device()
+    dq, dk, dv = (_desc(q, 3, dt, dev, "q"), _desc(k, 3, dt, dev, "k"), _desc(v, 3, dt, dev, "v"))
+    dqo, dko = _desc(q_offsets, 1, i32, dev, "q_offsets"), _desc(k_offsets, 1, i32, dev, "k_offsets")
     T, H, D = q.shape
     if out is None:
         out = q.new_empty((T, H, D))
-    if lse is None:
-        if want_lse:
-            lse = q.new_empty((H, T), dtype=f32)
-    else:
-        _check_dtype(f32, lse=lse)
-    _launch("_mlir_ciface_nova_hip_attention", (q, k, v, q_offsets, k_offsets, out, lse), dq,
-            _desc(k, 3, "k"), _desc(v, 3, "v"), _desc(q_offsets, 1, "q_offsets"),
-            _desc(k_offsets, 1, "k_offsets"), _desc(out, 3, "out"), _desc(lse, 2, "lse"),
-            D ** -0.5 if scale is None else scale, 1 if causal else 0, _dt(q))
+    if lse is None and want_lse:
+        lse = q.new_empty((H, T), dtype=f32)
+    _launch(lib()._mlir_ciface_nova_hip_attention, dev, dq, dk, dv, dqo, dko,
+            _desc(out, 3, dt, dev, "out"), _desc(lse, 2, f32, dev, "lse"),
+            (D or 1) ** -0.5 if scale is None else scale, 1 if causal else 0, _dt(q))
     return out, lse
 
 
@@ -645,27 +634,26 @@ def attention_backward(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, cau
     """Gradients of ``attention``'s result, from its ``out`` and ``lse``:
     returns (dq, dk, dv) in the operands' dtype."""
     torch = _torch()
-    f32, i32 = torch.float32, torch.int32
-    _check_dtype(q.dtype, grad_out=grad_out, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
-    _check_dtype(i32, q_offsets=q_offsets, k_offsets=k_offsets)
-    _check_dtype(f32, lse=lse)
-    desc_q, desc_k = _desc(q, 3, "q"), _desc(k, 3, "k")
+    f32, i32, dt, dev = torch.float32, torch.int32, q.dtype, q.get_device()
+    d = (_desc(grad_out, 3, dt, dev, "grad_out"), _desc(q, 3, dt, dev, "q"),
+         _desc(k, 3, dt, dev, "k"), _desc(v, 3, dt, dev, "v"), _desc(out, 3, dt, dev, "out"),
+         _desc(lse, 2, f32, dev, "lse"), _desc(q_offsets, 1, i32, dev, "q_offsets"),
+         _desc(k_offsets, 1, i32, dev, "k_offsets"))
     T, H, D = q.shape
+    Tk, G, _ = k.shape
     if dq is None:
         dq = q.new_empty((T, H, D))
     if dk is None:
-        dk = k.new_empty(tuple(k.shape))
+        dk = k.new_empty((Tk, G, D))
     if dv is None:
-        dv = k.new_empty(tuple(k.shape))
-    need = lib().nova_hip_attention_backward_scratch(T, k.shape[0], max(q_offsets.numel() - 1, 0), H,
-                                                     k.shape[1], D, 1 if causal else 0)
-    scratch = q.new_empty(need, dtype=f32)
-    _launch("_mlir_ciface_nova_hip_attention_backward",
-            (q, grad_out, k, v, out, lse, q_offsets, k_offsets, dq, dk, dv),
-            _desc(grad_out, 3, "grad_out"), desc_q, desc_k, _desc(v, 3, "v"), _desc(out, 3, "out"),
-            _desc(lse, 2, "lse"), _desc(q_offsets, 1, "q_offsets"), _desc(k_offsets, 1, "k_offsets"),
-            _desc(dq, 3, "dq"), _desc(dk, 3, "dk"), _desc(dv, 3, "dv"), _desc(scratch, 1, "scratch"),
-            D ** -0.5 if scale is None else scale, 1 if causal else 0, _dt(q))
+        dv = k.new_empty((Tk, G, D))
+    L = lib()
+    scratch = q.new_empty(L.nova_hip_attention_backward_scratch(
+        T, Tk, max(q_offsets.shape[0] - 1, 0), H, G, D, 1 if causal else 0), dtype=f32)
+    _launch(L._mlir_ciface_nova_hip_attention_backward, dev, *d, _desc(dq, 3, dt, dev, "dq"),
+            _desc(dk, 3, dt, dev, "dk"), _desc(dv, 3, dt, dev, "dv"),
+            _desc(scratch, 1, f32, dev, "scratch"), (D or 1) ** -0.5 if scale is None else scale,
+            1 if causal else 0, _dt(q))
     return dq, dk, dv
 
 
@@ -675,18 +663,19 @@ def attention_decode(q, k, v, lengths, *, scale=None, out=None, lse=None):
     first three dims in memory), lengths [sequences] i32.  Returns out;
     ``lse`` [sequences, heads] f32 is written when given."""
     torch = _torch()
-    _check_dtype(q.dtype, k=k, v=v, out=out)
-    _check_dtype(torch.int32, lengths=lengths)
-    _check_dtype(torch.float32, lse=lse)
-    dq, dk = _desc(q, 3, "q"), _desc(k, 4, "k")
+    f32, dt, dev = torch.float32, q.dtype, q.get_device()
+    dq, dk, dv = (_desc(q, 3, dt, dev, "q"), _desc(k, 4, dt, dev, "k"), _desc(v, 4, dt, dev, "v"))
+    dl = _desc(lengths, 1, torch.int32, dev, "lengths")
     B, H, D = q.shape
     if out is None:
         out = q.new_empty((B, H, D))
-    need = lib().nova_hip_attention_decode_scratch(B, k.shape[1], H, k.shape[2], D)
-    scratch = q.new_empty(need, dtype=torch.float32) if need else None
-    _launch("_mlir_ciface_nova_hip_attention_decode", (q, k, v, lengths, out, lse), dq, dk,
-            _desc(v, 4, "v"), _desc(lengths, 1, "lengths"), _desc(out, 3, "out"), _desc(lse, 2, "lse"),
-            _desc(scratch, 1, "scratch"), D ** -0.5 if scale is None else scale, _dt(q))
+    L = lib()
+    need = L.nova_hip_attention_decode_scratch(B, k.shape[1], H, k.shape[2], D)
+    scratch = q.new_empty(need, dtype=f32) if need else None
+    _launch(L._mlir_ciface_nova_hip_attention_decode, dev, dq, dk, dv, dl,
+            _desc(out, 3, dt, dev, "out"), _desc(lse, 2, f32, dev, "lse"),
+            _desc(scratch, 1, f32, dev, "scratch"), (D or 1) ** -0.5 if scale is None else scale,
+            _dt(q))
     return out
 
 
@@ -694,13 +683,12 @@ def token_logp(logits, labels, *, logp=None, lse=None):
     """The log-probability of each row's label [rows] f32 (0 where the label is
     negative); ``lse`` [rows] f32 is written when given."""
     torch = _torch()
-    _check_dtype(torch.int32, labels=labels)
-    _check_dtype(torch.float32, logp=logp, lse=lse)
-    d = _desc(logits, 2, "logits")
+    f32, dev = torch.float32, logits.get_device()
+    d, dl = _desc(logits, 2, logits.dtype, dev, "logits"), _desc(labels, 1, torch.int32, dev, "labels")
     if logp is None:
-        logp = logits.new_empty(logits.shape[0], dtype=torch.float32)
-    _launch("_mlir_ciface_nova_hip_token_logp", (logits, labels, logp, lse), d,
-            _desc(labels, 1, "labels"), _desc(logp, 1, "logp"), _desc(lse, 1, "lse"), _dt(logits))
+        logp = logits.new_empty(logits.shape[0], dtype=f32)
+    _launch(lib()._mlir_ciface_nova_hip_token_logp, dev, d, dl, _desc(logp, 1, f32, dev, "logp"),
+            _desc(lse, 1, f32, dev, "lse"), _dt(logits))
     return logp
 
 
@@ -712,12 +700,10 @@ def policy_loss(logits, labels, old_logp, advantage, weight, *, ref_logp=None, c
     with ``want_grad`` False.  ``clip`` is (low, high): the ratio is clamped to
     [1 - low, 1 + high].  Rows with a negative label or weight 0 take no part."""
     torch = _torch()
-    f32 = torch.float32
-    _check_dtype(torch.int32, labels=labels)
-    _check_dtype(f32, old_logp=old_logp, advantage=advantage, weight=weight, ref_logp=ref_logp,
-                 loss=loss, logp=logp, row_loss=row_loss)
-    _check_dtype(logits.dtype, grad=grad)
-    d = _desc(logits, 2, "logits")
+    f32, dt, dev = torch.float32, logits.dtype, logits.get_device()
+    d = (_desc(logits, 2, dt, dev, "logits"), _desc(labels, 1, torch.int32, dev, "labels"),
+         _desc(old_logp, 1, f32, dev, "old_logp"), _desc(ref_logp, 1, f32, dev, "ref_logp"),
+         _desc(advantage, 1, f32, dev, "advantage"), _desc(weight, 1, f32, dev, "weight"))
     rows, classes = logits.shape
     if loss is None:
         loss = logits.new_empty(1, dtype=f32)
@@ -727,12 +713,9 @@ def policy_loss(logits, labels, old_logp, advantage, weight, *, ref_logp=None, c
         row_loss = logits.new_empty(rows, dtype=f32)
     if grad is None and want_grad:
         grad = logits.new_empty((rows, classes))
-    _launch("_mlir_ciface_nova_hip_policy_loss",
-            (logits, labels, old_logp, advantage, weight, ref_logp, loss, logp, row_loss, grad), d,
-            _desc(labels, 1, "labels"), _desc(old_logp, 1, "old_logp"), _desc(ref_logp, 1, "ref_logp"),
-            _desc(advantage, 1, "advantage"), _desc(weight, 1, "weight"), _desc(loss, 1, "loss"),
-            _desc(logp, 1, "logp"), _desc(row_loss, 1, "row_loss"), _desc(grad, 2, "grad"),
-            clip[0], clip[1], kl_coef, grad_scale, _dt(logits))
+    _launch(lib()._mlir_ciface_nova_hip_policy_loss, dev, *d, _desc(loss, 1, f32, dev, "loss"),
+            _desc(logp, 1, f32, dev, "logp"), _desc(row_loss, 1, f32, dev, "row_loss"),
+            _desc(grad, 2, dt, dev, "grad"), clip[0], clip[1], kl_coef, grad_scale, _dt(logits))
     return loss, logp, grad
 
 
@@ -745,12 +728,9 @@ def preference_loss(logits, labels, offsets, ref_logp, *, beta: float = 0.1, smo
     False.  ``pair_loss`` [pairs] and ``token`` [3, rows] (logp, lse, slope) are
     written when given."""
     torch = _torch()
-    f32 = torch.float32
-    _check_dtype(torch.int32, labels=labels, offsets=offsets)
-    _check_dtype(f32, ref_logp=ref_logp, loss=loss, seq_logp=seq_logp, pair_loss=pair_loss,
-                 token=token)
-    _check_dtype(logits.dtype, grad=grad)
-    d, do = _desc(logits, 2, "logits"), _desc(offsets, 1, "offsets")
+    f32, i32, dt, dev = torch.float32, torch.int32, logits.dtype, logits.get_device()
+    d = (_desc(logits, 2, dt, dev, "logits"), _desc(labels, 1, i32, dev, "labels"),
+         _desc(offsets, 1, i32, dev, "offsets"), _desc(ref_logp, 1, f32, dev, "ref_logp"))
     rows, classes = logits.shape
     seqs = max(offsets.shape[0] - 1, 0)
     if loss is None:
@@ -763,9 +743,8 @@ def preference_loss(logits, labels, offsets, ref_logp, *, beta: float = 0.1, smo
         token = logits.new_empty((3, rows), dtype=f32)
     if grad is None and want_grad:
         grad = logits.new_empty((rows, classes))
-    _launch("_mlir_ciface_nova_hip_preference_loss",
-            (logits, labels, offsets, ref_logp, loss, seq_logp, pair_loss, token, grad), d,
-            _desc(labels, 1, "labels"), do, _desc(ref_logp, 1, "ref_logp"), _desc(loss, 1, "loss"),
-            _desc(seq_logp, 1, "seq_logp"), _desc(pair_loss, 1, "pair_loss"),
-            _desc(token, 2, "token"), _desc(grad, 2, "grad"), beta, smoothing, grad_scale, _dt(logits))
+    _launch(lib()._mlir_ciface_nova_hip_preference_loss, dev, *d, _desc(loss, 1, f32, dev, "loss"),
+            _desc(seq_logp, 1, f32, dev, "seq_logp"), _desc(pair_loss, 1, f32, dev, "pair_loss"),
+            _desc(token, 2, f32, dev, "token"), _desc(grad, 2, dt, dev, "grad"), beta, smoothing,
+            grad_scale, _dt(logits))
     return loss, seq_logp, grad
