@@ -2,8 +2,11 @@
 // single tokens.  Bound by HBM: keys and values are read once, for all query
 // heads of their group together (the group's heads are the MFMA's columns).
 //
-// A cache of S rows is cut into splits of `chunk` keys; a workgroup of one wave
-// takes one split of one sequence and key head, 32 keys at a time through a
+// A cache of up to 1024 rows is one workgroup's per sequence and key head: its
+// waves take a part each and join their sums through LDS, in one launch (one
+// sequence of 1000 rows, 6 heads of 64: 13.3 us in two launches, 9.2 in one; a
+// launch costs the host 3).  A longer cache is cut into splits of `chunk` keys; a
+// workgroup of one wave takes one split of one sequence and key head, 32 keys at a time through a
 // two-stage ring in LDS filled by DMA, without a barrier.  (Two waves sharing a
 // split joined their sums through LDS and took 2% longer.)  With more than
 // one split the sums go to the caller's scratch, and attention_join_kernel adds
@@ -28,6 +31,7 @@ struct DecodeArgs {
   uint16_t *o;
   float *lse;      // [B][heads] with row stride slse, or null
   float *partial;  // [B][heads][splits][D + 2]: sum, then m c and l (splits > 1)
+  // splits: 0 where one workgroup's waves take a sequence and join
   const int *lens;
   int64_t sqb, sqh, sob, soh, slse;
   int64_t skb, skt, skh, svb, svt, svh;
@@ -37,25 +41,27 @@ struct DecodeArgs {
 
 constexpr int kBN = 32;
 
-template <int DT, int DP>
-__global__ __launch_bounds__(64) void attention_decode_kernel(DecodeArgs a) {
+template <int DT, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void attention_decode_kernel(DecodeArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sk0_[kTile];
-  lds_char *const sk0 = (lds_char *)sk0_;
-  __shared__ __attribute__((aligned(1024))) char sk1_[kTile];
-  lds_char *const sk1 = (lds_char *)sk1_;
-  __shared__ __attribute__((aligned(1024))) char sv0_[kTile];
-  lds_char *const sv0 = (lds_char *)sv0_;
-  __shared__ __attribute__((aligned(1024))) char sv1_[kTile];
-  lds_char *const sv1 = (lds_char *)sv1_;
-  const int lane = threadIdx.x;
-  const int b = blockIdx.y, split = blockIdx.z;
+  const int lane = threadIdx.x & 63;
+  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float sm[NW][32], sl[NW][32];
+  __shared__ __attribute__((aligned(1024))) char sk0_[NW * kTile];
+  lds_char *const sk0 = (lds_char *)sk0_ + wave * kTile;
+  __shared__ __attribute__((aligned(1024))) char sk1_[NW * kTile];
+  lds_char *const sk1 = (lds_char *)sk1_ + wave * kTile;
+  __shared__ __attribute__((aligned(1024))) char sv0_[NW * kTile];
+  lds_char *const sv0 = (lds_char *)sv0_ + wave * kTile;
+  __shared__ __attribute__((aligned(1024))) char sv1_[NW * kTile];
+  lds_char *const sv1 = (lds_char *)sv1_ + wave * kTile;
+  const int b = blockIdx.y, split = NW == 1 ? blockIdx.z : wave;
   const int blocks = (a.group + 31) / 32;  // of 32 query heads
   const int kh = blockIdx.x / blocks, h0 = kh * a.group + 32 * (blockIdx.x - kh * blocks);
   const int hn = min(32, (kh + 1) * a.group - h0);
   const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
   const int from = split * a.chunk, to = min(len, from + a.chunk);
-  if (from >= len && split > 0) return;  // nothing here; the join does not read it
+  if (NW == 1 && from >= len && split > 0) return;  // nothing here; the join does not read it
 
   const uint16_t *kp = a.k + b * a.skb + kh * a.skh, *vp = a.v + b * a.svb + kh * a.svh;
 
@@ -160,7 +166,45 @@ __global__ __launch_bounds__(64) void attention_decode_kernel(DecodeArgs a) {
   }
 
   l = both_sum(l);
-  if (a.splits == 1) {
+  if constexpr (NW > 1) {
+    // Join the waves: to the largest of their maxima, then in wave order, each
+    // handing its sums over through its part of the ring.
+    if (lane < 32) {
+      sm[wave][lane] = mc;
+      sl[wave][lane] = l;
+    }
+    __syncthreads();
+    const int c = lane & 31;
+    float mx = sm[0][c];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sm[i][c]);
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i)
+      l += sm[i][c] == -INFINITY ? 0.0f : sl[i][c] * __builtin_amdgcn_exp2f(sm[i][c] - mx);
+    const float f = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - mx);
+    mc = mx;
+    static_assert(kTile >= 64 * 16 * 4, "a block of 32 x 32 sums");
+    lds_float *const box = (lds_float *)sk0 + lane;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+      if (db) __syncthreads();
+      if (wave) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[64 * r] = acc[db][r] * f;
+      }
+      __syncthreads();
+      if (wave == 0) {
+        acc[db] *= f;
+#pragma unroll
+        for (int i = 1; i < NW; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[db][r] += box[i * (kTile / 4) + 64 * r];
+      }
+    }
+    if (wave) return;
+  }
+  if (NW > 1 || a.splits == 1) {
     store_rows<DT, DP>(acc, l == 0.0f ? 0.0f : 1.0f / l, a.o + b * a.sob + h0 * a.soh, a.soh, hn,
                        a.D, lane);
     if (a.lse && lane < hn)
@@ -223,9 +267,17 @@ __global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a) {
     a.lse[b * a.slse + h] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
 }
 
+// Waves of the form that joins them itself: what the LDS of a CU holds.
+constexpr int kJoined = 1024;  // cache rows it takes
+constexpr int waves_joined(int64_t D) { return D <= 64 ? 8 : 4; }
+
 template <int DT, int DP>
 void launch_decode_t(const DecodeArgs &a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((attention_decode_kernel<DT, DP>), grid, dim3(64), 0, s, a);
+  constexpr int NW = waves_joined(DP);
+  if (a.splits == 0)
+    hipLaunchKernelGGL((attention_decode_kernel<DT, DP, NW>), grid, dim3(64 * NW), 0, s, a);
+  else
+    hipLaunchKernelGGL((attention_decode_kernel<DT, DP, 1>), grid, dim3(64), 0, s, a);
 }
 template <int DT>
 int32_t launch_decode(const DecodeArgs &a, dim3 grid, hipStream_t s) {
@@ -234,7 +286,7 @@ int32_t launch_decode(const DecodeArgs &a, dim3 grid, hipStream_t s) {
   else if (a.D <= 96) launch_decode_t<DT, 96>(a, grid, s);
   else launch_decode_t<DT, 128>(a, grid, s);
   const int32_t rc = check_hip(hipGetLastError(), "attention_decode launch");
-  if (rc || a.splits == 1) return rc;
+  if (rc || a.splits <= 1) return rc;
   hipLaunchKernelGGL(attention_join_kernel<DT>, dim3((unsigned)a.heads, grid.y), dim3(256), 0, s, a);
   return check_hip(hipGetLastError(), "attention_decode join launch");
 }
@@ -251,10 +303,17 @@ int32_t launch_decode(const DecodeArgs &a, dim3 grid, hipStream_t s) {
 //   8 x 8192                     69.2 / 57.7 / 51.5 / 48.5 / 50.8
 //   32 x 1500 .. 8192 of 8192     151 /  128 /  114 /  103 /  116
 //   8 x 131072                   1007 /  878 /  797 /  755 /  685
-int64_t attention_decode_chunk(int64_t B, int64_t S, int64_t kv_heads) {
+static int64_t decode_chunk(int64_t B, int64_t S, int64_t kv_heads) {
   const int64_t all = B * S * kv_heads;
   const int64_t keys = std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
-  return std::max<int64_t>(64, (keys + 63) / 64 * 64);
+  // At most 32768 splits (a dimension of the grid).
+  return std::max<int64_t>(64, (std::max(keys, S / 32768) + 63) / 64 * 64);
+}
+
+int64_t attention_decode_scratch(int64_t B, int64_t S, int64_t heads, int64_t kv_heads, int64_t D) {
+  if (S <= attn::kJoined) return 0;
+  const int64_t chunk = decode_chunk(B, S, kv_heads), splits = (S + chunk - 1) / chunk;
+  return splits <= 1 ? 0 : B * heads * splits * (D + 2);
 }
 
 int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s) {
@@ -276,15 +335,21 @@ int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s) 
   a.heads = (int)p.heads;
   a.group = (int)(p.heads / p.kv_heads);
   a.D = (int)p.D;
-  const int64_t chunk = attention_decode_chunk(p.B, p.S, p.kv_heads);
-  a.chunk = (int)chunk;
-  a.splits = (int)std::max<int64_t>(1, (p.S + chunk - 1) / chunk);
+  if (p.S <= attn::kJoined) {
+    const int64_t waves = attn::waves_joined(p.D);
+    a.chunk = (int)std::max<int64_t>(32, ((p.S + waves - 1) / waves + 31) / 32 * 32);
+    a.splits = 0;
+  } else {
+    a.chunk = (int)decode_chunk(p.B, p.S, p.kv_heads);
+    a.splits = (int)((p.S + a.chunk - 1) / a.chunk);
+  }
   a.c = p.scale * attn::kLog2e;
   // Splits outermost: sequences shorter than the cache leave the last splits
   // empty, and with splits innermost a power of two of them put every first
   // split on the same XCD (32 sequences of 300 rows in a cache of 8192, splits
   // of 512: 90 us, 16 with the order below).
-  const dim3 grid((unsigned)(p.kv_heads * ((a.group + 31) / 32)), (unsigned)p.B, (unsigned)a.splits);
+  const dim3 grid((unsigned)(p.kv_heads * ((a.group + 31) / 32)), (unsigned)p.B,
+                  (unsigned)std::max(1, a.splits));
   return p.dt == NOVA_HIP_DT_BF16 ? attn::launch_decode<NOVA_HIP_DT_BF16>(a, grid, s)
                                   : attn::launch_decode<NOVA_HIP_DT_F16>(a, grid, s);
 }

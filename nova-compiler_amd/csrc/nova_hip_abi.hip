@@ -1034,9 +1034,7 @@ int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int6
   if (sequences <= 0 || cache <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0) return 0;
   if (sequences > 0xffff || cache > 0x7fffffff || heads > 0xffff || kv_heads > heads || D > 128)
     return 0;  // the call itself refuses these
-  const int64_t chunk = attention_decode_chunk(sequences, cache, kv_heads);
-  const int64_t splits = (cache + chunk - 1) / chunk;
-  return splits <= 1 ? 0 : sequences * heads * splits * (D + 2);
+  return attention_decode_scratch(sequences, cache, heads, kv_heads, D);
 }
 
 int32_t _mlir_ciface_nova_hip_attention_decode(const NovaMemRef3D *q, const NovaMemRef4D *k,

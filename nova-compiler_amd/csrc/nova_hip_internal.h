@@ -161,8 +161,7 @@ struct AttentionDecodeProblem {
   float scale;
   int dt;
 };
-// Keys of one split of a cache of S rows.
-int64_t attention_decode_chunk(int64_t B, int64_t S, int64_t kv_heads);
+int64_t attention_decode_scratch(int64_t B, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
 int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s);
 
 // ---- losses over token log-probabilities (losses.hip) --------------------------

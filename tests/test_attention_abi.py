@@ -102,7 +102,7 @@ def test_attention_empty_calls_do_nothing():
 # ---- decode ----------------------------------------------------------------------------
 
 def dec(scale=0.125, dt=BF, **kw):
-    o = dict(q=d((3, 4, 64)), k=d((3, 200, 2, 64)), v=d((3, 200, 2, 64)), lens=d((3,)),
+    o = dict(q=d((3, 4, 64)), k=d((3, 2000, 2, 64)), v=d((3, 2000, 2, 64)), lens=d((3,)),
              out=d((3, 4, 64)), lse=None, scratch=d((10 ** 6,)))
     o.update(kw)
     return call("_mlir_ciface_nova_hip_attention_decode", list(o.values()), scale, dt)
@@ -110,22 +110,22 @@ def dec(scale=0.125, dt=BF, **kw):
 
 @pytest.mark.parametrize("want,kw", [
     (EINVAL, dict(q=None)), (EINVAL, dict(lens=None)), (EINVAL, dict(scale=0.0)),
-    (EINVAL, dict(k=d((3, 200, 2, 64), ptr=0))), (EINVAL, dict(lens=d((3,), ptr=0))),
+    (EINVAL, dict(k=d((3, 2000, 2, 64), ptr=0))), (EINVAL, dict(lens=d((3,), ptr=0))),
     (EINVAL, dict(scratch=None)), (EINVAL, dict(lse=d((3, 4), ptr=0))),
     (EDTYPE, dict(dt=F32)),
-    (ESHAPE, dict(v=d((3, 199, 2, 64)))), (ESHAPE, dict(lens=d((2,)))), (ESHAPE, dict(out=d((3, 2, 64)))),
-    (ESHAPE, dict(k=d((2, 200, 2, 64)), v=d((2, 200, 2, 64)))),
-    (ESHAPE, dict(k=d((3, 200, 3, 64)), v=d((3, 200, 3, 64)))), (ESHAPE, dict(lse=d((4, 3)))),
+    (ESHAPE, dict(v=d((3, 1999, 2, 64)))), (ESHAPE, dict(lens=d((2,)))), (ESHAPE, dict(out=d((3, 2, 64)))),
+    (ESHAPE, dict(k=d((2, 2000, 2, 64)), v=d((2, 2000, 2, 64)))),
+    (ESHAPE, dict(k=d((3, 2000, 3, 64)), v=d((3, 2000, 3, 64)))), (ESHAPE, dict(lse=d((4, 3)))),
     (ESHAPE, dict(scratch=d((10,)))),
-    (ESTRIDE, dict(k=d((3, 200, 2, 64), (25600, 32, 6400, 1)))),
-    (ESTRIDE, dict(k=d((3, 200, 2, 64), (25600, 128, 64, 2)))),
-    (ESTRIDE, dict(k=d((3, 200, 2, 64), ptr=FAKE + 8))),
-    (ESTRIDE, dict(v=d((3, 200, 2, 64), (25604, 128, 64, 1)))),
+    (ESTRIDE, dict(k=d((3, 2000, 2, 64), (256000, 32, 64000, 1)))),
+    (ESTRIDE, dict(k=d((3, 2000, 2, 64), (256000, 128, 64, 2)))),
+    (ESTRIDE, dict(k=d((3, 2000, 2, 64), ptr=FAKE + 8))),
+    (ESTRIDE, dict(v=d((3, 2000, 2, 64), (256004, 128, 64, 1)))),
     (ESTRIDE, dict(q=d((3, 4, 64), (256, 0, 1)))), (ESTRIDE, dict(out=d((3, 4, 64), (64, 64, 1)))),
     (ESTRIDE, dict(lens=d((3,), (2,)))), (ESTRIDE, dict(scratch=d((10 ** 6,), ptr=FAKE + 4))),
     (ESTRIDE, dict(lse=d((3, 4), (2, 1)))),
-    (ERANGE, dict(k=d((3, 200, 2, 64), (1 << 32, (1 << 23) + 64, 64, 1)))),
-    (ERANGE, dict(q=d((3, 4, 136)), out=d((3, 4, 136)), k=d((3, 200, 2, 136)), v=d((3, 200, 2, 136)))),
+    (ERANGE, dict(k=d((3, 2000, 2, 64), (1 << 32, (1 << 23) + 64, 64, 1)))),
+    (ERANGE, dict(q=d((3, 4, 136)), out=d((3, 4, 136)), k=d((3, 2000, 2, 136)), v=d((3, 2000, 2, 136)))),
 ])
 def test_decode_refuses(want, kw):
     assert dec(**kw) == want, nh.lib().nova_hip_last_error()
@@ -133,11 +133,14 @@ def test_decode_refuses(want, kw):
 
 def test_decode_scratch_and_empty_calls():
     L = nh.lib()
-    assert L.nova_hip_attention_decode_scratch(3, 64, 4, 2, 64) == 0  # one split
-    assert L.nova_hip_attention_decode_scratch(3, 200, 4, 2, 64) == 3 * 4 * 4 * 66
-    assert L.nova_hip_attention_decode_scratch(0, 200, 4, 2, 64) == 0
+    assert L.nova_hip_attention_decode_scratch(3, 1024, 4, 2, 64) == 0  # one workgroup's work
+    assert L.nova_hip_attention_decode_scratch(3, 1025, 4, 2, 64) == 3 * 4 * 17 * 66
+    assert L.nova_hip_attention_decode_scratch(0, 2000, 4, 2, 64) == 0
+    # At most 32768 splits whatever the cache.
+    most = L.nova_hip_attention_decode_scratch(1, 2 ** 31 - 2 ** 20, 1, 1, 8)
+    assert most <= 32768 * 10
     assert dec(q=d((0, 4, 64), ptr=0), out=d((0, 4, 64), ptr=0), lens=d((0,), ptr=0),
-               k=d((0, 200, 2, 64), ptr=0), v=d((0, 200, 2, 64), ptr=0)) == 0
+               k=d((0, 2000, 2, 64), ptr=0), v=d((0, 2000, 2, 64), ptr=0)) == 0
 
 
 # ---- losses over token log-probabilities --------------------------------------------------

@@ -46,9 +46,16 @@ def test_orders_and_shared_heads(cuda, order, H, G):
     run(cuda, [33, 200, 1], 200, H, G, 64, BF, order)
 
 
-@pytest.mark.parametrize("S", [1, 31, 32, 33, 63, 64, 65, 128, 129, 1000])
-def test_cache_sizes(cuda, S):
-    run(cuda, [S, 1, S // 2], S, 4, 2, 128, BF)
+@pytest.mark.parametrize("S", [1, 31, 32, 33, 63, 64, 65, 128, 129, 1000, 1023, 1024, 1025, 1100, 3001])
+@pytest.mark.parametrize("D", [64, 128])
+def test_cache_sizes(cuda, S, D):
+    run(cuda, [S, 1, S // 2, 0, S - 1], S, 4, 2, D, BF)
+
+
+@pytest.mark.parametrize("D", [32, 40, 64, 80, 96, 128])
+def test_head_dims_of_a_long_cache(cuda, D):
+    run(cuda, [1500, 1, 64, 130, 1437], 1500, 8, 2, D, HF)
+    run(cuda, [1500, 700], 1500, 35, 1, D, BF, "bhsd")  # more heads than one block of 32
 
 
 def test_lengths_zero_and_out_of_range(cuda):
