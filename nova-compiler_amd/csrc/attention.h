@@ -21,6 +21,8 @@
 // once.
 #pragma once
 
+#include <algorithm>
+
 #include "gemm_common.h"
 
 namespace nova_hip {
@@ -101,16 +103,20 @@ struct Tile {
 };
 
 // Tile t of the sequences' tiles of BM rows, off[0 .. B] being the sequences'
-// first rows and other[0 .. B] those of the other operand (whatever they hold,
-// every sequence is cut to rows inside [0, T) and [0, To)), in the order of
-// falling index within the sequence: the last tiles of the longest sequences
-// first.  That is the order of falling work of causal attention (or of rising
-// index counted from the end, for keys), so that what runs last is short.
-// False when t lies behind the last tile.
-// Wave-uniform; every wave searches for itself: with S(l) = sum over sequences
-// of max(0, tiles - l), the tiles of index l and above, it finds the largest
-// l with S(l) > t, bit by bit.  The first 64 sequences' rows are loaded together
-// and stay in registers: a call of few sequences waits for one load.
+// first rows and other[0 .. B] those of the other operand; whatever they hold,
+// every sequence is cut to rows inside [0, T) and [0, To).  False when there is
+// no such tile.  Wave-uniform; every wave searches for itself.
+//
+// Up to 64 sequences, whose rows one load brings into registers: in the order of
+// falling index within the sequence, the last tiles of the longest sequences
+// first, which is the order of falling work of causal attention (or of rising
+// index counted from the end, for keys), so that what runs last is short.  With
+// S(l) = sum over sequences of max(0, tiles - l), the tiles of index l and above,
+// that is the largest l with S(l) > t, found bit by bit.
+//
+// More: sequence b's tiles are numbered from off[b] / BM + b, which leaves it at
+// least as many numbers as it has tiles and needs no sums; 64 sequences are
+// probed at a time (three loads for 2^18 sequences), the last ones first.
 __device__ __forceinline__ bool find_tile(const int *off, const int *other, int B, int T, int To,
                                           int BM, int t, Tile &tile) {
   const int lane = threadIdx.x & 63;
@@ -121,51 +127,58 @@ __device__ __forceinline__ bool find_tile(const int *off, const int *other, int 
       e = max(s, min(max(o[b + 1], 0), n));
     }
   };
-  auto tiles_of = [&](int b) __attribute__((always_inline)) {
-    int s, e;
-    rows_of(off, T, b, s, e);
-    return (e - s + BM - 1) / BM;
-  };
-  int s0, e0, os0, oe0;
-  rows_of(off, T, lane, s0, e0);
-  rows_of(other, To, lane, os0, oe0);
-  const int n0 = (e0 - s0 + BM - 1) / BM;
-  auto above = [&](int l) __attribute__((always_inline)) {
-    int v = max(0, n0 - l);
-    for (int b0 = 64; b0 < B; b0 += 64) v += max(0, tiles_of(b0 + lane) - l);
-    return wave_sum_int(v);
-  };
-  if (above(0) <= t) return false;
-  int level = 0;
-  // No sequence has 2^k tiles once S(2^k) is 0.
-  int bit = 1;
-  while (bit < (1 << 26) && above(bit) > t) bit <<= 1;
-  for (bit >>= 1; bit > 0; bit >>= 1)
-    if (above(level + bit) > t) level += bit;
-  int k = t - above(level + 1);  // among the sequences with a tile of that index
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    if (b0) {
-      rows_of(off, T, b0 + lane, s0, e0);
-      rows_of(other, To, b0 + lane, os0, oe0);
-    }
+  int s0, e0, os0, oe0, l;
+  if (B <= 64) {
+    rows_of(off, T, lane, s0, e0);
+    rows_of(other, To, lane, os0, oe0);
     const int n = (e0 - s0 + BM - 1) / BM;
+    auto above = [&](int k) __attribute__((always_inline)) { return wave_sum_int(max(0, n - k)); };
+    if (above(0) <= t) return false;
+    int level = 0, bit = 1;
+    while (bit < (1 << 25) && above(bit) > t) bit <<= 1;
+    for (bit >>= 1; bit > 0; bit >>= 1)
+      if (above(level + bit) > t) level += bit;
+    const int k = t - above(level + 1);  // among the sequences with a tile of that index
     const uint64_t has = __ballot(n > level);
-    const int count = __builtin_popcountll(has);
-    if (k < count) {
-      const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
-                                                 __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
-      const int l = __builtin_ctzll(__ballot(n > level && rank == k));
-      tile.index = __builtin_amdgcn_readfirstlane(level);
-      tile.tiles = __builtin_amdgcn_readlane(n, l);
-      tile.s = __builtin_amdgcn_readlane(s0, l);
-      tile.e = __builtin_amdgcn_readlane(e0, l);
-      tile.os = __builtin_amdgcn_readlane(os0, l);
-      tile.oe = __builtin_amdgcn_readlane(oe0, l);
-      return true;
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
+                                               __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+    const uint64_t hit = __ballot(n > level && rank == k);
+    if (!hit) return false;
+    l = __builtin_ctzll(hit);
+    tile.index = level;
+    tile.tiles = __builtin_amdgcn_readlane(n, l);
+  } else {
+    t = T / BM + B - 1 - t;
+    int lo = 0, n = B;
+    for (;;) {
+      const int step = (n + 63) / 64, b = lo + lane * step;
+      const bool at = lane * step < n && min(max(off[b], 0), T) / BM + b <= t;
+      const int c = __builtin_popcountll(__ballot(at));
+      if (c == 0) return false;
+      lo += (c - 1) * step;
+      n = min(step, n - (c - 1) * step);
+      if (step == 1) break;
     }
-    k -= count;
+    rows_of(off, T, lo, s0, e0);
+    rows_of(other, To, lo, os0, oe0);
+    l = 0;
+    tile.index = t - (s0 / BM + lo);
+    tile.tiles = (e0 - s0 + BM - 1) / BM;
+    if (tile.index < 0 || tile.index >= tile.tiles) return false;
   }
-  return false;
+  tile.index = __builtin_amdgcn_readfirstlane(tile.index);
+  tile.tiles = __builtin_amdgcn_readfirstlane(tile.tiles);
+  tile.s = __builtin_amdgcn_readlane(s0, l);
+  tile.e = __builtin_amdgcn_readlane(e0, l);
+  tile.os = __builtin_amdgcn_readlane(os0, l);
+  tile.oe = __builtin_amdgcn_readlane(oe0, l);
+  return true;
+}
+
+// The tiles find_tile may give: whole ones and, for each sequence, at most one
+// that is not.
+inline int64_t tile_bound(int64_t T, int64_t B, int64_t BM) {
+  return B <= 64 ? std::min(T, T / BM + B) : T / BM + B;
 }
 
 // Loads of one LDS tile of ROWS rows by NW waves: per thread, the byte offset

@@ -193,10 +193,10 @@ int32_t launch_attention(const AttentionProblem &p, hipStream_t s) {
   a.group = (int)(p.heads / p.kv_heads);
   a.D = (int)p.D;
   a.c = p.scale * attn::kLog2e;
-  // Whole tiles and, for each sequence, at most one that is not.
-  const int64_t tiles = std::min(p.Tq, p.Tq / attn::kBM + p.B);
-  if (tiles * p.heads > 0x7fffffff)
-    return fail(NOVA_HIP_ERANGE, "attention: %lld tiles of %lld heads exceed 2^31 - 1",
+  const int64_t tiles = attn::tile_bound(p.Tq, p.B, attn::kBM);
+  // A grid's dimension holds less than 2^32 threads.
+  if (tiles * p.heads >= 1 << 24)
+    return fail(NOVA_HIP_ERANGE, "attention: %lld tiles of %lld heads exceed 2^24 - 1",
                 (long long)tiles, (long long)p.heads);
   a.tiles = (int)tiles;
   const unsigned grid = (unsigned)(tiles * p.heads);

@@ -425,8 +425,7 @@ int32_t launch_bwd(const BwdArgs &a, bool causal, int64_t qt, int64_t kt, hipStr
 
 namespace {
 int64_t padded_dim(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-// Tiles of BM rows: whole ones and, for each sequence, at most one that is not.
-int64_t tile_bound(int64_t T, int64_t B) { return std::min(T, T / attn::kBM + B); }
+int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::kBM); }
 
 // Runs of queries that a tile of keys is split into: as many as fill the chip
 // (256 workgroups at once, 512 at D <= 64), with four tiles of queries to a run
@@ -490,8 +489,9 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   a.scale = p.f.scale;
   a.splits = (int)dkv_splits(p.f.Tq, p.f.Tk, p.f.B, p.f.heads, p.f.kv_heads, p.f.D, p.f.causal);
   const int64_t qt = tile_bound(p.f.Tq, p.f.B), kt = tile_bound(p.f.Tk, p.f.B);
-  if (std::max(qt * p.f.heads, kt * p.f.kv_heads * a.splits) > 0x7fffffff)
-    return fail(NOVA_HIP_ERANGE, "attention_backward: more than 2^31 - 1 tiles");
+  // A grid's dimension holds less than 2^32 threads.
+  if (std::max(qt * p.f.heads, kt * p.f.kv_heads * a.splits) >= 1 << 24)
+    return fail(NOVA_HIP_ERANGE, "attention_backward: more than 2^24 - 1 tiles");
   return p.f.dt == NOVA_HIP_DT_BF16
              ? attn::launch_bwd<NOVA_HIP_DT_BF16>(a, p.f.causal, qt, kt, s)
              : attn::launch_bwd<NOVA_HIP_DT_F16>(a, p.f.causal, qt, kt, s);

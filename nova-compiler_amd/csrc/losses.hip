@@ -497,6 +497,12 @@ RowArgs row_args(const TokenLossProblem &p) {
 int32_t in_range(const TokenLossProblem &p, const char *w) {
   if (p.rows > 0x7fffffff - (1 << 20) || p.C > 0x7fffffff - (1 << 20))
     return fail(NOVA_HIP_ERANGE, "%s: rows or classes exceed 2^31 - 2^20", w);
+  // A grid's dimension holds less than 2^32 threads: 64 to a row of 1024 f32 or
+  // 2048 16-bit classes, at most 1024 to longer ones.
+  const int64_t threads = p.C <= (p.dt == NOVA_HIP_DT_F32 ? 1024 : 2048) ? 64 : 1024;
+  if (p.rows * threads >= (int64_t)1 << 32)
+    return fail(NOVA_HIP_ERANGE, "%s: %lld rows of %lld classes are more than one grid holds", w,
+                (long long)p.rows, (long long)p.C);
   return NOVA_HIP_SUCCESS;
 }
 

@@ -947,7 +947,7 @@ int32_t attn_common(const NovaMemRef3D *q, const NovaMemRef3D *k, const NovaMemR
     return fail(NOVA_HIP_ESTRIDE, "%s: offsets must be dense", w);
   if (!q_off->aligned || !k_off->aligned) return fail(NOVA_HIP_EINVAL, "%s: null offsets pointer", w);
   p.B = q_off->sizes[0] - 1;
-  if (p.B > (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 sequences", w);
+  if (p.B >= (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 - 1 sequences", w);
   p.q_off = reinterpret_cast<const int32_t *>(data_of(q_off)) + q_off->offset;
   p.k_off = reinterpret_cast<const int32_t *>(data_of(k_off)) + k_off->offset;
   p.lse = nullptr;
@@ -1251,7 +1251,8 @@ int32_t _mlir_ciface_nova_hip_preference_loss(
   if (n < 2 || n % 2)
     return fail(NOVA_HIP_ESHAPE, "%s: offsets must be [2 pairs + 1], at least one pair", w);
   p.pairs = n / 2;
-  if (p.pairs > (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 pairs", w);
+  // A grid's dimension holds less than 2^32 threads, 256 to a pair.
+  if (p.pairs >= (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 - 1 pairs", w);
   if (!dense_i32(offsets)) return fail(NOVA_HIP_ESTRIDE, "%s: offsets must be dense", w);
   if (!offsets->aligned) return fail(NOVA_HIP_EINVAL, "%s: null offsets pointer", w);
   if ((rc = vector_f32(ref_logp, n, w, "ref_logp")) || (rc = vector_f32(loss, 1, w, "loss")) ||

@@ -93,6 +93,17 @@ def test_attention_backward_refuses_its_own():
     assert L.nova_hip_attention_backward_scratch(-1, 4096, 1, 4, 1, 128, 0) == 0
 
 
+def test_calls_beyond_a_grid_are_refused():
+    # 2^20 one-token sequences of 32 heads: 2^25 tiles.
+    n = 1 << 20
+    q, off = d((n, 32, 64)), d((n + 1,))
+    kw = dict(q=q, k=d((n, 2, 64)), v=d((n, 2, 64)), qo=off, ko=off, out=q, lse=d((32, n)))
+    assert fwd(**kw) == ERANGE
+    assert bwd(**kw, go=q, dq=q, dk=d((n, 2, 64)), dv=d((n, 2, 64)), scratch=d((1 << 40,))) == ERANGE
+    assert logp(x=d((1 << 26, 4)), y=d((1 << 26,)), logp=d((1 << 26,))) == ERANGE
+    assert logp(x=d((1 << 22, 5000)), y=d((1 << 22,)), logp=d((1 << 22,))) == ERANGE
+
+
 def test_attention_empty_calls_do_nothing():
     none = dict(q=d((0, 4, 64), ptr=0), out=d((0, 4, 64), ptr=0), lse=d((4, 0), ptr=0))
     assert fwd(**none) == 0

@@ -152,3 +152,21 @@ def test_against_differences_of_the_forward(cuda):
         # Rounded weights and dS: their sums err by at most the same again.
         noise = 6 * 2 * u * ((grads[i].double() * d) ** 2).sum().sqrt().item() + 6 * u * d.norm().item()
         assert abs(ours - numeric) <= noise + 1e-6 * abs(numeric), (i, ours, numeric, noise)
+
+
+@pytest.mark.parametrize("B", [64, 65, 200])
+def test_many_sequences(cuda, B):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 4, (B,), generator=g).tolist()
+    for i, n in ((0, 150), (B // 2, 130), (B - 1, 129)):
+        lens[i] = n
+    run(cuda, lens, lens, 4, 2, 64, BF, True, pad=2)
+
+
+def test_split_runs_of_queries(cuda):
+    """Few tiles of keys under many queries are split into runs whose sums are
+    joined: head groups, ragged and empty ends among them."""
+    assert nh.lib().nova_hip_attention_backward_scratch(1500, 700, 2, 4, 1, 64, 1) > 2 * 4 * 1500
+    run(cuda, [1300, 200], [500, 200], 4, 1, 64, BF, True, pad=1)
+    run(cuda, [1300, 200], [500, 200], 4, 1, 128, HF, False)
+    run(cuda, [1100], [1100], 2, 2, 128, BF, True)

@@ -174,3 +174,52 @@ def test_rows_of_other_sequences_do_not_leak(cuda):
 
 def test_long_sequence(cuda):
     run(cuda, [2500], [4001], 2, 1, 128, BF, True)
+
+
+@pytest.mark.parametrize("B", [63, 64, 65, 128, 200, 4100])
+def test_many_sequences(cuda, B):
+    """Around the 64 sequences that are searched in registers, and far beyond:
+    lengths 0 to 3 and a few long ones, first, last and in the middle."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 4, (B,), generator=g).tolist()
+    for i, n in ((0, 150), (B // 2, 130), (B - 1, 129)):
+        lens[i] = n
+    if B < 1000:
+        for causal in (False, True):
+            run(cuda, lens, lens, 2, 1, 64, BF, causal, pad=2)
+        return
+    # The reference takes a loop turn per sequence: whole sequences of one batch
+    # against the same ones alone.
+    q, k, v = make(cuda, lens, lens, 2, 1, 64, BF)
+    out, lse = nh.attention(q, k, v, offsets(lens, cuda), offsets(lens, cuda))
+    start = [0]
+    for n in lens:
+        start.append(start[-1] + n)
+    for i in (0, 1, 2, 63, 64, 65, B // 2, B - 2, B - 1):
+        sl = slice(start[i], start[i + 1])
+        check(out[sl], lse[:, sl], q[sl], k[sl], v[sl], [lens[i]], [lens[i]], True, 0.125, i)
+    one = offsets([1] * B, cuda)
+    q1, k1, v1 = make(cuda, [1] * B, [1] * B, 2, 1, 64, BF)
+    out, _ = nh.attention(q1, k1, v1, one, one)  # a row that sees itself alone is its value
+    assert torch.equal(out, v1.expand(B, 2, 64))
+
+
+@pytest.mark.parametrize("bad", [[5, 2 ** 31 - 1, -7, 40], [-9, 20, 10, 10 ** 9], [60, 0, 60, 0],
+                                 [0] + [60, 0] * 40])
+def test_offsets_outside_the_operands(cuda, bad):
+    """Sequences are cut to the operands' rows: nothing else is read or written."""
+    H, G, D, T = 2, 1, 64, 60
+    guard = 64
+    q = torch.randn(T + 2 * guard, H, D, device=cuda).to(BF)
+    kv = torch.randn(T + 2 * guard, G, D, device=cuda).to(BF)
+    out = torch.full_like(q, 7.0)
+    off = torch.tensor(bad, dtype=torch.int32, device=cuda)
+    mid = slice(guard, guard + T)
+    lse = torch.full((H, T), 7.0, device=cuda)
+    nh.attention(q[mid], kv[mid], kv[mid], off, off, out=out[mid], lse=lse)
+    d = [torch.full_like(t, 7.0) for t in (q, kv, kv)]
+    nh.attention_backward(q[mid], q[mid], kv[mid], kv[mid], out[mid], lse, off, off, dq=d[0][mid],
+                          dk=d[1][mid], dv=d[2][mid])
+    torch.cuda.synchronize()
+    for t in [out] + d:
+        assert (t[:guard] == 7.0).all() and (t[guard + T:] == 7.0).all()
