@@ -193,8 +193,9 @@ struct TileLoad {
   uint32_t off;   // of the thread's first chunk, or kOOB
   uint32_t step;  // bytes to the next one
 
+  // By threads 0 .. 64 NW - 1 of each group of that many.
   __device__ __forceinline__ void init(int64_t stride, int D) {
-    const int slot = threadIdx.x, row = slot / CH, c = (slot & (CH - 1)) ^ swz<CH>(row);
+    const int slot = threadIdx.x % (64 * NW), row = slot / CH, c = (slot & (CH - 1)) ^ swz<CH>(row);
     off = c * 8 < D ? (uint32_t)(row * stride + c * 8) * 2u : kOOB;
     step = (uint32_t)(kStep * stride) * 2u;
   }
@@ -204,7 +205,7 @@ struct TileLoad {
     const int n = min(rows, ROWS);
     const uint32_t bytes = n > 0 ? ((uint32_t)(n - 1) * (uint32_t)stride + D) * 2u : 0u;
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(p, bytes);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % NW;
 #pragma unroll
     for (int i = 0; i < kN; ++i)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(

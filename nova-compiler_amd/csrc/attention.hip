@@ -7,6 +7,14 @@
 // when one is more than 2^8 above it (the factor is exact either way, and
 // f32 sums and 16-bit weights have that much room), so most tiles multiply no
 // accumulator.
+//
+// Four waves hold 32 queries each and stream tiles of 64 keys and values through
+// a two-stage ring in LDS filled by DMA; two workgroups share a CU at D = 128
+// (230 registers), so that one's exponentials run beside the other's products.
+// What bounds it: at D = 128 the matrix cores and the board's power (8192 causal
+// tokens, 32 heads: 535 us, 1.03 PFLOP/s, where a plain 8192^3 product of the
+// library reaches 1.40 and a 4096^3 one 1.17); at D = 64 the exponentials and
+// the rest of the softmax (2 x 4096 tokens, 32 heads: 337 us, 0.82 PFLOP/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,19 +39,25 @@ struct FwdArgs {
 constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
 constexpr float kSlack = 8.0f;  // m c may lag the largest score by this much
 
-template <int DT, int DP, bool CAUSAL>
-__global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a) {
+// KS groups of four waves share a tile of queries: group g takes the tiles of
+// keys g, g + KS, ... through a ring of its own, and the groups' sums are joined
+// at the end.  Two where the chip holds every tile of queries at once and waits
+// for the longest (see launch_fwd).
+template <int DT, int DP, bool CAUSAL, int KS>
+__global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_fwd_kernel(FwdArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sk0_[kTile];
-  lds_char *const sk0 = (lds_char *)sk0_;
-  __shared__ __attribute__((aligned(1024))) char sk1_[kTile];
-  lds_char *const sk1 = (lds_char *)sk1_;
-  __shared__ __attribute__((aligned(1024))) char sv0_[kTile];
-  lds_char *const sv0 = (lds_char *)sv0_;
-  __shared__ __attribute__((aligned(1024))) char sv1_[kTile];
-  lds_char *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
+  const int part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWaves;
+  __shared__ float sm[KS > 1 ? kWaves : 1][32], sl[KS > 1 ? kWaves : 1][32];
+  __shared__ __attribute__((aligned(1024))) char sk0_[KS * kTile];
+  lds_char *const sk0 = (lds_char *)sk0_ + part * kTile;
+  __shared__ __attribute__((aligned(1024))) char sk1_[KS * kTile];
+  lds_char *const sk1 = (lds_char *)sk1_ + part * kTile;
+  __shared__ __attribute__((aligned(1024))) char sv0_[KS * kTile];
+  lds_char *const sv0 = (lds_char *)sv0_ + part * kTile;
+  __shared__ __attribute__((aligned(1024))) char sv1_[KS * kTile];
+  lds_char *const sv1 = (lds_char *)sv1_ + part * kTile;
   int head, tile;
   unit_of(blockIdx.x, a.heads, a.tiles, CAUSAL, head, tile);
   Tile at;
@@ -134,18 +148,54 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's DMA has landed
     __syncthreads();
   };
-  if (nt > 0) fetch(0, sk0, sv0);
-  for (int t = 0; t < nt; t += 2) {
+  // Every group takes as many turns; one behind the last tile does nothing.
+  const int nu = (nt + KS - 1) / KS;
+  auto turn = [&](int u, const lds_char *sk, const lds_char *sv) __attribute__((always_inline)) {
+    if (KS == 1 || u * KS + part < nt) step(u * KS + part, sk, sv);
+  };
+  if (nu > 0) fetch(part, sk0, sv0);
+  for (int u = 0; u < nu; u += 2) {
     sync();
-    if (t + 1 < nt) fetch(t + 1, sk1, sv1);
-    step(t, sk0, sv0);
-    if (t + 1 >= nt) break;
+    if (u + 1 < nu) fetch((u + 1) * KS + part, sk1, sv1);
+    turn(u, sk0, sv0);
+    if (u + 1 >= nu) break;
     sync();
-    if (t + 2 < nt) fetch(t + 2, sk0, sv0);
-    step(t + 1, sk1, sv1);
+    if (u + 2 < nu) fetch((u + 2) * KS + part, sk0, sv0);
+    turn(u + 1, sk1, sv1);
+  }
+  l = both_sum(l);
+  if constexpr (KS > 1) {
+    static_assert(KS == 2 && KS * kTile >= kWaves * 64 * 16 * 4, "one block of each wave's sums");
+    lds_float *const box = (lds_float *)(lds_char *)sk0_ + wave * 1024 + lane;
+    __syncthreads();
+    if (part == 1 && lane < 32) {
+      sm[wave][lane] = mc;
+      sl[wave][lane] = l;
+    }
+    float mine = 0.0f, other = 0.0f;  // factors of the two groups' sums
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      if (i) __syncthreads();
+      if (part == 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) box[64 * r] = acc[i][r];
+      }
+      __syncthreads();
+      if (part == 0) {
+        if (i == 0) {
+          const float m1 = sm[wave][lane & 31], to = fmaxf(mc, m1);
+          mine = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - to);
+          other = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - to);
+          l = l * mine + sl[wave][lane & 31] * other;
+          mc = to;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = acc[i][r] * mine + box[64 * r] * other;
+      }
+    }
+    if (part == 1) return;
   }
   if (qn <= 0) return;
-  l = both_sum(l);
   // A row that sees no key is zero, its lse -inf.
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   store_rows<DT, DP>(acc, inv, a.o + (qs + q0) * a.so.t + head * a.so.h, a.so.t, qn, a.D, lane);
@@ -153,12 +203,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_fwd_kernel(FwdArgs a
     a.lse[head * a.slse + qs + q0 + lane] = l == 0.0f ? -INFINITY : (mc + __log2f(l)) * kLn2;
 }
 
+template <int DT, int DP, int KS>
+void launch_fwd_k(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {
+  if (causal)
+    hipLaunchKernelGGL((attention_fwd_kernel<DT, DP, true, KS>), dim3(grid), dim3(64 * kWaves * KS),
+                       0, s, a);
+  else
+    hipLaunchKernelGGL((attention_fwd_kernel<DT, DP, false, KS>), dim3(grid), dim3(64 * kWaves * KS),
+                       0, s, a);
+}
 template <int DT, int DP>
 void launch_fwd(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {
-  if (causal)
-    hipLaunchKernelGGL((attention_fwd_kernel<DT, DP, true>), dim3(grid), dim3(64 * kWaves), 0, s, a);
-  else
-    hipLaunchKernelGGL((attention_fwd_kernel<DT, DP, false>), dim3(grid), dim3(64 * kWaves), 0, s, a);
+  // Two groups while one workgroup of them per CU (of causal ones, whose work
+  // differs, two at D <= 64) holds all tiles.  One group against two, us: 1000
+  // causal tokens of 6 heads of 64 18.1 / 15.6, packed 1 to 4096 of these heads
+  // (432 tiles) 62.7 / 50.2, 3000 of 8 heads of 128 57.9 / 47.1; beyond, 4 x
+  // 1024 of 12 heads of 128 (432 tiles) 37.6 / 45.0.
+  const unsigned few = causal && a.D <= 64 ? 512 : 256;
+  if (grid <= few) launch_fwd_k<DT, DP, 2>(a, causal, grid, s);
+  else launch_fwd_k<DT, DP, 1>(a, causal, grid, s);
 }
 template <int DT>
 void launch_fwd(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {

@@ -508,12 +508,15 @@ int32_t in_range(const TokenLossProblem &p, const char *w) {
 
 template <int DT>
 void launch_grad_t(const GradArgs &a, hipStream_t s) {
-  // A wave per row as long as four strides of it cover the row.
+  // A wave per row as long as four strides of it cover the row; 1024 threads to
+  // the longest (8192 x 50304 bf16: 324 us, 330 with 512, 341 with 256).
   if (a.C <= 256 * Chunk<DT>::kE)
     hipLaunchKernelGGL((logits_grad_kernel<DT, 64>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 0,
                        s, a);
-  else
+  else if (a.C <= 2048 * Chunk<DT>::kE)
     hipLaunchKernelGGL((logits_grad_kernel<DT, 512>), dim3((unsigned)a.rows), dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((logits_grad_kernel<DT, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, s, a);
 }
 
 }  // namespace
