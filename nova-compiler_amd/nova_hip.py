@@ -10,6 +10,11 @@ i.e. batch matmul), ``linear`` (+ GELU epilogue), ``layer_norm`` and ``sce``
 * ``sce`` returns ``(softmax, loss)`` with ``loss`` of shape [1]
   (NovaOps.td:880-896, NovaToLinalgGeneric.cpp:1008).
 
+Beside them, without a reference counterpart: ``attention`` of packed
+sequences with its backward and its form for single tokens, and the losses
+over token log-probabilities (``token_logp``, ``policy_loss``,
+``preference_loss``).
+
 Tensors are torch tensors on the GPU; each call passes MLIR strided-memref
 descriptors built from the tensors' data pointers, sizes and strides, and
 launches on torch's current stream.  There is no fallback: if the library is
