@@ -14,7 +14,7 @@
 //
 // What bounds them at D = 128 (2 x 4096 tokens, 32 heads, not causal): the matrix
 // cores and the board's power for dQ (755 us, 1.09 PFLOP/s of its three
-// products), the issue of one wave per SIMD for dK and dV (1230 us, 0.89 of
+// products), the issue of one wave per SIMD for dK and dV (1045 us, 1.05 of
 // four).
 #include <hip/hip_runtime.h>
 
@@ -277,7 +277,6 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (kMask && q0 + 32 * i + 31 + shift < k0) continue;  // none of these sees these keys
-        if (i) __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_iglp_opt(0);  // a product, an LDS read, a product, ...
         f32x16 s = {}, dp;
 #pragma unroll
@@ -325,6 +324,13 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
     };
     fetch(sq0, sg0, sc0);
     for (int u = lo; u < hi; u += 2) {
+      if constexpr (DP > 64) {
+        // The gradients stay in the accumulation registers: left to the compiler
+        // they moved between the files in each tile (2 x 4096 tokens, not causal,
+        // 32 heads of 128: 1310 -> 1045 us).
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+a"(dk[i]), "+a"(dv[i]));
+      }
       sync();
       if (u + 1 < hi) fetch(sq1, sg1, sc1);
       step(sq0, sg0, sc0);
