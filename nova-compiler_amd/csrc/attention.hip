@@ -219,8 +219,10 @@ void launch_fwd(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {
   // causal tokens of 6 heads of 64 18.1 / 15.6, packed 1 to 4096 of these heads
   // (432 tiles) 62.7 / 50.2, 3000 of 8 heads of 128 57.9 / 47.1; beyond, 4 x
   // 1024 of 12 heads of 128 (432 tiles) 37.6 / 45.0.
+  // Not for sequences of less than eight tiles of keys in the mean, which lose
+  // to the join what they gain (8 x 197 of 12 heads of 64: 8.7 / 9.2).
   const unsigned few = causal && a.D <= 64 ? 512 : 256;
-  if (grid <= few) launch_fwd_k<DT, DP, 2>(a, causal, grid, s);
+  if (grid <= few && a.Tk / a.B >= 8 * kBN) launch_fwd_k<DT, DP, 2>(a, causal, grid, s);
   else launch_fwd_k<DT, DP, 1>(a, causal, grid, s);
 }
 template <int DT>

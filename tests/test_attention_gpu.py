@@ -176,6 +176,55 @@ def test_long_sequence(cuda):
     run(cuda, [2500], [4001], 2, 1, 128, BF, True)
 
 
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_keys_shared_by_two_groups_of_waves(cuda, D, causal):
+    """Few tiles of queries over long keys: odd numbers of tiles of keys, rows
+    that see none, sequences without any."""
+    run(cuda, [1000, 0, 70, 5], [1500, 700, 3, 1], 2, 1, D, HF, causal, pad=1)
+    run(cuda, [900], [577], 3, 3, D, BF, causal)
+
+
+def test_long_sequences_of_many_heads(cuda):
+    run(cuda, [700, 600], [700, 600], 64, 8, 64, BF, True, "fused")
+    run(cuda, [700, 600], [700, 600], 64, 64, 128, BF, False)
+
+
+def test_no_keys_or_no_queries_at_all(cuda):
+    for qlens, klens in (([5, 3], [0, 0]), ([0, 0], [4, 70])):
+        q, k, v = make(cuda, qlens, klens, 2, 1, 64, BF)
+        qo, ko = offsets(qlens, cuda), offsets(klens, cuda)
+        out, lse = nh.attention(q, k, v, qo, ko)
+        assert (out == 0).all() and torch.isinf(lse).all()
+        dq, dk, dv = nh.attention_backward(q, q, k, v, out, lse, qo, ko)
+        assert all((t == 0).all() for t in (dq, dk, dv))
+        assert dq.shape == q.shape and dk.shape == k.shape
+
+
+def test_strides_far_apart(cuda):
+    """Rows 2^22 elements apart (8 MB), the largest stride's half: offsets inside
+    a tile of 64 or 128 rows stay in range; heads past 2^32 bytes."""
+    n, D, step = 130, 64, 1 << 22
+    flat = torch.empty(n * step + (1 << 31) + 4096, dtype=BF, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(1)
+
+    def view(T, heads):
+        x = flat.as_strided((T, heads, D), (step, (1 << 31) // 2 + 64, 1))
+        for h in range(heads):
+            x[:, h] = torch.randn(T, D, generator=g, device=cuda).to(BF)
+        return x
+
+    k = view(n, 2)
+    q = torch.randn(n, 2, D, generator=g, device=cuda).to(BF)
+    off = offsets([n], cuda)
+    out, lse = nh.attention(q, k, k, off, off)
+    check(out, lse, q, k, k, [n], [n], True, 0.125)
+    a = nh.attention_backward(q, q, k, k, out, lse, off, off)
+    kc = k.contiguous()
+    b = nh.attention_backward(q, q, kc, kc, out, lse, off, off)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 @pytest.mark.parametrize("B", [63, 64, 65, 128, 200, 4100])
 def test_many_sequences(cuda, B):
     """Around the 64 sequences that are searched in registers, and far beyond:

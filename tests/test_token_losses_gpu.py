@@ -297,3 +297,25 @@ def test_gradients_against_differences(cuda):
         scale = (grad.double() * d).abs().sum().item()
         # f32 gradients: 3e-5 of each term; the difference: h^2 and 64-bit noise / h.
         assert abs(ours - num) <= 3e-5 * scale + 1e-8, (ours, num)
+
+
+def test_rows_far_apart(cuda):
+    """Rows 2^31 elements apart: a row's offset passes 32 bits in elements and
+    bytes, in the logits and in the gradient."""
+    C, step = 3000, 1 << 31
+    flat = torch.empty(2 * step + C, dtype=BF, device=cuda)
+    far = flat.as_strided((3, C), (step, 1))
+    x, y, g = make(cuda, 3, C, BF, masked=0)
+    one = torch.ones(3, device=cuda)
+    lp = nh.token_logp(x, y)
+    want = nh.policy_loss(x, y, lp - 0.1, one, one)
+    off = torch.tensor([0, 1, 3], dtype=torch.int32, device=cuda)
+    pref = nh.preference_loss(x, y, off, one[:2])
+    far.copy_(x)
+    assert torch.equal(nh.token_logp(far, y), lp)
+    assert all(torch.equal(a, b) for a, b in zip(nh.policy_loss(far, y, lp - 0.1, one, one), want))
+    assert all(torch.equal(a, b) for a, b in zip(nh.preference_loss(far, y, off, one[:2]), pref))
+    nh.policy_loss(x, y, lp - 0.1, one, one, grad=far)
+    assert torch.equal(far, want[2])
+    nh.preference_loss(x, y, off, one[:2], grad=far)
+    assert torch.equal(far, pref[2])
