@@ -419,8 +419,9 @@ int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D
  *   lse : [heads, query tokens] f32, log sum exp of the scaled scores, or
  *   NULL.
  * Scores, softmax and sums are f32; the weights are rounded to dt for the
- * product with v.  Rows outside every sequence are left as they were.  No
- * workspace: concurrent calls and captured graphs share nothing.
+ * product with v.  Rows outside every sequence are left as they were; out must
+ * not overlap q, k or v.  No workspace: concurrent calls and captured graphs
+ * share nothing.
  * ---------------------------------------------------------------------- */
 int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3D *k,
                                         const NovaMemRef3D *v, const NovaMemRef1D *q_offsets,
@@ -434,10 +435,12 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
  * dk and dv summed over the query heads that share a key head.  Shapes and
  * strides as for the forward (grad_out, out, dq as q; dk, dv as k); lse
  * [heads, query tokens]; scratch : at least
- * nova_hip_attention_backward_scratch() f32, dense, used by this call only.  P and dS are rounded to dt for the
- * products, sums are f32 in a fixed order (no atomics: the same bits on every
- * run).  A query that sees no key has gradient zero and adds none; rows
- * outside every sequence are left as they were. */
+ * nova_hip_attention_backward_scratch() f32, dense, used by this call only.  dq,
+ * dk and dv must not overlap the other operands or each other (views of one
+ * buffer are apart).  P and dS are rounded to dt for the products (an f16 dS
+ * beyond 65504 is an infinity), sums are f32 in a fixed order (no atomics: the
+ * same bits on every run).  A query that sees no key has gradient zero and
+ * adds none; rows outside every sequence are left as they were. */
 int32_t _mlir_ciface_nova_hip_attention_backward(
     const NovaMemRef3D *grad_out, const NovaMemRef3D *q, const NovaMemRef3D *k,
     const NovaMemRef3D *v, const NovaMemRef3D *out, const NovaMemRef2D *lse,
@@ -469,7 +472,8 @@ int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int6
  * Losses over token log-probabilities (HBM bound), beside nova.sce.  No
  * reference counterpart.  For all three:
  *   logits, grad : [R, C] of dt NOVA_HIP_DT_F32, _BF16 or _F16; any row
- *   stride; grad must not overlap logits; labels : [R] i32.
+ *   stride; grad must not overlap logits (column ranges of the same rows are
+ *   apart); labels : [R] i32.
  * A row with a negative label (a prompt token, padding) takes no part: its
  * logits are not read, its log-probability is 0 and its gradient row zero.  A
  * label of C or more makes the row's results NaN.  Row results and sums are

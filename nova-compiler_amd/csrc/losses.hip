@@ -402,7 +402,7 @@ struct GradArgs {
   const void *logits;
   void *grad;
   const int32_t *labels;
-  const float *lse, *slope;
+  const float *logp, *lse, *slope;
   int64_t sx, sg;
   int rows, C, pairs;
   const float *pair_loss;
@@ -428,8 +428,15 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH) void logits_grad_kernel(GradAr
   T *g = static_cast<T *>(a.grad) + row * a.sg;
   const int nc = a.C / X::kE, tail = a.C - nc * X::kE;
   const bool none = slope == 0.0f;  // the logits are not read
+  // log p = x - lse, or (x - x[y]) + lp where that is the smaller number: an lse
+  // of 10^4 is rounded by 2^-11, and the probabilities with it.
+  float pivot = lse, add = 0.0f;
+  if (fabsf(lse) > 64.0f && !none && y < a.C && fabsf(a.logp[row]) < fabsf(lse)) {
+    pivot = X::widen(x[y]);
+    add = a.logp[row];
+  }
   auto value = [&](float xv, int64_t col) __attribute__((always_inline)) {
-    const float p = -slope * exp_diff(xv, lse);
+    const float p = -slope * __builtin_amdgcn_exp2f(((xv - pivot) + add) * kL2e);
     return col == y ? p + slope : p;
   };
 #pragma unroll 4
@@ -573,7 +580,7 @@ int32_t launch_preference_loss(const PreferenceProblem &p, hipStream_t s) {
   if (!grad)
     return launch_loss_sum(p.pair_loss, p.pairs, 1.0 / (double)p.pairs, p.loss,
                            "preference_loss sum launch", s);
-  const GradArgs g = {p.t.logits, p.t.grad, p.t.labels, p.lse, p.slope, p.t.sx, p.t.sg,
+  const GradArgs g = {p.t.logits, p.t.grad, p.t.labels, p.logp, p.lse, p.slope, p.t.sx, p.t.sg,
                       (int)p.t.rows, (int)p.t.C, (int)p.pairs, p.pair_loss, p.loss};
   if (p.t.dt == NOVA_HIP_DT_F32) launch_grad_t<NOVA_HIP_DT_F32>(g, s);
   else if (p.t.dt == NOVA_HIP_DT_BF16) launch_grad_t<NOVA_HIP_DT_BF16>(g, s);

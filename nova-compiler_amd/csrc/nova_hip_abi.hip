@@ -1177,6 +1177,18 @@ int32_t token_common(const NovaMemRef2D *logits, const NovaMemRef1D *labels, Nov
   return NOVA_HIP_SUCCESS;
 }
 
+// The gradient apart from the logits, or column ranges of the same rows.
+int32_t grad_apart(const TokenLossProblem &p, const char *w) {
+  if (!p.grad || p.rows == 0) return NOVA_HIP_SUCCESS;
+  const int64_t sz = dtype_size(p.dt), sx = p.rows > 1 ? p.sx : p.C, sg = p.rows > 1 ? p.sg : p.C;
+  const intptr_t x = reinterpret_cast<intptr_t>(p.logits), g = reinterpret_cast<intptr_t>(p.grad);
+  if (x >= g + ((p.rows - 1) * sg + p.C) * sz || g >= x + ((p.rows - 1) * sx + p.C) * sz)
+    return NOVA_HIP_SUCCESS;
+  const int64_t pitch = sx * sz, row = p.C * sz, at = ((g - x) % pitch + pitch) % pitch;
+  if (sx == sg && at >= row && pitch - at >= row) return NOVA_HIP_SUCCESS;
+  return fail(NOVA_HIP_EINVAL, "%s: grad overlaps logits", w);
+}
+
 // A dense f32 vector of n values.
 int32_t vector_f32(const NovaMemRef1D *d, int64_t n, const char *w, const char *what) {
   int32_t rc = dense1(d, w, what);
@@ -1233,6 +1245,7 @@ int32_t _mlir_ciface_nova_hip_policy_loss(
   p.clip_high = clip_high;
   p.kl_coef = kl_coef;
   p.grad_scale = grad_scale;
+  if ((rc = grad_apart(p.t, w))) return rc;
   return launch_policy_loss(p, current_stream());
 }
 
@@ -1280,6 +1293,7 @@ int32_t _mlir_ciface_nova_hip_preference_loss(
   p.beta = beta;
   p.smoothing = smoothing;
   p.grad_scale = grad_scale;
+  if ((rc = grad_apart(p.t, w))) return rc;
   return launch_preference_loss(p, current_stream());
 }
 

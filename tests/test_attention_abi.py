@@ -210,6 +210,19 @@ def test_losses_refuse_their_own(f, want, kw):
     assert f(**kw) == want, nh.lib().nova_hip_last_error()
 
 
+@pytest.mark.parametrize("f", [policy, pref])
+@pytest.mark.parametrize("kw", [
+    dict(grad=d((6, 100))), dict(grad=d((6, 100), ptr=FAKE + 4 * 599)),
+    dict(x=d((6, 100), ptr=FAKE + 4 * 599)),
+    dict(grad=d((6, 100), (150, 1), ptr=FAKE + 400)),            # other row strides
+    dict(x=d((6, 100), (200, 1)), grad=d((6, 100), (200, 1), ptr=FAKE + 4 * 99)),
+    dict(x=d((6, 100), (200, 1)), grad=d((6, 100), (200, 1), ptr=FAKE + 4 * 101)),
+    dict(x=d((6, 100), (200, 1), ptr=FAKE + 4 * 301), grad=d((6, 100), (200, 1))),
+])
+def test_gradients_on_the_logits_are_refused(f, kw):
+    assert f(**kw) == EINVAL and b"overlaps" in nh.lib().nova_hip_last_error()
+
+
 # ---- the Python wrappers' own checks ---------------------------------------------------------
 
 def test_wrappers_refuse_before_the_call():

@@ -319,3 +319,29 @@ def test_rows_far_apart(cuda):
     assert torch.equal(far, want[2])
     nh.preference_loss(x, y, off, one[:2], grad=far)
     assert torch.equal(far, pref[2])
+
+
+@pytest.mark.parametrize("C", [100, 5000, 50304, 60000])
+@pytest.mark.parametrize("shift", [8192.0, -8192.0])
+def test_logits_far_from_zero(cuda, C, shift):
+    """Logits that are multiples of 2^-9 keep their exact differences 8192 away
+    from zero, so log-probabilities and gradients keep the bounds of the logits
+    around zero: |x - x_y| and |lp| stay under 40, and 2^-23 of those within the
+    2e-5 the bounds leave to a softmax value.  (The lse itself rounds by 2^-11.)"""
+    x, y, _ = make(cuda, 12, C, F32, seed=C)
+    x = (x * 512).round() / 512
+    y[0], y[7] = 3, C - 1  # a label in each sequence
+    lp, p, dist, ok = rows64(x, y)
+    assert dist.max() < 20 and lp.abs().max() < 40
+    far = x + shift
+    assert torch.equal(far - shift, x)
+    assert ((nh.token_logp(far, y).double() - lp).abs() <= lp_tol(lp, dist) * ok).all()
+    off = torch.tensor([0, 6, 12], dtype=torch.int32, device=cuda)
+    ref = torch.stack([lp[:6].sum(), lp[6:].sum()]).float()
+    token = torch.empty(3, 12, device=cuda)
+    _, _, grad = nh.preference_loss(far, y, off, ref, token=token)
+    slope = token[2].double()
+    check_grad(grad, slope, slope.abs() * 2e-5, p, y, ok)
+    one = torch.ones(12, device=cuda)
+    _, _, grad = nh.policy_loss(far, y, lp.float(), one, one)
+    check_grad(grad, -torch.ones_like(lp), lp_tol(lp, dist) + 2.0 ** -24 * lp.abs() + 2.0 ** -22, p, y, ok)
