@@ -7,10 +7,11 @@
 // in a fixed order: no atomics, the same bits on every run, and the gradients of
 // keys shared by a group of query heads are summed over the group inside the
 // workgroup (or, where its queries are split into runs, over the runs in order
-// by a third kernel).  That is seven products where five are the least.  attention_dq_kernel holds 32
-// queries per wave and streams keys and values; it also writes the rows' two
-// constants (lse in base 2, delta), which attention_dkv_kernel, behind it on
-// the stream, reads while it holds keys and values and streams Q and dO.
+// by a third kernel).  That is seven products where five are the least.
+// attention_dq_kernel holds 32 queries per wave and streams keys and values; it
+// also writes the rows' two constants (lse in base 2, delta), which
+// attention_dkv_kernel, behind it on the stream, reads while it holds keys and
+// values and streams Q and dO.
 //
 // What bounds them at D = 128 (2 x 4096 tokens, 32 heads, not causal): the matrix
 // cores and the board's power for dQ (755 us, 1.09 PFLOP/s of its three
@@ -75,19 +76,43 @@ __device__ __forceinline__ float row_dot(const u32x4 (&x)[DP / 16], const u32x4 
   return both_sum(s);
 }
 
-template <int DT, int DP, bool CAUSAL>
-__global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a) {
+// Adds the second group of waves' sums to the first's, block by block through
+// 16 KB of LDS, all of whose readers are done when every wave has come here.
+template <int DP>
+__device__ __forceinline__ void add_group(f32x16 (&acc)[DP / 32], lds_char *lds, int wave, int part,
+                                          int lane) {
+  lds_float *const box = (lds_float *)lds + wave * 1024 + lane;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) {
+    __syncthreads();
+    if (part == 1) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) box[64 * r] = acc[i][r];
+    }
+    __syncthreads();
+    if (part == 0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][r] += box[64 * r];
+    }
+  }
+}
+
+// KS groups of four waves share a tile of queries, as in the forward: group g
+// takes the tiles of keys g, g + KS, ... and the groups' sums are added at the end.
+template <int DT, int DP, bool CAUSAL, int KS>
+__global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_dq_kernel(BwdArgs a) {
   constexpr int CH = kPitch<DP>, kTile = kBN * CH * 16;
-  __shared__ __attribute__((aligned(1024))) char sk0_[kTile];
-  lds_char *const sk0 = (lds_char *)sk0_;
-  __shared__ __attribute__((aligned(1024))) char sk1_[kTile];
-  lds_char *const sk1 = (lds_char *)sk1_;
-  __shared__ __attribute__((aligned(1024))) char sv0_[kTile];
-  lds_char *const sv0 = (lds_char *)sv0_;
-  __shared__ __attribute__((aligned(1024))) char sv1_[kTile];
-  lds_char *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWaves;
+  const int part = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWaves;
+  __shared__ __attribute__((aligned(1024))) char sk0_[KS * kTile];
+  lds_char *const sk0 = (lds_char *)sk0_ + part * kTile;
+  __shared__ __attribute__((aligned(1024))) char sk1_[KS * kTile];
+  lds_char *const sk1 = (lds_char *)sk1_ + part * kTile;
+  __shared__ __attribute__((aligned(1024))) char sv0_[KS * kTile];
+  lds_char *const sv0 = (lds_char *)sv0_ + part * kTile;
+  __shared__ __attribute__((aligned(1024))) char sv1_[KS * kTile];
+  lds_char *const sv1 = (lds_char *)sv1_ + part * kTile;
   int head, tile;
   unit_of(blockIdx.x, a.heads, a.tiles, CAUSAL, head, tile);
   Tile place;
@@ -112,7 +137,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
     const float lse = a.lse[head * a.slse + qs + q0 + (lane & 31)];
     // A row without keys (lse -inf): every weight is masked below.
     nl = lse == -INFINITY ? 0.0f : lse * kLog2e;
-    if (lane < 32) {
+    if (lane < 32 && part == 0) {
       a.rows[at] = nl - kWeightLog2<DT>;
       a.rows[(int64_t)a.heads * a.Tq + at] = -delta;
     }
@@ -168,15 +193,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attention_dq_kernel(BwdArgs a)
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __syncthreads();
   };
-  if (nt > 0) fetch(0, sk0, sv0);
-  for (int t = 0; t < nt; t += 2) {
+  // Every group takes as many turns; one behind the last tile does nothing.
+  const int nu = (nt + KS - 1) / KS;
+  auto turn = [&](int u, const lds_char *sk, const lds_char *sv) __attribute__((always_inline)) {
+    if (KS == 1 || u * KS + part < nt) step(u * KS + part, sk, sv);
+  };
+  if (nu > 0) fetch(part, sk0, sv0);
+  for (int u = 0; u < nu; u += 2) {
     sync();
-    if (t + 1 < nt) fetch(t + 1, sk1, sv1);
-    step(t, sk0, sv0);
-    if (t + 1 >= nt) break;
+    if (u + 1 < nu) fetch((u + 1) * KS + part, sk1, sv1);
+    turn(u, sk0, sv0);
+    if (u + 1 >= nu) break;
     sync();
-    if (t + 2 < nt) fetch(t + 2, sk0, sv0);
-    step(t + 1, sk1, sv1);
+    if (u + 2 < nu) fetch((u + 2) * KS + part, sk0, sv0);
+    turn(u + 1, sk1, sv1);
+  }
+  if constexpr (KS > 1) {
+    static_assert(KS == 2, "one group hands its sums to the other");
+    add_group<DP>(acc, (lds_char *)sk0_, wave, part, lane);
+    if (part == 1) return;
   }
   if (qn <= 0) return;
   store_rows<DT, DP>(acc, a.scale, a.dq + (qs + q0) * a.sdq.t + head * a.sdq.h, a.sdq.t, qn, a.D,
@@ -401,8 +436,19 @@ template <int DT, int DP, bool CAUSAL>
 int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s) {
   if (q_tiles > 0) {
     a.tiles = (int)q_tiles;
-    hipLaunchKernelGGL((attention_dq_kernel<DT, DP, CAUSAL>), dim3((unsigned)(q_tiles * a.heads)),
-                       dim3(64 * kWaves), 0, s, a);
+    const unsigned grid = (unsigned)(q_tiles * a.heads);
+    // Two groups while the chip, which holds two workgroups of one group per CU,
+    // holds every tile at once and waits for the longest.  The whole backward
+    // with one group and with two, us, 2048 causal tokens of 6 heads of 64 70.5 /
+    // 65.3, packed 1 to 4096 of these 137.7 / 121.4, 2048 of 8 heads of 128 120 /
+    // 106; beyond, 8 x 1024 not causal of 6 heads of 64 (432 tiles) 65 / 76.
+    // Short sequences lose it to the join (8 x 512 of 6 heads of 64 27.1 / 27.9).
+    if (grid <= (CAUSAL ? 512 : 256) && a.Tk / a.B >= 10 * kBN)
+      hipLaunchKernelGGL((attention_dq_kernel<DT, DP, CAUSAL, 2>), dim3(grid), dim3(128 * kWaves), 0,
+                         s, a);
+    else
+      hipLaunchKernelGGL((attention_dq_kernel<DT, DP, CAUSAL, 1>), dim3(grid), dim3(64 * kWaves), 0,
+                         s, a);
     const int32_t rc = check_hip(hipGetLastError(), "attention_backward launch");
     if (rc) return rc;
   }
@@ -438,22 +484,33 @@ namespace {
 int64_t padded_dim(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::kBM); }
 
-// Runs of queries that a tile of keys is split into: as many as fill the chip
-// (256 workgroups at once, 512 at D <= 64), with four tiles of queries to a run
-// at least, by the mean length; and two for causal sequences of four rounds or
-// fewer, whose first tiles take twice the mean, where the products (of mean
-// length x group queries per key) outweigh writing and reading the sums.
-// Measured without / with two: packed causal sequences of 1 to 4096 tokens, 32
-// heads in groups of four of 128, 506 / 446 + 35 us; 8 x 1024 of 6 heads of 64
-// 36.8 / 33.5 + 14.5.
+// Runs of queries that a tile of keys is split into.  The chip takes 256 of
+// the workgroups at once, 512 at D <= 64.  With fewer tiles than that, runs to
+// fill it once (one and a half times where causal tiles differ in work), of at
+// least eight tiles of queries in the mean, or sixteen where half of it is busy
+// anyway; with up to four times as many, causal, two, if they are long: the first
+// tiles take twice the mean.  More runs cost more to write and add than they
+// save.  The whole backward with 1 / 2 / 4 / 8 runs, us:
+//   4096 causal tokens, 8 heads in groups of 4 of 128 (66 tiles)  520 / 333 / 239 / 211
+//   2 x 2048, 16 in groups of 4 of 128 (136)                      279 / 194 / 164 / 191
+//   2 x 2048 not causal, 8 of 128 (272)                           132 / 160 / 190 / 265
+//   packed 1 to 4096, 32 in groups of 4 of 128 (568)              706 / 682 / 742 / 882
+//   4 x 4096, 8 of 128 (1056)                                     465 / 571 / 719 / 998
+//   8192, 12 in groups of 3 of 64 (260)                           557 / 417 / 384 / 389
+//   8 x 1024, 6 of 64 (432)                                       50 / 64 / 78
 int64_t dkv_splits(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
                    bool causal) {
   if (B == 0 || kv_heads == 0 || Tk == 0) return 1;
   const int64_t units = tile_bound(Tk, B) * kv_heads, slots = D <= 64 ? 512 : 256;
-  const int64_t group = heads / kv_heads, queries = Tq / B * group;
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(8, queries / (4 * attn::kBN)));
-  if (units < slots) return std::min(most, slots / units);
-  return causal && units < 4 * slots && queries >= 2048 ? 2 : 1;
+  const int64_t tiles = Tq / B * (heads / kv_heads) / attn::kBN;
+  int64_t runs = 1, least = 24;
+  if (units < slots) {
+    runs = ((causal ? 3 : 2) * slots + units) / (2 * units);
+    least = units < slots / 2 ? 8 : 16;
+  } else if (causal && units < 4 * slots) {
+    runs = 2;
+  }
+  return std::max<int64_t>(1, std::min({runs, tiles / least, (int64_t)8}));
 }
 }  // namespace
 

@@ -170,3 +170,21 @@ def test_split_runs_of_queries(cuda):
     run(cuda, [1300, 200], [500, 200], 4, 1, 64, BF, True, pad=1)
     run(cuda, [1300, 200], [500, 200], 4, 1, 128, HF, False)
     run(cuda, [1100], [1100], 2, 2, 128, BF, True)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+def test_keys_shared_by_two_groups_of_waves(cuda, dt, D):
+    """Few tiles of long sequences: two groups of waves take a tile's keys in
+    turn.  Odd and even numbers of tiles, one tile alone, none at all."""
+    run(cuda, [700, 65, 1, 200], [2600, 64, 0, 129], 2, 1, D, dt, True)
+    run(cuda, [33, 90], [1281, 1], 4, 2, D, dt, False, pad=1)
+
+
+def test_many_runs_of_queries(cuda):
+    """Eight runs to a tile of keys, some of them of masked tiles alone, and a
+    sequence with fewer tiles of queries than runs."""
+    need = nh.lib().nova_hip_attention_backward_scratch(2100, 300, 2, 8, 1, 128, 1)
+    assert need == 2 * 8 * 2100 + 4 * 8 * 4 * 64 * 128
+    run(cuda, [2000, 100], [200, 100], 8, 1, 128, BF, True)
+    run(cuda, [2000, 3], [200, 100], 8, 1, 64, HF, True)
