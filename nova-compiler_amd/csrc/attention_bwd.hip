@@ -22,6 +22,7 @@
 #include <algorithm>
 
 #include "attention.h"
+#include "wave.h"
 
 namespace nova_hip {
 namespace attn {
@@ -37,6 +38,9 @@ struct BwdArgs {
   Rows sq, sk, sv, so, sgo, sdq, sdk, sdv;
   int64_t slse;
   int Tq, Tk, B, heads, group, D, tiles, splits;
+  int least;        // tiles of queries in a run
+  float share;      // half of one over the workgroups that the chip takes at once
+  bool last_first;  // the last runs are launched first
   float c, scale;
 };
 
@@ -218,10 +222,40 @@ __global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_dq_kernel(BwdAr
                      lane);
 }
 
+// Runs that the `total` tiles of queries of a tile of keys are split into: none
+// shorter than the least, nor than a.share of the batch's work, which the offsets
+// give.  Two kernels must come to the same number, so no product here can be
+// fused with a sum but the one that is.
+template <bool CAUSAL>
+__device__ __forceinline__ int runs_of(const BwdArgs &a, int total) {
+  if (a.splits == 1) return 1;
+  const int lane = threadIdx.x & 63;
+  float work = 0.0f;
+  for (int b = lane; b < a.B; b += 64) {
+    const float k = (float)a.k_off[b + 1] - (float)a.k_off[b];
+    const float q = (float)a.q_off[b + 1] - (float)a.q_off[b];
+    work = __builtin_fmaf(k, q, work);
+  }
+  work = wave_sum(work) * (CAUSAL ? 0.5f : 1.0f) / (kBM * kBN) * (float)a.heads;
+  const int length = max(a.least, (int)fminf(fmaxf(work, 0.0f) * a.share, 1e9f));
+  return __builtin_amdgcn_readfirstlane(min(a.splits, max(1, total / length)));
+}
+
+// The first query of a sequence that sees a key from row0 on.
+template <bool CAUSAL>
+__device__ __forceinline__ int first_query(int row0, int Lq, int Lk) {
+  return CAUSAL ? min(Lq, max(0, row0 - (Lk - Lq))) : 0;
+}
+
 // 128 keys, 32 to a wave, x the queries that see them in every query head of the
 // group: `total` tiles of 64 queries, or, where tiles of keys alone are too few
-// or too uneven for the chip, one of `splits` runs of them; the runs' sums
-// then go to scratch and attention_dkv_join_kernel adds them in order.
+// or too uneven for the chip, one of up to `splits` runs of them; the runs' sums
+// then go to scratch and attention_dkv_join_kernel adds them in order.  (The run
+// that ends last adding them, behind a fence, made the L2s write back and forget:
+// 680 -> 1470 us packed as below.)  Runs are the grid's outer dimension, so that
+// those which a shorter tile has not got lie together: between the others they
+// keep whole shader engines idle (8192 tokens, 32 heads in groups of 4 of 128,
+// two runs at most: 1755 us, 2394 the other way).
 //
 // At D = 128 the keys, the values and the two gradients of a wave's 32 keys
 // take 192 registers, so one wave runs per SIMD (two at D <= 64).  What then
@@ -248,9 +282,10 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kv_heads = a.heads / a.group;
   int kh, tile;
-  unit_of(blockIdx.x, kv_heads, a.tiles * a.splits, CAUSAL, kh, tile);
-  const int split = tile % a.splits, unit = kh * a.tiles * a.splits + tile;
-  tile /= a.splits;
+  if ((int)blockIdx.x >= kv_heads * a.tiles) return;
+  unit_of(blockIdx.x, kv_heads, a.tiles, CAUSAL, kh, tile);
+  const int split = a.last_first ? a.splits - 1 - blockIdx.y : blockIdx.y;
+  const int unit = kh * a.tiles + tile;
   Tile place;
   if (!find_tile(a.k_off, a.q_off, a.B, a.Tk, a.Tq, kBM, tile, place)) return;
   // Causal: the first keys have the most queries.
@@ -258,15 +293,17 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   const int qs = place.os, qe = place.oe, ks = place.s, ke = place.e;
   const int Lq = qe - qs, Lk = ke - ks, shift = Lk - Lq;
   // Causal: key j is seen by the queries j - shift and on.
-  const int first = CAUSAL ? min(Lq, max(0, row0 - shift)) : 0;
+  const int first = first_query<CAUSAL>(row0, Lq, Lk);
   const int nt = (Lq - first + kBN - 1) / kBN, total = nt * a.group;
   // The first `nm` of a head's tiles of queries hold some that do not see all of
   // the keys.  Every head's come first, the others behind them, in a loop of
   // its own without masks.
   const int nm = CAUSAL ? min(nt, max(0, (row0 + kBM - shift - first + kBN - 2) / kBN)) : 0;
   const int masked = nm * a.group;
-  const int from = (int)((int64_t)total * split / a.splits);
-  const int to = (int)((int64_t)total * (split + 1) / a.splits);
+  const int runs = runs_of<CAUSAL>(a, total);
+  if (split >= runs) return;
+  const int from = (int)((int64_t)total * split / runs);
+  const int to = (int)((int64_t)total * (split + 1) / runs);
 
   const int k0 = row0 + 32 * wave, kn = min(32, Lk - k0);
   u32x4 kf[DP / 16], vf[DP / 16];
@@ -379,8 +416,8 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   if constexpr (CAUSAL) run(std::true_type(), from, min(to, masked), 0, nm);
   run(std::false_type(), max(from - masked, 0), to - masked, nm, nt);
   if (kn <= 0) return;
-  if (a.splits > 1) {
-    float *p = a.partial + ((int64_t)unit * kWaves + wave) * kPartial<DP> + lane;
+  if (runs > 1) {
+    float *p = a.partial + (((int64_t)unit * a.splits + split) * kWaves + wave) * kPartial<DP> + lane;
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -397,7 +434,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
 }
 
 // The sums of a tile of keys from those of its splits, in split order.
-template <int DT, int DP>
+template <int DT, int DP, bool CAUSAL>
 __global__ __launch_bounds__(64 * kWaves) void attention_dkv_join_kernel(BwdArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -405,8 +442,12 @@ __global__ __launch_bounds__(64 * kWaves) void attention_dkv_join_kernel(BwdArgs
   Tile place;
   if (!find_tile(a.k_off, a.q_off, a.B, a.Tk, a.Tq, kBM, w - kh * a.tiles, place)) return;
   const int ks = place.s, ke = place.e;
-  const int k0 = (place.tiles - 1 - place.index) * kBM + 32 * wave, kn = min(32, ke - ks - k0);
+  const int row0 = (place.tiles - 1 - place.index) * kBM;
+  const int k0 = row0 + 32 * wave, kn = min(32, ke - ks - k0);
   if (kn <= 0) return;
+  const int Lq = place.oe - place.os, first = first_query<CAUSAL>(row0, Lq, ke - ks);
+  const int runs = runs_of<CAUSAL>(a, (Lq - first + kBN - 1) / kBN * a.group);
+  if (runs == 1) return;
   f32x16 x[DP / 32];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -416,7 +457,7 @@ __global__ __launch_bounds__(64 * kWaves) void attention_dkv_join_kernel(BwdArgs
     for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[i][r] = p[(16 * i + r) * 64];
-    for (int s = 1; s < a.splits; ++s) {
+    for (int s = 1; s < runs; ++s) {
       p += (int64_t)kWaves * kPartial<DP>;
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i)
@@ -455,12 +496,12 @@ int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s)
   if (k_tiles > 0) {
     a.tiles = (int)k_tiles;
     const unsigned grid = (unsigned)(k_tiles * (a.heads / a.group));
-    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL>), dim3(grid * a.splits),
+    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL>), dim3(a.splits > 1 ? (grid + 7) / 8 * 8 : grid, a.splits),
                        dim3(64 * kWaves), 0, s, a);
     if (a.splits > 1) {
       const int32_t rc = check_hip(hipGetLastError(), "attention_backward launch");
       if (rc) return rc;
-      hipLaunchKernelGGL((attention_dkv_join_kernel<DT, DP>), dim3(grid), dim3(64 * kWaves), 0, s, a);
+      hipLaunchKernelGGL((attention_dkv_join_kernel<DT, DP, CAUSAL>), dim3(grid), dim3(64 * kWaves), 0, s, a);
     }
   }
   return check_hip(hipGetLastError(), "attention_backward launch");
@@ -484,41 +525,47 @@ namespace {
 int64_t padded_dim(int64_t D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
 int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::kBM); }
 
-// Runs of queries that a tile of keys is split into.  The chip takes 256 of
-// the workgroups at once, 512 at D <= 64.  With fewer tiles than that, runs to
-// fill it once (one and a half times where causal tiles differ in work), of at
-// least eight tiles of queries in the mean, or sixteen where half of it is busy
-// anyway; with up to four times as many, causal, two, if they are long: the first
-// tiles take twice the mean.  More runs cost more to write and add than they
-// save.  The whole backward with 1 / 2 / 4 / 8 runs, us:
-//   4096 causal tokens, 8 heads in groups of 4 of 128 (66 tiles)  520 / 333 / 239 / 211
-//   2 x 2048, 16 in groups of 4 of 128 (136)                      279 / 194 / 164 / 191
-//   2 x 2048 not causal, 8 of 128 (272)                           132 / 160 / 190 / 265
-//   packed 1 to 4096, 32 in groups of 4 of 128 (568)              706 / 682 / 742 / 882
-//   4 x 4096, 8 of 128 (1056)                                     465 / 571 / 719 / 998
-//   8192, 12 in groups of 3 of 64 (260)                           557 / 417 / 384 / 389
-//   8 x 1024, 6 of 64 (432)                                       50 / 64 / 78
-int64_t dkv_splits(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
-                   bool causal) {
-  if (B == 0 || kv_heads == 0 || Tk == 0) return 1;
+// Runs of queries that tiles of keys are split into, where the longest of them
+// would keep the chip waiting.  The host knows the sequences' number and tokens;
+// `most` follows from them, and the device splits those tiles that are long.
+// With fewer tiles than the chip takes at once (256, 512 at D <= 64), up to four
+// runs, or eight for very few tiles; with up to four times as many, causal, two,
+// the last ones first (the longest tiles have them).  No run is shorter than half
+// the mean work of a slot (a quarter / a half / three eighths, us, packed 568
+// tiles as below 687 / 674 / 679, 2 x 4096 tokens of 8 heads of 128 312 / 283 /
+// 297).  Nothing is split where no sequence is likely to have two runs of the
+// least length: between all of one length and one that has all tokens, the
+// geometric mean decides.  The whole backward without runs and with them, us:
+//   4096 causal tokens, 8 heads in groups of 4 of 128 (66 tiles)  487 / 212
+//   2 x 2048, 16 in groups of 4 of 128 (136)                      277 / 184
+//   packed 1 to 4096, 32 in groups of 4 of 128 (568)              711 / 664
+//   packed 1 to 4096, 6 of 64 (426)                               133 / 116
+//   8192, 12 in groups of 3 of 64 (260)                           555 / 417
+//   2 x 4096 not causal, 8 in groups of 4 of 64 (132)             481 / 279
+//   8 x 1024, 6 of 64 (432): none is split                        53 / 54
+struct Runs {
+  int64_t most;
+  int least;
+  bool last_first;
+};
+Runs dkv_runs(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
+              bool causal) {
+  if (B == 0 || kv_heads == 0 || Tk == 0) return {1, 1, false};
   const int64_t units = tile_bound(Tk, B) * kv_heads, slots = D <= 64 ? 512 : 256;
-  const int64_t tiles = Tq / B * (heads / kv_heads) / attn::kBN;
-  int64_t runs = 1, least = 24;
-  if (units < slots) {
-    runs = ((causal ? 3 : 2) * slots + units) / (2 * units);
-    least = units < slots / 2 ? 8 : 16;
-  } else if (causal && units < 4 * slots) {
-    runs = 2;
-  }
-  return std::max<int64_t>(1, std::min({runs, tiles / least, (int64_t)8}));
+  const double tiles = (double)Tq * (heads / kv_heads) / attn::kBN, likely = tiles * tiles / B;
+  const bool few = units < slots / 4;
+  if (likely < (few ? 16.0 * 16.0 : 24.0 * 24.0) || units >= (causal ? 4 : 1) * slots)
+    return {1, 1, false};
+  return {units < slots / 8 ? 8 : units < slots ? 4 : 2,
+          few || (D > 64 && units < slots) ? 8 : 16, units >= slots};
 }
 }  // namespace
 
 int64_t attention_backward_scratch(int64_t Tq, int64_t Tk, int64_t B, int64_t heads,
                                    int64_t kv_heads, int64_t D, bool causal) {
-  const int64_t rows = 2 * heads * Tq, splits = dkv_splits(Tq, Tk, B, heads, kv_heads, D, causal);
+  const int64_t rows = 2 * heads * Tq, splits = dkv_runs(Tq, Tk, B, heads, kv_heads, D, causal).most;
   if (splits <= 1) return rows;
-  return rows + tile_bound(Tk, B) * kv_heads * splits * attn::kWaves * 64 * padded_dim(D);
+  return (rows + 63) / 64 * 64 + tile_bound(Tk, B) * kv_heads * splits * attn::kWaves * 64 * padded_dim(D);
 }
 
 int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t s) {
@@ -535,7 +582,6 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   a.lse = p.f.lse;
   a.slse = p.f.slse;
   a.rows = p.scratch;
-  a.partial = p.scratch + 2 * p.f.heads * p.f.Tq;
   a.q_off = p.f.q_off;
   a.k_off = p.f.k_off;
   a.sq = {p.f.q.st, p.f.q.sh};
@@ -555,8 +601,13 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   a.tiles = 0;
   a.c = p.f.scale * attn::kLog2e;
   a.scale = p.f.scale;
-  a.splits = (int)dkv_splits(p.f.Tq, p.f.Tk, p.f.B, p.f.heads, p.f.kv_heads, p.f.D, p.f.causal);
+  const Runs runs = dkv_runs(p.f.Tq, p.f.Tk, p.f.B, p.f.heads, p.f.kv_heads, p.f.D, p.f.causal);
+  a.splits = (int)runs.most;
+  a.least = runs.least;
+  a.last_first = runs.last_first;
+  a.share = 0.5f / (p.f.D <= 64 ? 512 : 256);
   const int64_t qt = tile_bound(p.f.Tq, p.f.B), kt = tile_bound(p.f.Tk, p.f.B);
+  a.partial = p.scratch + (2 * p.f.heads * p.f.Tq + 63) / 64 * 64;
   // A grid's dimension holds less than 2^32 threads.
   if (std::max(qt * p.f.heads, kt * p.f.kv_heads * a.splits) >= 1 << 24)
     return fail(NOVA_HIP_ERANGE, "attention_backward: more than 2^24 - 1 tiles");
