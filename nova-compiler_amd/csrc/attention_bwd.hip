@@ -533,16 +533,17 @@ int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::k
 // the last ones first (the longest tiles have them).  No run is shorter than half
 // the mean work of a slot (a quarter / a half / three eighths, us, packed 568
 // tiles as below 687 / 674 / 679, 2 x 4096 tokens of 8 heads of 128 312 / 283 /
-// 297).  Nothing is split where no sequence is likely to have two runs of the
-// least length: between all of one length and one that has all tokens, the
-// geometric mean decides.  The whole backward without runs and with them, us:
+// 297).  Nothing is split where no sequence is likely to be long: between all of
+// one length and one that has all tokens, the geometric mean decides: of more
+// tiles where the products are short (D <= 64) and half of the chip is busy, since
+// the join's launch alone takes 3 us (8 x 1024 of 6 heads of 64 47 / 51.5 with
+// nothing to join).  The whole backward without runs and with them, us:
 //   4096 causal tokens, 8 heads in groups of 4 of 128 (66 tiles)  487 / 212
 //   2 x 2048, 16 in groups of 4 of 128 (136)                      277 / 184
 //   packed 1 to 4096, 32 in groups of 4 of 128 (568)              711 / 664
-//   packed 1 to 4096, 6 of 64 (426)                               133 / 116
+//   8192, 6 of 64 (390)                                           254 / 228
 //   8192, 12 in groups of 3 of 64 (260)                           555 / 417
 //   2 x 4096 not causal, 8 in groups of 4 of 64 (132)             481 / 279
-//   8 x 1024, 6 of 64 (432): none is split                        53 / 54
 struct Runs {
   int64_t most;
   int least;
@@ -554,8 +555,8 @@ Runs dkv_runs(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads
   const int64_t units = tile_bound(Tk, B) * kv_heads, slots = D <= 64 ? 512 : 256;
   const double tiles = (double)Tq * (heads / kv_heads) / attn::kBN, likely = tiles * tiles / B;
   const bool few = units < slots / 4;
-  if (likely < (few ? 16.0 * 16.0 : 24.0 * 24.0) || units >= (causal ? 4 : 1) * slots)
-    return {1, 1, false};
+  const double least = few ? 16 : D > 64 || units < slots / 2 ? 24 : 48;
+  if (likely < least * least || units >= (causal ? 4 : 1) * slots) return {1, 1, false};
   return {units < slots / 8 ? 8 : units < slots ? 4 : 2,
           few || (D > 64 && units < slots) ? 8 : 16, units >= slots};
 }
