@@ -39,7 +39,7 @@ struct BwdArgs {
   int64_t slse;
   int Tq, Tk, B, heads, group, D, tiles, splits;
   int least;        // tiles of queries in a run
-  float share;      // half of one over the workgroups that the chip takes at once
+  float share;      // and the part of the batch's work that it takes at least
   bool last_first;  // the last runs are launched first
   float c, scale;
 };
@@ -531,9 +531,10 @@ int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::k
 // With fewer tiles than the chip takes at once (256, 512 at D <= 64), up to four
 // runs, or eight for very few tiles; with up to four times as many, causal, two,
 // the last ones first (the longest tiles have them).  No run is shorter than half
-// the mean work of a slot (a quarter / a half / three eighths, us, packed 568
-// tiles as below 687 / 674 / 679, 2 x 4096 tokens of 8 heads of 128 312 / 283 /
-// 297).  Nothing is split where no sequence is likely to be long: between all of
+// the mean work of a slot (a quarter / a half, us, packed 568 tiles as below 687 /
+// 674, 2 x 4096 tokens of 8 heads of 128 312 / 283), but where the tiles are just
+// more than the chip takes, when halves of all of them fill it evenly (2 x 8192 of
+// 16 in groups of 8 of 128, 260 tiles: 2110 / 1830).  Nothing is split where no sequence is likely to be long: between all of
 // one length and one that has all tokens, the geometric mean decides: of more
 // tiles where the products are short (D <= 64) and half of the chip is busy, since
 // the join's launch alone takes 3 us (8 x 1024 of 6 heads of 64 47 / 51.5 with
@@ -547,18 +548,21 @@ int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::k
 struct Runs {
   int64_t most;
   int least;
+  float share;
   bool last_first;
 };
 Runs dkv_runs(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
               bool causal) {
-  if (B == 0 || kv_heads == 0 || Tk == 0) return {1, 1, false};
+  if (B == 0 || kv_heads == 0 || Tk == 0) return {1, 1, 0.0f, false};
   const int64_t units = tile_bound(Tk, B) * kv_heads, slots = D <= 64 ? 512 : 256;
   const double tiles = (double)Tq * (heads / kv_heads) / attn::kBN, likely = tiles * tiles / B;
   const bool few = units < slots / 4;
   const double least = few ? 16 : D > 64 || units < slots / 2 ? 24 : 48;
-  if (likely < least * least || units >= (causal ? 4 : 1) * slots) return {1, 1, false};
+  if (likely < least * least || units >= (causal ? 4 : 1) * slots)
+    return {1, 1, 0.0f, false};
   return {units < slots / 8 ? 8 : units < slots ? 4 : 2,
-          few || (D > 64 && units < slots) ? 8 : 16, units >= slots};
+          few || (D > 64 && units < slots) ? 8 : 16,
+          units >= slots && 2 * units < 3 * slots ? 0.0f : 0.5f / slots, units >= slots};
 }
 }  // namespace
 
@@ -606,7 +610,7 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   a.splits = (int)runs.most;
   a.least = runs.least;
   a.last_first = runs.last_first;
-  a.share = 0.5f / (p.f.D <= 64 ? 512 : 256);
+  a.share = runs.share;
   const int64_t qt = tile_bound(p.f.Tq, p.f.B), kt = tile_bound(p.f.Tk, p.f.B);
   a.partial = p.scratch + (2 * p.f.heads * p.f.Tq + 63) / 64 * 64;
   // A grid's dimension holds less than 2^32 threads.
