@@ -209,3 +209,32 @@ def test_two_runs_last_ones_first(cuda):
     tiles = sum(lens) // 128 + len(lens)
     assert need >= 2 * H * sum(lens) + 2 * H * tiles * 4 * 64 * 128
     run(cuda, lens, lens, H, H, 128, BF, True)
+
+
+def test_runs_in_a_captured_graph(cuda):
+    """Split and joined runs replayed with new inputs, eager calls of other
+    shapes between the replays: the same bits as eager calls."""
+    lens, H, G, D = [2000, 300, 5], 4, 1, 128
+    q, k, v = make(cuda, lens, lens, H, G, D, BF, 0, "thd", 0)
+    off = offsets(lens, cuda)
+    go = torch.randn(q.shape, device=cuda).to(BF)
+    o, lse = nh.attention(q, k, v, off, off)
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    nh.attention_backward(go, q, k, v, o, lse, off, off, dq=dq, dk=dk, dv=dv)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        nh.attention(q, k, v, off, off, out=o, lse=lse)
+        nh.attention_backward(go, q, k, v, o, lse, off, off, dq=dq, dk=dk, dv=dv)
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    for _ in range(4):
+        for t in (q, k, v, go):
+            t.copy_(torch.randn(t.shape, generator=gen, device=cuda))
+        for t in (dq, dk, dv):
+            t.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        run(cuda, [130, 70], [130, 70], 8, 1, 64, BF, True)
+        o2, lse2 = nh.attention(q, k, v, off, off)
+        want = nh.attention_backward(go, q, k, v, o2, lse2, off, off)
+        assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), want))
