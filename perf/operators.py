@@ -30,13 +30,11 @@ BETA, SMOOTHING = 0.1, 0.05           # preference loss
 CLIP_LOW, CLIP_HIGH, KL = 0.2, 0.28, 0.04  # policy loss
 
 
-_PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                        "nova-compiler_amd")
-
-
 def _nh():
-    if _PACKAGE not in sys.path:
-        sys.path.insert(0, _PACKAGE)
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       "nova-compiler_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     import nova_hip
     return nova_hip
 
