@@ -180,8 +180,9 @@ __global__ __launch_bounds__(64 * NW) void attention_decode_kernel(DecodeArgs a)
     for (int i = 1; i < NW; ++i) mx = fmaxf(mx, sm[i][c]);
     l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NW; ++i)
-      l += sm[i][c] == -INFINITY ? 0.0f : sl[i][c] * __builtin_amdgcn_exp2f(sm[i][c] - mx);
+    for (int i = 0; i < NW; ++i)  // 0 times a NaN stays one: all scores of a wave may be NaN
+      l += sl[i][c] *
+           (sm[i][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[i][c] - mx));
     const float f = mc == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc - mx);
     mc = mx;
     static_assert(kTile >= 64 * 16 * 4, "a block of 32 x 32 sums");

@@ -58,6 +58,27 @@ def test_head_dims_of_a_long_cache(cuda, D):
     run(cuda, [1500, 700], 1500, 35, 1, D, BF, "bhsd")  # more heads than one block of 32
 
 
+@pytest.mark.parametrize("S", [40, 300, 1024, 1025, 3001])  # one launch up to 1024 rows, two beyond
+@pytest.mark.parametrize("dt,D", [(BF, 64), (HF, 128)])
+def test_nan_scores_reach_the_lse(cuda, S, dt, D):
+    """A NaN query, and NaN in all keys that one wave of the joined form or one
+    split takes: result and log-sum-exp are both NaN there, whatever the cache's
+    size, and those of the other heads and sequences what they were."""
+    g = torch.Generator(device=cuda).manual_seed(S)
+    q = torch.randn(3, 4, D, generator=g, device=cuda).to(dt)
+    k, v = (torch.randn(3, S, 2, D, generator=g, device=cuda).to(dt) for _ in range(2))
+    n = torch.tensor([S, S - 1, S // 2], dtype=torch.int32, device=cuda)
+    lse, want = torch.empty(3, 4, device=cuda), torch.empty(3, 4, device=cuda)
+    plain = nh.attention_decode(q, k, v, n, lse=want)
+    q[0, 1] = float("nan")
+    k[1, 32:, 1] = float("nan")
+    out = nh.attention_decode(q, k, v, n, lse=lse)
+    bad = torch.zeros(3, 4, dtype=torch.bool, device=cuda)
+    bad[0, 1] = bad[1, 2] = bad[1, 3] = True
+    assert torch.isnan(lse[bad]).all() and torch.isnan(out[bad]).all()
+    assert torch.equal(lse[~bad], want[~bad]) and torch.equal(out[~bad], plain[~bad])
+
+
 def test_lengths_zero_and_out_of_range(cuda):
     q, k, v, length, out = run(cuda, [0, 300, -5, 70], 64, 4, 2, 64, BF)
     assert (out[0] == 0).all() and (out[2] == 0).all()
