@@ -38,6 +38,13 @@ struct FwdArgs {
 
 constexpr int kWaves = 4, kBM = 32 * kWaves, kBN = 64;
 constexpr float kSlack = 8.0f;  // m c may lag the largest score by this much
+// f16 weights are taken times 2^7: with the slack they stay under 2^15, and one
+// that rounds to zero is under 2^-32 of a row's largest, not 2^-25.  Thousands of
+// the latter behind one key far above them are a part of the result that f16
+// shows (2^-11): 4095 keys of weight 2^-25.2 together weigh 2^-13.2, and more
+// where their values are the larger ones.
+template <int DT>
+constexpr float kUp = DT == NOVA_HIP_DT_F16 ? 7.0f : 0.0f;
 
 // KS groups of four waves share a tile of queries: group g takes the tiles of
 // keys g, g + KS, ... through a ring of its own, and the groups' sums are joined
@@ -121,12 +128,12 @@ __global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_fwd_kernel(FwdA
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
     }
-    const float mu = mc == -INFINITY ? 0.0f : mc;
+    const float up = kUp<DT> - (mc == -INFINITY ? 0.0f : mc);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.c, -mu));
+        s[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.c, up));
         l += s[i][r];
       }
 #pragma unroll
@@ -200,7 +207,7 @@ __global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_fwd_kernel(FwdA
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   store_rows<DT, DP>(acc, inv, a.o + (qs + q0) * a.so.t + head * a.so.h, a.so.t, qn, a.D, lane);
   if (a.lse && lane < qn)
-    a.lse[head * a.slse + qs + q0 + lane] = l == 0.0f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+    a.lse[head * a.slse + qs + q0 + lane] = l == 0.0f ? -INFINITY : (mc + (__log2f(l) - kUp<DT>)) * kLn2;
 }
 
 template <int DT, int DP, int KS>

@@ -40,6 +40,10 @@ struct DecodeArgs {
 };
 
 constexpr int kBN = 32;
+// f16 weights, at most 1, are taken times 2^15: one that rounds to zero is under
+// 2^-40 of the largest in its part of the cache, not 2^-25 (see the forward).
+template <int DT>
+constexpr float kUp = DT == NOVA_HIP_DT_F16 ? 15.0f : 0.0f;
 
 template <int DT, int DP, int NW>
 __global__ __launch_bounds__(64 * NW) void attention_decode_kernel(DecodeArgs a) {
@@ -124,10 +128,10 @@ __global__ __launch_bounds__(64 * NW) void attention_decode_kernel(DecodeArgs a)
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
     }
-    const float mu = mc == -INFINITY ? 0.0f : mc;
+    const float up = kUp<DT> - (mc == -INFINITY ? 0.0f : mc);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -mu));
+      s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, up));
       l += s[r];
     }
 #pragma unroll
@@ -209,7 +213,7 @@ __global__ __launch_bounds__(64 * NW) void attention_decode_kernel(DecodeArgs a)
     store_rows<DT, DP>(acc, l == 0.0f ? 0.0f : 1.0f / l, a.o + b * a.sob + h0 * a.soh, a.soh, hn,
                        a.D, lane);
     if (a.lse && lane < hn)
-      a.lse[b * a.slse + h0 + lane] = l == 0.0f ? -INFINITY : (mc + __log2f(l)) * kLn2;
+      a.lse[b * a.slse + h0 + lane] = l == 0.0f ? -INFINITY : (mc + (__log2f(l) - kUp<DT>)) * kLn2;
     return;
   }
   const int col = lane & 31;
@@ -265,7 +269,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a) {
   if (d < a.D)
     *reinterpret_cast<uint32_t *>(a.o + b * a.sob + h * a.soh + d) = pack<DT>(x0 * inv, x1 * inv);
   if (a.lse && lane == 0)
-    a.lse[b * a.slse + h] = sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * kLn2;
+    a.lse[b * a.slse + h] = sum == 0.0f ? -INFINITY : (mx + (__log2f(sum) - kUp<DT>)) * kLn2;
 }
 
 // Waves of the form that joins them itself: what the LDS of a CU holds.

@@ -272,3 +272,44 @@ def test_offsets_outside_the_operands(cuda, bad):
     torch.cuda.synchronize()
     for t in [out] + d:
         assert (t[:guard] == 7.0).all() and (t[guard + T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("form", ["prompt", "causal", "two groups", "single token", "long cache"])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_many_small_weights_behind_a_large_one(cuda, dt, form):
+    """One key's score 17.5 above those of n - 1 others, whose weights of e^-17.5 =
+    2^-25.2 lie under half of f16's least number and whose values alone differ from
+    zero.  A weight rounds by u of itself or, in f16, by 2^-32 at most (n - 1
+    times), the result by u; scores are exact and exponentials within 4e-5.  A row's
+    sum is added up by two lanes, n / 2 f32 additions each (long cache: in parts of
+    at most 2048 keys): 2^-25 of it for each of n, here SUM."""
+    SUM = 2.0 ** -25 * 4096
+    n = 70000 if form == "long cache" else 1000 if form == "single token" else 4095
+    D, rows = 64, 1 if form in ("single token", "long cache") else 300 if form == "two groups" else 3000
+    heads = 2 if form == "two groups" else 32  # few tiles: two groups of waves share the keys
+    q = torch.zeros(rows, heads, D, dtype=dt, device=cuda)
+    q[:, :, 0] = 17.5
+    k = torch.zeros(n, 1, D, dtype=dt, device=cuda)
+    v = torch.full((n, 1, D), 1000.0, dtype=dt, device=cuda)
+    k[7, 0, 0], v[7] = 1.0, 0.0
+    if rows == 1:
+        lse = torch.empty(1, heads, device=cuda)
+        out = nh.attention_decode(q, k[None], v[None], torch.tensor([n], dtype=torch.int32, device=cuda),
+                                  scale=1.0, lse=lse)
+        lse = lse.t()
+    else:
+        out, lse = nh.attention(q, k, v, offsets([rows], cuda), offsets([n], cuda), scale=1.0,
+                                causal=form == "causal")
+    # Causal: query i sees n - rows + i + 1 keys, the seventh among them.
+    seen = torch.full((rows,), float(n), dtype=F64, device=cuda)
+    if form == "causal":
+        seen = torch.arange(n - rows + 1, n + 1, device=cuda, dtype=F64)
+    w = math.exp(-17.5)
+    total = 1.0 + (seen - 1) * w
+    want = 1000.0 * (seen - 1) * w / total
+    u = torch.finfo(dt).eps / 2
+    tol = 2 * u * want * 1.01 + (4e-5 + SUM) * want + (1000.0 * 2.0 ** -32 * (seen - 1) if dt == HF else 0.0)
+    err = (out.double() - want[:, None, None]).abs()
+    assert (err <= tol[:, None, None]).all(), (err.max().item(), want.max().item(), tol.max().item())
+    d = (lse.double() - (17.5 + torch.log(total))[None]).abs().max().item()
+    assert d <= 4e-5 + SUM, d
