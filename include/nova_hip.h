@@ -437,9 +437,10 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
  * [heads, query tokens]; scratch : at least
  * nova_hip_attention_backward_scratch() f32, dense, used by this call only.  dq,
  * dk and dv must not overlap the other operands or each other (views of one
- * buffer are apart).  P and dS are rounded to dt for the products (an f16 dS
- * beyond 65504 is an infinity), sums are f32 in a fixed order (no atomics: the
- * same bits on every run).  A query that sees no key has gradient zero and
+ * buffer are apart).  P and dS are rounded to dt for the products (in f16 each
+ * column of dS takes a power of two of its own, so that small and large gradients
+ * keep their bits), sums are f32 in a fixed order (no atomics: the same bits on
+ * every run).  A query that sees no key has gradient zero and
  * adds none; rows outside every sequence are left as they were. */
 int32_t _mlir_ciface_nova_hip_attention_backward(
     const NovaMemRef3D *grad_out, const NovaMemRef3D *q, const NovaMemRef3D *k,

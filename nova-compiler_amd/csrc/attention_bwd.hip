@@ -58,6 +58,40 @@ constexpr int64_t kPartial = DP * 64;
 template <int DT>
 constexpr float kWeightLog2 = DT == NOVA_HIP_DT_F16 ? 8.0f : 0.0f;
 
+// f16 dS is as small as the gradient that came in (a mean over thousands of
+// tokens: under 2^-24, where f16 has nothing left) and as large as its loss scale
+// makes it, so each column of a product with it (a lane and its partner) has a
+// factor 2^up of its own, which its sums carry until they are complete.  It starts
+// at 2^40, and is lowered, with the sums so far, where a value would pass 2^15: the
+// largest comes to [2^5, 2^6) then, so that what rounds to zero is under 2^-30 of
+// the column's largest.  (Factors of two are exact.)  bf16 has f32's exponents.
+constexpr float kUp = 40.0f;
+template <int DP>
+__device__ __forceinline__ void fit_f16(f32x16 &ds, f32x16 (&acc)[DP / 32], float &up) {
+  float t = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) t = fmaxf(t, fabsf(ds[r]));
+  if (__ballot(t > 32768.0f)) {
+    keep_branch();
+    t = both_max(t);
+    const int by = t > 32768.0f && t < INFINITY ? 6 - __builtin_amdgcn_frexp_expf(t) : 0;
+    const float f = __builtin_amdgcn_ldexpf(1.0f, by);
+    up += (float)by;
+    ds *= f;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
+  }
+}
+// Takes the factor back.
+template <int DT, int DP>
+__device__ __forceinline__ void unfit(f32x16 (&acc)[DP / 32], float up) {
+  if constexpr (DT == NOVA_HIP_DT_F16) {
+    const float f = __builtin_amdgcn_ldexpf(1.0f, -(int)up);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] *= f;
+  }
+}
+
 // sum over d of a row's products, the row held as load_cols gives it.
 template <int DT, int DP>
 __device__ __forceinline__ float row_dot(const u32x4 (&x)[DP / 16], const u32x4 (&y)[DP / 16]) {
@@ -155,6 +189,7 @@ __global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_dq_kernel(BwdAr
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16{};
+  float up = DT == NOVA_HIP_DT_F16 ? kUp : 0.0f;  // of dS, see fit_f16
   const int last = q0 + (lane & 31) + shift;
 
   auto fetch = [&](int t, lds_char *sk, lds_char *sv) __attribute__((always_inline)) {
@@ -174,15 +209,17 @@ __global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_dq_kernel(BwdAr
         s = mfma_32x32x16<DT>(read_row_frag(sk, row_frag<CH>(32 * i, kk, lane)), qf[kk], s);
         dp = mfma_32x32x16<DT>(read_row_frag(sv, row_frag<CH>(32 * i, kk, lane)), gf[kk], dp);
       }
+      const float add = up - nl;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl)) * (dp[r] - delta);
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, add)) * (dp[r] - delta);
       if (edge) {
         keep_branch();
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (k0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[r] = 0.0f;
       }
+      if constexpr (DT == NOVA_HIP_DT_F16) fit_f16<DP>(s, acc, up);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const u32x4 sf = pack_frag<DT>(s, kk);  // dS rounds to the operands' type
@@ -212,6 +249,7 @@ __global__ __launch_bounds__(64 * kWaves * KS, 2) void attention_dq_kernel(BwdAr
     if (u + 2 < nu) fetch((u + 2) * KS + part, sk0, sv0);
     turn(u + 1, sk1, sv1);
   }
+  unfit<DT, DP>(acc, up);
   if constexpr (KS > 1) {
     static_assert(KS == 2, "one group hands its sums to the other");
     add_group<DP>(acc, (lds_char *)sk0_, wave, part, lane);
@@ -312,6 +350,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   TileLoad<kBN, CH, kWaves> lq, lg;
   lq.init(a.sq.t, a.D);
   lg.init(a.sgo.t, a.D);
+  float up = DT == NOVA_HIP_DT_F16 ? kUp : 0.0f;  // of dS, see fit_f16
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) dk[i] = dv[i] = f32x16{};
@@ -343,7 +382,6 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
     };
     auto step = [&](const lds_char *sq, const lds_char *sg, const lds_float *sc)
         __attribute__((always_inline)) {
-      constexpr float kDown = DT == NOVA_HIP_DT_F16 ? 1.0f / 256.0f : 1.0f;
       const int q0 = first + cj * kBN;
       if (kMask && ++cj == j1) cj = j0;
 #pragma unroll
@@ -362,6 +400,9 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
           s = mfma_32x32x16<DT>(read_row_frag(sq, row_frag<CH>(32 * i, kk, lane)), kf[kk], s);
           dp = mfma_32x32x16<DT>(read_row_frag(sg, row_frag<CH>(32 * i, kk, lane)), vf[kk], dp);
         }
+        // From the weights' factor to that of dS.
+        const float down =
+            DT == NOVA_HIP_DT_F16 ? __builtin_amdgcn_exp2f(up - kWeightLog2<DT>) : 1.0f;
         // Rows of this block from which on the lane's key is seen.
         const int seen = kMask ? k0 + (lane & 31) - shift - q0 - 32 * i - 4 * (lane >> 5) : 0;
 #pragma unroll
@@ -371,11 +412,12 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * r4 + e;
             s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], a.c, -nl[e]));
-            dp[r] = s[r] * (DT == NOVA_HIP_DT_F16 ? dp[r] * kDown : dp[r]);
+            dp[r] = s[r] * (DT == NOVA_HIP_DT_F16 ? dp[r] * down : dp[r]);
             if constexpr (kMask)
               if (8 * (r >> 2) + (r & 3) < seen) s[r] = dp[r] = 0.0f;
           }
         }
+        if constexpr (DT == NOVA_HIP_DT_F16) fit_f16<DP>(dp, dk, up);
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
           // Weights and dS round to the operands' type for these products.
@@ -416,6 +458,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 64 ? 2 : 1) void attention_dkv_k
   if constexpr (CAUSAL) run(std::true_type(), from, min(to, masked), 0, nm);
   run(std::false_type(), max(from - masked, 0), to - masked, nm, nt);
   if (kn <= 0) return;
+  unfit<DT, DP>(dk, up);
   if (runs > 1) {
     float *p = a.partial + (((int64_t)unit * a.splits + split) * kWaves + wave) * kPartial<DP> + lane;
 #pragma unroll

@@ -238,3 +238,97 @@ def test_runs_in_a_captured_graph(cuda):
         o2, lse2 = nh.attention(q, k, v, off, off)
         want = nh.attention_backward(go, q, k, v, o2, lse2, off, off)
         assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), want))
+
+
+def scaled(dev, qlens, klens, H, G, D, dt, causal, grad, q_up=1.0, k_up=1.0, v_up=1.0, rows=None):
+    """(grads, reference, bounds) with grad_out of size `grad` and q, k, v of the
+    given sizes (their products kept where scores are of size 1).  dS rounds by u
+    of itself and in f16, where a column of the product with it (a query's row for
+    dQ, a key's for dK) has a factor that keeps its largest value above 2^5, by
+    2^-25 of 2^-5 of that."""
+    q, k, v = make(dev, qlens, klens, H, G, D, dt)
+    q, k, v = ((x.float() * up).to(dt) for x, up in ((q, q_up), (k, k_up), (v, v_up)))
+    g = torch.Generator(device=dev).manual_seed(5)
+    go = torch.randn(q.shape, generator=g, device=dev) * grad
+    if rows is not None:
+        go *= rows[:, None, None]
+    go = go.to(dt)
+    scale = D ** -0.5 / (q_up * k_up)
+    qo, ko = offsets(qlens, dev), offsets(klens, dev)
+    o, lse = nh.attention(q, k, v, qo, ko, causal=causal, scale=scale)
+    got = nh.attention_backward(go, q, k, v, o, lse, qo, ko, causal=causal, scale=scale)
+    u = torch.finfo(dt).eps / 2
+    want = [torch.zeros(t.shape, dtype=F64, device=dev) for t in (q, k, k)]
+    tol = [torch.zeros_like(w) for w in want]
+    a = c = 0
+    for n, m in zip(qlens, klens):
+        keep = torch.ones(n, m, dtype=torch.bool, device=dev)
+        if causal:
+            keep = keep.tril(m - n)
+        sl, kl = slice(a, a + n), slice(c, c + m)
+        for j in range(G):
+            K, V = k[c:c + m, j].double(), v[c:c + m, j].double()
+            heads = []
+            for h in range(j * H // G, (j + 1) * H // G):
+                Q, GO, O = (t[a:a + n, h].double() for t in (q, go, o))
+                s = torch.mm(Q, K.t().contiguous()) * scale
+                p = torch.where(keep, torch.exp(s - lse[h, a:a + n].double()[:, None]), torch.zeros_like(s))
+                delta = (GO * O).sum(1)[:, None]
+                ds = p * (torch.mm(GO, V.t().contiguous()) - delta)
+                slack = p * (torch.mm(GO.abs(), V.t().abs().contiguous()) + (GO * O).abs().sum(1)[:, None])
+                heads.append((h, Q, GO, p, ds, (u * 1.01 + 4e-5) * ds.abs() + 1e-5 * slack,
+                              2.0 ** -30 * (ds.abs() + 1e-5 * slack) * (dt == HF)))
+            # A key's factor is common to the heads of its group.
+            least = torch.stack([x[6].amax(0, keepdim=True) for x in heads]).amax(0)
+            for h, Q, GO, p, ds, err, tiny in heads:
+                row, col = err + tiny.amax(1, keepdim=True) * keep, err + least * keep
+                want[0][sl, h] = torch.mm(ds, K) * scale
+                tol[0][sl, h] = torch.mm(row, K.abs()) * scale
+                want[1][kl, j] += torch.mm(ds.t().contiguous(), Q) * scale
+                tol[1][kl, j] += torch.mm(col.t().contiguous(), Q.abs()) * scale
+                want[2][kl, j] += torch.mm(p.t().contiguous(), GO)
+                tol[2][kl, j] += torch.mm(((u * 1.01 + 4e-5) * p + 2.0 ** -33 * keep * (dt == HF)).t().contiguous(),
+                                          GO.abs())
+        a, c = a + n, c + m
+    for name, x, w, t in zip(("dq", "dk", "dv"), got, want, tol):
+        bound = t * 1.01 + u * w.abs() * 1.01 + 2.0 ** -25 * (dt == HF) + 1e-30
+        # Beyond the type's largest value there is no bound to hold.
+        fits = w.abs() + t < 0.99 * torch.finfo(dt).max
+        err = (x.double() - w).abs()
+        assert (err <= bound)[fits].all(), (name, (err - bound)[fits].max().item(), w.abs().max().item())
+        assert torch.isfinite(x[fits]).all(), name
+    return got, want
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_small_gradients(cuda, dt, causal, D):
+    """grad_out as a mean over thousands of tokens leaves it: dS lies under f16's
+    least number where dQ and dK, products with large K and Q, do not."""
+    for grad in (2.0 ** -10, 2.0 ** -16, 2.0 ** -20):
+        got, want = scaled(cuda, [700, 130], [700, 130], 4, 2, D, dt, causal, grad, k_up=64.0, q_up=1 / 64)
+        assert want[0].abs().max() > 2.0 ** -17
+        got, want = scaled(cuda, [700, 130], [700, 130], 4, 2, D, dt, causal, grad, q_up=64.0, k_up=1 / 64)
+        assert want[1].abs().max() > 2.0 ** -17
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_gradients(cuda, D):
+    """grad_out and values whose dS passes f16's largest number (a loss scale) where
+    dQ (small K) or dK (small Q) does not."""
+    for i, up in ((0, 64.0), (1, 1 / 64)):
+        got, want = scaled(cuda, [300, 40], [300, 40], 4, 2, D, HF, True, 256.0, v_up=256.0, q_up=up, k_up=1 / up)
+        assert 100.0 < want[i].abs().max() < 60000.0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("shape", [([900], [900]), ([1300, 200], [500, 200]), ([700, 65], [2600, 64])])
+def test_gradients_of_rows_of_all_sizes(cuda, shape, D):
+    """Rows of grad_out from 2^-20 to 2^4, the small ones first, last and in turn:
+    the factors of keys fall on the way, in runs of queries and in two groups of
+    waves as well."""
+    n = sum(shape[0])
+    for rows in (torch.linspace(-20, 4, n), torch.linspace(4, -20, n),
+                 torch.where(torch.arange(n) % 97 == 0, 4.0, -20.0)):
+        scaled(cuda, *shape, 4, 1, D, HF, True, 1.0, k_up=8.0, q_up=1 / 8, rows=(2.0 ** rows).to(cuda))
