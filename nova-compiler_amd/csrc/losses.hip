@@ -136,11 +136,23 @@ __device__ __forceinline__ float exp_diff(float x, float m) {
   return __builtin_amdgcn_exp2f((x - m) * kL2e);
 }
 
+// A row's inputs.  Every thread reads them ahead of the reductions' barriers, so
+// that logp and row_loss may be written over them.
+struct Row {
+  float old_logp, ref_logp, advantage, weight;
+  __device__ __forceinline__ void load(const RowArgs &a, int row) {
+    old_logp = a.old_logp[row];
+    ref_logp = a.ref_logp ? a.ref_logp[row] : 0.0f;
+    advantage = a.advantage[row];
+    weight = a.weight[row];
+  }
+};
+
 // A row's slope d loss / d lp and its loss, from its log-probability.
-__device__ __forceinline__ void policy_row(const RowArgs &a, int row, float lp, float &loss,
+__device__ __forceinline__ void policy_row(const RowArgs &a, const Row &in, float lp, float &loss,
                                            float &slope) {
-  const float w = a.weight[row], adv = a.advantage[row];
-  const float ratio = expf(lp - a.old_logp[row]);
+  const float w = in.weight, adv = in.advantage;
+  const float ratio = expf(lp - in.old_logp);
   const float plain = ratio * adv;
   // fminf / fmaxf drop a NaN, which the products with the ratio bring back.
   const float clipped = fminf(fmaxf(ratio, a.lo), a.hi) * adv;
@@ -149,7 +161,7 @@ __device__ __forceinline__ void policy_row(const RowArgs &a, int row, float lp, 
   float g = take ? -plain : 0.0f;
   if (ratio != ratio) l = g = ratio;
   if (a.ref_logp) {
-    const float d = a.ref_logp[row] - lp;
+    const float d = in.ref_logp - lp;
     // exp(d) - 1 - d cancels near 0: expm1.
     const float em1 = expm1f(d);
     l += a.kl * (em1 - d);
@@ -187,6 +199,8 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH >= 512 ? 4 : 1) void logp_r
     }
     return;
   }
+  Row in = {};
+  if constexpr (MODE == kPolicy) in.load(a, row);
   u32x4 v[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -226,7 +240,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH >= 512 ? 4 : 1) void logp_r
     return;
   } else {
     float loss, slope;
-    policy_row(a, row, lp, loss, slope);
+    policy_row(a, in, lp, loss, slope);
     if (tid == 0) {
       a.logp[row] = lp;
       a.row_loss[row] = loss;
@@ -276,6 +290,8 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
     }
     return;
   }
+  Row in = {};
+  if constexpr (MODE == kPolicy) in.load(a, row);
   const float xt = tid < tail ? X::widen(x[(int64_t)nc * X::kE + tid]) : -INFINITY;
   const float xy = y < a.C ? X::widen(x[y]) : __builtin_nanf("");
   float m = xt, s = tid < tail && xt > -INFINITY ? 1.0f : 0.0f;
@@ -308,7 +324,7 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
     }
   } else {
     float loss, slope;
-    policy_row(a, row, lp, loss, slope);
+    policy_row(a, in, lp, loss, slope);
     if (tid == 0) {
       a.logp[row] = lp;
       a.row_loss[row] = loss;
@@ -367,6 +383,8 @@ struct PairArgs {
 __global__ __launch_bounds__(256) void preference_pair_kernel(PairArgs a) {
   __shared__ double part[256];
   const int pair = blockIdx.x, tid = threadIdx.x;
+  // Ahead of the barriers: seq_logp may be written over them.
+  const float ref0 = a.ref[2 * pair], ref1 = a.ref[2 * pair + 1];
   double seq[2];
   int s[2], e[2];
 #pragma unroll
@@ -384,7 +402,7 @@ __global__ __launch_bounds__(256) void preference_pair_kernel(PairArgs a) {
     __syncthreads();
     seq[j] = part[0];
   }
-  const double h = a.beta * ((seq[0] - (double)a.ref[2 * pair]) - (seq[1] - (double)a.ref[2 * pair + 1]));
+  const double h = a.beta * ((seq[0] - (double)ref0) - (seq[1] - (double)ref1));
   const double soft = log1p(exp(-fabs(h)));
   const double neg = 1.0 / (1.0 + exp(h));  // sigmoid(-h)
   const double c = a.beta * (a.smoothing * (1.0 - neg) - (1.0 - a.smoothing) * neg) / a.P;

@@ -345,3 +345,27 @@ def test_logits_far_from_zero(cuda, C, shift):
     one = torch.ones(12, device=cuda)
     _, _, grad = nh.policy_loss(far, y, lp.float(), one, one)
     check_grad(grad, -torch.ones_like(lp), lp_tol(lp, dist) + 2.0 ** -24 * lp.abs() + 2.0 ** -22, p, y, ok)
+
+
+@pytest.mark.parametrize("C", [300, 5000, 32000, 50304, 60000, 120000])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_results_written_over_the_inputs(cuda, dt, C):
+    """logp over old_logp, ref_logp or advantage, row_loss over weight, seq_logp
+    over the sequences' ref_logp: the bits of separate memory."""
+    R = 700
+    x, y, g = make(cuda, R, C, dt, masked=0.2)
+    old = nh.token_logp(x, y) - 0.1 * torch.randn(R, generator=g, device=cuda)
+    ref, adv, w = old + 0.05, torch.randn(R, generator=g, device=cuda), torch.rand(R, generator=g, device=cuda)
+    row = torch.empty(R, device=cuda)
+    call = lambda o, f, a, v, **k: nh.policy_loss(x, y, o, a, v, ref_logp=f, kl_coef=0.1, **k)
+    want = call(old, ref, adv, w, row_loss=row)
+    for i in range(3):
+        ins = [t.clone() for t in (old, ref, adv, w)]
+        got = call(*ins, logp=ins[i], row_loss=ins[3])
+        assert torch.equal(ins[i], want[1]) and torch.equal(ins[3], row)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    off = torch.tensor([0, 100, 350, 420, 700], dtype=torch.int32, device=cuda)
+    ref = torch.randn(4, generator=g, device=cuda) * 10 - 900
+    want = nh.preference_loss(x, y, off, ref)
+    got = nh.preference_loss(x, y, off, ref, seq_logp=ref)
+    assert torch.equal(ref, want[1]) and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
