@@ -492,8 +492,9 @@ int32_t _mlir_ciface_nova_hip_token_logp(const NovaMemRef2D *logits, const NovaM
  *   grad_scale * d loss / d logits in the same pass over the logits.
  * Where both sides of the min are equal the gradient is the first's.
  *   old_logp, ref_logp, advantage (A), weight, logp, row_loss : [R] f32;
- *   ref_logp may be NULL when kl_coef is 0.  A row with weight 0 takes no
- *   part either.  weight carries the mean a caller wants (1 / valid tokens,
+ *   ref_logp may be NULL when kl_coef is 0.  A row with weight 0 adds no
+ *   loss, whatever its ratio, and its gradient is zero; its logp is that of its
+ *   label all the same (0 for a label of C or more).  weight carries the mean a caller wants (1 / valid tokens,
  *   1 / (sequences length), ...); grad_scale is a loss scale.  logp and row_loss
  *   may be written over old_logp, ref_logp, advantage or weight (logp over
  *   old_logp: the next step's), whole vectors over each other. */

@@ -167,8 +167,17 @@ __device__ __forceinline__ void policy_row(const RowArgs &a, const Row &in, floa
     l += a.kl * (em1 - d);
     g -= a.kl * em1;
   }
-  loss = w * l;
-  slope = w * g;
+  // Weight 0: nothing of an infinite or NaN loss either.
+  loss = w == 0.0f ? 0.0f : w * l;
+  slope = w == 0.0f ? 0.0f : w * g;
+}
+
+template <int DT, int TH>
+__device__ __forceinline__ void zero_row(typename Chunk<DT>::T *g, int C, int tid) {
+  typedef Chunk<DT> X;
+  const int nc = C / X::kE, tail = C - nc * X::kE;
+  for (int c = tid; c < nc; c += TH) X::store(g + (int64_t)c * X::kE, u32x4{0, 0, 0, 0});
+  if (tid < tail) g[(int64_t)nc * X::kE + tid] = typename X::T(0);
 }
 
 // TH threads per row, NC chunks per thread; TH == 64: four rows a workgroup.
@@ -181,7 +190,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH >= 512 ? 4 : 1) void logp_r
   const int row = TH == 64 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= a.rows) return;
   const int y = __builtin_amdgcn_readfirstlane(a.labels[row]);
-  const bool skip = y < 0 || (MODE == kPolicy && a.weight[row] == 0.0f);
+  const bool skip = y < 0 || (MODE == kPolicy && y >= a.C && a.weight[row] == 0.0f);
   const T *x = static_cast<const T *>(a.logits) + row * a.sx;
   T *g = a.grad ? static_cast<T *>(a.grad) + row * a.sg : nullptr;
   const int nc = a.C / X::kE, tail = a.C - nc * X::kE;
@@ -193,10 +202,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH >= 512 ? 4 : 1) void logp_r
       if (a.slope) a.slope[row] = 0.0f;
       if (MODE == kPolicy) a.row_loss[row] = 0.0f;
     }
-    if (MODE == kPolicy && g) {
-      for (int c = tid; c < nc; c += TH) X::store(g + c * X::kE, u32x4{0, 0, 0, 0});
-      if (tid < tail) g[nc * X::kE + tid] = T(0);
-    }
+    if (MODE == kPolicy && g) zero_row<DT, TH>(g, a.C, tid);
     return;
   }
   Row in = {};
@@ -246,6 +252,7 @@ __global__ __launch_bounds__(TH == 64 ? 256 : TH, TH >= 512 ? 4 : 1) void logp_r
       a.row_loss[row] = loss;
     }
     if (!g) return;
+    if (in.weight == 0.0f) return zero_row<DT, TH>(g, a.C, tid);
     slope *= a.grad_scale;
     const float k = -slope / s;
     auto value = [&](float xv, int col) __attribute__((always_inline)) {
@@ -273,7 +280,7 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
   __shared__ float red[TH / 64];
   const int tid = threadIdx.x, row = blockIdx.x;
   const int y = __builtin_amdgcn_readfirstlane(a.labels[row]);
-  const bool skip = y < 0 || (MODE == kPolicy && a.weight[row] == 0.0f);
+  const bool skip = y < 0 || (MODE == kPolicy && y >= a.C && a.weight[row] == 0.0f);
   const T *x = static_cast<const T *>(a.logits) + row * a.sx;
   T *g = a.grad ? static_cast<T *>(a.grad) + row * a.sg : nullptr;
   const int nc = a.C / X::kE, tail = a.C - nc * X::kE;
@@ -284,10 +291,7 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
       if (a.slope) a.slope[row] = 0.0f;
       if (MODE == kPolicy) a.row_loss[row] = 0.0f;
     }
-    if (MODE == kPolicy && g) {
-      for (int c = tid; c < nc; c += TH) X::store(g + (int64_t)c * X::kE, u32x4{0, 0, 0, 0});
-      if (tid < tail) g[(int64_t)nc * X::kE + tid] = T(0);
-    }
+    if (MODE == kPolicy && g) zero_row<DT, TH>(g, a.C, tid);
     return;
   }
   Row in = {};
@@ -330,6 +334,7 @@ __global__ __launch_bounds__(512) void logp_long_kernel(RowArgs a) {
       a.row_loss[row] = loss;
     }
     if (!g) return;
+    if (in.weight == 0.0f) return zero_row<DT, TH>(g, a.C, tid);
     slope *= a.grad_scale;
     const float k = -slope / s;
     auto value = [&](float xv, int64_t col) __attribute__((always_inline)) {

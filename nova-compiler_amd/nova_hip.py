@@ -703,7 +703,8 @@ def policy_loss(logits, labels, old_logp, advantage, weight, *, ref_logp=None, c
     """The clipped policy loss over tokens, weighted by ``weight``, with a KL
     term to ``ref_logp``: returns (loss[1], logp [rows], grad), grad None
     with ``want_grad`` False.  ``clip`` is (low, high): the ratio is clamped to
-    [1 - low, 1 + high].  Rows with a negative label or weight 0 take no part."""
+    [1 - low, 1 + high].  Rows with a negative label take no part; rows with
+    weight 0 have a log-probability but no loss and a zero gradient."""
     torch = _torch()
     f32, dt, dev = torch.float32, logits.dtype, logits.get_device()
     d = (_desc(logits, 2, dt, dev, "logits"), _desc(labels, 1, torch.int32, dev, "labels"),

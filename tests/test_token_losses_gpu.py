@@ -369,3 +369,33 @@ def test_results_written_over_the_inputs(cuda, dt, C):
     want = nh.preference_loss(x, y, off, ref)
     got = nh.preference_loss(x, y, off, ref, seq_logp=ref)
     assert torch.equal(ref, want[1]) and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+
+
+@pytest.mark.parametrize("C", [300, 5000, 50304, 110001])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_rows_of_weight_zero(cuda, dt, C):
+    """Their log-probability is the label's, so that it can be the next step's
+    old_logp (within LP of the module's docstring: calls with and without a
+    gradient give a row different numbers of threads and so add it up in different
+    orders, each within LP); they add no loss and have a zero gradient, even where
+    their logits or ratio are infinite or NaN; the other rows are what they were."""
+    x, y, g = make(cuda, 12, C, dt, masked=0)
+    y[3] = -1
+    x[5, 7], x[6, 0] = float("nan"), float("inf")
+    old = torch.zeros(12, device=cuda)
+    old[7] = -1e30
+    adv, w = torch.randn(12, generator=g, device=cuda), torch.rand(12, generator=g, device=cuda) + 0.1
+    none = torch.tensor([1, 3, 5, 6, 7], device=cuda)
+    w[none] = 0.0
+    row = torch.full((12,), 7.0, device=cuda)
+    loss, logp, grad = nh.policy_loss(x, y, old, adv, w, ref_logp=old, kl_coef=0.1, row_loss=row)
+    want, _, dist, _ = rows64(x, y)
+    assert torch.isnan(logp[[5, 6]]).all() and torch.isnan(want[[5, 6]]).all()
+    fine = torch.tensor([i for i in range(12) if i not in (5, 6)], device=cuda)
+    assert ((logp.double() - want).abs() <= lp_tol(want, dist))[fine].all()
+    assert logp[1] < 0 and logp[3] == 0
+    assert (row[none] == 0).all() and (grad[none] == 0).all() and torch.isfinite(loss).all()
+    rest = torch.tensor([i for i in range(12) if i not in none.tolist()], device=cuda)
+    a = nh.policy_loss(x[rest], y[rest], old[rest], adv[rest], w[rest], ref_logp=old[rest], kl_coef=0.1)
+    assert torch.equal(grad[rest], a[2]) and torch.equal(logp[rest], a[1])
+    assert abs(loss.item() - a[0].item()) <= 2.0 ** -23 * abs(a[0].item())
