@@ -419,9 +419,10 @@ int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D
  *   lse : [heads, query tokens] f32, log sum exp of the scaled scores, or
  *   NULL.
  * Scores, softmax and sums are f32; the weights are rounded to dt for the
- * product with v.  Rows outside every sequence are left as they were; out must
- * not overlap q, k or v.  No workspace: concurrent calls and captured graphs
- * share nothing.
+ * product with v.  Rows outside every sequence are left as they were.  Results
+ * that overlap an operand or each other are refused (views of one buffer, whose
+ * rows, heads or tokens lie beside each other, are apart).  No workspace:
+ * concurrent calls and captured graphs share nothing.
  * ---------------------------------------------------------------------- */
 int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3D *k,
                                         const NovaMemRef3D *v, const NovaMemRef1D *q_offsets,
@@ -436,12 +437,12 @@ int32_t _mlir_ciface_nova_hip_attention(const NovaMemRef3D *q, const NovaMemRef3
  * strides as for the forward (grad_out, out, dq as q; dk, dv as k); lse
  * [heads, query tokens]; scratch : at least
  * nova_hip_attention_backward_scratch() f32, dense, used by this call only.  dq,
- * dk and dv must not overlap the other operands or each other (views of one
- * buffer are apart).  P and dS are rounded to dt for the products (in f16 each
- * column of dS takes a power of two of its own, so that small and large gradients
- * keep their bits), sums are f32 in a fixed order (no atomics: the same bits on
- * every run).  A query that sees no key has gradient zero and
- * adds none; rows outside every sequence are left as they were. */
+ * dk and dv that overlap the other operands or each other are refused.  P and dS
+ * are rounded to dt for the products (in f16 each column of dS takes a power of
+ * two of its own, so that small and large gradients keep their bits), sums are f32
+ * in a fixed order (no atomics: the same bits on every run).  A query that sees no
+ * key has gradient zero and adds none; rows outside every sequence are left as
+ * they were. */
 int32_t _mlir_ciface_nova_hip_attention_backward(
     const NovaMemRef3D *grad_out, const NovaMemRef3D *q, const NovaMemRef3D *k,
     const NovaMemRef3D *v, const NovaMemRef3D *out, const NovaMemRef2D *lse,
@@ -460,8 +461,8 @@ int64_t nova_hip_attention_backward_scratch(int64_t q_tokens, int64_t k_tokens, 
  *   rows behind a length are not read.  lse : [sequences, heads] f32 or NULL.
  *   scratch : nova_hip_attention_decode_scratch() f32, dense and 8-byte aligned,
  *   used by this call only (NULL when that is 0).
- * A length of 0 gives a zero row and lse -inf.  Types and roundings as for
- * _mlir_ciface_nova_hip_attention. */
+ * A length of 0 gives a zero row and lse -inf.  Results on operands are refused.
+ * Types and roundings as for _mlir_ciface_nova_hip_attention. */
 int32_t _mlir_ciface_nova_hip_attention_decode(const NovaMemRef3D *q, const NovaMemRef4D *k,
                                                const NovaMemRef4D *v, const NovaMemRef1D *lengths,
                                                NovaMemRef3D *out, NovaMemRef2D *lse,

@@ -270,6 +270,14 @@ int32_t launch_attention(const AttentionProblem &p, hipStream_t s) {
   if (tiles * p.heads >= 1 << 24)
     return fail(NOVA_HIP_ERANGE, "attention: %lld tiles of %lld heads exceed 2^24 - 1",
                 (long long)tiles, (long long)p.heads);
+  const Extent q = extent("q", p.q, p.Tq, p.heads, p.D), k = extent("k", p.k, p.Tk, p.kv_heads, p.D),
+               v = extent("v", p.v, p.Tk, p.kv_heads, p.D),
+               out = extent("out", p.o, p.Tq, p.heads, p.D),
+               lse = {"lse", p.lse, p.lse ? 4 * p.Tq : 0, {p.heads, 1, 1}, {4 * p.slse, 0, 0}};
+  int32_t rc;
+  if ((rc = check_apart("attention", out, {q, k, v})) ||
+      (rc = check_apart("attention", lse, {q, k, v, out})))
+    return rc;
   a.tiles = (int)tiles;
   const unsigned grid = (unsigned)(tiles * p.heads);
   if (p.dt == NOVA_HIP_DT_BF16) attn::launch_fwd<NOVA_HIP_DT_BF16>(a, p.causal, grid, s);

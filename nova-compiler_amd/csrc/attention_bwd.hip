@@ -659,6 +659,18 @@ int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t
   // A grid's dimension holds less than 2^32 threads.
   if (std::max(qt * p.f.heads, kt * p.f.kv_heads * a.splits) >= 1 << 24)
     return fail(NOVA_HIP_ERANGE, "attention_backward: more than 2^24 - 1 tiles");
+  const char *w = "attention_backward";
+  const int64_t Tq = p.f.Tq, Tk = p.f.Tk, H = p.f.heads, G = p.f.kv_heads, D = p.f.D;
+  const Extent q = extent("q", p.f.q, Tq, H, D), k = extent("k", p.f.k, Tk, G, D),
+               v = extent("v", p.f.v, Tk, G, D), out = extent("out", p.f.o, Tq, H, D),
+               go = extent("grad_out", p.go, Tq, H, D), dq = extent("dq", p.dq, Tq, H, D),
+               dk = extent("dk", p.dk, Tk, G, D), dv = extent("dv", p.dv, Tk, G, D),
+               lse = {"lse", p.f.lse, 4 * Tq, {H, 1, 1}, {4 * p.f.slse, 0, 0}};
+  int32_t rc;
+  if ((rc = check_apart(w, dq, {q, k, v, out, go, lse, dk, dv})) ||
+      (rc = check_apart(w, dk, {q, k, v, out, go, lse, dv})) ||
+      (rc = check_apart(w, dv, {q, k, v, out, go, lse})))
+    return rc;
   return p.f.dt == NOVA_HIP_DT_BF16
              ? attn::launch_bwd<NOVA_HIP_DT_BF16>(a, p.f.causal, qt, kt, s)
              : attn::launch_bwd<NOVA_HIP_DT_F16>(a, p.f.causal, qt, kt, s);

@@ -323,6 +323,16 @@ int64_t attention_decode_scratch(int64_t B, int64_t S, int64_t heads, int64_t kv
 
 int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s) {
   if (p.B == 0 || p.heads == 0 || p.D == 0) return NOVA_HIP_SUCCESS;
+  const int64_t B = p.B, S = p.S, H = p.heads, G = p.kv_heads, run = 2 * p.D;
+  const Extent q = {"q", p.q, run, {B, H, 1}, {2 * p.sqb, 2 * p.sqh, 0}},
+               k = {"k", p.k, S ? run : 0, {B, S, G}, {2 * p.skb, 2 * p.skt, 2 * p.skh}},
+               v = {"v", p.v, S ? run : 0, {B, S, G}, {2 * p.svb, 2 * p.svt, 2 * p.svh}},
+               out = {"out", p.o, run, {B, H, 1}, {2 * p.sob, 2 * p.soh, 0}},
+               lse = {"lse", p.lse, p.lse ? 4 * H : 0, {B, 1, 1}, {4 * p.slse, 0, 0}};
+  int32_t rc;
+  if ((rc = check_apart("attention_decode", out, {q, k, v})) ||
+      (rc = check_apart("attention_decode", lse, {q, k, v, out})))
+    return rc;
   attn::DecodeArgs a;
   a.q = static_cast<const uint16_t *>(p.q);
   a.k = static_cast<const uint16_t *>(p.k);

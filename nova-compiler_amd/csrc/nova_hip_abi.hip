@@ -12,6 +12,7 @@
 #include <cmath>
 #include <mutex>
 #include <memory>
+#include <numeric>
 #include <unordered_map>
 #include <vector>
 
@@ -404,6 +405,40 @@ const float *in_f32(const D *d) {
 }
 
 }  // namespace
+
+// Two operands are apart where their ranges are, or, views of one buffer, where
+// modulo a step common to their longer strides what is left of each (the shorter
+// strides and the runs) lies beside the other's.
+static bool apart(const Extent &a, const Extent &b) {
+  auto span = [](const Extent &x, int64_t below) {
+    int64_t s = x.run;
+    for (int i = 0; i < 3; ++i)
+      if (x.n[i] > 1 && x.st[i] < below) s += (x.n[i] - 1) * x.st[i];
+    return s;
+  };
+  if (!a.run || !b.run) return true;
+  const intptr_t pa = reinterpret_cast<intptr_t>(a.p), pb = reinterpret_cast<intptr_t>(b.p);
+  if (pa >= pb + span(b, INT64_MAX) || pb >= pa + span(a, INT64_MAX)) return true;
+  for (const Extent *x : {&a, &b})
+    for (int i = 0; i < 3; ++i) {
+      const int64_t least = x->st[i];
+      if (x->n[i] <= 1 || least == 0) continue;
+      int64_t step = 0;
+      for (const Extent *y : {&a, &b})
+        for (int j = 0; j < 3; ++j)
+          if (y->n[j] > 1 && y->st[j] >= least) step = std::gcd(step, y->st[j]);
+      const int64_t at = ((pb - pa) % step + step) % step;
+      if (at >= span(a, least) && step - at >= span(b, least)) return true;
+    }
+  return false;
+}
+
+int32_t check_apart(const char *w, const Extent &result,
+                              std::initializer_list<Extent> others) {
+  for (const Extent &x : others)
+    if (!apart(result, x)) return fail(NOVA_HIP_EINVAL, "%s: %s overlaps %s", w, result.name, x.name);
+  return NOVA_HIP_SUCCESS;
+}
 }  // namespace nova_hip
 
 using namespace nova_hip;

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/nova_hip.h"
@@ -139,6 +140,19 @@ struct AttentionProblem {
   int dt;
 };
 int32_t launch_attention(const AttentionProblem &p, hipStream_t s);
+
+// The bytes of an operand: runs of `run` bytes in up to three dims (strides in
+// bytes, not negative).
+struct Extent {
+  const char *name;
+  const void *p;
+  int64_t run, n[3], st[3];
+};
+inline Extent extent(const char *name, const AttentionOperand &o, int64_t T, int64_t H, int64_t D) {
+  return {name, o.p, T && H ? 2 * D : 0, {T, H, 1}, {2 * o.st, 2 * o.sh, 0}};
+}
+// Refuses a result that overlaps one of `others`.
+int32_t check_apart(const char *w, const Extent &result, std::initializer_list<Extent> others);
 
 struct AttentionBackwardProblem {
   AttentionProblem f;  // the forward's operands, result and lse

@@ -253,3 +253,88 @@ def test_wrappers_refuse_before_the_call():
     assert code(nh.policy_loss, x, y, v, v, v, grad=x.to(bf)) == EDTYPE
     assert code(nh.preference_loss, x, y, off, v.to(bf)) == EDTYPE
     assert code(nh.preference_loss, x, y, off, v) == EINVAL
+
+
+# ---- results on operands ---------------------------------------------------------------------
+
+def shifted(sizes, at, strides=None):
+    """A view `at` elements of 2 bytes behind FAKE."""
+    return d(sizes, strides, ptr=FAKE + 2 * at)
+
+
+def refused(rc):
+    return rc == EINVAL and b"overlaps" in nh.lib().nova_hip_last_error()
+
+
+FAR = 1 << 24
+Q, K = (10, 4, 64), (12, 2, 64)
+
+
+def fwd_at(**kw):
+    o = dict(q=shifted(Q, 0), k=shifted(K, FAR), v=shifted(K, 2 * FAR), out=shifted(Q, 3 * FAR),
+             lse=shifted((4, 10), 4 * FAR))
+    o.update(kw)
+    return fwd(**o)
+
+
+def bwd_at(**kw):
+    o = dict(q=shifted(Q, 0), k=shifted(K, FAR), v=shifted(K, 2 * FAR), out=shifted(Q, 3 * FAR),
+             lse=shifted((4, 10), 4 * FAR), go=shifted(Q, 5 * FAR), dq=shifted(Q, 6 * FAR),
+             dk=shifted(K, 7 * FAR), dv=shifted(K, 8 * FAR), scratch=d((10 ** 6,), ptr=FAKE + 18 * FAR))
+    o.update(kw)
+    return bwd(**o)
+
+
+def dec_at(**kw):
+    o = dict(q=shifted((3, 4, 64), 0), k=shifted((3, 2000, 2, 64), FAR), v=shifted((3, 2000, 2, 64), 2 * FAR),
+             out=shifted((3, 4, 64), 3 * FAR), lse=shifted((3, 4), 4 * FAR),
+             scratch=d((10 ** 6,), ptr=FAKE + 10 * FAR))
+    o.update(kw)
+    return dec(**o)
+
+
+@pytest.mark.parametrize("at", [0, 8, 2560 - 8, -(2560 - 8)])
+def test_results_on_operands_are_refused(at):
+    assert refused(fwd_at(out=shifted(Q, at)))
+    assert refused(fwd_at(out=shifted(Q, FAR + min(at, 1536 - 8))))
+    assert refused(fwd_at(lse=shifted((4, 10), max(-72, min(at, 2400)))))
+    for i in (0, 3, 5):  # q, out, grad_out
+        assert refused(bwd_at(dq=shifted(Q, i * FAR + at)))
+    at = max(-(1536 - 8), min(at, 1536 - 8))
+    for i in (1, 2):  # k, v
+        assert refused(bwd_at(dk=shifted(K, i * FAR + at))) and refused(bwd_at(dv=shifted(K, i * FAR + at)))
+    assert refused(bwd_at(dv=shifted(K, 7 * FAR + at))) and refused(bwd_at(dk=shifted(K, 6 * FAR)))
+    assert refused(bwd_at(dq=shifted(Q, 4 * FAR)))
+    for i in (0, 1, 2):
+        assert refused(dec_at(out=shifted((3, 4, 64), i * FAR + max(at, 0) % 768 // 8 * 8)))
+    assert refused(dec_at(lse=shifted((3, 4), 3 * FAR)))
+
+
+@pytest.mark.parametrize("view,strides", [
+    # Views of one buffer that share bytes: heads of one projection that
+    # overlap by one, halves of rows by eight values, tokens by one.
+    (256 - 64, (640, 64, 1)), (64 - 8, (640, 128, 1)), (9 * 256, (256, 64, 1)),
+    (64, (128, 1280, 1)),  # every second token, but from the heads' side the same rows
+])
+def test_views_that_share_bytes_are_refused(view, strides):
+    other = strides if strides != (128, 1280, 1) else (128, 1344, 1)
+    assert refused(fwd_at(q=shifted(Q, 0, strides), out=shifted(Q, view, other)))
+    assert refused(bwd_at(q=shifted(Q, 0, strides), dq=shifted(Q, view, other)))
+
+
+@pytest.mark.parametrize("view,strides", [
+    (256, (640, 64, 1)),       # heads beside each other in one projection's rows
+    (-256, (640, 64, 1)), (640 - 256, (640, 64, 1)),
+    (64, (512, 128, 1)),       # halves of each head's row
+    (64, (128, 1280, 1)),      # tokens in turn, heads outermost
+    (2560, (256, 64, 1)),      # one behind the other
+    (640, (64, 1280, 1)),      # heads in turn
+])
+def test_views_beside_each_other_pass(view, strides):
+    """(What comes behind the check, a launch without a GPU, fails otherwise.)"""
+    assert not refused(fwd_at(q=shifted(Q, 0, strides), out=shifted(Q, view, strides)))
+    assert not refused(bwd_at(q=shifted(Q, 0, strides), dq=shifted(Q, view, strides)))
+    kv = strides[0] // 2 // 64 * 64 if strides == (640, 64, 1) else None
+    if kv:  # dq, dk and dv as the three parts of a fused projection's gradient
+        assert not refused(bwd_at(dq=shifted(Q, 6 * FAR, (512, 64, 1)), dk=shifted(K, 6 * FAR + 256, (512, 64, 1)),
+                                  dv=shifted(K, 6 * FAR + 384, (512, 64, 1))))
