@@ -539,12 +539,14 @@ int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s)
   if (k_tiles > 0) {
     a.tiles = (int)k_tiles;
     const unsigned grid = (unsigned)(k_tiles * (a.heads / a.group));
-    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL>), dim3(a.splits > 1 ? (grid + 7) / 8 * 8 : grid, a.splits),
-                       dim3(64 * kWaves), 0, s, a);
+    hipLaunchKernelGGL((attention_dkv_kernel<DT, DP, CAUSAL>),
+                       dim3(a.splits > 1 ? (grid + 7) / 8 * 8 : grid, a.splits), dim3(64 * kWaves),
+                       0, s, a);
     if (a.splits > 1) {
       const int32_t rc = check_hip(hipGetLastError(), "attention_backward launch");
       if (rc) return rc;
-      hipLaunchKernelGGL((attention_dkv_join_kernel<DT, DP, CAUSAL>), dim3(grid), dim3(64 * kWaves), 0, s, a);
+      hipLaunchKernelGGL((attention_dkv_join_kernel<DT, DP, CAUSAL>), dim3(grid),
+                         dim3(64 * kWaves), 0, s, a);
     }
   }
   return check_hip(hipGetLastError(), "attention_backward launch");
@@ -573,21 +575,35 @@ int64_t tile_bound(int64_t T, int64_t B) { return attn::tile_bound(T, B, attn::k
 // `most` follows from them, and the device splits those tiles that are long.
 // With fewer tiles than the chip takes at once (256, 512 at D <= 64), up to four
 // runs, or eight for very few tiles; with up to four times as many, causal, two,
-// the last ones first (the longest tiles have them).  No run is shorter than half
-// the mean work of a slot (a quarter / a half, us, packed 568 tiles as below 687 /
-// 674, 2 x 4096 tokens of 8 heads of 128 312 / 283), but where the tiles are just
-// more than the chip takes, when halves of all of them fill it evenly (2 x 8192 of
-// 16 in groups of 8 of 128, 260 tiles: 2110 / 1830).  Nothing is split where no sequence is likely to be long: between all of
-// one length and one that has all tokens, the geometric mean decides: of more
-// tiles where the products are short (D <= 64) and half of the chip is busy, since
-// the join's launch alone takes 3 us (8 x 1024 of 6 heads of 64 47 / 51.5 with
-// nothing to join).  The whole backward without runs and with them, us:
-//   4096 causal tokens, 8 heads in groups of 4 of 128 (66 tiles)  487 / 212
-//   2 x 2048, 16 in groups of 4 of 128 (136)                      277 / 184
-//   packed 1 to 4096, 32 in groups of 4 of 128 (568)              711 / 664
-//   8192, 6 of 64 (390)                                           254 / 228
-//   8192, 12 in groups of 3 of 64 (260)                           555 / 417
-//   2 x 4096 not causal, 8 in groups of 4 of 64 (132)             481 / 279
+// the last ones first (the longest tiles have them).
+//
+// A run has `least` tiles of 64 queries at least: 8 where tiles are few or long in
+// time (D > 64), else 16.  And at least a slot's share of the batch's work, of which
+// causal tiles, the longest twice the mean, take a half (a quarter / a half, us,
+// packed 568 tiles as below 687 / 674, 2 x 4096 tokens of 8 heads of 128 312 / 283)
+// and the others, as long as their sequence, all (a half / all: 4 x 2048 of 6 heads
+// of 64 134 / 116, 8 x 1024 of 3 of 128 90 / 73, packed 1 to 4096 of 6 of 64 199 /
+// 187).  Where the tiles are just more than the chip takes, halves of all of them
+// fill it evenly (2 x 8192 of 16 in groups of 8 of 128, 260 tiles: 2380 / 1800).
+//
+// Nothing is split where no sequence is likely to be long enough: two runs of 16 or
+// three of 8 in the geometric mean of all sequences of one length and one that has
+// all tokens.  The host cannot tell these apart, so equal sequences pay for the
+// join's launch (3 us, 6 at D > 64) and packed ones of the same number gain.  The
+// whole backward without runs and with them, us, causal unless said otherwise:
+//   8 x 1024 / 1 to 4096 packed, 6 heads of 64 (432, 426 tiles)  49.3 / 52.1, 122 / 116
+//   9 x 1024, 4 x 2048, 6 of 64                                   54.7 / 58.0, 73.6 / 78.3
+//   4000 and seven shorter to 50, 6 of 64                         117 / 99
+//   8 x 1024 / 1 to 4096 packed, 3 of 128                         65 / 71, 192 / 163
+//   8 x 1024, 4 x 2048 / 1 to 4096 packed, 8 of 128               89 / 96, 146 / 162, 236 / 241
+//   1 to 4096 packed, 32 in groups of 4 of 128 (568)              720 / 666
+//   8 x 1024, 8 in groups of 4 of 128                             151 / 112
+//   4096, 8 in groups of 4 of 128 (66)                            491 / 218
+//   2 x 2048, 16 in groups of 4 of 128 (136)                      278 / 182
+//   8192, 6 of 64 (390); 12 in groups of 3 of 64 (260)            244 / 230, 553 / 424
+//   2 x 4096 not causal, 8 in groups of 4 of 64 (132)             482 / 281
+// and under the bound, with runs from half of it on: 2 x 1024 of 6 of 64 39.9 /
+// 43.8, 1024 39.8 / 43.2, but 2000 and 48 65 / 58.
 struct Runs {
   int64_t most;
   int least;
@@ -599,13 +615,12 @@ Runs dkv_runs(int64_t Tq, int64_t Tk, int64_t B, int64_t heads, int64_t kv_heads
   if (B == 0 || kv_heads == 0 || Tk == 0) return {1, 1, 0.0f, false};
   const int64_t units = tile_bound(Tk, B) * kv_heads, slots = D <= 64 ? 512 : 256;
   const double tiles = (double)Tq * (heads / kv_heads) / attn::kBN, likely = tiles * tiles / B;
-  const bool few = units < slots / 4;
-  const double least = few ? 16 : D > 64 || units < slots / 2 ? 24 : 48;
-  if (likely < least * least || units >= (causal ? 4 : 1) * slots)
-    return {1, 1, 0.0f, false};
-  return {units < slots / 8 ? 8 : units < slots ? 4 : 2,
-          few || (D > 64 && units < slots) ? 8 : 16,
-          units >= slots && 2 * units < 3 * slots ? 0.0f : 0.5f / slots, units >= slots};
+  const int least = units < slots / 4 || (D > 64 && units < slots) ? 8 : 16;
+  const double enough = least == 8 ? 24 : 32;
+  if (likely < enough * enough || units >= (causal ? 4 : 1) * slots) return {1, 1, 0.0f, false};
+  return {units < slots / 8 ? 8 : units < slots ? 4 : 2, least,
+          units >= slots && 2 * units < 3 * slots ? 0.0f : (causal ? 0.5f : 1.0f) / slots,
+          units >= slots};
 }
 }  // namespace
 
@@ -613,7 +628,8 @@ int64_t attention_backward_scratch(int64_t Tq, int64_t Tk, int64_t B, int64_t he
                                    int64_t kv_heads, int64_t D, bool causal) {
   const int64_t rows = 2 * heads * Tq, splits = dkv_runs(Tq, Tk, B, heads, kv_heads, D, causal).most;
   if (splits <= 1) return rows;
-  return (rows + 63) / 64 * 64 + tile_bound(Tk, B) * kv_heads * splits * attn::kWaves * 64 * padded_dim(D);
+  return (rows + 63) / 64 * 64 +
+         tile_bound(Tk, B) * kv_heads * splits * attn::kWaves * 64 * padded_dim(D);
 }
 
 int32_t launch_attention_backward(const AttentionBackwardProblem &p, hipStream_t s) {

@@ -338,3 +338,19 @@ def test_views_beside_each_other_pass(view, strides):
     if kv:  # dq, dk and dv as the three parts of a fused projection's gradient
         assert not refused(bwd_at(dq=shifted(Q, 6 * FAR, (512, 64, 1)), dk=shifted(K, 6 * FAR + 256, (512, 64, 1)),
                                   dv=shifted(K, 6 * FAR + 384, (512, 64, 1))))
+
+
+def test_runs_of_queries_follow_tokens_and_sequences():
+    """Scratch for runs where two runs of 16 tiles of 64 queries (three of 8 for few
+    tiles, or heads of more than 64) fit the likely longest sequence, and by no
+    other sign of a batch: between a little under and a little over the bound the
+    answer changes once."""
+    def runs(T, B, H, D, causal=1):
+        return nh.lib().nova_hip_attention_backward_scratch(T, T, B, H, H, D, causal) > 2 * H * T
+    # sqrt(T / 64 * T / B / 64) tiles in the likely longest.
+    for H, D, B, tiles in ((6, 64, 8, 32), (6, 64, 9, 32), (12, 64, 4, 32), (1, 64, 4, 24), (3, 128, 8, 24),
+                           (8, 128, 8, 32)):
+        least = int(64 * tiles * B ** 0.5)
+        assert [runs(T, B, H, D) for T in (least // 2, least - 1, least + 64, 2 * least)] == [0, 0, 1, 1], (H, D, B)
+    # Equal and unequal sequences of the same number and tokens have the same bound.
+    assert runs(8192, 8, 6, 64) and runs(8120, 8, 6, 64) and runs(9216, 9, 6, 64)

@@ -332,3 +332,36 @@ def test_gradients_of_rows_of_all_sizes(cuda, shape, D):
     for rows in (torch.linspace(-20, 4, n), torch.linspace(4, -20, n),
                  torch.where(torch.arange(n) % 97 == 0, 4.0, -20.0)):
         scaled(cuda, *shape, 4, 1, D, HF, True, 1.0, k_up=8.0, q_up=1 / 8, rows=(2.0 ** rows).to(cuda))
+
+
+def runs_scratch(lens, H, G, D, causal=True):
+    """Floats of scratch beyond the rows' constants, over those of one run of all
+    tiles of keys: the most runs a tile may have."""
+    T = sum(lens)
+    need = nh.lib().nova_hip_attention_backward_scratch(T, T, len(lens), H, G, D, causal)
+    tiles = (T // 128 + len(lens)) * G
+    return tiles, (need - (2 * H * T + 63) // 64 * 64) // (tiles * 4 * 64 * D)
+
+
+@pytest.mark.parametrize("D,H,G,lens", [
+    (128, 12, 12, [2500, 597]),  # every tile halved: just more than 256 tiles ...
+    (128, 26, 13, [2400, 130]),  # (heads in groups)
+    (64, 24, 24, [2500, 597]),   # ... or 512 at D <= 64
+    (64, 32, 32, [3300, 40, 65, 700]),    # two runs of the long tiles, the last ones first
+    (128, 16, 16, [4200, 40, 65, 700]),
+])
+def test_more_tiles_than_the_chip_takes_at_once(cuda, D, H, G, lens):
+    tiles, most = runs_scratch(lens, H, G, D)
+    slots = 512 if D <= 64 else 256
+    assert most == 2 and slots <= tiles < 4 * slots, (tiles, most)
+    assert (2 * tiles < 3 * slots) == (lens[0] in (2400, 2500)), tiles
+    run(cuda, lens, lens, H, G, D, BF, True, pad=1)
+
+
+@pytest.mark.parametrize("D,H,lens", [(64, 6, [1024] * 8), (64, 6, [2048] * 4), (128, 3, [1024] * 8)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_equal_sequences(cuda, D, H, lens, causal):
+    """Batches that may be split by their tokens, of which the device splits few
+    tiles or none."""
+    assert runs_scratch(lens, H, H, D, causal)[1] > 1
+    run(cuda, lens, lens, H, H, D, HF, causal)
