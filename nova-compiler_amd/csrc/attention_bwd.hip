@@ -521,12 +521,22 @@ int32_t launch_bwd_t(BwdArgs a, int64_t q_tiles, int64_t k_tiles, hipStream_t s)
   if (q_tiles > 0) {
     a.tiles = (int)q_tiles;
     const unsigned grid = (unsigned)(q_tiles * a.heads);
-    // Two groups while the chip, which holds two workgroups of one group per CU,
-    // holds every tile at once and waits for the longest.  The whole backward
-    // with one group and with two, us, 2048 causal tokens of 6 heads of 64 70.5 /
-    // 65.3, packed 1 to 4096 of these 137.7 / 121.4, 2048 of 8 heads of 128 120 /
-    // 106; beyond, 8 x 1024 not causal of 6 heads of 64 (432 tiles) 65 / 76.
-    // Short sequences lose it to the join (8 x 512 of 6 heads of 64 27.1 / 27.9).
+    // Two groups while the tiles' number is within the workgroups of one group that
+    // the chip holds (two per CU) and the longest tile decides.  At D > 64 it holds
+    // 256 of two groups, so that causal batches of more take a second round, of
+    // their shortest tiles: still less than the longest's turns.  The whole backward
+    // with one group and with two, us, causal:
+    //   2048 tokens, 8 heads of 128 (136 tiles); 3000, 12 (288)    115 / 102, 179 / 160
+    //   4096, 8 of 128 (264); 8192, 6 (390)                        221 / 194, 481 / 430
+    //   2 x 2048, 12 of 128 (408); 4 x 1024, 12 (432)              141 / 132, 85.5 / 88.1
+    //   packed 1 to 4096, 6 of 128 (426); of 96                    214 / 185, 168 / 152
+    //   8 x 1024, 7 of 128 (504); of 96                            92.6 / 97.3, 75.7 / 79.1
+    //   4096, 8 of 64 (264); packed 1 to 4096, 6 of 64 (426)       114 / 105, 134 / 122
+    //   4 x 1024, 12 of 64 (432); 8 x 1024, 6 of 64 (432)          46.2 / 48.2, 46.5 / 48.3
+    // so equal sequences of 1024 lose 3 to 5% by what packed batches of as many
+    // tokens gain 9 to 13% by.  Beyond, 8 x 1024 not causal of 6 heads of 64 (432
+    // tiles) 65 / 76.  Short sequences lose it to the join (8 x 512 of 6 heads of 64
+    // 27.1 / 27.9).
     if (grid <= (CAUSAL ? 512 : 256) && a.Tk / a.B >= 10 * kBN)
       hipLaunchKernelGGL((attention_dq_kernel<DT, DP, CAUSAL, 2>), dim3(grid), dim3(128 * kWaves), 0,
                          s, a);
