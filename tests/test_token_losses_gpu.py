@@ -399,3 +399,35 @@ def test_rows_of_weight_zero(cuda, dt, C):
     a = nh.policy_loss(x[rest], y[rest], old[rest], adv[rest], w[rest], ref_logp=old[rest], kl_coef=0.1)
     assert torch.equal(grad[rest], a[2]) and torch.equal(logp[rest], a[1])
     assert abs(loss.item() - a[0].item()) <= 2.0 ** -23 * abs(a[0].item())
+
+
+@pytest.mark.parametrize("kl", [0.0, 0.3, -0.2])
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_policy_wide_clip_with_a_kl_term(cuda, dt, kl):
+    """clip (1, 5): the ratio in [0, 6], so only ratios above 6 are clipped; the
+    loss, its rows and the gradient with a reference that differs from logp."""
+    R, C, lo, hi, scale = 60, 700, 1.0, 5.0, 4.0
+    x, y, g = make(cuda, R, C, dt, seed=5)
+    lp, p, dist, ok = rows64(x, y)
+    step = torch.linspace(-3.0, 3.0, R, device=cuda, dtype=F64)  # no step within 0.01 of log 6
+    assert (step - math.log(1 + hi)).abs().min() > 0.01
+    old, ref = (lp - step).float(), (lp + 0.7 * torch.randn(R, generator=g, device=cuda, dtype=F64)).float()
+    adv, w = torch.randn(R, generator=g, device=cuda), torch.rand(R, generator=g, device=cuda)
+    row = torch.empty(R, device=cuda)
+    loss, logp, grad = nh.policy_loss(x, y, old, adv, w, ref_logp=ref, kl_coef=kl, clip=(lo, hi),
+                                      grad_scale=scale, row_loss=row)
+    tol = lp_tol(lp, dist)
+    assert ((logp.double() - lp).abs() <= tol).all()
+    A, W, k = adv.double(), w.double() * ok, float(torch.tensor(kl, dtype=F32))
+    ratio = torch.exp(lp - old.double())
+    plain, clipped, d = ratio * A, ratio.clamp(1 - lo, 1 + hi) * A, ref.double() - lp
+    per = -torch.minimum(plain, clipped) + k * (torch.expm1(d) - d)
+    slope = torch.where(plain <= clipped, -plain, torch.zeros_like(plain)) - k * torch.expm1(d)
+    # A ratio is off by lp's error and expf's 2 ulp, a clipped one by nothing; the
+    # KL term by lp's error times its slope (d.exp() + 1) and a few ulp.
+    rel = (tol + 1e-6) * 1.01
+    err = rel * plain.abs() + 2.0 ** -23 * clipped.abs() + abs(k) * (rel * (d.exp() + 1) + 1e-6 * d.abs())
+    err = W * (err + 2.0 ** -22 * per.abs())
+    assert ((row.double() - W * per).abs() <= err + 1e-38).all()
+    assert abs(loss.item() - (W * per).sum().item()) <= err.sum().item() + 2.0 ** -23 * abs(loss.item())
+    check_grad(grad, slope * W, err + 2.0 ** -22 * (slope * W).abs(), p, y, ok, scale)
