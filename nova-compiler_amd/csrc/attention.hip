@@ -11,10 +11,12 @@
 // Four waves hold 32 queries each and stream tiles of 64 keys and values through
 // a two-stage ring in LDS filled by DMA; two workgroups share a CU at D = 128
 // (230 registers), so that one's exponentials run beside the other's products.
-// What bounds it: at D = 128 the matrix cores and the board's power (8192 causal
-// tokens, 32 heads: 535 us, 1.03 PFLOP/s, where a plain 8192^3 product of the
-// library reaches 1.40 and a 4096^3 one 1.17); at D = 64 the exponentials and
-// the rest of the softmax (2 x 4096 tokens, 32 heads: 337 us, 0.82 PFLOP/s).
+// What bounds it: at D = 128 the products and the softmax, which hardly overlap
+// (counters, packed causal 1 to 4096 tokens: the matrix cores 49% busy and the
+// vector units 55% of the time; 8192 causal tokens, 32 heads: 535 us, 1.03 PFLOP/s,
+// where a plain 8192^3 product of the library reaches 1.40 and a 4096^3 one 1.17);
+// at D = 64 the exponentials and the rest of the softmax (2 x 4096 tokens, 32
+// heads: 334 us, 0.82 PFLOP/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -224,7 +226,7 @@ void launch_fwd(const FwdArgs &a, bool causal, unsigned grid, hipStream_t s) {
   // Two groups while one workgroup of them per CU (of causal ones, whose work
   // differs, two at D <= 64) holds all tiles.  One group against two, us: 1000
   // causal tokens of 6 heads of 64 18.1 / 15.6, packed 1 to 4096 of these heads
-  // (432 tiles) 62.7 / 50.2, 3000 of 8 heads of 128 57.9 / 47.1; beyond, 4 x
+  // (426 tiles) 62.7 / 50.2, 3000 of 8 heads of 128 57.9 / 47.1; beyond, 4 x
   // 1024 of 12 heads of 128 (432 tiles) 37.6 / 45.0.
   // Not for sequences of less than eight tiles of keys in the mean, which lose
   // to the join what they gain (8 x 197 of 12 heads of 64: 8.7 / 9.2).

@@ -13,10 +13,10 @@
 // attention_dkv_kernel, behind it on the stream, reads while it holds keys and
 // values and streams Q and dO.
 //
-// What bounds them at D = 128 (2 x 4096 tokens, 32 heads, not causal): the matrix
-// cores and the board's power for dQ (755 us, 1.09 PFLOP/s of its three
-// products), the issue of one wave per SIMD for dK and dV (1045 us, 1.05 of
-// four).
+// What bounds them at D = 128 (2 x 4096 tokens, 32 heads, not causal): products and
+// exponentials that overlap in part for dQ (755 us, 1.09 PFLOP/s of its three
+// products; counters: the matrix cores 51% busy, the vector units 37%), the issue
+// of one wave per SIMD for dK and dV (1045 us, 1.05 of four; 49% and 30%).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -3,17 +3,16 @@
 // heads of their group together (the group's heads are the MFMA's columns).
 //
 // A cache of up to 1024 rows is one workgroup's per sequence and key head: its
-// waves take a part each and join their sums through LDS, in one launch (one
-// sequence of 1000 rows, 6 heads of 64: 13.3 us in two launches, 9.2 in one; a
-// launch costs the host 3).  A longer cache is cut into splits of `chunk` keys; a
-// workgroup of one wave takes one split of one sequence and key head, 32 keys at a time through a
+// waves take a part each and join their sums through LDS, in one launch (see
+// kJoined).  A longer cache is cut into splits of `chunk` keys; a workgroup of one
+// wave takes one split of one sequence and key head, 32 keys at a time through a
 // two-stage ring in LDS filled by DMA, without a barrier.  (Two waves sharing a
 // split joined their sums through LDS and took 2% longer.)  With more than
 // one split the sums go to the caller's scratch, and attention_join_kernel adds
 // them in a fixed order.
 //
 // Measured: 32 sequences of 1500 to 8192 rows, 597 MB of keys and values, in
-// 100 us (5.8 TB/s); 8 of 131072 in 685 us (6.3 TB/s).  Without the products
+// 104 us (5.7 TB/s); 8 of 131072 in 685 us (6.3 TB/s).  Without the products
 // (the DMA alone) it takes the same: the loads are the time.
 #include <hip/hip_runtime.h>
 
@@ -31,11 +30,11 @@ struct DecodeArgs {
   uint16_t *o;
   float *lse;      // [B][heads] with row stride slse, or null
   float *partial;  // [B][heads][splits][D + 2]: sum, then m c and l (splits > 1)
-  // splits: 0 where one workgroup's waves take a sequence and join
   const int *lens;
   int64_t sqb, sqh, sob, soh, slse;
   int64_t skb, skt, skh, svb, svt, svh;
-  int S, heads, group, D, chunk, splits;
+  int S, heads, group, D, chunk;
+  int splits;  // 0 where one workgroup's waves take a sequence and join
   float c;
 };
 
@@ -272,8 +271,23 @@ __global__ __launch_bounds__(256) void attention_join_kernel(DecodeArgs a) {
     a.lse[b * a.slse + h] = sum == 0.0f ? -INFINITY : (mx + (__log2f(sum) - kUp<DT>)) * kLn2;
 }
 
-// Waves of the form that joins them itself: what the LDS of a CU holds.
-constexpr int kJoined = 1024;  // cache rows it takes
+// Cache rows that the form takes whose waves join by themselves.  One launch costs
+// the host 4 us less than two, but one workgroup is slower than many splits, the
+// more so the longer the cache.  Two launches / one, us, of eager calls and of
+// replays of a captured graph, where the host's part is none:
+//   1 x 512 rows, 6 heads of 64                17.3 / 12.8    7.4 /  6.7
+//   1 x 1024                                   17.0 / 12.7    8.1 /  8.6
+//   1 x 2048                                   17.3 / 13.1    7.8 / 12.2
+//   1 x 512, 32 heads in groups of 4 of 128    17.3 / 13.0    9.2 / 11.1
+//   1 x 1024                                   17.6 / 16.6    9.9 / 16.4
+//   1 x 1536                                   17.5 / 21.1   10.5 / 21.1
+//   32 x 1024                                  30.0 / 24.3   30.1 / 24.4
+//   32 x 2048                                  51.4 / 43.6   51.8 / 43.3
+//   64 x 1024, 6 of 64                         19.9 / 21.9   19.6 / 22.0
+// Eager calls of one sequence gain up to 1024 rows of 128 and 2000 of 64, replays up
+// to about 350 and 768.
+constexpr int kJoined = 1024;
+// Its waves: what the LDS of a CU holds.
 constexpr int waves_joined(int64_t D) { return D <= 64 ? 8 : 4; }
 
 template <int DT, int DP>

@@ -7,17 +7,18 @@
 // between the maximum, the sum and the gradient, so the policy loss reads the
 // logits once and writes the gradient once.  The preference loss knows a row's
 // slope only when both sequences of the pair are summed, so its gradient is
-// a second pass over the logits, from the last row to the first: the rows
-// read last are still in the cache between HBM and the L2s.
+// a second pass over the logits, from the last row to the first: some of the rows
+// read last are still cached beyond the L2s (8192 x 50304 bf16 326 us, 361 from the
+// first row on; 4096 x 32000 bf16 100 either way, 2048 x 50304 f32 169 and 166).
 //
 // 16-bit logits are widened exactly; maxima, sums and log-probabilities are
 // f32, sums over rows 64 bits; the gradient is rounded once, to the logits'
 // type.
 //
 // Measured, of the bytes that have to move: policy loss 8192 x 50304 f32, 80% of
-// the rows valid, 525 us (5.65 TB/s, 0.87 of the copy's 6.5); bf16 272 us;
+// the rows valid, 525 us (5.65 TB/s, 0.87 of the copy's 6.5); bf16 263 us;
 // token_logp 8192 x 50304 190 us in f32 (6.95 TB/s), 96 us in bf16; preference
-// loss 8192 x 50304 bf16, 70% valid, 324 us (4.3 TB/s counting the logits once,
+// loss 8192 x 50304 bf16, 70% valid, 327 us (4.3 TB/s counting the logits once,
 // 6.1 as read).  Small calls are their launches' time on the host.
 #include <hip/hip_runtime.h>
 
