@@ -407,12 +407,12 @@ int32_t _mlir_ciface_nova_hip_index_to_i32(const NovaMemRef1D *src, NovaMemRef1D
  *   out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G]) v[j, h / G],
  *   G = heads / key heads; causal: query i of a sequence sees the keys
  *   j <= i + (keys - queries), so that the last query sees the last key.
- * A query that sees no key gives a zero row and lse -inf.  Rows of other
- * sequences and rows outside the sequences never take part, whatever they
- * hold.  Inside a causal sequence a key less than 128 rows ahead of a query has
- * weight 0 there: an infinity or NaN in its v (backward: in its k and v, and in
- * a query's q and grad_out for the keys as near behind it) still reaches that
- * query, as 0 times it does in a dense product.
+ * A query that sees no key, or whose scores are all -inf, gives a zero row and
+ * lse -inf.  Rows of other sequences and rows outside the sequences never take
+ * part, whatever they hold.  Inside a causal sequence a key less than 128 rows
+ * ahead of a query has weight 0 there: an infinity or NaN in its v (backward: in
+ * its k and v, and in a query's q and grad_out for the keys as near behind it)
+ * still reaches that query, as 0 times it does in a dense product.
  *   q, out : [query tokens, heads, D]; k, v : [key tokens, key heads, D];
  *   dt NOVA_HIP_DT_BF16 or _F16; D a multiple of 8 up to 128; unit stride on
  *   D, any order of the other dims, rows 16-byte aligned.

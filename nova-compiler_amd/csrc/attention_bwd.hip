@@ -15,7 +15,7 @@
 //
 // What bounds them at D = 128 (2 x 4096 tokens, 32 heads, not causal): products and
 // exponentials that overlap in part for dQ (755 us, 1.09 PFLOP/s of its three
-// products; counters: the matrix cores 51% busy, the vector units 37%), the issue
+// products; counters: the matrix cores 51% busy, the vector units 36%), the issue
 // of one wave per SIMD for dK and dV (1045 us, 1.05 of four; 49% and 30%).
 #include <hip/hip_runtime.h>
 

@@ -637,7 +637,8 @@ def attention(q, k, v, q_offsets, k_offsets, *, causal: bool = True, scale=None,
 def attention_backward(grad_out, q, k, v, out, lse, q_offsets, k_offsets, *, causal: bool = True,
                        scale=None, dq=None, dk=None, dv=None):
     """Gradients of ``attention``'s result, from its ``out`` and ``lse``:
-    returns (dq, dk, dv) in the operands' dtype."""
+    returns (dq, dk, dv) in the operands' dtype; their rows outside every sequence
+    are not written."""
     torch = _torch()
     f32, i32, dt, dev = torch.float32, torch.int32, q.dtype, q.get_device()
     d = (_desc(grad_out, 3, dt, dev, "grad_out"), _desc(q, 3, dt, dev, "q"),
