@@ -497,8 +497,8 @@ int32_t _mlir_ciface_nova_hip_token_logp(const NovaMemRef2D *logits, const NovaM
  *   loss, whatever its ratio, and its gradient is zero; its logp is that of its
  *   label all the same (0 for a label of C or more).  weight carries the mean a caller wants (1 / valid tokens,
  *   1 / (sequences length), ...); grad_scale is a loss scale.  logp and row_loss
- *   may be written over old_logp, ref_logp, advantage or weight (logp over
- *   old_logp: the next step's), whole vectors over each other. */
+ *   may be the memory of old_logp, ref_logp, advantage or weight (logp that of
+ *   old_logp: the next step's), the whole vector and not a part of it. */
 int32_t _mlir_ciface_nova_hip_policy_loss(
     const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *old_logp,
     const NovaMemRef1D *ref_logp, const NovaMemRef1D *advantage, const NovaMemRef1D *weight,
@@ -515,7 +515,7 @@ int32_t _mlir_ciface_nova_hip_policy_loss(
  *   offsets : [2 pairs + 1]; ref_logp, seq_logp : [2 pairs] f32; pair_loss :
  *   [pairs] f32; token : [3, R] f32, written with the rows' logp, lse and slope
  *   (grad_scale * d loss / d logp of every row of a sequence, 0 elsewhere).
- *   seq_logp may be written over ref_logp. */
+ *   seq_logp may be the memory of ref_logp. */
 int32_t _mlir_ciface_nova_hip_preference_loss(
     const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *offsets,
     const NovaMemRef1D *ref_logp, NovaMemRef1D *loss, NovaMemRef1D *seq_logp,
