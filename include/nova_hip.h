@@ -495,10 +495,11 @@ int32_t _mlir_ciface_nova_hip_token_logp(const NovaMemRef2D *logits, const NovaM
  *   old_logp, ref_logp, advantage (A), weight, logp, row_loss : [R] f32;
  *   ref_logp may be NULL when kl_coef is 0.  A row with weight 0 adds no
  *   loss, whatever its ratio, and its gradient is zero; its logp is that of its
- *   label all the same (0 for a label of C or more).  weight carries the mean a caller wants (1 / valid tokens,
- *   1 / (sequences length), ...); grad_scale is a loss scale.  logp and row_loss
- *   may be the memory of old_logp, ref_logp, advantage or weight (logp that of
- *   old_logp: the next step's), the whole vector and not a part of it. */
+ *   label all the same (0 for a label of C or more).  weight carries the mean a
+ *   caller wants (1 / valid tokens, 1 / (sequences length), ...); grad_scale is a
+ *   loss scale.  logp and row_loss may be the memory of old_logp, ref_logp,
+ *   advantage or weight (logp that of old_logp: the next step's), the whole vector
+ *   and not a part of it. */
 int32_t _mlir_ciface_nova_hip_policy_loss(
     const NovaMemRef2D *logits, const NovaMemRef1D *labels, const NovaMemRef1D *old_logp,
     const NovaMemRef1D *ref_logp, const NovaMemRef1D *advantage, const NovaMemRef1D *weight,
