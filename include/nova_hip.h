@@ -471,6 +471,108 @@ int32_t _mlir_ciface_nova_hip_attention_decode(const NovaMemRef3D *q, const Nova
 int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int64_t heads,
                                           int64_t kv_heads, int64_t D);
 /* ------------------------------------------------------------------------
+ * Rotary positions and the norm of query and key heads (HBM bound), the rows
+ * of nova.linear's output on their way to an attention call.  No reference
+ * counterpart.  For all of them:
+ *   rows : [tokens, heads, D], D a multiple of 8 up to 256, unit stride on D,
+ *   any order of the other dims, rows 16-byte aligned; dt NOVA_HIP_DT_F32, _BF16
+ *   or _F16 (paged calls: 16-bit).
+ *   freqs : [R / 2] f32, R a multiple of 8 up to D: the first R values of a row
+ *   are rotated, the others stay.  With t = position * freqs[i], the pair (a, b)
+ *   being values (i, i + R / 2) of the row, or (2 i, 2 i + 1) when interleaved is
+ *   1, becomes scale (a cos t - b sin t, b cos t + a sin t).  Angles are taken in
+ *   64 bits, everything else in f32, results are rounded once.
+ *   positions : [tokens] i32 in device memory, any value.
+ * A result may take the place of the rows it is made from (the same address and
+ * strides); any other overlap with an operand or result is refused.
+ * ---------------------------------------------------------------------- */
+/* freqs[i] = base^(-2 i / R), R = 2 (size of freqs, at most 128), for contexts
+ * `factor` times longer than the model's: with original = 0 all divided by
+ * factor; with original the context it was trained on, those that turn `high`
+ * times over it stay, those that turn `low` times are divided by factor, with
+ *   keep = clamp((original freqs[i] / 2 pi - low) / (high - low), 0, 1):
+ *   freqs[i] (keep + (1 - keep) / factor).
+ * Computed in 64 bits.  factor = 1 changes nothing. */
+int32_t _mlir_ciface_nova_hip_rotary_frequencies(NovaMemRef1D *freqs, float base, float factor,
+                                                 float low, float high, int64_t original);
+/* out = x rotated; inverse = 1 rotates back (by -t, still times scale): the
+ * gradient of x from that of out. */
+int32_t _mlir_ciface_nova_hip_rotary(const NovaMemRef3D *x, const NovaMemRef1D *positions,
+                                     const NovaMemRef1D *freqs, NovaMemRef3D *out, float scale,
+                                     int32_t interleaved, int32_t inverse, int32_t dt);
+/* Each row of q and k normed and rotated in one pass:
+ *   y = x (mean x^2 + eps)^(-1/2) weight, then the rotation.
+ *   q_weight, k_weight : [D] of weight_dt, f32 or dt; positions and freqs may
+ *   both be NULL (the norm alone). */
+int32_t _mlir_ciface_nova_hip_qk_norm_rotary(
+    const NovaMemRef3D *q, const NovaMemRef3D *k, const NovaMemRef1D *q_weight,
+    const NovaMemRef1D *k_weight, const NovaMemRef1D *positions, const NovaMemRef1D *freqs,
+    NovaMemRef3D *q_out, NovaMemRef3D *k_out, float eps, float scale, int32_t interleaved, int32_t dt,
+    int32_t weight_dt);
+/* Its gradients of q and k (dq, dk, of dt) and of the weights (f32, [D]), from
+ * those of its results and its operands.  dq may take the place of q or grad_q, dk
+ * of k or grad_k.  scratch : at least
+ * nova_hip_qk_norm_rotary_backward_scratch() f32, dense, used by this call only
+ * (NULL when that is 0).  Sums over rows are f32 in a fixed order (the same bits on
+ * every run). */
+int32_t _mlir_ciface_nova_hip_qk_norm_rotary_backward(
+    const NovaMemRef3D *grad_q, const NovaMemRef3D *grad_k, const NovaMemRef3D *q,
+    const NovaMemRef3D *k, const NovaMemRef1D *q_weight, const NovaMemRef1D *k_weight,
+    const NovaMemRef1D *positions, const NovaMemRef1D *freqs, NovaMemRef3D *dq, NovaMemRef3D *dk,
+    NovaMemRef1D *dq_weight, NovaMemRef1D *dk_weight, NovaMemRef1D *scratch, float eps, float scale,
+    int32_t interleaved, int32_t dt, int32_t weight_dt);
+/* Floats of scratch the call above needs on sizes it accepts. */
+int64_t nova_hip_qk_norm_rotary_backward_scratch(int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                 int64_t D);
+/* ------------------------------------------------------------------------
+ * A paged cache: rows of keys and values in pages, k_pages and v_pages
+ * [pages, rows of a page, key heads, D] of dt NOVA_HIP_DT_BF16 or _F16, unit
+ * stride on D, any order of the other dims, rows 16-byte aligned, any page size.
+ * Row i of sequence b is row i % page of page table[b, i / page].
+ *   offsets : [sequences + 1] i32, not decreasing: the new tokens of sequence b
+ *   are the packed rows [offsets[b], offsets[b + 1]);
+ *   lengths : [sequences] i32: rows of the sequence, the new ones being the last
+ *   of them (new token i of n has position lengths[b] - n + i);
+ *   table : [sequences, pages of each] i32, rows dense; a view of its first columns
+ *   says that no sequence is longer.
+ * All three are device memory; whatever they hold, no access leaves an operand.
+ * ---------------------------------------------------------------------- */
+/* New tokens' keys and values to their places, keys rotated by their position
+ * on the way (freqs NULL: as they are), and q rotated to q_out in the same
+ * launch (both NULL: keys and values alone).
+ *   k, v : [tokens, key heads, D]; q, q_out : [tokens, heads, D].
+ * A token outside every sequence takes no part; one whose position is negative
+ * or beyond the table, or whose page is not one of the pages, is not stored.  Rows
+ * of the pages that no token goes to are left as they were.  Two tokens must not
+ * go to the same row. */
+int32_t _mlir_ciface_nova_hip_paged_append(
+    const NovaMemRef3D *k, const NovaMemRef3D *v, NovaMemRef4D *k_pages, NovaMemRef4D *v_pages,
+    const NovaMemRef1D *offsets, const NovaMemRef1D *lengths, const NovaMemRef2D *table,
+    const NovaMemRef1D *freqs, const NovaMemRef3D *q, NovaMemRef3D *q_out, float scale,
+    int32_t interleaved, int32_t dt);
+/* Attention of the new tokens over their sequences' rows, as
+ * _mlir_ciface_nova_hip_attention has it (causal: a token sees the rows up to its
+ * own position; groups, types, roundings, empty rows and near masked infinities
+ * the same).  Lengths are cut to what the table holds, entries of the table to the
+ * pages that there are; rows behind a length are not read.
+ *   q, out : [tokens, heads, D], D a multiple of 8 up to 128; lse : [heads,
+ *   tokens] f32 or NULL; rows outside every sequence are left as they were.
+ *   max_queries : no sequence has more new tokens (0: not known); tokens beyond it
+ *   may be left out.
+ *   scratch : nova_hip_paged_attention_scratch() f32, dense and 8-byte aligned,
+ *   used by this call only (NULL when that is 0). */
+int32_t _mlir_ciface_nova_hip_paged_attention(
+    const NovaMemRef3D *q, const NovaMemRef4D *k_pages, const NovaMemRef4D *v_pages,
+    const NovaMemRef1D *offsets, const NovaMemRef1D *lengths, const NovaMemRef2D *table,
+    NovaMemRef3D *out, NovaMemRef2D *lse, NovaMemRef1D *scratch, float scale, int32_t causal,
+    int64_t max_queries, int32_t dt);
+/* Floats of scratch the call above needs on sizes it accepts: rows = columns of
+ * the table times the page size, max_queries as there but at most `tokens` (not
+ * known: tokens). */
+int64_t nova_hip_paged_attention_scratch(int64_t tokens, int64_t sequences, int64_t heads,
+                                         int64_t kv_heads, int64_t D, int64_t rows,
+                                         int64_t max_queries);
+/* ------------------------------------------------------------------------
  * Losses over token log-probabilities (HBM bound), beside nova.sce.  No
  * reference counterpart.  For all three:
  *   logits, grad : [R, C] of dt NOVA_HIP_DT_F32, _BF16 or _F16; any row

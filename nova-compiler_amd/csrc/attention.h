@@ -286,13 +286,11 @@ __device__ __forceinline__ float both_max(float v) { return fmaxf(v, __shfl_xor(
 __device__ __forceinline__ float both_sum(float v) { return v + __shfl_xor(v, 32); }
 
 // A wave's transposed result [DP columns d][32 rows], times `mul` of the
-// lane's row, to 16-bit rows at p: row l % 32 < rows.  Lane halves trade 8-byte
-// pieces so that each lane stores 16 bytes.
+// lane's row, to 16-bit rows: row l % 32 at dst where `ok`.  Lane halves trade
+// 8-byte pieces so that each lane stores 16 bytes.
 template <int DT, int DP>
-__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], float mul, uint16_t *p,
-                                           int64_t stride, int rows, int D, int lane) {
-  uint16_t *dst = p + (lane & 31) * stride;
-  const bool ok = (lane & 31) < rows;
+__device__ __forceinline__ void store_row(const f32x16 (&acc)[DP / 32], float mul, uint16_t *dst,
+                                          bool ok, int D, int lane) {
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
@@ -309,6 +307,12 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], float m
       const int d = 32 * b + 8 * (i + (lane >> 5));
       if (ok && d < D) *reinterpret_cast<u32x4 *>(dst + d) = u32x4{x[0], x[1], y[0], y[1]};
     }
+}
+// The same to rows `stride` apart from p on: row l % 32 < rows.
+template <int DT, int DP>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], float mul, uint16_t *p,
+                                           int64_t stride, int rows, int D, int lane) {
+  store_row<DT, DP>(acc, mul, p + (lane & 31) * stride, (lane & 31) < rows, D, lane);
 }
 
 }  // namespace attn

@@ -914,7 +914,7 @@ constexpr int64_t kAttnMaxStride = 1 << 23;  // elements; 128 rows stay below 2^
 // the row's own length, so that the rows a tile holds behind the last one lie
 // outside the operand, where loads return zero.
 int32_t attn_operand(const NovaMemRef3D *d, const char *w, const char *what, bool out,
-                     AttentionOperand &o) {
+                     AttentionOperand &o, int size = 2, int64_t max_stride = kAttnMaxStride) {
   if (!d) return fail(NOVA_HIP_EINVAL, "%s: null %s descriptor", w, what);
   if (!nonneg_sizes(d, 3)) return fail(NOVA_HIP_ESHAPE, "%s: negative size", w);
   const int64_t T = d->sizes[0], H = d->sizes[1], D = d->sizes[2];
@@ -931,10 +931,10 @@ int32_t attn_operand(const NovaMemRef3D *d, const char *w, const char *what, boo
     return fail(NOVA_HIP_ESTRIDE, "%s: %s must have unit stride on the head dim", w, what);
   if ((T > 1 && o.st < D) || o.sh < 0)
     return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
-  o.p = const_cast<char *>(data_of(d)) + d->offset * 2;
-  if (o.st % 8 || o.sh % 8 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
+  o.p = const_cast<char *>(data_of(d)) + d->offset * size;
+  if (o.st * size % 16 || o.sh * size % 16 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
     return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s must start at 16-byte aligned addresses", w, what);
-  if (o.st > kAttnMaxStride)
+  if (o.st > max_stride)
     return fail(NOVA_HIP_ERANGE, "%s: token stride of %s exceeds 2^23 elements", w, what);
   if (out && H > 1) {
     const bool apart = o.sh >= D && (T <= 1 || (o.st <= o.sh ? o.sh >= (T - 1) * o.st + D
@@ -1330,6 +1330,498 @@ int32_t _mlir_ciface_nova_hip_preference_loss(
   p.grad_scale = grad_scale;
   if ((rc = grad_apart(p.t, w))) return rc;
   return launch_preference_loss(p, current_stream());
+}
+
+// ---- positions and the paged cache ---------------------------------------------------
+namespace {
+constexpr int64_t kAnyStride = INT64_MAX;
+
+// A dense i32 vector of n values.
+int32_t vector_i32(const NovaMemRef1D *d, int64_t n, const char *w, const char *what,
+                   const int32_t *&p) {
+  int32_t rc = dense1(d, w, what);
+  if (rc) return rc;
+  if (d->sizes[0] != n)
+    return fail(NOVA_HIP_ESHAPE, "%s: %s has %lld values, not %lld", w, what,
+                (long long)d->sizes[0], (long long)n);
+  p = reinterpret_cast<const int32_t *>(data_of(d)) + d->offset;
+  return NOVA_HIP_SUCCESS;
+}
+
+int32_t head_dim_ok(int64_t D, const char *w) {
+  if (D % 8 || D > kMaxHeadDim)
+    return fail(NOVA_HIP_ERANGE, "%s: head dim %lld is not a multiple of 8 up to %lld", w,
+                (long long)D, (long long)kMaxHeadDim);
+  return NOVA_HIP_SUCCESS;
+}
+
+// The frequencies [R / 2] of rows of D values (NULL: nothing is rotated), and
+// what goes with them.
+int32_t rotation(const NovaMemRef1D *freqs, float scale, int32_t interleaved, int64_t D,
+                 const char *w, const float *&p, int64_t &R) {
+  int32_t rc;
+  if (!(scale > -INFINITY) || !(scale < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: scale must be finite", w);
+  if (interleaved != 0 && interleaved != 1)
+    return fail(NOVA_HIP_EINVAL, "%s: interleaved is %d", w, interleaved);
+  p = nullptr;
+  R = 0;
+  if (!freqs) return NOVA_HIP_SUCCESS;
+  if ((rc = dense1(freqs, w, "freqs"))) return rc;
+  R = 2 * freqs->sizes[0];
+  if (R % 8 || R > D)
+    return fail(NOVA_HIP_ERANGE, "%s: %lld rotated values are not a multiple of 8 up to the head dim %lld",
+                w, (long long)R, (long long)D);
+  p = in_f32(freqs);
+  return NOVA_HIP_SUCCESS;
+}
+
+int32_t row_type(int32_t dt, const char *w) {
+  if (dt != NOVA_HIP_DT_F32 && dt != NOVA_HIP_DT_BF16 && dt != NOVA_HIP_DT_F16)
+    return fail(NOVA_HIP_EDTYPE, "%s: dtype %d (f32, bf16 and f16 are provided)", w, dt);
+  return NOVA_HIP_SUCCESS;
+}
+
+// A norm's weight [D], of f32 or the rows' type.
+int32_t norm_weight(const NovaMemRef1D *d, int64_t D, int32_t w_dt, int32_t dt, const char *w,
+                    const char *what, const void *&p) {
+  if (w_dt != NOVA_HIP_DT_F32 && w_dt != dt)
+    return fail(NOVA_HIP_EDTYPE, "%s: weights are f32 or of the rows' dtype, not %d", w, w_dt);
+  int32_t rc = dense1(d, w, what);
+  if (rc) return rc;
+  if (d->sizes[0] != D)
+    return fail(NOVA_HIP_ESHAPE, "%s: %s has %lld values, not %lld", w, what,
+                (long long)d->sizes[0], (long long)D);
+  p = data_of(d) + d->offset * dtype_size(w_dt);
+  return NOVA_HIP_SUCCESS;
+}
+
+Extent rows_extent(const char *name, const AttentionOperand &o, const NovaMemRef3D *d, int size) {
+  const int64_t T = d->sizes[0], H = d->sizes[1], D = d->sizes[2];
+  return {name, o.p, T && H ? size * D : 0, {T, H, 1}, {size * o.st, size * o.sh, 0}};
+}
+Extent vector_extent(const char *name, const void *p, int64_t bytes) {
+  return {name, p, p ? bytes : 0, {1, 1, 1}, {0, 0, 0}};
+}
+// Rows may be written where they are read, whole operand over whole operand.
+bool same_rows(const AttentionOperand &a, const AttentionOperand &b) {
+  return a.p == b.p && a.st == b.st && a.sh == b.sh;
+}
+// Result `y` of the rows `x` apart from all of `others`, and from x unless it is x.
+int32_t rows_apart(const char *w, const Extent &y, const Extent &x, bool same,
+                   std::initializer_list<Extent> others) {
+  int32_t rc = same ? NOVA_HIP_SUCCESS : check_apart(w, y, {x});
+  return rc ? rc : check_apart(w, y, others);
+}
+
+int32_t eps_ok(float eps, const char *w) {
+  if (!(eps >= 0.0f) || !(eps < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: eps must be finite and not negative", w);
+  return NOVA_HIP_SUCCESS;
+}
+
+// Pages [pages, page, key heads, D] of 16-bit values.
+int32_t page_operand(const NovaMemRef4D *d, const char *w, const char *what, bool out,
+                     PageOperand &o) {
+  const int64_t n[3] = {d->sizes[0], d->sizes[1], d->sizes[2]}, D = d->sizes[3];
+  int64_t st[3];
+  for (int i = 0; i < 3; ++i) st[i] = n[i] > 1 ? d->strides[i] : D;
+  o = {nullptr, st[0], st[1], st[2]};
+  if (n[0] == 0 || n[1] == 0 || n[2] == 0 || D == 0) return NOVA_HIP_SUCCESS;
+  if (!d->aligned) return fail(NOVA_HIP_EINVAL, "%s: null %s data pointer", w, what);
+  if (D > 1 && d->strides[3] != 1)
+    return fail(NOVA_HIP_ESTRIDE, "%s: %s must have unit stride on the head dim", w, what);
+  o.p = const_cast<char *>(data_of(d)) + d->offset * 2;
+  if (st[0] % 8 || st[1] % 8 || st[2] % 8 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s must start at 16-byte aligned addresses", w, what);
+  if (st[0] < 0 || st[1] < 0 || st[2] < 0)
+    return fail(NOVA_HIP_ESTRIDE, "%s: negative stride of %s", w, what);
+  if (out) {  // in the order of their strides, each beyond what the ones before it span
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return st[a] < st[b]; });
+    int64_t span = D;
+    for (int i : order) {
+      if (n[i] <= 1) continue;
+      if (st[i] < span) return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
+      span += (n[i] - 1) * st[i];
+    }
+  }
+  return NOVA_HIP_SUCCESS;
+}
+
+// The pages and what says where a sequence's rows lie in them.
+int32_t paged_cache(const NovaMemRef4D *k, const NovaMemRef4D *v, const NovaMemRef1D *offsets,
+                    const NovaMemRef1D *lengths, const NovaMemRef2D *table, bool out, const char *w,
+                    PagedCache &c) {
+  if (!k || !v || !offsets || !lengths || !table)
+    return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if (!nonneg_sizes(k, 4) || !nonneg_sizes(v, 4) || !nonneg_sizes(table, 2))
+    return fail(NOVA_HIP_ESHAPE, "%s: negative size", w);
+  for (int i = 0; i < 4; ++i)
+    if (k->sizes[i] != v->sizes[i])
+      return fail(NOVA_HIP_ESHAPE, "%s: shapes of k_pages and v_pages differ", w);
+  c.pages = k->sizes[0];
+  c.page = k->sizes[1];
+  c.kv_heads = k->sizes[2];
+  c.D = k->sizes[3];
+  if (offsets->sizes[0] < 1) return fail(NOVA_HIP_ESHAPE, "%s: offsets must be [sequences + 1]", w);
+  c.B = offsets->sizes[0] - 1;
+  int32_t rc;
+  if ((rc = vector_i32(offsets, c.B + 1, w, "offsets", c.offsets)) ||
+      (rc = vector_i32(lengths, c.B, w, "lengths", c.lengths)))
+    return rc;
+  c.width = table->sizes[1];
+  c.stable = c.B > 1 ? table->strides[0] : c.width;
+  if (table->sizes[0] != c.B)
+    return fail(NOVA_HIP_ESHAPE, "%s: table must be [sequences, pages of each]", w);
+  if ((c.width > 1 && c.B > 0 && table->strides[1] != 1) || c.stable < 0)
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows of the table must be dense", w);
+  if (c.B > 0 && c.width > 0 && !table->aligned)
+    return fail(NOVA_HIP_EINVAL, "%s: null table pointer", w);
+  c.table = reinterpret_cast<const int32_t *>(data_of(table)) + table->offset;
+  if (c.B >= (1 << 24)) return fail(NOVA_HIP_ERANGE, "%s: more than 2^24 - 1 sequences", w);
+  if (c.kv_heads > 0xffff) return fail(NOVA_HIP_ERANGE, "%s: more than 65535 heads", w);
+  if (c.pages > 0x7fffffff || c.page > 0x7fffffff - (1 << 20) || c.width > 0x7fffffff ||
+      c.width * c.page > 0x7fffffff - (1 << 20))
+    return fail(NOVA_HIP_ERANGE, "%s: more than 2^31 - 1 pages or 2^31 - 2^20 rows of a sequence", w);
+  if ((rc = page_operand(k, w, "k_pages", out, c.k)) ||
+      (rc = page_operand(v, w, "v_pages", out, c.v)))
+    return rc;
+  // No rows to address: every place lies outside.
+  if (c.page == 0 || c.pages == 0 || c.kv_heads == 0 || c.D == 0) c.width = 0;
+  c.page = std::max<int64_t>(c.page, 1);
+  return NOVA_HIP_SUCCESS;
+}
+Extent pages_extent(const char *name, const PageOperand &o, const PagedCache &c) {
+  return {name, o.p, o.p ? 2 * c.D : 0, {c.pages, c.page, c.kv_heads}, {2 * o.sp, 2 * o.st, 2 * o.sh}};
+}
+Extent table_extent(const PagedCache &c) {
+  return {"table", c.table, c.B && c.width ? 4 * c.width : 0, {c.B, 1, 1}, {4 * c.stable, 0, 0}};
+}
+}  // namespace
+
+int32_t _mlir_ciface_nova_hip_rotary_frequencies(NovaMemRef1D *freqs, float base, float factor,
+                                                 float low, float high, int64_t original) {
+  clear_error();
+  const char *w = "rotary_frequencies";
+  int32_t rc = dense1(freqs, w, "freqs");
+  if (rc) return rc;
+  if (freqs->sizes[0] > kMaxHeadDim / 2)
+    return fail(NOVA_HIP_ERANGE, "%s: more than %lld frequencies", w, (long long)kMaxHeadDim / 2);
+  if (!(base > 0.0f) || !(base < INFINITY) || !(factor > 0.0f) || !(factor < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: base and factor must be positive and finite", w);
+  if (original < 0) return fail(NOVA_HIP_EINVAL, "%s: negative original length", w);
+  if (original > 0 && (!(low < high) || !(low > -INFINITY) || !(high < INFINITY)))
+    return fail(NOVA_HIP_EINVAL, "%s: low must lie below high, both finite", w);
+  return launch_rotary_frequencies(out_f32(freqs), freqs->sizes[0], base, factor, low, high,
+                                   (double)original, current_stream());
+}
+
+int32_t _mlir_ciface_nova_hip_rotary(const NovaMemRef3D *x, const NovaMemRef1D *positions,
+                                     const NovaMemRef1D *freqs, NovaMemRef3D *out, float scale,
+                                     int32_t interleaved, int32_t inverse, int32_t dt) {
+  clear_error();
+  const char *w = "rotary";
+  PositionProblem p = {};
+  p.what = w;
+  int32_t rc;
+  if (!x || !freqs) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if ((rc = row_type(dt, w)) || (rc = same_shape(out, x, w, "out"))) return rc;
+  const int size = dtype_size(dt);
+  auto &r = p.rows[0];
+  p.T = x->sizes[0];
+  r.heads = x->sizes[1];
+  p.D = x->sizes[2];
+  if (inverse != 0 && inverse != 1) return fail(NOVA_HIP_EINVAL, "%s: inverse is %d", w, inverse);
+  if ((rc = attn_operand(x, w, "x", false, r.src, size, kAnyStride)) ||
+      (rc = attn_operand(out, w, "out", true, r.dst, size, kAnyStride)) || (rc = head_dim_ok(p.D, w)) ||
+      (rc = vector_i32(positions, p.T, w, "positions", p.positions)) ||
+      (rc = rotation(freqs, scale, interleaved, p.D, w, p.freqs, p.R)) ||
+      (rc = rows_apart(w, rows_extent("out", r.dst, out, size), rows_extent("x", r.src, x, size),
+                       same_rows(r.dst, r.src),
+                       {vector_extent("positions", p.positions, 4 * p.T),
+                        vector_extent("freqs", p.freqs, 2 * p.R)})))
+    return rc;
+  p.scale = scale;
+  p.interleaved = interleaved != 0;
+  p.inverse = inverse != 0;
+  p.dt = dt;
+  return launch_positions(p, current_stream());
+}
+
+int32_t _mlir_ciface_nova_hip_qk_norm_rotary(
+    const NovaMemRef3D *q, const NovaMemRef3D *k, const NovaMemRef1D *q_weight,
+    const NovaMemRef1D *k_weight, const NovaMemRef1D *positions, const NovaMemRef1D *freqs,
+    NovaMemRef3D *q_out, NovaMemRef3D *k_out, float eps, float scale, int32_t interleaved, int32_t dt,
+    int32_t weight_dt) {
+  clear_error();
+  const char *w = "qk_norm_rotary";
+  PositionProblem p = {};
+  p.what = w;
+  int32_t rc;
+  if (!q || !k) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if ((rc = row_type(dt, w)) || (rc = same_shape(q_out, q, w, "q_out")) ||
+      (rc = same_shape(k_out, k, w, "k_out")))
+    return rc;
+  const int size = dtype_size(dt);
+  auto &rq = p.rows[0], &rk = p.rows[1];
+  p.T = q->sizes[0];
+  p.D = q->sizes[2];
+  rq.heads = q->sizes[1];
+  rk.heads = k->sizes[1];
+  if (k->sizes[0] != p.T || k->sizes[2] != p.D)
+    return fail(NOVA_HIP_ESHAPE, "%s: tokens and head dim of q and k differ", w);
+  if (!positions != !freqs)
+    return fail(NOVA_HIP_EINVAL, "%s: positions and freqs go together", w);
+  if ((rc = attn_operand(q, w, "q", false, rq.src, size, kAnyStride)) ||
+      (rc = attn_operand(k, w, "k", false, rk.src, size, kAnyStride)) ||
+      (rc = attn_operand(q_out, w, "q_out", true, rq.dst, size, kAnyStride)) ||
+      (rc = attn_operand(k_out, w, "k_out", true, rk.dst, size, kAnyStride)) ||
+      (rc = head_dim_ok(p.D, w)) || (rc = eps_ok(eps, w)) ||
+      (rc = norm_weight(q_weight, p.D, weight_dt, dt, w, "q_weight", rq.w)) ||
+      (rc = norm_weight(k_weight, p.D, weight_dt, dt, w, "k_weight", rk.w)) ||
+      (positions && (rc = vector_i32(positions, p.T, w, "positions", p.positions))) ||
+      (rc = rotation(freqs, scale, interleaved, p.D, w, p.freqs, p.R)))
+    return rc;
+  const int64_t wb = p.D * dtype_size(weight_dt);
+  const Extent xq = rows_extent("q", rq.src, q, size), xk = rows_extent("k", rk.src, k, size),
+               yq = rows_extent("q_out", rq.dst, q_out, size), yk = rows_extent("k_out", rk.dst, k_out, size),
+               wq = vector_extent("q_weight", rq.w, wb), wk = vector_extent("k_weight", rk.w, wb),
+               at = vector_extent("positions", p.positions, 4 * p.T),
+               fr = vector_extent("freqs", p.freqs, 2 * p.R);
+  if ((rc = rows_apart(w, yq, xq, same_rows(rq.dst, rq.src), {xk, wq, wk, at, fr})) ||
+      (rc = rows_apart(w, yk, xk, same_rows(rk.dst, rk.src), {xq, wq, wk, at, fr, yq})))
+    return rc;
+  p.scale = scale;
+  p.eps = eps;
+  p.norm = true;
+  p.interleaved = interleaved != 0;
+  p.dt = dt;
+  p.w_dt = weight_dt;
+  return launch_positions(p, current_stream());
+}
+
+int64_t nova_hip_qk_norm_rotary_backward_scratch(int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                 int64_t D) {
+  if (tokens <= 0 || heads < 0 || kv_heads < 0 || D <= 0 || tokens > 0x7fffffff || heads > 0xffff ||
+      kv_heads > 0xffff || D > kMaxHeadDim)
+    return 0;  // the call itself refuses these, or has nothing to sum
+  return qk_norm_backward_scratch(tokens, heads, kv_heads, D);
+}
+
+int32_t _mlir_ciface_nova_hip_qk_norm_rotary_backward(
+    const NovaMemRef3D *grad_q, const NovaMemRef3D *grad_k, const NovaMemRef3D *q,
+    const NovaMemRef3D *k, const NovaMemRef1D *q_weight, const NovaMemRef1D *k_weight,
+    const NovaMemRef1D *positions, const NovaMemRef1D *freqs, NovaMemRef3D *dq, NovaMemRef3D *dk,
+    NovaMemRef1D *dq_weight, NovaMemRef1D *dk_weight, NovaMemRef1D *scratch, float eps, float scale,
+    int32_t interleaved, int32_t dt, int32_t weight_dt) {
+  clear_error();
+  const char *w = "qk_norm_rotary_backward";
+  QkNormBackwardProblem p = {};
+  int32_t rc;
+  if (!q || !k) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if ((rc = row_type(dt, w)) || (rc = same_shape(grad_q, q, w, "grad_q")) ||
+      (rc = same_shape(grad_k, k, w, "grad_k")) || (rc = same_shape(dq, q, w, "dq")) ||
+      (rc = same_shape(dk, k, w, "dk")))
+    return rc;
+  const int size = dtype_size(dt);
+  auto &a = p.part[0], &b = p.part[1];
+  p.T = q->sizes[0];
+  p.D = q->sizes[2];
+  a.heads = q->sizes[1];
+  b.heads = k->sizes[1];
+  if (k->sizes[0] != p.T || k->sizes[2] != p.D)
+    return fail(NOVA_HIP_ESHAPE, "%s: tokens and head dim of q and k differ", w);
+  if (!positions != !freqs)
+    return fail(NOVA_HIP_EINVAL, "%s: positions and freqs go together", w);
+  if ((rc = attn_operand(q, w, "q", false, a.x, size, kAnyStride)) ||
+      (rc = attn_operand(k, w, "k", false, b.x, size, kAnyStride)) ||
+      (rc = attn_operand(grad_q, w, "grad_q", false, a.g, size, kAnyStride)) ||
+      (rc = attn_operand(grad_k, w, "grad_k", false, b.g, size, kAnyStride)) ||
+      (rc = attn_operand(dq, w, "dq", true, a.dx, size, kAnyStride)) ||
+      (rc = attn_operand(dk, w, "dk", true, b.dx, size, kAnyStride)) || (rc = head_dim_ok(p.D, w)) ||
+      (rc = eps_ok(eps, w)) || (rc = norm_weight(q_weight, p.D, weight_dt, dt, w, "q_weight", a.w)) ||
+      (rc = norm_weight(k_weight, p.D, weight_dt, dt, w, "k_weight", b.w)) ||
+      (rc = vector_f32(dq_weight, p.D, w, "dq_weight")) ||
+      (rc = vector_f32(dk_weight, p.D, w, "dk_weight")) ||
+      (positions && (rc = vector_i32(positions, p.T, w, "positions", p.positions))) ||
+      (rc = rotation(freqs, scale, interleaved, p.D, w, p.freqs, p.R)))
+    return rc;
+  const int64_t need = nova_hip_qk_norm_rotary_backward_scratch(p.T, a.heads, b.heads, p.D);
+  if (need > 0) {
+    if (!scratch) return fail(NOVA_HIP_EINVAL, "%s: null scratch descriptor", w);
+    if ((rc = dense1(scratch, w, "scratch"))) return rc;
+    if (scratch->sizes[0] < need)
+      return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, %lld are needed", w,
+                  (long long)scratch->sizes[0], (long long)need);
+    p.scratch = out_f32(scratch);
+  }
+  a.dw = out_f32(dq_weight);
+  b.dw = out_f32(dk_weight);
+  const int64_t wb = p.D * dtype_size(weight_dt);
+  const Extent xq = rows_extent("q", a.x, q, size), xk = rows_extent("k", b.x, k, size),
+               gq = rows_extent("grad_q", a.g, grad_q, size), gk = rows_extent("grad_k", b.g, grad_k, size),
+               yq = rows_extent("dq", a.dx, dq, size), yk = rows_extent("dk", b.dx, dk, size),
+               wq = vector_extent("q_weight", a.w, wb), wk = vector_extent("k_weight", b.w, wb),
+               at = vector_extent("positions", p.positions, 4 * p.T),
+               fr = vector_extent("freqs", p.freqs, 2 * p.R),
+               sq = vector_extent("dq_weight", a.dw, 4 * p.D), sk = vector_extent("dk_weight", b.dw, 4 * p.D),
+               sc = vector_extent("scratch", p.scratch, 4 * need);
+  // A row's gradient may take the place of the row or of its own gradient.
+  if ((rc = rows_apart(w, yq, xq, same_rows(a.dx, a.x), {xk, gk, wq, wk, at, fr})) ||
+      (rc = rows_apart(w, yq, gq, same_rows(a.dx, a.g), {})) ||
+      (rc = rows_apart(w, yk, xk, same_rows(b.dx, b.x), {xq, gq, wq, wk, at, fr, yq})) ||
+      (rc = rows_apart(w, yk, gk, same_rows(b.dx, b.g), {})) ||
+      (rc = check_apart(w, sq, {xq, xk, gq, gk, wq, wk, at, fr, yq, yk})) ||
+      (rc = check_apart(w, sk, {xq, xk, gq, gk, wq, wk, at, fr, yq, yk, sq})) ||
+      (rc = check_apart(w, sc, {xq, xk, gq, gk, wq, wk, at, fr, yq, yk, sq, sk})))
+    return rc;
+  p.scale = scale;
+  p.eps = eps;
+  p.interleaved = interleaved != 0;
+  p.dt = dt;
+  p.w_dt = weight_dt;
+  return launch_qk_norm_backward(p, current_stream());
+}
+
+int32_t _mlir_ciface_nova_hip_paged_append(
+    const NovaMemRef3D *k, const NovaMemRef3D *v, NovaMemRef4D *k_pages, NovaMemRef4D *v_pages,
+    const NovaMemRef1D *offsets, const NovaMemRef1D *lengths, const NovaMemRef2D *table,
+    const NovaMemRef1D *freqs, const NovaMemRef3D *q, NovaMemRef3D *q_out, float scale,
+    int32_t interleaved, int32_t dt) {
+  clear_error();
+  const char *w = "paged_append";
+  PositionProblem p = {};
+  PagedCache c;
+  p.what = w;
+  int32_t rc;
+  if (!k || !v) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if (dt != NOVA_HIP_DT_BF16 && dt != NOVA_HIP_DT_F16)
+    return fail(NOVA_HIP_EDTYPE, "%s: dtype %d (bf16 and f16 are provided)", w, dt);
+  if (!q != !q_out) return fail(NOVA_HIP_EINVAL, "%s: q and q_out go together", w);
+  auto &rq = p.rows[0], &rk = p.rows[1], &rv = p.rows[2];
+  p.T = k->sizes[0];
+  p.D = k->sizes[2];
+  rk.heads = rv.heads = k->sizes[1];
+  if ((rc = same_shape(v, k, w, "v")) || (rc = attn_operand(k, w, "k", false, rk.src, 2, kAnyStride)) ||
+      (rc = attn_operand(v, w, "v", false, rv.src, 2, kAnyStride)) || (rc = head_dim_ok(p.D, w)) ||
+      (rc = paged_cache(k_pages, v_pages, offsets, lengths, table, true, w, c)) ||
+      (rc = rotation(freqs, scale, interleaved, p.D, w, p.freqs, p.R)))
+    return rc;
+  if (c.kv_heads != rk.heads || c.D != p.D)
+    return fail(NOVA_HIP_ESHAPE, "%s: k [%lld,%lld,%lld], pages [%lld,%lld,%lld,%lld]", w,
+                (long long)p.T, (long long)rk.heads, (long long)p.D, (long long)k_pages->sizes[0],
+                (long long)k_pages->sizes[1], (long long)c.kv_heads, (long long)c.D);
+  const Extent xk = rows_extent("k", rk.src, k, 2), xv = rows_extent("v", rv.src, v, 2),
+               pk = pages_extent("k_pages", c.k, c), pv = pages_extent("v_pages", c.v, c),
+               off = vector_extent("offsets", c.offsets, 4 * (c.B + 1)),
+               len = vector_extent("lengths", c.lengths, 4 * c.B), tab = table_extent(c),
+               fr = vector_extent("freqs", p.freqs, 2 * p.R);
+  if ((rc = check_apart(w, pk, {xk, xv, off, len, tab, fr})) ||
+      (rc = check_apart(w, pv, {xk, xv, off, len, tab, fr, pk})))
+    return rc;
+  if (q) {
+    if ((rc = same_shape(q_out, q, w, "q_out")) ||
+        (rc = attn_operand(q, w, "q", false, rq.src, 2, kAnyStride)) ||
+        (rc = attn_operand(q_out, w, "q_out", true, rq.dst, 2, kAnyStride)))
+      return rc;
+    if (q->sizes[0] != p.T || q->sizes[2] != p.D)
+      return fail(NOVA_HIP_ESHAPE, "%s: tokens and head dim of q and k differ", w);
+    rq.heads = q->sizes[1];
+    const Extent xq = rows_extent("q", rq.src, q, 2), yq = rows_extent("q_out", rq.dst, q_out, 2);
+    if ((rc = rows_apart(w, yq, xq, same_rows(rq.dst, rq.src), {xk, xv, off, len, tab, fr, pk, pv})) ||
+        (rc = check_apart(w, pk, {xq})) || (rc = check_apart(w, pv, {xq})))
+      return rc;
+  }
+  rk.dst = {c.k.p, 0, c.k.sh};
+  rv.dst = {c.v.p, 0, c.v.sh};
+  p.paged = &c;
+  p.scale = scale;
+  p.interleaved = interleaved != 0;
+  p.dt = dt;
+  return launch_positions(p, current_stream());
+}
+
+int64_t nova_hip_paged_attention_scratch(int64_t tokens, int64_t sequences, int64_t heads,
+                                         int64_t kv_heads, int64_t D, int64_t rows,
+                                         int64_t max_queries) {
+  if (tokens <= 0 || sequences <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0 || rows <= 0 ||
+      max_queries <= 0 || tokens > 0x7fffffff || sequences >= (1 << 24) || heads > 0xffff ||
+      kv_heads > heads || heads % kv_heads || D > 128 || rows > 0x7fffffff)
+    return 0;  // the call itself refuses these, or has nothing to do
+  return paged_attention_scratch(tokens, sequences, heads, kv_heads, D, rows, max_queries);
+}
+
+int32_t _mlir_ciface_nova_hip_paged_attention(
+    const NovaMemRef3D *q, const NovaMemRef4D *k_pages, const NovaMemRef4D *v_pages,
+    const NovaMemRef1D *offsets, const NovaMemRef1D *lengths, const NovaMemRef2D *table,
+    NovaMemRef3D *out, NovaMemRef2D *lse, NovaMemRef1D *scratch, float scale, int32_t causal,
+    int64_t max_queries, int32_t dt) {
+  clear_error();
+  const char *w = "paged_attention";
+  PagedAttentionProblem p = {};
+  int32_t rc;
+  if (!q) return fail(NOVA_HIP_EINVAL, "%s: null descriptor", w);
+  if (dt != NOVA_HIP_DT_BF16 && dt != NOVA_HIP_DT_F16)
+    return fail(NOVA_HIP_EDTYPE, "%s: dtype %d (bf16 and f16 are provided)", w, dt);
+  if (!(scale > 0.0f) || !(scale < INFINITY))
+    return fail(NOVA_HIP_EINVAL, "%s: scale must be positive and finite", w);
+  if (causal != 0 && causal != 1) return fail(NOVA_HIP_EINVAL, "%s: causal is %d", w, causal);
+  if (max_queries < 0) return fail(NOVA_HIP_EINVAL, "%s: max_queries is negative", w);
+  if ((rc = same_shape(out, q, w, "out")) || (rc = attn_operand(q, w, "q", false, p.q)) ||
+      (rc = attn_operand(out, w, "out", true, p.o)) ||
+      (rc = paged_cache(k_pages, v_pages, offsets, lengths, table, false, w, p.c)))
+    return rc;
+  p.T = q->sizes[0];
+  p.heads = q->sizes[1];
+  const int64_t D = q->sizes[2];
+  if (p.c.D != D)
+    return fail(NOVA_HIP_ESHAPE, "%s: head dim of q is %lld, of the pages %lld", w, (long long)D,
+                (long long)p.c.D);
+  if (p.heads > 0 && (p.c.kv_heads == 0 || p.heads % p.c.kv_heads))
+    return fail(NOVA_HIP_ESHAPE, "%s: %lld query heads do not share %lld key heads evenly", w,
+                (long long)p.heads, (long long)p.c.kv_heads);
+  if (D % 8 || D > 128)
+    return fail(NOVA_HIP_ERANGE, "%s: head dim %lld is not a multiple of 8 up to 128", w, (long long)D);
+  if (p.c.k.st > kAttnMaxStride || p.c.v.st > kAttnMaxStride)
+    return fail(NOVA_HIP_ERANGE, "%s: row stride of the pages exceeds 2^23 elements", w);
+  if (lse) {
+    if (lse->sizes[0] != p.heads || lse->sizes[1] != p.T)
+      return fail(NOVA_HIP_ESHAPE, "%s: lse must be [heads, query tokens]", w);
+    if ((p.T > 1 && lse->strides[1] != 1) || (p.heads > 1 && lse->strides[0] < p.T))
+      return fail(NOVA_HIP_ESTRIDE, "%s: lse rows must be dense and not overlap", w);
+    if (!lse->aligned && p.heads * p.T > 0) return fail(NOVA_HIP_EINVAL, "%s: null lse pointer", w);
+    p.lse = out_f32(lse);
+    p.slse = lse->strides[0];
+  }
+  // 0: not known, one sequence may have all.
+  p.max_queries = max_queries == 0 ? p.T : std::min(max_queries, p.T);
+  const int64_t need = nova_hip_paged_attention_scratch(p.T, p.c.B, p.heads, p.c.kv_heads, D,
+                                                        p.c.width * p.c.page, p.max_queries);
+  if (need > 0) {
+    if (!scratch) return fail(NOVA_HIP_EINVAL, "%s: null scratch descriptor", w);
+    if ((rc = dense1(scratch, w, "scratch"))) return rc;
+    if (scratch->sizes[0] < need)
+      return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, %lld are needed", w,
+                  (long long)scratch->sizes[0], (long long)need);
+    p.partial = out_f32(scratch);
+    if (reinterpret_cast<uintptr_t>(p.partial) & 7u)
+      return fail(NOVA_HIP_ESTRIDE, "%s: scratch must be 8-byte aligned", w);
+  }
+  const Extent xq = rows_extent("q", p.q, q, 2), y = rows_extent("out", p.o, out, 2),
+               pk = pages_extent("k_pages", p.c.k, p.c), pv = pages_extent("v_pages", p.c.v, p.c),
+               off = vector_extent("offsets", p.c.offsets, 4 * (p.c.B + 1)),
+               len = vector_extent("lengths", p.c.lengths, 4 * p.c.B), tab = table_extent(p.c),
+               ls = {"lse", p.lse, p.lse ? 4 * p.T : 0, {p.heads, 1, 1}, {4 * p.slse, 0, 0}},
+               sc = vector_extent("scratch", p.partial, 4 * need);
+  if ((rc = check_apart(w, y, {xq, pk, pv, off, len, tab})) ||
+      (rc = check_apart(w, ls, {xq, pk, pv, off, len, tab, y})) ||
+      (rc = check_apart(w, sc, {xq, pk, pv, off, len, tab, y, ls})))
+    return rc;
+  p.scale = scale;
+  p.causal = causal != 0;
+  p.dt = dt;
+  return launch_paged_attention(p, current_stream());
 }
 
 void nova_hip_set_stream(void *stream) { t_stream = static_cast<hipStream_t>(stream); }

@@ -178,6 +178,74 @@ struct AttentionDecodeProblem {
 int64_t attention_decode_scratch(int64_t B, int64_t S, int64_t heads, int64_t kv_heads, int64_t D);
 int32_t launch_attention_decode(const AttentionDecodeProblem &p, hipStream_t s);
 
+// ---- positions and the paged cache (positions.hip, attention_paged.hip) ---------
+constexpr int64_t kMaxHeadDim = 256;  // of the rows of positions.hip
+// Pages [pages, page, key heads, D]: strides in elements.
+struct PageOperand {
+  void *p;
+  int64_t sp, st, sh;  // page, row and head strides
+};
+struct PagedCache {
+  PageOperand k, v;
+  const int32_t *offsets;  // [B + 1]: the new tokens of each sequence
+  const int32_t *lengths;  // [B]: rows of the cache, the new ones among them
+  const int32_t *table;    // [B, width], row stride stable
+  int64_t stable, B, width, pages, page, kv_heads, D;
+};
+// Rows [T, heads, D] read at src and written at dst (paged keys and values: dst
+// holds the pages' base and head stride).
+struct PositionRows {
+  AttentionOperand src, dst;
+  const void *w;
+  int64_t heads;
+};
+struct PositionProblem {
+  const char *what;      // the entry point, for errors
+  PositionRows rows[3];  // unused ones have no heads
+  const PagedCache *paged;   // or null; then rows are queries, keys, values
+  const int32_t *positions;  // [T], not for paged
+  const float *freqs;        // [R / 2]
+  int64_t T, D, R;
+  float scale, eps;
+  bool norm, interleaved, inverse;
+  int dt, w_dt;
+};
+int32_t launch_positions(const PositionProblem &p, hipStream_t s);
+int32_t launch_rotary_frequencies(float *freqs, int64_t n, double base, double factor, double low,
+                                  double high, double original, hipStream_t s);
+
+struct QkNormBackwardProblem {
+  struct Part {
+    AttentionOperand x, g, dx;
+    const void *w;
+    float *dw;
+    int64_t heads;
+  } part[2];  // queries, keys
+  const int32_t *positions;
+  const float *freqs;
+  float *scratch;  // of qk_norm_backward_scratch() floats
+  int64_t T, D, R;
+  float scale, eps;
+  bool interleaved;
+  int dt, w_dt;
+};
+int64_t qk_norm_backward_scratch(int64_t T, int64_t heads, int64_t kv_heads, int64_t D);
+int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s);
+
+struct PagedAttentionProblem {
+  PagedCache c;
+  AttentionOperand q, o;  // [T, heads, D]
+  float *lse;             // [heads, T], row stride slse; may be null
+  float *partial;         // scratch of paged_attention_scratch() floats
+  int64_t slse, T, heads, max_queries;
+  float scale;
+  bool causal;
+  int dt;
+};
+int64_t paged_attention_scratch(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
+                                int64_t rows, int64_t max_queries);
+int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s);
+
 // ---- losses over token log-probabilities (losses.hip) --------------------------
 struct TokenLossProblem {
   const void *logits;

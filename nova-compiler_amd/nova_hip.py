@@ -11,7 +11,9 @@ i.e. batch matmul), ``linear`` (+ GELU epilogue), ``layer_norm`` and ``sce``
   (NovaOps.td:880-896, NovaToLinalgGeneric.cpp:1008).
 
 Beside them, without a reference counterpart: ``attention`` of packed
-sequences with its backward and its form for single tokens, and the losses
+sequences with its backward and its form for single tokens, rotary positions
+with the norm of query and key heads (``rotary``, ``qk_norm_rotary``), a paged
+cache with its attention (``paged_append``, ``paged_attention``), and the losses
 over token log-probabilities (``token_logp``, ``policy_loss``,
 ``preference_loss``).
 
@@ -75,6 +77,14 @@ EXPORTS = (
     "_mlir_ciface_nova_hip_attention_decode",
     "nova_hip_attention_backward_scratch",
     "nova_hip_attention_decode_scratch",
+    "_mlir_ciface_nova_hip_rotary_frequencies",
+    "_mlir_ciface_nova_hip_rotary",
+    "_mlir_ciface_nova_hip_qk_norm_rotary",
+    "_mlir_ciface_nova_hip_qk_norm_rotary_backward",
+    "nova_hip_qk_norm_rotary_backward_scratch",
+    "_mlir_ciface_nova_hip_paged_append",
+    "_mlir_ciface_nova_hip_paged_attention",
+    "nova_hip_paged_attention_scratch",
     "_mlir_ciface_nova_hip_token_logp",
     "_mlir_ciface_nova_hip_policy_loss",
     "_mlir_ciface_nova_hip_preference_loss",
@@ -181,6 +191,16 @@ def lib() -> ctypes.CDLL:
     L.nova_hip_attention_backward_scratch.restype = ctypes.c_int64
     L.nova_hip_attention_decode_scratch.argtypes = [ctypes.c_int64] * 5
     L.nova_hip_attention_decode_scratch.restype = ctypes.c_int64
+    L._mlir_ciface_nova_hip_rotary_frequencies.argtypes = [P] + [F] * 4 + [ctypes.c_int64]
+    L._mlir_ciface_nova_hip_rotary.argtypes = [P] * 4 + [F, I, I, I]
+    L._mlir_ciface_nova_hip_qk_norm_rotary.argtypes = [P] * 8 + [F, F, I, I, I]
+    L._mlir_ciface_nova_hip_qk_norm_rotary_backward.argtypes = [P] * 13 + [F, F, I, I, I]
+    L.nova_hip_qk_norm_rotary_backward_scratch.argtypes = [ctypes.c_int64] * 4
+    L.nova_hip_qk_norm_rotary_backward_scratch.restype = ctypes.c_int64
+    L._mlir_ciface_nova_hip_paged_append.argtypes = [P] * 10 + [F, I, I]
+    L._mlir_ciface_nova_hip_paged_attention.argtypes = [P] * 9 + [F, I, ctypes.c_int64, I]
+    L.nova_hip_paged_attention_scratch.argtypes = [ctypes.c_int64] * 7
+    L.nova_hip_paged_attention_scratch.restype = ctypes.c_int64
     L._mlir_ciface_nova_hip_token_logp.argtypes = [P] * 4 + [I]
     L._mlir_ciface_nova_hip_policy_loss.argtypes = [P] * 10 + [F] * 4 + [I]
     L._mlir_ciface_nova_hip_preference_loss.argtypes = [P] * 9 + [F] * 3 + [I]
@@ -682,6 +702,148 @@ def attention_decode(q, k, v, lengths, *, scale=None, out=None, lse=None):
             _desc(out, 3, dt, dev, "out"), _desc(lse, 2, f32, dev, "lse"),
             _desc(scratch, 1, f32, dev, "scratch"), (D or 1) ** -0.5 if scale is None else scale,
             _dt(q))
+    return out
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, original: int = 0,
+                       low: float = 1.0, high: float = 32.0, freqs=None, device=None):
+    """base^(-2 i / dim) [dim / 2] f32 on the GPU, for contexts ``factor`` times
+    longer than the model's: all divided by it, or, with ``original`` the context
+    it was trained on, only those that turn few times over that (divided in full
+    at ``low`` turns, kept from ``high`` on)."""
+    torch = _torch()
+    if freqs is None:
+        if dim % 2:
+            raise NovaHipError(2, f"rotary_frequencies: {dim} values do not pair up")
+        freqs = torch.empty(dim // 2, dtype=torch.float32, device="cuda" if device is None else device)
+    elif 2 * freqs.shape[0] != dim:
+        raise NovaHipError(2, f"rotary_frequencies: freqs must have {dim} / 2 values")
+    dev = freqs.get_device()
+    _launch(lib()._mlir_ciface_nova_hip_rotary_frequencies, dev,
+            _desc(freqs, 1, torch.float32, dev, "freqs"), base, factor, low, high, original)
+    return freqs
+
+
+def rotary(x, positions, freqs, *, interleaved: bool = False, scale: float = 1.0,
+           inverse: bool = False, out=None):
+    """x [tokens, heads, D] (f32 / bf16 / f16) with the first 2 len(freqs) values
+    of each head rotated by ``positions`` [tokens] i32 times ``freqs`` f32, cosines
+    and sines times ``scale``; pairs are the two halves' values or, interleaved,
+    neighbours.  ``inverse`` rotates back: x's gradient from the result's.  ``out``
+    may be x."""
+    torch = _torch()
+    dt, dev = x.dtype, x.get_device()
+    d = (_desc(x, 3, dt, dev, "x"), _desc(positions, 1, torch.int32, dev, "positions"),
+         _desc(freqs, 1, torch.float32, dev, "freqs"))
+    if out is None:
+        out = x.new_empty(x.shape)
+    _launch(lib()._mlir_ciface_nova_hip_rotary, dev, *d, _desc(out, 3, dt, dev, "out"), scale,
+            1 if interleaved else 0, 1 if inverse else 0, _dt(x))
+    return out
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, positions=None, freqs=None, *, eps: float = 1e-6,
+                   interleaved: bool = False, scale: float = 1.0, q_out=None, k_out=None):
+    """RMS norm of each head of q [tokens, heads, D] and k [tokens, key heads, D]
+    times its weight [D] (f32 or q's dtype, both alike), then ``rotary`` in the
+    same pass (``positions`` and ``freqs`` None: the norm alone).  Returns (q_out,
+    k_out), which may be q and k."""
+    torch = _torch()
+    dt, dev, wt = q.dtype, q.get_device(), q_weight.dtype
+    d = (_desc(q, 3, dt, dev, "q"), _desc(k, 3, dt, dev, "k"), _desc(q_weight, 1, wt, dev, "q_weight"),
+         _desc(k_weight, 1, wt, dev, "k_weight"), _desc(positions, 1, torch.int32, dev, "positions"),
+         _desc(freqs, 1, torch.float32, dev, "freqs"))
+    if q_out is None:
+        q_out = q.new_empty(q.shape)
+    if k_out is None:
+        k_out = k.new_empty(k.shape)
+    _launch(lib()._mlir_ciface_nova_hip_qk_norm_rotary, dev, *d, _desc(q_out, 3, dt, dev, "q_out"),
+            _desc(k_out, 3, dt, dev, "k_out"), eps, scale, 1 if interleaved else 0, _dt(q),
+            _dt(q_weight))
+    return q_out, k_out
+
+
+def qk_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, positions=None, freqs=None, *,
+                            eps: float = 1e-6, interleaved: bool = False, scale: float = 1.0, dq=None,
+                            dk=None, dq_weight=None, dk_weight=None):
+    """Gradients of ``qk_norm_rotary``'s results with respect to q, k and both
+    weights: returns (dq, dk, dq_weight, dk_weight), the last two f32.  ``dq`` may
+    be q or grad_q, ``dk`` k or grad_k."""
+    torch = _torch()
+    f32, dt, dev, wt = torch.float32, q.dtype, q.get_device(), q_weight.dtype
+    d = (_desc(grad_q, 3, dt, dev, "grad_q"), _desc(grad_k, 3, dt, dev, "grad_k"),
+         _desc(q, 3, dt, dev, "q"), _desc(k, 3, dt, dev, "k"), _desc(q_weight, 1, wt, dev, "q_weight"),
+         _desc(k_weight, 1, wt, dev, "k_weight"), _desc(positions, 1, torch.int32, dev, "positions"),
+         _desc(freqs, 1, f32, dev, "freqs"))
+    T, H, D = q.shape
+    if dq is None:
+        dq = q.new_empty(q.shape)
+    if dk is None:
+        dk = k.new_empty(k.shape)
+    if dq_weight is None:
+        dq_weight = q.new_empty(D, dtype=f32)
+    if dk_weight is None:
+        dk_weight = q.new_empty(D, dtype=f32)
+    L = lib()
+    scratch = q.new_empty(L.nova_hip_qk_norm_rotary_backward_scratch(T, H, k.shape[1], D), dtype=f32)
+    _launch(L._mlir_ciface_nova_hip_qk_norm_rotary_backward, dev, *d, _desc(dq, 3, dt, dev, "dq"),
+            _desc(dk, 3, dt, dev, "dk"), _desc(dq_weight, 1, f32, dev, "dq_weight"),
+            _desc(dk_weight, 1, f32, dev, "dk_weight"), _desc(scratch, 1, f32, dev, "scratch"), eps,
+            scale, 1 if interleaved else 0, _dt(q), _dt(q_weight))
+    return dq, dk, dq_weight, dk_weight
+
+
+def paged_append(k, v, k_pages, v_pages, offsets, lengths, table, *, freqs=None,
+                 interleaved: bool = False, scale: float = 1.0, q=None, q_out=None):
+    """New tokens' keys and values [tokens, key heads, D] (bf16 / f16) to their
+    places in k_pages and v_pages [pages, rows of a page, key heads, D].  Sequence
+    b's tokens are the packed rows offsets[b] .. offsets[b + 1] and the last of its
+    lengths[b] rows; its row i lies in page table[b, i // page] (all i32 on the
+    GPU).  With ``freqs`` keys, and ``q`` [tokens, heads, D] if given, are rotated
+    by their position as ``rotary`` does.  Returns q_out (None without q), which
+    may be q."""
+    torch = _torch()
+    f32, i32, dt, dev = torch.float32, torch.int32, k.dtype, k.get_device()
+    d = (_desc(k, 3, dt, dev, "k"), _desc(v, 3, dt, dev, "v"), _desc(k_pages, 4, dt, dev, "k_pages"),
+         _desc(v_pages, 4, dt, dev, "v_pages"), _desc(offsets, 1, i32, dev, "offsets"),
+         _desc(lengths, 1, i32, dev, "lengths"), _desc(table, 2, i32, dev, "table"),
+         _desc(freqs, 1, f32, dev, "freqs"), _desc(q, 3, dt, dev, "q"))
+    if q_out is None and q is not None:
+        q_out = q.new_empty(q.shape)
+    _launch(lib()._mlir_ciface_nova_hip_paged_append, dev, *d, _desc(q_out, 3, dt, dev, "q_out"), scale,
+            1 if interleaved else 0, _dt(k))
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, offsets, lengths, table, *, causal: bool = True, scale=None,
+                    max_queries=None, out=None, lse=None):
+    """Attention of new tokens q [tokens, heads, D] (bf16 / f16) over the rows of
+    their sequences in the pages, described as for ``paged_append``; causal: a
+    token sees the rows up to its own position.  ``max_queries`` says that no
+    sequence has more new tokens (1: single tokens); a view of the table's first
+    columns that none is longer.  Returns out; ``lse`` [heads, tokens] f32 is
+    written when given."""
+    torch = _torch()
+    f32, i32, dt, dev = torch.float32, torch.int32, q.dtype, q.get_device()
+    d = (_desc(q, 3, dt, dev, "q"), _desc(k_pages, 4, dt, dev, "k_pages"),
+         _desc(v_pages, 4, dt, dev, "v_pages"), _desc(offsets, 1, i32, dev, "offsets"),
+         _desc(lengths, 1, i32, dev, "lengths"), _desc(table, 2, i32, dev, "table"))
+    T, H, D = q.shape
+    if max_queries is None:
+        max_queries = 0
+    elif max_queries < 1:
+        raise NovaHipError(1, f"paged_attention: max_queries is {max_queries}")
+    if out is None:
+        out = q.new_empty((T, H, D))
+    L = lib()
+    B, width = table.shape
+    _, page, G, _ = k_pages.shape
+    need = L.nova_hip_paged_attention_scratch(T, B, H, G, D, width * page,
+                                              min(max_queries or T, T))
+    scratch = q.new_empty(need, dtype=f32) if need else None
+    _launch(L._mlir_ciface_nova_hip_paged_attention, dev, *d, _desc(out, 3, dt, dev, "out"),
+            _desc(lse, 2, f32, dev, "lse"), _desc(scratch, 1, f32, dev, "scratch"),
+            (D or 1) ** -0.5 if scale is None else scale, 1 if causal else 0, max_queries, _dt(q))
     return out
 
 
