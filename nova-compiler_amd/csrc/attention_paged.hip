@@ -11,13 +11,14 @@
 // per sequence (single tokens): a wave per split of the keys, tiles of 32, without
 // a barrier; bound by HBM.  Either cuts the keys of a tile of rows into splits of
 // `chunk` where there are few tiles; a tile whose rows see at most one split
-// writes its result, the others' sums go to the caller's scratch and
-// paged_join_kernel adds them in order.
+// writes its result, the others' sums go to the caller's scratch, where a second
+// kernel adds them in order.
 //
 // Keys come by DMA into LDS.  Where a page holds whole loads (rows that are a
-// multiple of the 4 or 8 of one instruction) its address is a scalar: 64 entries of
-// the table lie in a register, and a buffer of the load's rows that are there makes
-// the others zero.  Other page sizes go through registers, a row's address per lane.
+// multiple of the 4 or 8 of one instruction) its address is a scalar: a lane looks up
+// each load of a tile, a tile ahead, and a buffer of the load's rows that are there
+// makes the others zero.  Other page sizes go through registers, a row's address per
+// lane.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -33,16 +34,21 @@ struct PagedArgs {
   const uint16_t *q, *k, *v;
   uint16_t *o;
   float *lse;      // [heads][T] with row stride slse, or null
-  float *partial;  // [T][heads][splits][D + 2]: sum, then m c and l (splits > 1)
+  // Rows of D + 2: sum, then m c and l.  [T][heads][splits], or, with slots, [key
+  // heads][slots][rows of a tile].
+  float *partial;
+  int2 *rows;  // [T][heads] of the scratch: a row's splits (0: written) and its place, with slots
   const int *off, *lens, *table;
   Rows sq, so;
   int64_t skp, skt, skh, svp, svt, svh, stb, slse;
   double per_page;  // 1 / page
   int T, B, heads, kv_heads, group, D, page, pages, width, cap;  // cap: rows of a sequence
-  int tiles, splits, chunk;
-  float c;  // scale log2 e
+  int tiles;  // per key head; with all their splits where these are slots'
+  int splits, chunk;  // chunk: what `splits` cover all rows with, at least 1
+  int slots, least;  // splits are found from the sequences' lengths: room for them, their least keys
+  float c;           // scale log2 e
+  float places;      // workgroups resident at once, to a key head
   bool causal;
-  bool whole;  // a load's rows lie in one page
 };
 
 constexpr float kSlack = 8.0f;  // as in the packed forward
@@ -65,53 +71,177 @@ __device__ __forceinline__ Seq seq_of(const PagedArgs &a, int b) {
   return q;
 }
 
-// Tile t of the sequences' tiles of BM rows (n group rows each): the sequence, or
-// -1, and the tile's index in it.  Wave-uniform.  The order and the two searches
-// are find_tile's.
-__device__ __forceinline__ int find_rows(const PagedArgs &a, int BM, int t, int &index) {
+__device__ __forceinline__ int wave_max_int(int v) {
+#define NOVA_DPP_MAX(c) v = max(v, __builtin_amdgcn_mov_dpp(v, c, 0xF, 0xF, false))
+  NOVA_DPP_MAX(0xB1);   // quad_perm [1,0,3,2]
+  NOVA_DPP_MAX(0x4E);   // quad_perm [2,3,0,1]
+  NOVA_DPP_MAX(0x141);  // row_half_mirror
+  NOVA_DPP_MAX(0x140);  // row_mirror
+#undef NOVA_DPP_MAX
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
+__device__ __forceinline__ Seq lane_seq(const Seq &q, int l) {
+  return {__builtin_amdgcn_readlane(q.s, l), __builtin_amdgcn_readlane(q.n, l),
+          __builtin_amdgcn_readlane(q.len, l)};
+}
+// Sum of the lanes below: within the rows of 16, then over rows.
+__device__ __forceinline__ int lanes_below(int v) {
+  int x = v;
+#define NOVA_DPP_SCAN(c, rows) x += __builtin_amdgcn_update_dpp(0, x, c, rows, 0xF, false)
+  NOVA_DPP_SCAN(0x111, 0xF);  // row_shr:1
+  NOVA_DPP_SCAN(0x112, 0xF);  // row_shr:2
+  NOVA_DPP_SCAN(0x114, 0xF);  // row_shr:4
+  NOVA_DPP_SCAN(0x118, 0xF);  // row_shr:8
+  NOVA_DPP_SCAN(0x142, 0xA);  // row_bcast:15 to rows 1 and 3
+  NOVA_DPP_SCAN(0x143, 0xC);  // row_bcast:31 to rows 2 and 3
+#undef NOVA_DPP_SCAN
+  return x - v;
+}
+
+// The work is cut so that it fills the chip's places for workgroups and no place is
+// left with a long remainder: a tile that sees `vis` keys into ceil(vis / chunk)
+// splits.  With fewer tiles than places, into as many as fill them once; with more,
+// only tiles that see kLong times the keys a place has in the mean (one token over a
+// long cache among prompts).
+constexpr float kLong = 2.0f;
+constexpr int kBM = 128;
+
+__device__ __forceinline__ int splits_for(int vis, int chunk) { return max(1, (vis - 1) / chunk + 1); }
+__device__ __forceinline__ int piece_of(int vis, int n) { return ((vis - 1) / n + 64) / 64 * 64; }
+// Keys that the tiles of a sequence see in the mean, or more.
+__device__ __forceinline__ float mean_keys(const PagedArgs &a, const Seq &q) {
+  return a.causal ? fmaxf(0.5f * (float)q.len, (float)q.len - 0.5f * (float)q.n) : (float)q.len;
+}
+__device__ __forceinline__ int tiles_of(const PagedArgs &a, const Seq &q) {
+  return (q.n * a.group + kBM - 1) / kBM;
+}
+
+// Up to 64 sequences, one to a lane (none in the others), read in one go by a whole
+// wave; the same for every wave of a call.  Each of a sequence's tiles may have `n`
+// splits; those of sequences with more than one have slots from `base` on.
+struct Work {
+  Seq q;
+  int tiles, n, base, chunk;
+};
+__device__ __forceinline__ Work work_of(const PagedArgs &a, int BM) {
   const int lane = threadIdx.x & 63;
-  if (a.B <= 64) {
-    int n = 0;
-    if (lane < a.B) {
-      const int s = min(max(a.off[lane], 0), a.T), e = max(s, min(a.off[lane + 1], a.T));
-      n = ((e - s) * a.group + BM - 1) / BM;
+  Work w;
+  w.q = lane < a.B ? seq_of(a, lane) : Seq{0, 0, 0};
+  w.tiles = BM == kBM ? tiles_of(a, w.q) : (w.q.n > 0 ? 1 : 0);
+  w.n = 1;
+  w.base = 0;
+  w.chunk = a.chunk;
+  if (a.slots == 0) return w;
+  const float tiles = (float)w.tiles;
+  float c = wave_sum(tiles * mean_keys(a, w.q)) / a.places;
+  if (wave_sum(tiles) >= a.places) {
+    c *= kLong;
+  } else {
+    for (int i = 0; i < 8; ++i) {
+      const float units = wave_sum(tiles * ceilf((float)w.q.len / fmaxf(c, 1.0f)));
+      if (units <= a.places) break;
+      c *= fmaxf(1.02f, units / a.places);
     }
-    auto above = [&](int k) __attribute__((always_inline)) { return wave_sum_int(max(0, n - k)); };
-    if (above(0) <= t) return -1;
-    int level = 0, bit = 1;
-    while (bit < (1 << 25) && above(bit) > t) bit <<= 1;
-    for (bit >>= 1; bit > 0; bit >>= 1)
-      if (above(level + bit) > t) level += bit;
-    const int k = t - above(level + 1);
-    const uint64_t has = __ballot(n > level);
-    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32),
-                                               __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
-    const uint64_t hit = __ballot(n > level && rank == k);
-    if (!hit) return -1;
-    index = level;
-    return __builtin_ctzll(hit);
   }
-  // Sequence b's tiles are numbered from off[b] group / BM + b.
-  t = a.T * a.group / BM + a.B - 1 - t;
+  w.chunk = __builtin_amdgcn_readfirstlane(max(a.least, (int)fminf(c + 1.0f, (float)a.cap)));
+  w.n = splits_for(w.q.len, w.chunk);
+  // As many slots as the host counted on, or no splits.
+  const float mine = w.n > 1 ? tiles * (float)w.n : 0.0f;
+  if (!(wave_sum(mine) <= (float)a.slots)) {
+    w.n = 1;
+    w.chunk = a.chunk;
+    return w;
+  }
+  w.base = lanes_below((int)mine);
+  return w;
+}
+
+// A tile of rows (n group to a sequence: of kBM, or the one that has all 32) and a
+// split of its keys.
+struct Unit {
+  Seq seq;
+  int b, index, split;
+  int slots, base;  // the sequence's, as in Work
+};
+
+// Unit t, wave-uniform; false where there is none.
+__device__ __forceinline__ bool unit_at(const Work &w, int first, int count, int k, Unit &u) {
+  const uint64_t hit = __ballot(k >= first && k < first + count);
+  if (!hit) return false;
+  u.b = __builtin_ctzll(hit);
+  u.seq = lane_seq(w.q, u.b);
+  u.split = k - __builtin_amdgcn_readlane(first, u.b);
+  u.slots = __builtin_amdgcn_readlane(w.n, u.b);
+  u.base = __builtin_amdgcn_readlane(w.base, u.b);
+  return true;
+}
+// One tile to a sequence, and splits of like size: one behind the other.
+__device__ __forceinline__ bool find_split(const Work &w, int t, Unit &u) {
+  const int n = w.tiles * w.n;
+  u.index = 0;
+  return unit_at(w, lanes_below(n), n, t, u);
+}
+// In the order of falling work, so that what runs last is short.  A sequence's tiles, the last first, see falling
+// numbers of keys, one tile's tokens less each; counted in such steps from the
+// longest sequence's end (a split's share of it) tile j of b lies at d(b) + j.  With
+// S(x) = sum over sequences of the units below x, the unit's place is the largest x
+// with S(x) <= t, found bit by bit.
+__device__ __forceinline__ bool find_unit(const PagedArgs &a, const Work &w, int t, Unit &u) {
+  const int len = w.q.len / w.n, longest = wave_max_int(w.tiles > 0 ? len : 0);
+  const int d = (int)min((int64_t)(longest - min(len, longest)) * a.group / kBM, (int64_t)1 << 24);
+  auto below = [&](int x) __attribute__((always_inline)) {
+    return wave_sum_int(w.n * min(max(x - d, 0), w.tiles));
+  };
+  if (wave_sum_int(w.n * w.tiles) <= t) return false;
+  int x = 0, bit = 1;
+  while (bit < (1 << 26) && below(bit) <= t) bit <<= 1;
+  for (bit >>= 1; bit > 0; bit >>= 1)
+    if (below(x + bit) <= t) x += bit;
+  const int k = t - below(x);  // among the units at x
+  const int here = x >= d && x - d < w.tiles ? w.n : 0;
+  if (!unit_at(w, lanes_below(here), here, k, u)) return false;
+  u.index = __builtin_amdgcn_readlane(w.tiles - 1 - (x - d), u.b);
+  return true;
+}
+
+// More than 64 sequences: the tiles by find_tile's numbering and search, at most
+// a.splits splits.
+__device__ __forceinline__ bool find_tile_of_many(const PagedArgs &a, int t, Unit &u) {
+  const int lane = threadIdx.x & 63;
+  t = a.T * a.group / kBM + a.B - 1 - t;
   int lo = 0, n = a.B;
   for (;;) {
-    const int step = (n + 63) / 64, b = lo + lane * step;
-    const bool at = lane * step < n && min(max(a.off[b], 0), a.T) * a.group / BM + b <= t;
+    const int step = (n + 63) / 64, i = lo + lane * step;
+    const bool at = lane * step < n && min(max(a.off[i], 0), a.T) * a.group / kBM + i <= t;
     const int c = __builtin_popcountll(__ballot(at));
-    if (c == 0) return -1;
+    if (c == 0) return false;
     lo += (c - 1) * step;
     n = min(step, n - (c - 1) * step);
     if (step == 1) break;
   }
-  const Seq q = seq_of(a, lo);
-  index = __builtin_amdgcn_readfirstlane(t - (q.s * a.group / BM + lo));
-  if (index < 0 || index >= (q.n * a.group + BM - 1) / BM) return -1;
-  return __builtin_amdgcn_readfirstlane(lo);
+  u.b = __builtin_amdgcn_readfirstlane(lo);
+  u.seq = seq_of(a, u.b);
+  u.index = __builtin_amdgcn_readfirstlane(t - (u.seq.s * a.group / kBM + u.b));
+  return u.index >= 0 && u.index < tiles_of(a, u.seq);
+}
+constexpr int kSummed = 4096;  // sequences; more are not looked at
+__device__ __forceinline__ int chunk_of_many(const PagedArgs &a) {
+  if (a.splits == 1 || a.B > kSummed) return a.chunk;
+  float tiles = 0.0f, keys = 0.0f;
+  for (int b = threadIdx.x & 63; b < a.B; b += 64) {
+    const Seq q = seq_of(a, b);
+    tiles += (float)tiles_of(a, q);
+    keys += (float)tiles_of(a, q) * mean_keys(a, q);
+  }
+  const float c = wave_sum(keys) / a.places * (wave_sum(tiles) >= a.places ? kLong : 1.25f);
+  return __builtin_amdgcn_readfirstlane(max(a.chunk, (int)fminf(c, (float)a.cap)));
 }
 
-// NW waves of 32 rows each.
-template <int DT, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_paged_kernel(PagedArgs a) {
+// NW waves of 32 rows each.  WHOLE: a load's rows lie in one page.
+template <int DT, int DP, int NW, bool WHOLE>
+__global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a) {
   constexpr int CH = kPitch<DP>, BN = NW == 1 ? 32 : 64, kTile = BN * CH * 16;
   constexpr int kRows = 64 / CH;               // rows of one DMA instruction
   constexpr int kN = BN / kRows / NW;          // instructions of a wave and tile
@@ -120,25 +250,37 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_paged_kern
   lds_char *const sv0 = (lds_char *)sv0_, *const sv1 = (lds_char *)sv1_;
   const int lane = threadIdx.x & 63;
   const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int kh, b, index = 0, split;
-  if constexpr (NW == 1) {
+  static_assert(NW == 1 || 32 * NW == kBM, "rows of a tile");
+  int kh, chunk = a.chunk;
+  Unit u;
+  if (a.slots || (NW > 1 && a.B <= 64)) {
+    int unit;
+    unit_of(blockIdx.x, a.kv_heads, a.tiles, true, kh, unit);
+    const Work w = work_of(a, 32 * NW);
+    if (!(NW == 1 ? find_split(w, unit, u) : find_unit(a, w, unit, u))) return;
+    chunk = w.chunk;
+  } else if constexpr (NW == 1) {
     kh = blockIdx.x;
-    b = blockIdx.y;
-    split = blockIdx.z;
+    u.b = blockIdx.y;
+    u.split = blockIdx.z;
+    u.seq = seq_of(a, u.b);
+    u.index = 0;
   } else {
     int tile;
-    unit_of(blockIdx.x, a.kv_heads, a.tiles, a.causal, kh, tile);
-    split = blockIdx.y;
-    b = find_rows(a, 32 * NW, tile, index);
-    if (b < 0) return;
+    unit_of(blockIdx.x, a.kv_heads, a.tiles, true, kh, tile);
+    u.split = a.splits - 1 - blockIdx.y;  // first splits last: others are long tiles'
+    if (!find_tile_of_many(a, tile, u)) return;
+    chunk = chunk_of_many(a);
   }
-  const Seq seq = seq_of(a, b);
-  const int row0 = index * 32 * NW, R = NW == 1 ? min(seq.n, 32 / a.group) * a.group : seq.n * a.group;
+  const Seq seq = u.seq;
+  const int b = u.b, split = u.split;
+  const int row0 = u.index * 32 * NW, R = NW == 1 ? min(seq.n, 32 / a.group) * a.group : seq.n * a.group;
   if (R <= row0) return;
   const int vis = seq.seen((min(row0 + 32 * NW, R) - 1) / a.group, a.causal);
-  const int from = split * a.chunk, to = min(vis, from + a.chunk);
-  if (split > 0 && from >= vis) return;
-  const bool direct = vis <= a.chunk;
+  const int ns = splits_for(vis, chunk), piece = NW == 1 && !a.slots ? chunk : piece_of(vis, ns);
+  const int from = split * piece, to = min(vis, from + piece);
+  if (split > 0 && (split >= ns || from >= vis)) return;
+  const bool direct = ns <= 1;
 
   const int q0 = row0 + 32 * wave, qn = min(32, R - q0);  // this wave's rows, maybe none
   const int row = min(q0 + (lane & 31), R - 1), token = row / a.group;
@@ -166,57 +308,71 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_paged_kern
   auto page_of = [&](int key) __attribute__((always_inline)) {
     return (int)(((double)key + 0.5) * a.per_page);
   };
-  int first = 0, ids = 0;  // entries first .. first + 63 of the table
-  bool loaded = false;
+  // WHOLE: a lane to each of the next tile's loads finds its page and row there, a
+  // tile ahead of the load itself.
+  int id = 0, at = 0;
+  auto look = [&](int t) __attribute__((always_inline)) {
+    const int key = min(from + t * BN + (lane & (BN / kRows - 1)) * kRows, to - 1), pg = page_of(key);
+    id = table[pg];
+    at = key - pg * a.page;
+  };
+  if (WHOLE && to > from) look(0);
+  // The queries are waited for here: at their use in the loop the compiler would
+  // wait for every load.
+  __builtin_amdgcn_s_waitcnt(0x0F70);
   auto fetch = [&](int t, lds_char *sk, lds_char *sv) __attribute__((always_inline)) {
     const int k0 = from + t * BN;
-    if (a.whole) {
-      const int p0 = __builtin_amdgcn_readfirstlane(page_of(k0));
-      const int p1 = __builtin_amdgcn_readfirstlane(page_of(min(k0 + BN, to) - 1));
-      if (!loaded || p1 >= first + 64) {
-        loaded = true;
-        first = p0;
-        ids = min(max(table[min(p0 + lane, a.width - 1)], 0), a.pages - 1);
-      }
+    if constexpr (WHOLE) {
+      const int skt = (int)a.skt * 2, svt = (int)a.svt * 2;  // bytes
+      const int pg = min(max(id, 0), a.pages - 1);
+      const uint64_t ka = reinterpret_cast<uint64_t>(kp + pg * a.skp) + (uint32_t)(at * skt);
+      const uint64_t va = reinterpret_cast<uint64_t>(vp + pg * a.svp) + (uint32_t)(at * svt);
+      // Rows behind the last read zero.
+      const int n = min(to - k0 - (lane & (BN / kRows - 1)) * kRows, kRows);
+      const int kb = max((n - 1) * skt + 2 * a.D, 0), vb = max((n - 1) * svt + 2 * a.D, 0);
+      look(t + 1);
+      // Ahead of the loads: a wait for it is then none for them.
+      __builtin_amdgcn_sched_barrier(0);
+      auto buffer = [&](uint64_t p, int bytes, int l) __attribute__((always_inline)) {
+        const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)p, l);
+        const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), l);
+        return make_rsrc(reinterpret_cast<const uint16_t *>(hi << 32 | lo),
+                         __builtin_amdgcn_readlane(bytes, l));
+      };
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int r0 = (i * NW + wave) * kRows, key = k0 + r0, n = min(to - key, kRows);
-        const int pg = __builtin_amdgcn_readfirstlane(page_of(min(key, to - 1)));
-        const int id = __builtin_amdgcn_readlane(ids, pg - first);
-        const int r = key - pg * a.page;
-        const __amdgpu_buffer_rsrc_t rk =
-            make_rsrc(kp + id * a.skp + r * a.skt, n > 0 ? (uint32_t)(((n - 1) * a.skt + a.D) * 2) : 0u);
-        const __amdgpu_buffer_rsrc_t rv =
-            make_rsrc(vp + id * a.svp + r * a.svt, n > 0 ? (uint32_t)(((n - 1) * a.svt + a.D) * 2) : 0u);
+        const int l = i * NW + wave, r0 = l * kRows;
+        const __amdgpu_buffer_rsrc_t rk = buffer(ka, kb, l), rv = buffer(va, vb, l);
         const int lr = lane / CH, ch = (lane & (CH - 1)) ^ swz<CH>(r0 + lr);
+        // Single tokens: read once by the whole chip, see attention_decode.hip.
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rk, (lds_void *)(sk + r0 * CH * 16), 16,
-            ch * 8 < a.D ? (uint32_t)(lr * a.skt + ch * 8) * 2u : kOOB, 0, 0, NW == 1 ? 2 : 0);
+            ch * 8 < a.D ? (uint32_t)(lr * skt + ch * 16) : kOOB, 0, 0, NW == 1 ? 2 : 0);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rv, (lds_void *)(sv + r0 * CH * 16), 16,
-            ch * 8 < a.D ? (uint32_t)(lr * a.svt + ch * 8) * 2u : kOOB, 0, 0, NW == 1 ? 2 : 0);
+            ch * 8 < a.D ? (uint32_t)(lr * svt + ch * 16) : kOOB, 0, 0, NW == 1 ? 2 : 0);
       }
     } else {
       typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-      u32x4 x[kN], y[kN];
+      auto rows = [&](const uint16_t *p, int64_t sp, int64_t st, lds_char *tile) __attribute__((always_inline)) {
+        u32x4 x[kN];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int r0 = (i * NW + wave) * kRows, lr = lane / CH, key = k0 + r0 + lr;
-        const int ch = (lane & (CH - 1)) ^ swz<CH>(r0 + lr);
-        x[i] = y[i] = u32x4{0, 0, 0, 0};
-        if (key < to && ch * 8 < a.D) {
-          const int pg = page_of(key), r = key - pg * a.page;
-          const int id = min(max(table[pg], 0), a.pages - 1);
-          x[i] = *reinterpret_cast<const u32x4 *>(kp + id * a.skp + r * a.skt + ch * 8);
-          y[i] = *reinterpret_cast<const u32x4 *>(vp + id * a.svp + r * a.svt + ch * 8);
+        for (int i = 0; i < kN; ++i) {
+          const int r0 = (i * NW + wave) * kRows, lr = lane / CH, key = k0 + r0 + lr;
+          const int ch = (lane & (CH - 1)) ^ swz<CH>(r0 + lr);
+          x[i] = u32x4{0, 0, 0, 0};
+          if (key < to && ch * 8 < a.D) {
+            const int pg = page_of(key), r = key - pg * a.page;
+            const int id = min(max(table[pg], 0), a.pages - 1);
+            x[i] = *reinterpret_cast<const u32x4 *>(p + (id * sp + r * st) + ch * 8);
+          }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int r0 = (i * NW + wave) * kRows;
-        *(lds_u32x4 *)(sk + r0 * CH * 16 + lane * 16) = x[i];
-        *(lds_u32x4 *)(sv + r0 * CH * 16 + lane * 16) = y[i];
-      }
+        for (int i = 0; i < kN; ++i)
+          *(lds_u32x4 *)(tile + (i * NW + wave) * kRows * CH * 16 + lane * 16) = x[i];
+      };
+      rows(kp, a.skp, a.skt, sk);
+      rows(vp, a.svp, a.svt, sv);
     }
   };
 
@@ -297,36 +453,34 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_paged_kern
     }
   } else {
     // A stage is refilled when the reads of it have returned, and read when all
-    // but the next stage's loads have landed.
-    constexpr int kInFlight = 2 * kN;
-    auto landed = [&](bool more) __attribute__((always_inline)) {
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) __builtin_amdgcn_s_waitcnt(0x0F70 | (kInFlight & 15) | ((kInFlight >> 4) << 14));
-      else __builtin_amdgcn_s_waitcnt(0x0F70);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    auto drained = [&]() __attribute__((always_inline)) {
+    // but the next stage's loads have landed.  Behind the last tile empty ones are
+    // fetched: with branches around the waits the compiler adds stricter ones.
+    auto turn = [&](int t, lds_char *sk, lds_char *sv, lds_char *nk, lds_char *nv) __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
+      fetch(t + 1, nk, nv);
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int kInFlight = WHOLE ? 2 * kN : 0;
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (kInFlight & 15) | ((kInFlight >> 4) << 14));
+      __builtin_amdgcn_sched_barrier(0);
+      step(t, sk, sv);
     };
     if (nt > 0) fetch(0, sk0, sv0);
     for (int t = 0; t < nt; t += 2) {
-      const bool two = t + 1 < nt;
-      drained();
-      if (two) fetch(t + 1, sk1, sv1);
-      landed(two && a.whole);
-      step(t, sk0, sv0);
-      if (!two) break;
-      const bool three = t + 2 < nt;
-      drained();
-      if (three) fetch(t + 2, sk0, sv0);
-      landed(three && a.whole);
-      step(t + 1, sk1, sv1);
+      turn(t, sk0, sv0, sk1, sv1);
+      turn(t + 1, sk1, sv1, sk0, sv0);
     }
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // the LDS is no longer written
   }
   l = both_sum(l);
   if (qn <= 0) return;
+  int64_t at_row = ((int64_t)(seq.s + token) * a.heads + head) * a.splits + split;
+  if (a.slots)
+    at_row = ((int64_t)kh * a.slots + u.base + u.index * u.slots + split) * (32 * NW) + (row - row0);
+  if (a.rows && split == 0 && lane < qn)
+    a.rows[(int64_t)(seq.s + token) * a.heads + head] =
+        int2{direct ? 0 : (vis - 1) / piece + 1, (int)at_row};
   if (direct) {
     // A row that sees no key is zero, its lse -inf.
     store_row<DT, DP>(acc, l == 0.0f ? 0.0f : 1.0f / l,
@@ -337,7 +491,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_paged_kern
     return;
   }
   if (!mine) return;
-  float *p = a.partial + (((int64_t)(seq.s + token) * a.heads + head) * a.splits + split) * (a.D + 2);
+  float *p = a.partial + at_row * (a.D + 2);
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -348,9 +502,15 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_paged_kern
   if (lane < 32) *reinterpret_cast<float2 *>(p + a.D) = float2{mc, l};
 }
 
-// The sequence of a token, or -1: 64 sequences are probed at a time.
-__device__ __forceinline__ int sequence_of(const PagedArgs &a, int t) {
-  const int lane = threadIdx.x & 63;
+// Whether a token's rows are in a tile of its sequence (of 32 rows: the first ones).
+// By a whole wave.
+__device__ __forceinline__ bool in_tile(const PagedArgs &a, int BM, int t) {
+  const int lane = threadIdx.x & 63, most = BM == kBM ? a.T : 32 / a.group;
+  if (a.B <= 64) {
+    const int s = lane < a.B ? max(a.off[lane], 0) : a.T;
+    return __ballot(s <= t && t < a.off[min(lane, a.B - 1) + 1] && t - s < most) != 0;
+  }
+  // The sequences that end at or before t are counted out, 64 probes at a time.
   int lo = 0, n = a.B;
   while (n > 0) {
     const int step = (n + 63) / 64, i = min(lo + (lane + 1) * step, lo + n);
@@ -363,71 +523,185 @@ __device__ __forceinline__ int sequence_of(const PagedArgs &a, int t) {
     lo += skip;
     n = min(step, n - skip);
   }
-  return lo < a.B ? lo : -1;
+  return lo < a.B && a.off[lo] <= t && t < a.off[lo + 1] && t - max(a.off[lo], 0) < most;
 }
 
-// One workgroup per (token, head) whose tile of BM rows left sums of several
-// splits: to their largest maximum, added in split order within each wave's share
-// (splits w, w + 4, ...), then the four shares in order.
+// A row's sums as its tile left them: its splits (0: none), the first one's place and
+// the rows from one to the next.  What a.rows holds of a row that no tile had (where
+// sequences overlap) is cut to the scratch.
+struct Sums {
+  int n;
+  const float *p;
+};
+__device__ __forceinline__ int64_t sums_step(const PagedArgs &a, int BM) {
+  return (a.slots ? BM : 1) * (int64_t)(a.D + 2);
+}
+__device__ __forceinline__ Sums sums_of(const PagedArgs &a, int BM, int t, int head) {
+  const int2 r = a.rows[(int64_t)t * a.heads + head];
+  if (!a.slots)
+    return {min(max(r.x, 0), a.splits),
+            a.partial + ((int64_t)t * a.heads + head) * a.splits * (a.D + 2)};
+  const int all = a.kv_heads * a.slots * BM, at = min(max(r.y, 0), all - 1);
+  return {min(max(r.x, 0), (all - 1 - at) / BM + 1), a.partial + (int64_t)at * (a.D + 2)};
+}
+
+// The sums of splits first, first + STEP, ... of a row (p: split 0's, `step` from one
+// to the next), by a wave: to the largest maximum mx, in the splits' order.  A lane holds values
+// 2 lane and 2 lane + 1; a split's maximum and sum of weights are a lane's.
+struct Joined {
+  float mx, sum, x0, x1;
+};
+template <int STEP>
+__device__ __forceinline__ Joined join(const PagedArgs &a, const float *p, int64_t step, int first,
+                                       int n) {
+  const int lane = threadIdx.x & 63;
+  Joined j = {-INFINITY, 0.0f, 0.0f, 0.0f};
+  const float *v = p + min(2 * lane, a.D - 2);
+  for (int i0 = first; i0 < n; i0 += 64 * STEP) {
+    const int i = i0 + lane * STEP, count = min(64, (n - i0 + STEP - 1) / STEP);
+    float2 ml = {-INFINITY, 0.0f};
+    if (i < n) ml = *reinterpret_cast<const float2 *>(p + i * step + a.D);
+    const float mx = fmaxf(j.mx, wave_max(ml.x));
+    const float old = j.mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(j.mx - mx);
+    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    j = {mx, j.sum * old + wave_sum(ml.y * f), j.x0 * old, j.x1 * old};
+    for (int k0 = 0; k0 < count; k0 += 8) {
+      float2 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        x[k] = *reinterpret_cast<const float2 *>(v + (i0 + min(k0 + k, count - 1) * STEP) * step);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const bool there = k0 + k < count;
+        const float g = lane_value(f, (k0 + k) & 63);
+        j.x0 = there ? __builtin_fmaf(x[k].x, g, j.x0) : j.x0;
+        j.x1 = there ? __builtin_fmaf(x[k].y, g, j.x1) : j.x1;
+      }
+    }
+  }
+  return j;
+}
+
+template <int DT>
+__device__ __forceinline__ void store_joined(const PagedArgs &a, int t, int head, int lane,
+                                             const Joined &j) {
+  const float inv = j.sum == 0.0f ? 0.0f : 1.0f / j.sum;
+  if (2 * lane < a.D)
+    *reinterpret_cast<uint32_t *>(a.o + t * a.so.t + head * a.so.h + 2 * lane) =
+        pack<DT>(j.x0 * inv, j.x1 * inv);
+  if (a.lse && lane == 0)
+    a.lse[head * a.slse + t] = j.sum == 0.0f ? -INFINITY : (j.mx + (__log2f(j.sum) - kUp<DT>)) * kLn2;
+}
+
+// Few rows: one workgroup per (token, head), its waves take every fourth split and
+// join in order.
 template <int DT>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int BM) {
   __shared__ float smax[4], ssum[4], sx[4][128];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = blockIdx.x / a.heads, head = blockIdx.x - t * a.heads;
-  const int b = sequence_of(a, t);
-  if (b < 0) return;
-  const Seq seq = seq_of(a, b);
-  const int token = t - seq.s;
-  if (token < 0 || token >= seq.n) return;
-  // As the rows' tile decided it.
-  const int R = BM == 32 ? min(seq.n, 32 / a.group) * a.group : seq.n * a.group;
-  const int row = token * a.group + head % a.group;
-  if (row >= R) return;
-  const int vis = seq.seen((min(row / BM * BM + BM, R) - 1) / a.group, a.causal);
-  if (vis <= a.chunk) return;
-  const int n = (vis + a.chunk - 1) / a.chunk;
-  const float *p = a.partial + ((int64_t)t * a.heads + head) * a.splits * (a.D + 2);
-  float mx = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 256) mx = fmaxf(mx, p[(int64_t)i * (a.D + 2) + a.D]);
-  mx = wave_max(mx);
-  if (lane == 0) smax[wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
-  float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
-  const int d = 2 * lane;
-#pragma unroll 8
-  for (int i = wave; i < n; i += 4) {
-    const float *r = p + (int64_t)i * (a.D + 2);
-    const float2 ml = *reinterpret_cast<const float2 *>(r + a.D);
-    const float2 v = *reinterpret_cast<const float2 *>(r + min(d, a.D - 2));
-    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
-    sum = __builtin_fmaf(ml.y, f, sum);
-    x0 = __builtin_fmaf(v.x, f, x0);
-    x1 = __builtin_fmaf(v.y, f, x1);
+  const Sums s = sums_of(a, BM, t, head);
+  if (!in_tile(a, BM, t) || s.n == 0) return;
+  Joined j = join<4>(a, s.p, sums_step(a, BM), wave, s.n);
+  sx[wave][2 * lane] = j.x0;
+  sx[wave][2 * lane + 1] = j.x1;
+  if (lane == 0) {
+    smax[wave] = j.mx;
+    ssum[wave] = j.sum;
   }
-  sx[wave][d] = x0;
-  sx[wave][d + 1] = x1;
-  if (lane == 0) ssum[wave] = sum;
   __syncthreads();
   if (wave) return;
-  sum = (ssum[0] + ssum[1]) + (ssum[2] + ssum[3]);
-  x0 = (sx[0][d] + sx[1][d]) + (sx[2][d] + sx[3][d]);
-  x1 = (sx[0][d + 1] + sx[1][d + 1]) + (sx[2][d + 1] + sx[3][d + 1]);
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  if (d < a.D)
-    *reinterpret_cast<uint32_t *>(a.o + t * a.so.t + head * a.so.h + d) = pack<DT>(x0 * inv, x1 * inv);
-  if (a.lse && lane == 0)
-    a.lse[head * a.slse + t] = sum == 0.0f ? -INFINITY : (mx + (__log2f(sum) - kUp<DT>)) * kLn2;
+  j = {fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3])), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = smax[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(smax[w] - j.mx);
+    j.sum = __builtin_fmaf(ssum[w], f, j.sum);
+    j.x0 = __builtin_fmaf(sx[w][2 * lane], f, j.x0);
+    j.x1 = __builtin_fmaf(sx[w][2 * lane + 1], f, j.x1);
+  }
+  store_joined<DT>(a, t, head, lane, j);
 }
 
+// Many rows: a workgroup per token and `per` heads.  A wave takes eight rows at a
+// time, so that their loads are on their way together: lane 8 r + i has row r's split
+// i.  Rows of more than eight splits, of which there are few, one by one.
+template <int DT>
+__global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int per) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x;
+  const int64_t step = sums_step(a, kBM);
+  const int end = min(a.heads, ((int)blockIdx.y + 1) * per);
+  for (int h0 = blockIdx.y * per + 8 * wave; h0 < end; h0 += 8 * (blockDim.x >> 6)) {
+    const int rows = min(8, end - h0), r = lane >> 3, i = lane & 7;
+    const Sums s = sums_of(a, kBM, t, h0 + min(r, rows - 1));
+    if (!in_tile(a, kBM, t)) return;
+    const int n = r < rows ? s.n : 0;
+    auto row_of = [&](int q) __attribute__((always_inline)) {
+      const uint64_t p = reinterpret_cast<uint64_t>(s.p);
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)p, 8 * q);
+      const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), 8 * q);
+      return reinterpret_cast<const float *>(hi << 32 | lo);
+    };
+    if (__ballot(n > 8)) {
+      for (int k = 0; k < rows; ++k) {
+        const int nk = __builtin_amdgcn_readlane(n, 8 * k);
+        if (nk) store_joined<DT>(a, t, h0 + k, lane, join<1>(a, row_of(k), step, 0, nk));
+      }
+      continue;
+    }
+    const int most = wave_max_int(n), d = min(2 * lane, a.D - 2);
+    if (most == 0) continue;
+    float2 ml = {-INFINITY, 0.0f};
+    if (i < n) ml = *reinterpret_cast<const float2 *>(s.p + i * step + a.D);
+    float mx = ml.x;
+    mx = fmaxf(mx, dpp_mov<0xB1>(mx));   // quad_perm [1,0,3,2]
+    mx = fmaxf(mx, dpp_mov<0x4E>(mx));   // quad_perm [2,3,0,1]
+    mx = fmaxf(mx, dpp_mov<0x141>(mx));  // row_half_mirror
+    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    float sum = ml.y * f;
+    sum += dpp_mov<0xB1>(sum);
+    sum += dpp_mov<0x4E>(sum);
+    sum += dpp_mov<0x141>(sum);
+    float x0[8] = {}, x1[8] = {};
+    for (int k = 0; k < most; ++k) {
+      float2 x[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)  // (a row without the split: its first one's values, unused)
+        x[q] = *reinterpret_cast<const float2 *>(
+            row_of(q) + (k < __builtin_amdgcn_readlane(n, 8 * q) ? k : 0) * step + d);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const bool there = k < __builtin_amdgcn_readlane(n, 8 * q);
+        const float g = lane_value(f, 8 * q + k);
+        x0[q] = there ? __builtin_fmaf(x[q].x, g, x0[q]) : x0[q];
+        x1[q] = there ? __builtin_fmaf(x[q].y, g, x1[q]) : x1[q];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (__builtin_amdgcn_readlane(n, 8 * q))
+        store_joined<DT>(a, t, h0 + q, lane,
+                         {lane_value(mx, 8 * q), lane_value(sum, 8 * q), x0[q], x1[q]});
+  }
+}
+
+template <int DT, int DP, bool WHOLE>
+void launch_paged_t(const PagedArgs &a, bool narrow, hipStream_t s) {
+  const unsigned units = (unsigned)(a.tiles * a.kv_heads);
+  if (narrow)
+    hipLaunchKernelGGL(
+        (attention_paged_kernel<DT, DP, 1, WHOLE>),
+        a.slots ? dim3(units) : dim3((unsigned)a.kv_heads, (unsigned)a.B, (unsigned)a.splits), dim3(64),
+        0, s, a);
+  else
+    hipLaunchKernelGGL((attention_paged_kernel<DT, DP, 4, WHOLE>),
+                       dim3(units, a.slots ? 1u : (unsigned)a.splits), dim3(256), 0, s, a);
+}
 template <int DT, int DP>
 void launch_paged_t(const PagedArgs &a, bool narrow, hipStream_t s) {
-  if (narrow)
-    hipLaunchKernelGGL((attention_paged_kernel<DT, DP, 1>),
-                       dim3((unsigned)a.kv_heads, (unsigned)a.B, (unsigned)a.splits), dim3(64), 0, s, a);
-  else
-    hipLaunchKernelGGL((attention_paged_kernel<DT, DP, 4>),
-                       dim3((unsigned)(a.tiles * a.kv_heads), (unsigned)a.splits), dim3(256), 0, s, a);
+  // A load is of 8 rows up to D = 64, of 4 beyond.
+  if (a.page % (64 / kPitch<DP>) == 0) launch_paged_t<DT, DP, true>(a, narrow, s);
+  else launch_paged_t<DT, DP, false>(a, narrow, s);
 }
 template <int DT>
 int32_t launch_paged(const PagedArgs &a, bool narrow, hipStream_t s) {
@@ -436,34 +710,58 @@ int32_t launch_paged(const PagedArgs &a, bool narrow, hipStream_t s) {
   else if (a.D <= 96) launch_paged_t<DT, 96>(a, narrow, s);
   else launch_paged_t<DT, 128>(a, narrow, s);
   const int32_t rc = check_hip(hipGetLastError(), "paged_attention launch");
-  if (rc || a.splits <= 1) return rc;
-  hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((unsigned)(a.T * a.heads)), dim3(256), 0, s, a,
-                     narrow ? 32 : 128);
+  if (rc || (a.splits <= 1 && a.slots == 0)) return rc;
+  if (a.T * a.heads <= 4096 || narrow) {
+    hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((unsigned)(a.T * a.heads)), dim3(256), 0, s, a,
+                       narrow ? 32 : attn::kBM);
+  } else {
+    const int per = 32, waves = std::min(4, (a.heads + 7) / 8);
+    hipLaunchKernelGGL(paged_join_rows_kernel<DT>, dim3((unsigned)a.T, (unsigned)((a.heads + per - 1) / per)),
+                       dim3(64 * waves), 0, s, a, per);
+  }
   return check_hip(hipGetLastError(), "paged_attention join launch");
 }
 
-// The form of a call, its tiles of rows and its splits.
+
+// The form of a call, its tiles of rows (units with their splits where there are
+// slots for these) per key head, its splits and slots.
 struct Plan {
   bool narrow;
-  int64_t tiles, chunk, splits;
+  int64_t tiles, chunk, splits, slots, least, places;
 };
-Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t rows, int64_t max_queries) {
-  Plan p;
+Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D, int64_t rows,
+             int64_t max_queries) {
+  Plan p = {};
   const int64_t group = heads / kv_heads;
   p.narrow = max_queries * group <= 32 && B <= 0xffff;
+  p.chunk = std::max<int64_t>(rows, 1);
+  // Workgroups resident at once, by LDS (a wave's 32 or 16 KB) and registers.
+  p.places = p.narrow ? (D <= 64 ? 1536 : 768) : (D <= 64 ? 768 : 512);
+  p.least = p.narrow ? 64 : 256;
+  const int64_t most = (rows + p.least - 1) / p.least, mine = (p.places + kv_heads - 1) / kv_heads;
   if (p.narrow) {
-    p.tiles = 0;
-    // As for the padded cache (attention_decode.hip).
-    const int64_t all = B * rows * kv_heads;
-    const int64_t keys = std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
-    p.chunk = std::max<int64_t>(64, (std::max(keys, rows / 32768) + 63) / 64 * 64);
+    p.tiles = std::min(B, T);
+    if (B <= 64 && B * kv_heads * most > p.places) {
+      p.slots = std::min(B * most, B < mine ? mine : 2 * mine);
+    } else {
+      // As for the padded cache (attention_decode.hip).
+      const int64_t all = B * rows * kv_heads;
+      const int64_t keys =
+          std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
+      p.chunk = std::max<int64_t>(64, (std::max(keys, rows / 32768) + 63) / 64 * 64);
+    }
+  } else if (B <= 64) {
+    p.tiles = std::min(T * group, T * group / kBM + B);
+    // Work::n: fewer tiles than places have as many units as places at most; with more
+    // tiles, those that are split have less than 4 / kLong units to a place.
+    if (most > 1) p.slots = std::min(p.tiles * most, p.tiles < mine ? mine : 2 * mine);
   } else {
-    // Two workgroups to a CU, four rounds of them at most.
-    p.tiles = B <= 64 ? std::min(T * group, T * group / 128 + B) : T * group / 128 + B;
-    const int64_t units = p.tiles * kv_heads;
-    const int64_t splits = std::max<int64_t>(1, std::min(2048 / units, rows / 512));
+    p.tiles = T * group / kBM + B;
+    const int64_t splits =
+        std::max<int64_t>(1, std::min(3 * p.places / (2 * p.tiles * kv_heads), rows / 512));
     p.chunk = std::max<int64_t>(64, ((rows + splits - 1) / splits + 63) / 64 * 64);
   }
+  p.tiles += p.slots;
   p.splits = std::max<int64_t>(1, (rows + p.chunk - 1) / p.chunk);
   return p;
 }
@@ -473,8 +771,11 @@ Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t rows
 
 int64_t paged_attention_scratch(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
                                 int64_t rows, int64_t max_queries) {
-  const attn::Plan p = attn::plan_of(T, B, heads, kv_heads, rows, max_queries);
-  return p.splits <= 1 ? 0 : T * heads * p.splits * (D + 2);
+  const attn::Plan p = attn::plan_of(T, B, heads, kv_heads, D, rows, max_queries);
+  const int64_t rows_of_sums = p.slots ? kv_heads * p.slots * (p.narrow ? 32 : attn::kBM)
+                               : p.splits > 1 ? T * heads * p.splits
+                                              : 0;
+  return rows_of_sums ? rows_of_sums * (D + 2) + 2 * T * heads : 0;
 }
 
 int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
@@ -487,7 +788,6 @@ int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
   a.o = static_cast<uint16_t *>(p.o.p);
   a.lse = p.lse;
   a.slse = p.slse;
-  a.partial = p.partial;
   a.off = c.offsets;
   a.lens = c.lengths;
   a.table = c.table;
@@ -507,18 +807,25 @@ int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
   a.pages = (int)c.pages;
   a.width = (int)c.width;
   a.cap = (int)(c.width * c.page);
-  const attn::Plan plan = attn::plan_of(p.T, c.B, p.heads, c.kv_heads, a.cap, p.max_queries);
+  const attn::Plan plan = attn::plan_of(p.T, c.B, p.heads, c.kv_heads, c.D, a.cap, p.max_queries);
   // Rows are counted in 32 bits, a grid's dimension holds less than 2^32 threads.
   if (p.T * p.heads >= (1LL << 31) - (1 << 20) || plan.tiles * c.kv_heads >= 1 << 24 ||
-      (plan.splits > 1 && p.T * p.heads >= 1 << 24))
+      ((plan.splits > 1 || plan.slots > 0) && p.T * ((p.heads + 31) / 32) >= 1 << 24) ||
+      (plan.narrow && (plan.splits > 1 || plan.slots > 0) && p.T * p.heads >= 1 << 24))
     return fail(NOVA_HIP_ERANGE, "paged_attention: %lld tokens of %lld heads in %lld sequences",
                 (long long)p.T, (long long)p.heads, (long long)c.B);
+  if (plan.splits > 1 || plan.slots) {
+    a.rows = reinterpret_cast<int2 *>(p.partial);
+    a.partial = p.partial + 2 * p.T * p.heads;
+  }
   a.tiles = (int)plan.tiles;
   a.splits = (int)plan.splits;
   a.chunk = (int)plan.chunk;
   a.c = p.scale * attn::kLog2e;
   a.causal = p.causal;
-  a.whole = c.page % (c.D <= 64 ? 8 : 4) == 0;
+  a.slots = (int)plan.slots;
+  a.least = (int)plan.least;
+  a.places = (float)plan.places / (float)c.kv_heads;
   return p.dt == NOVA_HIP_DT_BF16 ? attn::launch_paged<NOVA_HIP_DT_BF16>(a, plan.narrow, s)
                                   : attn::launch_paged<NOVA_HIP_DT_F16>(a, plan.narrow, s);
 }

@@ -1434,8 +1434,8 @@ int32_t page_operand(const NovaMemRef4D *d, const char *w, const char *what, boo
   o.p = const_cast<char *>(data_of(d)) + d->offset * 2;
   if (st[0] % 8 || st[1] % 8 || st[2] % 8 || (reinterpret_cast<uintptr_t>(o.p) & 15u))
     return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s must start at 16-byte aligned addresses", w, what);
-  if (st[0] < 0 || st[1] < 0 || st[2] < 0)
-    return fail(NOVA_HIP_ESTRIDE, "%s: negative stride of %s", w, what);
+  if (st[0] < 0 || st[1] < D || st[2] < 0)
+    return fail(NOVA_HIP_ESTRIDE, "%s: rows of %s overlap", w, what);
   if (out) {  // in the order of their strides, each beyond what the ones before it span
     int order[3] = {0, 1, 2};
     std::sort(order, order + 3, [&](int a, int b) { return st[a] < st[b]; });
@@ -1783,8 +1783,9 @@ int32_t _mlir_ciface_nova_hip_paged_attention(
                 (long long)p.heads, (long long)p.c.kv_heads);
   if (D % 8 || D > 128)
     return fail(NOVA_HIP_ERANGE, "%s: head dim %lld is not a multiple of 8 up to 128", w, (long long)D);
-  if (p.c.k.st > kAttnMaxStride || p.c.v.st > kAttnMaxStride)
-    return fail(NOVA_HIP_ERANGE, "%s: row stride of the pages exceeds 2^23 elements", w);
+  const int64_t wide = std::max(p.c.k.st, p.c.v.st);
+  if (wide > kAttnMaxStride || wide * (p.c.page - 1) >= 1 << 30)
+    return fail(NOVA_HIP_ERANGE, "%s: rows of a page 2^23, or its first and last 2^30, elements apart", w);
   if (lse) {
     if (lse->sizes[0] != p.heads || lse->sizes[1] != p.T)
       return fail(NOVA_HIP_ESHAPE, "%s: lse must be [heads, query tokens]", w);

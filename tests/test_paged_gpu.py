@@ -271,3 +271,15 @@ def test_append_stores_nothing_outside(cuda):
     # No pages at all: only q.
     nh.paged_append(x, x, c.k[:0], c.v[:0], off, lens, c.table, q=q, q_out=q)
     assert (q == 3.0).all()
+
+
+def test_tokens_beyond_the_hint_are_left_out(cuda):
+    """Seven new tokens where the call is told of one: the first ones that a tile
+    of 32 rows holds are computed, the others' rows stay, whatever the splits."""
+    for rows in (60, 3000):
+        q, c, off, out, lse = run(cuda, [(7, rows), (1, rows)], 20, 2, 64)  # 10 heads to a key head
+        got, l2 = torch.full_like(out, 5.0), torch.full_like(lse, 5.0)
+        nh.paged_attention(q, c.k, c.v, off, c.lengths, c.table, out=got, lse=l2, max_queries=1)
+        near = (got.double() - out.double()).abs() <= 2.0 ** -6
+        assert near[:3].all() and near[7:].all() and (l2[:, :3] - lse[:, :3]).abs().max() < 1e-4
+        assert (got[3:7] == 5.0).all() and (l2[:, 3:7] == 5.0).all()
