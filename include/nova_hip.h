@@ -529,7 +529,8 @@ int64_t nova_hip_qk_norm_rotary_backward_scratch(int64_t tokens, int64_t heads, 
  * [pages, rows of a page, key heads, D] of dt NOVA_HIP_DT_BF16 or _F16, unit
  * stride on D, any order of the other dims, rows 16-byte aligned, any page size
  * (attention reads keys fastest from pages of a multiple of 8 rows, or of 4 where D
- * is above 64; it takes pages of up to 2^30 elements from first to last row).
+ * is above 64; it takes tables of up to 2^30 rows and pages of up to
+ * 2^30 elements from first to last row).
  * Row i of sequence b is row i % page of page table[b, i / page].
  *   offsets : [sequences + 1] i32, not decreasing: the new tokens of sequence b
  *   are the packed rows [offsets[b], offsets[b + 1]);
@@ -561,7 +562,7 @@ int32_t _mlir_ciface_nova_hip_paged_append(
  *   tokens] f32 or NULL; rows outside every sequence are left as they were.
  *   max_queries : no sequence has more new tokens (0: not known); tokens beyond it
  *   may be left out.
- *   scratch : nova_hip_paged_attention_scratch() f32, dense and 8-byte aligned,
+ *   scratch : nova_hip_paged_attention_scratch() f32, dense and 16-byte aligned,
  *   used by this call only (NULL when that is 0). */
 int32_t _mlir_ciface_nova_hip_paged_attention(
     const NovaMemRef3D *q, const NovaMemRef4D *k_pages, const NovaMemRef4D *v_pages,

@@ -30,24 +30,41 @@ namespace nova_hip {
 namespace attn {
 namespace {
 
+// n / d for n < 2^31: the upper bits of n m, m the least number above 2^(31 + l) / d.
+struct Divider {
+  uint32_t d, m;
+  int l;
+  Divider() = default;
+  __host__ explicit Divider(int64_t by) : d((uint32_t)by), l(0) {
+    while (((int64_t)1 << l) < by) ++l;
+    m = (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)by) + 1);
+  }
+  __device__ __forceinline__ int of(int n) const {
+    return (int)(((uint64_t)(uint32_t)n * m) >> (31 + l));
+  }
+};
+
 struct PagedArgs {
   const uint16_t *q, *k, *v;
   uint16_t *o;
-  float *lse;      // [heads][T] with row stride slse, or null
-  // Rows of D + 2: sum, then m c and l.  [T][heads][splits], or, with slots, [key
-  // heads][slots][rows of a tile].
+  float *lse;  // [heads][T] with row stride slse, or null
+  // Sums of splits.  Chunks: [key heads][slots] of a tile each (see sums_at).  Up to 32
+  // rows: rows of D + 2, the sum, then m c and l: [key heads][slots][32], or without
+  // slots [T][heads][splits]; and for each of [T][heads] its splits (0: written) and place.
   float *partial;
-  int2 *rows;  // [T][heads] of the scratch: a row's splits (0: written) and its place, with slots
+  int2 *rows;
   const int *off, *lens, *table;
   Rows sq, so;
   int64_t skp, skt, skh, svp, svt, svh, stb, slse;
   double per_page;  // 1 / page
-  int T, B, heads, kv_heads, group, D, page, pages, width, cap;  // cap: rows of a sequence
-  int tiles;  // per key head; with all their splits where these are slots'
+  Divider group;    // query heads to a key head
+  int T, B, heads, kv_heads, D, page, pages, width, cap;  // cap: rows of a sequence
+  int tiles;          // per key head; up to 64 sequences: with their splits
+  int split_tiles;    // those that may have several
   int splits, chunk;  // chunk: what `splits` cover all rows with, at least 1
-  int slots, least;  // splits are found from the sequences' lengths: room for them, their least keys
-  float c;           // scale log2 e
-  float places;      // workgroups resident at once, to a key head
+  int slots, least;   // of splits found from the lengths: room for them, their least keys
+  float c;            // scale log2 e
+  float places;       // workgroups resident at once, to a key head
   bool causal;
 };
 
@@ -101,29 +118,26 @@ __device__ __forceinline__ int lanes_below(int v) {
 }
 
 // The work is cut so that it fills the chip's places for workgroups and no place is
-// left with a long remainder: a tile that sees `vis` keys into ceil(vis / chunk)
-// splits.  With fewer tiles than places, into as many as fill them once; with more,
-// only tiles that see kLong times the keys a place has in the mean (one token over a
-// long cache among prompts).
+// left with a long remainder.  With fewer tiles than places, a sequence's keys into as
+// many splits as fill the places once; with more, only where its tiles see kLong times
+// the keys that a place has in the mean (one token over a long cache among prompts).
 constexpr float kLong = 2.0f;
 constexpr int kBM = 128;
 
-__device__ __forceinline__ int splits_for(int vis, int chunk) { return max(1, (vis - 1) / chunk + 1); }
-__device__ __forceinline__ int piece_of(int vis, int n) { return ((vis - 1) / n + 64) / 64 * 64; }
 // Keys that the tiles of a sequence see in the mean, or more.
 __device__ __forceinline__ float mean_keys(const PagedArgs &a, const Seq &q) {
   return a.causal ? fmaxf(0.5f * (float)q.len, (float)q.len - 0.5f * (float)q.n) : (float)q.len;
 }
 __device__ __forceinline__ int tiles_of(const PagedArgs &a, const Seq &q) {
-  return (q.n * a.group + kBM - 1) / kBM;
+  return (q.n * (int)a.group.d + kBM - 1) / kBM;
 }
 
 // Up to 64 sequences, one to a lane (none in the others), read in one go by a whole
-// wave; the same for every wave of a call.  Each of a sequence's tiles may have `n`
-// splits; those of sequences with more than one have slots from `base` on.
+// wave; the same for every wave of a call.  The tiles of a sequence have up to n
+// splits of `piece` keys; those of sequences with more than one have slots from `base`.
 struct Work {
   Seq q;
-  int tiles, n, base, chunk;
+  int tiles, n, piece, base;
 };
 __device__ __forceinline__ Work work_of(const PagedArgs &a, int BM) {
   const int lane = threadIdx.x & 63;
@@ -131,90 +145,99 @@ __device__ __forceinline__ Work work_of(const PagedArgs &a, int BM) {
   w.q = lane < a.B ? seq_of(a, lane) : Seq{0, 0, 0};
   w.tiles = BM == kBM ? tiles_of(a, w.q) : (w.q.n > 0 ? 1 : 0);
   w.n = 1;
+  w.piece = a.cap;
   w.base = 0;
-  w.chunk = a.chunk;
   if (a.slots == 0) return w;
-  const float tiles = (float)w.tiles;
+  const float tiles = (float)w.tiles, len = (float)w.q.len;
+  const float all = wave_sum(tiles);
   float c = wave_sum(tiles * mean_keys(a, w.q)) / a.places;
-  if (wave_sum(tiles) >= a.places) {
+  if (all >= a.places) {
     c *= kLong;
   } else {
     for (int i = 0; i < 8; ++i) {
-      const float units = wave_sum(tiles * ceilf((float)w.q.len / fmaxf(c, 1.0f)));
+      const float units = wave_sum(tiles * ceilf(len * __builtin_amdgcn_rcpf(fmaxf(c, 1.0f))));
       if (units <= a.places) break;
-      c *= fmaxf(1.02f, units / a.places);
+      c *= fmaxf(1.02f, units * __builtin_amdgcn_rcpf(a.places));
     }
   }
-  w.chunk = __builtin_amdgcn_readfirstlane(max(a.least, (int)fminf(c + 1.0f, (float)a.cap)));
-  w.n = splits_for(w.q.len, w.chunk);
+  c = fmaxf(c, (float)a.least);
+  const float n = fmaxf(1.0f, ceilf(len * __builtin_amdgcn_rcpf(c)));
   // As many slots as the host counted on, or no splits.
-  const float mine = w.n > 1 ? tiles * (float)w.n : 0.0f;
-  if (!(wave_sum(mine) <= (float)a.slots)) {
-    w.n = 1;
-    w.chunk = a.chunk;
-    return w;
-  }
+  const float mine = n > 1.0f ? tiles * n : 0.0f;
+  if (!(wave_sum(mine) <= (float)a.slots)) return w;
+  w.n = (int)n;
+  // n of them hold the sequence: what the quotient is off by is less than the margin.
+  if (n > 1.0f)
+    w.piece = ((int)(len * __builtin_amdgcn_rcpf(n)) + 2 + (w.q.len >> 20) + 63) / 64 * 64;
   w.base = lanes_below((int)mine);
   return w;
 }
 
 // A tile of rows (n group to a sequence: of kBM, or the one that has all 32) and a
-// split of its keys.
+// split of its keys; `slot` is its first split's.
 struct Unit {
   Seq seq;
-  int b, index, split;
-  int slots, base;  // the sequence's, as in Work
+  int b, index, split, piece, slot;
 };
-
-// Unit t, wave-uniform; false where there is none.
 __device__ __forceinline__ bool unit_at(const Work &w, int first, int count, int k, Unit &u) {
   const uint64_t hit = __ballot(k >= first && k < first + count);
   if (!hit) return false;
   u.b = __builtin_ctzll(hit);
   u.seq = lane_seq(w.q, u.b);
+  u.piece = __builtin_amdgcn_readlane(w.piece, u.b);
   u.split = k - __builtin_amdgcn_readlane(first, u.b);
-  u.slots = __builtin_amdgcn_readlane(w.n, u.b);
-  u.base = __builtin_amdgcn_readlane(w.base, u.b);
   return true;
 }
+// Unit t, wave-uniform; false where there is none.
+//
 // One tile to a sequence, and splits of like size: one behind the other.
 __device__ __forceinline__ bool find_split(const Work &w, int t, Unit &u) {
   const int n = w.tiles * w.n;
+  if (!unit_at(w, lanes_below(n), n, t, u)) return false;
   u.index = 0;
-  return unit_at(w, lanes_below(n), n, t, u);
+  u.slot = __builtin_amdgcn_readlane(w.base, u.b);
+  return true;
 }
-// In the order of falling work, so that what runs last is short.  A sequence's tiles, the last first, see falling
-// numbers of keys, one tile's tokens less each; counted in such steps from the
-// longest sequence's end (a split's share of it) tile j of b lies at d(b) + j.  With
-// S(x) = sum over sequences of the units below x, the unit's place is the largest x
-// with S(x) <= t, found bit by bit.
+// In the order of falling work, so that what runs last is short.  A sequence's tiles,
+// the last first, see falling numbers of keys, one tile's tokens less each; counted in
+// such steps from the longest piece's end tile j of b lies at d(b) + j.  With S(x) =
+// sum over sequences of the units below x, the unit's place is the largest x with
+// S(x) <= t, found bit by bit.
 __device__ __forceinline__ bool find_unit(const PagedArgs &a, const Work &w, int t, Unit &u) {
-  const int len = w.q.len / w.n, longest = wave_max_int(w.tiles > 0 ? len : 0);
-  const int d = (int)min((int64_t)(longest - min(len, longest)) * a.group / kBM, (int64_t)1 << 24);
+  const int len = min(w.piece, w.q.len), longest = wave_max_int(w.tiles > 0 ? len : 0);
+  const int d = (int)fminf((float)(longest - min(len, longest)) * (float)a.group.d * (1.0f / kBM), 1e7f);
   auto below = [&](int x) __attribute__((always_inline)) {
     return wave_sum_int(w.n * min(max(x - d, 0), w.tiles));
   };
-  if (wave_sum_int(w.n * w.tiles) <= t) return false;
-  int x = 0, bit = 1;
-  while (bit < (1 << 26) && below(bit) <= t) bit <<= 1;
-  for (bit >>= 1; bit > 0; bit >>= 1)
-    if (below(x + bit) <= t) x += bit;
-  const int k = t - below(x);  // among the units at x
+  int x = 0;
+  if (a.B > 1) {
+    int bit = 1;
+    while (bit < (1 << 26) && below(bit) <= t) bit <<= 1;
+    for (bit >>= 1; bit > 0; bit >>= 1)
+      if (below(x + bit) <= t) x += bit;
+    t -= below(x);  // among the units at x
+  } else {
+    // One sequence: (its n, of lane 0; at most 2^26 units).
+    const int n = __builtin_amdgcn_readlane(w.n, 0);
+    if (n > 1) x = (int)(((double)t + 0.5) / (double)n);
+    else x = t;
+    t -= x * n;
+  }
   const int here = x >= d && x - d < w.tiles ? w.n : 0;
-  if (!unit_at(w, lanes_below(here), here, k, u)) return false;
-  u.index = __builtin_amdgcn_readlane(w.tiles - 1 - (x - d), u.b);
+  if (!unit_at(w, lanes_below(here), here, t, u)) return false;
+  const int index = w.tiles - 1 - (x - d);
+  u.index = __builtin_amdgcn_readlane(index, u.b);
+  u.slot = __builtin_amdgcn_readlane(w.base + index * w.n, u.b);
   return true;
 }
 
-// More than 64 sequences: the tiles by find_tile's numbering and search, at most
-// a.splits splits.
+// More than 64 sequences: tile t by find_tile's numbering and search, from its end.
 __device__ __forceinline__ bool find_tile_of_many(const PagedArgs &a, int t, Unit &u) {
-  const int lane = threadIdx.x & 63;
-  t = a.T * a.group / kBM + a.B - 1 - t;
+  const int lane = threadIdx.x & 63, group = (int)a.group.d;
   int lo = 0, n = a.B;
   for (;;) {
     const int step = (n + 63) / 64, i = lo + lane * step;
-    const bool at = lane * step < n && min(max(a.off[i], 0), a.T) * a.group / kBM + i <= t;
+    const bool at = lane * step < n && min(max(a.off[i], 0), a.T) * group / kBM + i <= t;
     const int c = __builtin_popcountll(__ballot(at));
     if (c == 0) return false;
     lo += (c - 1) * step;
@@ -223,11 +246,13 @@ __device__ __forceinline__ bool find_tile_of_many(const PagedArgs &a, int t, Uni
   }
   u.b = __builtin_amdgcn_readfirstlane(lo);
   u.seq = seq_of(a, u.b);
-  u.index = __builtin_amdgcn_readfirstlane(t - (u.seq.s * a.group / kBM + u.b));
+  u.index = __builtin_amdgcn_readfirstlane(t - (u.seq.s * group / kBM + u.b));
+  u.slot = t * a.splits;
   return u.index >= 0 && u.index < tiles_of(a, u.seq);
 }
-constexpr int kSummed = 4096;  // sequences; more are not looked at
-__device__ __forceinline__ int chunk_of_many(const PagedArgs &a) {
+// Their pieces: at most a.splits of them, from the lengths of up to kSummed sequences.
+constexpr int kSummed = 4096;
+__device__ __forceinline__ int piece_of_many(const PagedArgs &a) {
   if (a.splits == 1 || a.B > kSummed) return a.chunk;
   float tiles = 0.0f, keys = 0.0f;
   for (int b = threadIdx.x & 63; b < a.B; b += 64) {
@@ -236,12 +261,20 @@ __device__ __forceinline__ int chunk_of_many(const PagedArgs &a) {
     keys += (float)tiles_of(a, q) * mean_keys(a, q);
   }
   const float c = wave_sum(keys) / a.places * (wave_sum(tiles) >= a.places ? kLong : 1.25f);
-  return __builtin_amdgcn_readfirstlane(max(a.chunk, (int)fminf(c, (float)a.cap)));
+  return __builtin_amdgcn_readfirstlane(max(a.chunk, ((int)fminf(c, (float)a.cap) + 63) / 64 * 64));
+}
+
+// A tile's sums of one split as its waves hold them: [4 waves][32-column blocks][4][64
+// lanes] of four values, the registers 4 g .. 4 g + 3 of a block, then m c and l of
+// [4 waves][32 rows].
+template <int DP>
+__device__ __forceinline__ float *sums_at(const PagedArgs &a, int kh, int slot) {
+  return a.partial + ((int64_t)kh * a.slots + slot) * (kBM * (DP + 2));
 }
 
 // NW waves of 32 rows each.  WHOLE: a load's rows lie in one page.
 template <int DT, int DP, int NW, bool WHOLE>
-__global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 1 && !WHOLE ? 1 : 2) void attention_paged_kernel(PagedArgs a) {
   constexpr int CH = kPitch<DP>, BN = NW == 1 ? 32 : 64, kTile = BN * CH * 16;
   constexpr int kRows = 64 / CH;               // rows of one DMA instruction
   constexpr int kN = BN / kRows / NW;          // instructions of a wave and tile
@@ -251,45 +284,45 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a
   const int lane = threadIdx.x & 63;
   const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   static_assert(NW == 1 || 32 * NW == kBM, "rows of a tile");
-  int kh, chunk = a.chunk;
+  const int group = (int)a.group.d;
+  int kh;
   Unit u;
-  if (a.slots || (NW > 1 && a.B <= 64)) {
-    int unit;
-    unit_of(blockIdx.x, a.kv_heads, a.tiles, true, kh, unit);
-    const Work w = work_of(a, 32 * NW);
-    if (!(NW == 1 ? find_split(w, unit, u) : find_unit(a, w, unit, u))) return;
-    chunk = w.chunk;
-  } else if constexpr (NW == 1) {
+  if (NW == 1 && !a.slots) {
     kh = blockIdx.x;
     u.b = blockIdx.y;
     u.split = blockIdx.z;
     u.seq = seq_of(a, u.b);
-    u.index = 0;
+    u.index = u.slot = 0;
+    u.piece = a.chunk;
   } else {
-    int tile;
-    unit_of(blockIdx.x, a.kv_heads, a.tiles, true, kh, tile);
-    u.split = a.splits - 1 - blockIdx.y;  // first splits last: others are long tiles'
-    if (!find_tile_of_many(a, tile, u)) return;
-    chunk = chunk_of_many(a);
+    int unit;
+    unit_of(blockIdx.x, a.kv_heads, a.tiles, true, kh, unit);
+    if (NW == 1 || a.B <= 64) {
+      const Work w = work_of(a, 32 * NW);
+      if (!(NW == 1 ? find_split(w, unit, u) : find_unit(a, w, unit, u))) return;
+    } else {
+      if (!find_tile_of_many(a, a.tiles - 1 - unit, u)) return;
+      u.split = a.splits - 1 - blockIdx.y;  // first splits last: others are long tiles'
+      u.piece = piece_of_many(a);
+    }
   }
   const Seq seq = u.seq;
   const int b = u.b, split = u.split;
-  const int row0 = u.index * 32 * NW, R = NW == 1 ? min(seq.n, 32 / a.group) * a.group : seq.n * a.group;
+  const int row0 = u.index * 32 * NW, R = NW == 1 ? min(seq.n, 32 / group) * group : seq.n * group;
   if (R <= row0) return;
-  const int vis = seq.seen((min(row0 + 32 * NW, R) - 1) / a.group, a.causal);
-  const int ns = splits_for(vis, chunk), piece = NW == 1 && !a.slots ? chunk : piece_of(vis, ns);
-  const int from = split * piece, to = min(vis, from + piece);
-  if (split > 0 && (split >= ns || from >= vis)) return;
-  const bool direct = ns <= 1;
+  const int vis = seq.seen(a.group.of(min(row0 + 32 * NW, R) - 1), a.causal);
+  const int from = split * u.piece, to = min(vis, from + u.piece);
+  if (split > 0 && from >= vis) return;
+  const bool direct = vis <= u.piece;
 
   const int q0 = row0 + 32 * wave, qn = min(32, R - q0);  // this wave's rows, maybe none
-  const int row = min(q0 + (lane & 31), R - 1), token = row / a.group;
-  const int head = kh * a.group + row - token * a.group;
+  const int row = min(q0 + (lane & 31), R - 1), token = a.group.of(row);
+  const int head = kh * group + row - token * group;
   const bool mine = (lane & 31) < qn;
   const int end = mine ? min(to, seq.seen(token, a.causal)) : 0;  // the keys this lane's row sees
   // ... and those that the wave's first and last rows see.
-  const int least = qn > 0 ? min(to, seq.seen(q0 / a.group, a.causal)) : 0;
-  const int most = qn > 0 ? min(to, seq.seen((q0 + qn - 1) / a.group, a.causal)) : 0;
+  const int least = __builtin_amdgcn_readlane(end, 0);
+  const int most = __builtin_amdgcn_readlane(end, max(qn, 1) - 1);
   u32x4 qf[DP / 16];
   {
     const uint16_t *p = a.q + (seq.s + token) * a.sq.t + head * a.sq.h;
@@ -475,12 +508,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a
   }
   l = both_sum(l);
   if (qn <= 0) return;
-  int64_t at_row = ((int64_t)(seq.s + token) * a.heads + head) * a.splits + split;
-  if (a.slots)
-    at_row = ((int64_t)kh * a.slots + u.base + u.index * u.slots + split) * (32 * NW) + (row - row0);
-  if (a.rows && split == 0 && lane < qn)
+  if (NW == 1 && a.rows && split == 0 && lane < qn)
     a.rows[(int64_t)(seq.s + token) * a.heads + head] =
-        int2{direct ? 0 : (vis - 1) / piece + 1, (int)at_row};
+        int2{direct ? 0 : (vis - 1) / u.piece + 1, (kh * a.slots + u.slot) * 32 + lane};
   if (direct) {
     // A row that sees no key is zero, its lse -inf.
     store_row<DT, DP>(acc, l == 0.0f ? 0.0f : 1.0f / l,
@@ -490,22 +520,124 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a
           l == 0.0f ? -INFINITY : (mc + (__log2f(l) - kUp<DT>)) * kLn2;
     return;
   }
-  if (!mine) return;
-  float *p = a.partial + at_row * (a.D + 2);
+  if constexpr (NW > 1) {
+    float *const p = sums_at<DP>(a, kh, u.slot + split);
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      const int d = 32 * db + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-      if (d < a.D) *reinterpret_cast<float2 *>(p + d) = float2{acc[db][r], acc[db][r + 1]};
-    }
-  if (lane < 32) *reinterpret_cast<float2 *>(p + a.D) = float2{mc, l};
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<gemm::f32x4 *>(p + ((wave * (DP / 32) + db) * 4 + g) * 256 + lane * 4) =
+            gemm::f32x4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+    if (lane < 32)
+      *reinterpret_cast<float2 *>(p + kBM * DP + (wave * 32 + lane) * 2) = float2{mc, l};
+  } else {
+    if (!mine) return;
+    const int64_t at = a.slots ? (int64_t)(kh * a.slots + u.slot + split) * 32 + row
+                               : ((int64_t)(seq.s + token) * a.heads + head) * a.splits + split;
+    float *const p = a.partial + at * (a.D + 2);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const int d = 32 * db + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+        if (d < a.D) *reinterpret_cast<float2 *>(p + d) = float2{acc[db][r], acc[db][r + 1]};
+      }
+    if (lane < 32) *reinterpret_cast<float2 *>(p + a.D) = float2{mc, l};
+  }
 }
 
-// Whether a token's rows are in a tile of its sequence (of 32 rows: the first ones).
-// By a whole wave.
-__device__ __forceinline__ bool in_tile(const PagedArgs &a, int BM, int t) {
-  const int lane = threadIdx.x & 63, most = BM == kBM ? a.T : 32 / a.group;
+// Chunks: the sums of a tile's splits.  A workgroup per tile that has any and 32
+// columns, in GROUPS groups of four waves that read what the tile's waves wrote, whole
+// lines of it: group g takes splits g, g + GROUPS, ..., each to the largest maximum so
+// far, and the groups join in order.
+template <int DT, int DP, int GROUPS>
+__global__ __launch_bounds__(2 * kBM * GROUPS) void paged_join_tile_kernel(PagedArgs a) {
+  __shared__ float box[GROUPS > 1 ? GROUPS - 1 : 1][4][18][GROUPS > 1 ? 64 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int kh = blockIdx.x, db = blockIdx.z, group = (int)a.group.d;
+  Unit u;
+  if (a.B <= 64) {
+    const Work w = work_of(a, kBM);
+    const int tiles = w.n > 1 ? w.tiles : 0;
+    if (!unit_at(w, lanes_below(tiles), tiles, blockIdx.y, u)) return;
+    u.index = u.split;
+    u.slot = __builtin_amdgcn_readlane(w.base + u.index * w.n, u.b);
+  } else {
+    if (!find_tile_of_many(a, blockIdx.y, u)) return;
+    u.piece = piece_of_many(a);
+  }
+  const Seq seq = u.seq;
+  const int row0 = u.index * kBM, R = seq.n * group;
+  const int vis = seq.seen(a.group.of(min(row0 + kBM, R) - 1), a.causal);
+  if (vis <= u.piece) return;
+  const int q0 = row0 + 32 * wave, qn = min(32, R - q0);
+  const float *const p = sums_at<DP>(a, kh, u.slot);
+  const float *const px = p + (wave * (DP / 32) + db) * 1024 + lane * 4;
+  const float *const pm = p + kBM * DP + (wave * 32 + (lane & 31)) * 2;
+  f32x16 acc[1] = {};
+  float mx = -INFINITY, sum = 0.0f;
+  // A further split's sums, or another group's.
+  auto add = [&](float m, float l, auto value) __attribute__((always_inline)) {
+    const float to = fmaxf(mx, m);
+    const float old = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mx - to);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+    mx = to;
+    sum = __builtin_fmaf(l, f, sum * old);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[0][r] = __builtin_fmaf(value(r), f, acc[0][r] * old);
+  };
+  constexpr int kAhead = 4;  // splits whose loads are on their way together
+  const int n = qn > 0 ? (vis - 1) / u.piece + 1 : 0;
+  for (int s0 = part; s0 < n; s0 += kAhead * GROUPS) {
+    gemm::f32x4 x[kAhead][4];
+    float2 ml[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const int64_t at = (int64_t)min(s0 + s * GROUPS, n - 1) * (kBM * (DP + 2));
+      ml[s] = *reinterpret_cast<const float2 *>(pm + at);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x[s][g] = *reinterpret_cast<const gemm::f32x4 *>(px + at + g * 256);
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      // (With a branch around the rest the compiler moves the loads into it.)
+      const bool there = s0 + s * GROUPS < n;
+      add(there ? ml[s].x : -INFINITY, there ? ml[s].y : 0.0f,
+          [&](int r) { return there ? x[s][r >> 2][r & 3] : 0.0f; });
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    if (part) {
+      float(*const mine)[64] = box[part - 1][wave];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[r][lane] = acc[0][r];
+      mine[16][lane] = mx;
+      mine[17][lane] = sum;
+    }
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int g = 0; g < GROUPS - 1; ++g) {
+      const float(*const other)[64] = box[g][wave];
+      add(other[16][lane], other[17][lane], [&](int r) { return other[r][lane]; });
+    }
+  }
+  if (qn <= 0) return;
+  const int row = min(q0 + (lane & 31), R - 1), token = a.group.of(row);
+  const int head = kh * group + row - token * group;
+  store_row<DT, 32>(acc, sum == 0.0f ? 0.0f : 1.0f / sum,
+                    a.o + (seq.s + token) * a.so.t + head * a.so.h + 32 * db, (lane & 31) < qn,
+                    a.D - 32 * db, lane);
+  if (a.lse && db == 0 && lane < qn)
+    a.lse[head * a.slse + seq.s + token] =
+        sum == 0.0f ? -INFINITY : (mx + (__log2f(sum) - kUp<DT>)) * kLn2;
+}
+
+// Whether a token is among the first of its sequence, which a tile of 32 rows has.  By
+// a whole wave.
+__device__ __forceinline__ bool in_tile(const PagedArgs &a, int t) {
+  const int lane = threadIdx.x & 63, most = 32 / (int)a.group.d;
   if (a.B <= 64) {
     const int s = lane < a.B ? max(a.off[lane], 0) : a.T;
     return __ballot(s <= t && t < a.off[min(lane, a.B - 1) + 1] && t - s < most) != 0;
@@ -533,16 +665,13 @@ struct Sums {
   int n;
   const float *p;
 };
-__device__ __forceinline__ int64_t sums_step(const PagedArgs &a, int BM) {
-  return (a.slots ? BM : 1) * (int64_t)(a.D + 2);
-}
-__device__ __forceinline__ Sums sums_of(const PagedArgs &a, int BM, int t, int head) {
+__device__ __forceinline__ Sums sums_of(const PagedArgs &a, int t, int head) {
   const int2 r = a.rows[(int64_t)t * a.heads + head];
   if (!a.slots)
     return {min(max(r.x, 0), a.splits),
             a.partial + ((int64_t)t * a.heads + head) * a.splits * (a.D + 2)};
-  const int all = a.kv_heads * a.slots * BM, at = min(max(r.y, 0), all - 1);
-  return {min(max(r.x, 0), (all - 1 - at) / BM + 1), a.partial + (int64_t)at * (a.D + 2)};
+  const int all = a.kv_heads * a.slots * 32, at = min(max(r.y, 0), all - 1);
+  return {min(max(r.x, 0), (all - 1 - at) / 32 + 1), a.partial + (int64_t)at * (a.D + 2)};
 }
 
 // The sums of splits first, first + STEP, ... of a row (p: split 0's, `step` from one
@@ -593,16 +722,16 @@ __device__ __forceinline__ void store_joined(const PagedArgs &a, int t, int head
     a.lse[head * a.slse + t] = j.sum == 0.0f ? -INFINITY : (j.mx + (__log2f(j.sum) - kUp<DT>)) * kLn2;
 }
 
-// Few rows: one workgroup per (token, head), its waves take every fourth split and
-// join in order.
+// Up to 32 rows of a sequence: one workgroup per (token, head), its waves take every
+// fourth split and join in order.
 template <int DT>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int BM) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
   __shared__ float smax[4], ssum[4], sx[4][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = blockIdx.x / a.heads, head = blockIdx.x - t * a.heads;
-  const Sums s = sums_of(a, BM, t, head);
-  if (!in_tile(a, BM, t) || s.n == 0) return;
-  Joined j = join<4>(a, s.p, sums_step(a, BM), wave, s.n);
+  const Sums s = sums_of(a, t, head);
+  if (!in_tile(a, t) || s.n == 0) return;
+  Joined j = join<4>(a, s.p, (a.slots ? 32 : 1) * (int64_t)(a.D + 2), wave, s.n);
   sx[wave][2 * lane] = j.x0;
   sx[wave][2 * lane + 1] = j.x1;
   if (lane == 0) {
@@ -622,69 +751,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int BM) {
   store_joined<DT>(a, t, head, lane, j);
 }
 
-// Many rows: a workgroup per token and `per` heads.  A wave takes eight rows at a
-// time, so that their loads are on their way together: lane 8 r + i has row r's split
-// i.  Rows of more than eight splits, of which there are few, one by one.
-template <int DT>
-__global__ __launch_bounds__(256) void paged_join_rows_kernel(PagedArgs a, int per) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x;
-  const int64_t step = sums_step(a, kBM);
-  const int end = min(a.heads, ((int)blockIdx.y + 1) * per);
-  for (int h0 = blockIdx.y * per + 8 * wave; h0 < end; h0 += 8 * (blockDim.x >> 6)) {
-    const int rows = min(8, end - h0), r = lane >> 3, i = lane & 7;
-    const Sums s = sums_of(a, kBM, t, h0 + min(r, rows - 1));
-    if (!in_tile(a, kBM, t)) return;
-    const int n = r < rows ? s.n : 0;
-    auto row_of = [&](int q) __attribute__((always_inline)) {
-      const uint64_t p = reinterpret_cast<uint64_t>(s.p);
-      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)p, 8 * q);
-      const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), 8 * q);
-      return reinterpret_cast<const float *>(hi << 32 | lo);
-    };
-    if (__ballot(n > 8)) {
-      for (int k = 0; k < rows; ++k) {
-        const int nk = __builtin_amdgcn_readlane(n, 8 * k);
-        if (nk) store_joined<DT>(a, t, h0 + k, lane, join<1>(a, row_of(k), step, 0, nk));
-      }
-      continue;
-    }
-    const int most = wave_max_int(n), d = min(2 * lane, a.D - 2);
-    if (most == 0) continue;
-    float2 ml = {-INFINITY, 0.0f};
-    if (i < n) ml = *reinterpret_cast<const float2 *>(s.p + i * step + a.D);
-    float mx = ml.x;
-    mx = fmaxf(mx, dpp_mov<0xB1>(mx));   // quad_perm [1,0,3,2]
-    mx = fmaxf(mx, dpp_mov<0x4E>(mx));   // quad_perm [2,3,0,1]
-    mx = fmaxf(mx, dpp_mov<0x141>(mx));  // row_half_mirror
-    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mx);
-    float sum = ml.y * f;
-    sum += dpp_mov<0xB1>(sum);
-    sum += dpp_mov<0x4E>(sum);
-    sum += dpp_mov<0x141>(sum);
-    float x0[8] = {}, x1[8] = {};
-    for (int k = 0; k < most; ++k) {
-      float2 x[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q)  // (a row without the split: its first one's values, unused)
-        x[q] = *reinterpret_cast<const float2 *>(
-            row_of(q) + (k < __builtin_amdgcn_readlane(n, 8 * q) ? k : 0) * step + d);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const bool there = k < __builtin_amdgcn_readlane(n, 8 * q);
-        const float g = lane_value(f, 8 * q + k);
-        x0[q] = there ? __builtin_fmaf(x[q].x, g, x0[q]) : x0[q];
-        x1[q] = there ? __builtin_fmaf(x[q].y, g, x1[q]) : x1[q];
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      if (__builtin_amdgcn_readlane(n, 8 * q))
-        store_joined<DT>(a, t, h0 + q, lane,
-                         {lane_value(mx, 8 * q), lane_value(sum, 8 * q), x0[q], x1[q]});
-  }
-}
-
 template <int DT, int DP, bool WHOLE>
 void launch_paged_t(const PagedArgs &a, bool narrow, hipStream_t s) {
   const unsigned units = (unsigned)(a.tiles * a.kv_heads);
@@ -695,36 +761,37 @@ void launch_paged_t(const PagedArgs &a, bool narrow, hipStream_t s) {
         0, s, a);
   else
     hipLaunchKernelGGL((attention_paged_kernel<DT, DP, 4, WHOLE>),
-                       dim3(units, a.slots ? 1u : (unsigned)a.splits), dim3(256), 0, s, a);
+                       dim3(units, a.B <= 64 ? 1u : (unsigned)a.splits), dim3(256), 0, s, a);
 }
 template <int DT, int DP>
-void launch_paged_t(const PagedArgs &a, bool narrow, hipStream_t s) {
+int32_t launch_paged_d(const PagedArgs &a, bool narrow, hipStream_t s) {
   // A load is of 8 rows up to D = 64, of 4 beyond.
   if (a.page % (64 / kPitch<DP>) == 0) launch_paged_t<DT, DP, true>(a, narrow, s);
   else launch_paged_t<DT, DP, false>(a, narrow, s);
-}
-template <int DT>
-int32_t launch_paged(const PagedArgs &a, bool narrow, hipStream_t s) {
-  if (a.D <= 32) launch_paged_t<DT, 32>(a, narrow, s);
-  else if (a.D <= 64) launch_paged_t<DT, 64>(a, narrow, s);
-  else if (a.D <= 96) launch_paged_t<DT, 96>(a, narrow, s);
-  else launch_paged_t<DT, 128>(a, narrow, s);
   const int32_t rc = check_hip(hipGetLastError(), "paged_attention launch");
-  if (rc || (a.splits <= 1 && a.slots == 0)) return rc;
-  if (a.T * a.heads <= 4096 || narrow) {
-    hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((unsigned)(a.T * a.heads)), dim3(256), 0, s, a,
-                       narrow ? 32 : attn::kBM);
-  } else {
-    const int per = 32, waves = std::min(4, (a.heads + 7) / 8);
-    hipLaunchKernelGGL(paged_join_rows_kernel<DT>, dim3((unsigned)a.T, (unsigned)((a.heads + per - 1) / per)),
-                       dim3(64 * waves), 0, s, a, per);
+  if (rc || !a.partial) return rc;
+  if (narrow)
+    hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((unsigned)(a.T * a.heads)), dim3(256), 0, s, a);
+  else {
+    // Groups where tiles are so few that they may have eight splits and more.
+    const dim3 grid((unsigned)a.kv_heads, (unsigned)a.split_tiles, DP / 32);
+    if (a.split_tiles * 8 <= a.places)
+      hipLaunchKernelGGL((paged_join_tile_kernel<DT, DP, 4>), grid, dim3(8 * kBM), 0, s, a);
+    else
+      hipLaunchKernelGGL((paged_join_tile_kernel<DT, DP, 1>), grid, dim3(2 * kBM), 0, s, a);
   }
   return check_hip(hipGetLastError(), "paged_attention join launch");
 }
+template <int DT>
+int32_t launch_paged(const PagedArgs &a, bool narrow, hipStream_t s) {
+  if (a.D <= 32) return launch_paged_d<DT, 32>(a, narrow, s);
+  if (a.D <= 64) return launch_paged_d<DT, 64>(a, narrow, s);
+  if (a.D <= 96) return launch_paged_d<DT, 96>(a, narrow, s);
+  return launch_paged_d<DT, 128>(a, narrow, s);
+}
 
-
-// The form of a call, its tiles of rows (units with their splits where there are
-// slots for these) per key head, its splits and slots.
+// The form of a call, its tiles of rows per key head (up to 64 sequences: with their
+// splits), its splits and slots.
 struct Plan {
   bool narrow;
   int64_t tiles, chunk, splits, slots, least, places;
@@ -735,34 +802,34 @@ Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D, i
   const int64_t group = heads / kv_heads;
   p.narrow = max_queries * group <= 32 && B <= 0xffff;
   p.chunk = std::max<int64_t>(rows, 1);
-  // Workgroups resident at once, by LDS (a wave's 32 or 16 KB) and registers.
+  // Workgroups resident at once, by LDS (a wave's 32 or 16 KB) and registers; single
+  // tokens: as many as it takes to fill the memory's pipes.
   p.places = p.narrow ? (D <= 64 ? 1536 : 768) : (D <= 64 ? 768 : 512);
   p.least = p.narrow ? 64 : 256;
   const int64_t most = (rows + p.least - 1) / p.least, mine = (p.places + kv_heads - 1) / kv_heads;
-  if (p.narrow) {
-    p.tiles = std::min(B, T);
-    if (B <= 64 && B * kv_heads * most > p.places) {
-      p.slots = std::min(B * most, B < mine ? mine : 2 * mine);
-    } else {
-      // As for the padded cache (attention_decode.hip).
-      const int64_t all = B * rows * kv_heads;
-      const int64_t keys =
-          std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
-      p.chunk = std::max<int64_t>(64, (std::max(keys, rows / 32768) + 63) / 64 * 64);
-    }
+  // Work::n: fewer tiles than places have as many units as places at most; with more
+  // tiles, those that are split have less than 4 / kLong units to a place.
+  auto room = [&](int64_t tiles) { return std::min(tiles * most, tiles < mine ? mine : 2 * mine); };
+  if (p.narrow && B <= 64 && B * kv_heads * most > p.places) {
+    p.slots = room(B);
+    p.tiles = B + p.slots;
+  } else if (p.narrow) {
+    // As for the padded cache (attention_decode.hip).
+    const int64_t all = B * rows * kv_heads;
+    const int64_t keys = std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
+    p.chunk = std::max<int64_t>(64, (std::max(keys, rows / 32768) + 63) / 64 * 64);
   } else if (B <= 64) {
     p.tiles = std::min(T * group, T * group / kBM + B);
-    // Work::n: fewer tiles than places have as many units as places at most; with more
-    // tiles, those that are split have less than 4 / kLong units to a place.
-    if (most > 1) p.slots = std::min(p.tiles * most, p.tiles < mine ? mine : 2 * mine);
+    if (most > 1) p.slots = room(p.tiles);
+    p.tiles += p.slots;
   } else {
     p.tiles = T * group / kBM + B;
     const int64_t splits =
         std::max<int64_t>(1, std::min(3 * p.places / (2 * p.tiles * kv_heads), rows / 512));
     p.chunk = std::max<int64_t>(64, ((rows + splits - 1) / splits + 63) / 64 * 64);
   }
-  p.tiles += p.slots;
   p.splits = std::max<int64_t>(1, (rows + p.chunk - 1) / p.chunk);
+  if (!p.narrow && p.splits > 1) p.slots = p.tiles * p.splits;
   return p;
 }
 
@@ -772,10 +839,9 @@ Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D, i
 int64_t paged_attention_scratch(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
                                 int64_t rows, int64_t max_queries) {
   const attn::Plan p = attn::plan_of(T, B, heads, kv_heads, D, rows, max_queries);
-  const int64_t rows_of_sums = p.slots ? kv_heads * p.slots * (p.narrow ? 32 : attn::kBM)
-                               : p.splits > 1 ? T * heads * p.splits
-                                              : 0;
-  return rows_of_sums ? rows_of_sums * (D + 2) + 2 * T * heads : 0;
+  if (!p.narrow) return kv_heads * p.slots * attn::kBM * ((D + 31) / 32 * 32 + 2);
+  const int64_t sums = p.slots ? kv_heads * p.slots * 32 : p.splits > 1 ? T * heads * p.splits : 0;
+  return sums ? sums * (D + 2) + (2 * T * heads + 3) / 4 * 4 : 0;
 }
 
 int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
@@ -801,7 +867,7 @@ int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
   a.B = (int)c.B;
   a.heads = (int)p.heads;
   a.kv_heads = (int)c.kv_heads;
-  a.group = (int)(p.heads / c.kv_heads);
+  a.group = attn::Divider(p.heads / c.kv_heads);
   a.D = (int)c.D;
   a.page = (int)c.page;
   a.pages = (int)c.pages;
@@ -810,15 +876,15 @@ int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
   const attn::Plan plan = attn::plan_of(p.T, c.B, p.heads, c.kv_heads, c.D, a.cap, p.max_queries);
   // Rows are counted in 32 bits, a grid's dimension holds less than 2^32 threads.
   if (p.T * p.heads >= (1LL << 31) - (1 << 20) || plan.tiles * c.kv_heads >= 1 << 24 ||
-      ((plan.splits > 1 || plan.slots > 0) && p.T * ((p.heads + 31) / 32) >= 1 << 24) ||
       (plan.narrow && (plan.splits > 1 || plan.slots > 0) && p.T * p.heads >= 1 << 24))
     return fail(NOVA_HIP_ERANGE, "paged_attention: %lld tokens of %lld heads in %lld sequences",
                 (long long)p.T, (long long)p.heads, (long long)c.B);
   if (plan.splits > 1 || plan.slots) {
-    a.rows = reinterpret_cast<int2 *>(p.partial);
-    a.partial = p.partial + 2 * p.T * p.heads;
+    a.rows = plan.narrow ? reinterpret_cast<int2 *>(p.partial) : nullptr;
+    a.partial = p.partial + (plan.narrow ? (2 * p.T * p.heads + 3) / 4 * 4 : 0);
   }
   a.tiles = (int)plan.tiles;
+  a.split_tiles = (int)(c.B <= 64 ? std::min(plan.tiles - plan.slots, plan.slots / 2) : plan.tiles);
   a.splits = (int)plan.splits;
   a.chunk = (int)plan.chunk;
   a.c = p.scale * attn::kLog2e;

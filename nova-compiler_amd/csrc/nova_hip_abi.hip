@@ -1783,6 +1783,8 @@ int32_t _mlir_ciface_nova_hip_paged_attention(
                 (long long)p.heads, (long long)p.c.kv_heads);
   if (D % 8 || D > 128)
     return fail(NOVA_HIP_ERANGE, "%s: head dim %lld is not a multiple of 8 up to 128", w, (long long)D);
+  if (p.c.width * p.c.page > 1 << 30)
+    return fail(NOVA_HIP_ERANGE, "%s: more than 2^30 rows of a sequence", w);
   const int64_t wide = std::max(p.c.k.st, p.c.v.st);
   if (wide > kAttnMaxStride || wide * (p.c.page - 1) >= 1 << 30)
     return fail(NOVA_HIP_ERANGE, "%s: rows of a page 2^23, or its first and last 2^30, elements apart", w);
@@ -1806,8 +1808,8 @@ int32_t _mlir_ciface_nova_hip_paged_attention(
       return fail(NOVA_HIP_ESHAPE, "%s: scratch holds %lld floats, %lld are needed", w,
                   (long long)scratch->sizes[0], (long long)need);
     p.partial = out_f32(scratch);
-    if (reinterpret_cast<uintptr_t>(p.partial) & 7u)
-      return fail(NOVA_HIP_ESTRIDE, "%s: scratch must be 8-byte aligned", w);
+    if (reinterpret_cast<uintptr_t>(p.partial) & 15u)
+      return fail(NOVA_HIP_ESTRIDE, "%s: scratch must be 16-byte aligned", w);
   }
   const Extent xq = rows_extent("q", p.q, q, 2), y = rows_extent("out", p.o, out, 2),
                pk = pages_extent("k_pages", p.c.k, p.c), pv = pages_extent("v_pages", p.c.v, p.c),

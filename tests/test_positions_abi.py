@@ -202,12 +202,13 @@ def test_paged_scratch():
     assert f(0, 3, 4, 2, 64, 64, 1) == 0 and f(3, 3, 5, 2, 64, 64, 1) == 0 and f(3, 3, 4, 2, 64, -1, 1) == 0
     assert (f(3, 3, 4, 2, 64, 12800, 1) - 2 * 3 * 4) % 66 == 0        # sums, and two numbers to a row
     # Single tokens: room for what fills the chip, or splits that are a grid's dimension.
-    assert f(1, 1, 1, 1, 8, 2 ** 31 - 2 ** 20, 1) <= 2560 * 32 * 10 + 2
-    assert f(100, 100, 1, 1, 8, 2 ** 31 - 2 ** 20, 1) <= 100 * 32768 * 10 + 200
+    assert f(1, 1, 1, 1, 8, 2 ** 30, 1) <= 1536 * 32 * 10 + 4
+    assert f(100, 100, 1, 1, 8, 2 ** 30, 1) <= 100 * 32768 * 10 + 200
     # Chunks: room for what fills the chip twice, whatever the tokens and rows.
-    assert 0 < f(1 << 16, 4, 32, 8, 128, 131072, 1 << 16) <= 2 * 512 * 128 * 130 + 2 * 32 * (1 << 16)
+    assert 0 < f(1 << 16, 4, 32, 8, 128, 131072, 1 << 16) <= 2 * 512 * 128 * 130
     assert f(1 << 16, 4, 32, 8, 128, 256, 1 << 16) == 0                # one split
     assert f(1 << 16, 100, 32, 8, 128, 131072, 1 << 16) == 0           # many tiles of many sequences
+    assert att(table=at(6, (3, (1 << 26) + 1)), scratch=at(11, (1 << 33,))) == ERANGE
 
 
 def test_empty_calls_do_nothing():
