@@ -9,25 +9,28 @@
 // and backward, with g the gradient rotated back and t = g w:
 //   dx = r (t - x r^2 mean(t x)),   dw = sum over rows of g x r.
 //
-// All of it is bound by HBM: a row is read and written once.  A row belongs to
-// L = 1 .. 32 neighbouring lanes, each with a "slot" of two 16-byte chunks that
-// hold whole pairs, so that the rotation needs no exchange between lanes and the
-// norm log2 L of them.  A workgroup takes a few tokens with all their heads and
-// works out their sines and cosines once, into LDS: angles are taken in 64 bits
-// (in 32 an angle of 10^5 is off by 4e-3) and only their fraction of a turn is
-// rounded.
+// All of it is bound by HBM: a row is read and written once.  A workgroup takes one to
+// kMaxTB tokens with all their heads, issues the loads of its rows, works out the tokens'
+// sines and cosines meanwhile, once, into LDS, and ends: angles are taken in 64 bits (in
+// 32 an angle of 10^5 is off by 4e-3).  A row belongs to L = 1 .. 32 neighbouring lanes,
+// each with a "slot" of two 16-byte chunks that hold whole pairs, so that the rotation
+// needs no exchange between lanes and the norm log2 L of them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "gemm_common.h"
+#include "wave.h"
 
 namespace nova_hip {
 namespace pos {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTB = 8;  // tokens whose angles a workgroup holds at once
+// Rows of a lane whose loads are on their way together (append, cold, at 2 / 3: 41.2 / 46.2
+// us).  They and the stores are such that the caches keep nothing for: 33.4 against 36.6.
+constexpr int kAhead = 2;
 constexpr int kMaxPairs = kMaxHeadDim / 2;
 
 // One operand's rows and where they go (strides in bytes).
@@ -53,7 +56,7 @@ struct Args {
   const int *positions;
   const float *freqs;
   float scale, eps;
-  int T, D, R, TB, L, NS, heads, w_dt;  // heads: of all rows together
+  int T, D, R, TB, L, heads, w_dt;  // heads: of all rows together
   bool inverse;
 };
 
@@ -63,51 +66,36 @@ __device__ __forceinline__ float widen(uint32_t h) {
   else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
 
-// V values at p, 16 or 8 bytes.
+// V values, 16 or 8 bytes.
 template <int DT, int V>
-__device__ __forceinline__ void load(const char *p, float (&x)[V]) {
-  if constexpr (DT == NOVA_HIP_DT_F32) {
-    static_assert(V == 4, "16 bytes");
-    const gemm::f32x4 r = *reinterpret_cast<const gemm::f32x4 *>(p);
+struct Chunk {
+  typedef uint32_t raw __attribute__((ext_vector_type(DT == NOVA_HIP_DT_F32 ? V : V / 2)));
+  static __device__ __forceinline__ void widen_to(const raw &r, float (&x)[V]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = r[i];
-  } else {
-    uint32_t r[V / 2];
-    if constexpr (V == 8) {
-      const gemm::u32x4 v = *reinterpret_cast<const gemm::u32x4 *>(p);
+    for (int i = 0; i < V; ++i) {
+      if constexpr (DT == NOVA_HIP_DT_F32) x[i] = __uint_as_float(r[i]);
+      else x[i] = widen<DT>(i & 1 ? r[i / 2] >> 16 : r[i / 2] & 0xffffu);
+    }
+  }
+  static __device__ __forceinline__ void store(char *p, const float (&x)[V]) {
+    raw r;
+    if constexpr (DT == NOVA_HIP_DT_F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = v[i];
+      for (int i = 0; i < V; ++i) r[i] = __float_as_uint(x[i]);
     } else {
-      const gemm::u32x2 v = *reinterpret_cast<const gemm::u32x2 *>(p);
-      r[0] = v[0];
-      r[1] = v[1];
-    }
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      x[2 * i] = widen<DT>(r[i] & 0xffffu);
-      x[2 * i + 1] = widen<DT>(r[i] >> 16);
+      for (int i = 0; i < V / 2; ++i)
+        r[i] = DT == NOVA_HIP_DT_BF16 ? gemm::pack_bf16(x[2 * i], x[2 * i + 1])
+                                      : gemm::pack_f16(x[2 * i], x[2 * i + 1]);
     }
+    __builtin_nontemporal_store(r, reinterpret_cast<raw *>(p));
   }
-}
-template <int DT, int V>
-__device__ __forceinline__ void store(char *p, const float (&x)[V]) {
-  if constexpr (DT == NOVA_HIP_DT_F32) {
-    *reinterpret_cast<gemm::f32x4 *>(p) = gemm::f32x4{x[0], x[1], x[2], x[3]};
-  } else {
-    uint32_t r[V / 2];
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i)
-      r[i] = DT == NOVA_HIP_DT_BF16 ? gemm::pack_bf16(x[2 * i], x[2 * i + 1])
-                                    : gemm::pack_f16(x[2 * i], x[2 * i + 1]);
-    if constexpr (V == 8) *reinterpret_cast<gemm::u32x4 *>(p) = gemm::u32x4{r[0], r[1], r[2], r[3]};
-    else *reinterpret_cast<gemm::u32x2 *>(p) = gemm::u32x2{r[0], r[1]};
-  }
-}
+};
 
 // A lane's slot of a row: its two chunks of V values, in elements from the row's
-// start, and which of them are there and rotated.  Halves: chunk j < R / 2 V goes
-// with the chunk R / 2 values on; what is not rotated lies in pairs of neighbours,
-// as all chunks do when pairs are interleaved.
+// start, and which of them are there and rotated.  Halves: chunk j < R / 2 V goes with
+// the chunk R / 2 values on; what is left (all, when pairs are interleaved) lies in two
+// runs, so that neighbouring lanes load neighbouring chunks.
 struct Slot {
   int e[2];
   bool has[2], rot[2];
@@ -115,10 +103,11 @@ struct Slot {
 template <int V, bool INTER>
 __device__ __forceinline__ Slot slot_of(int j, int D, int R) {
   Slot s;
-  const int np = R / 2 / V;
-  const bool pair = !INTER && j < np;
-  s.e[0] = (pair ? j : 2 * j) * V;
-  s.e[1] = pair ? s.e[0] + R / 2 : s.e[0] + V;
+  const int np = INTER ? 0 : R / 2 / V, run = (D / V - 2 * np + 1) / 2;
+  const bool pair = j < np;
+  s.e[0] = (pair ? j : np + j) * V;
+  s.e[1] = pair ? s.e[0] + R / 2 : j - np < run ? s.e[0] + run * V : D;
+  if (!pair && j - np >= run) s.e[0] = D;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     s.has[i] = s.e[i] < D;
@@ -127,7 +116,7 @@ __device__ __forceinline__ Slot slot_of(int j, int D, int R) {
   return s;
 }
 
-// Sines and cosines of a token, times the scale: cs[i] and cs[kMaxPairs + i].
+// Cosine and sine of a token's angle, times the scale.
 __device__ __forceinline__ void angle(double position, float freq, float scale, bool inverse,
                                       float &c, float &s) {
   double turns = position * (double)freq * 0.15915494309189533577;
@@ -139,7 +128,33 @@ __device__ __forceinline__ void angle(double position, float freq, float scale, 
   s = (inverse ? -scale : scale) * __builtin_fmaf(cx, rest, sx);
 }
 
-// Rotates the slot's values by the token's table.
+// The angles of tokens 0 .. nt - 1 by a workgroup: cs[t][i] and cs[t][kMaxPairs + i].
+template <typename Position>
+__device__ __forceinline__ void angles(float (&cs)[kMaxTB][2 * kMaxPairs], int nt, int pairs,
+                                       const float *freqs, float scale, bool inverse,
+                                       Position position) {
+  for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
+    const int t = i / pairs, k = i - t * pairs;
+    float c, s;
+    angle(position(t), freqs[k], scale, inverse, c, s);
+    cs[t][k] = c;
+    cs[t][kMaxPairs + k] = s;
+  }
+}
+
+// V values of LDS, from a multiple of four.
+template <int V>
+__device__ __forceinline__ void load_floats(const float *p, float (&x)[V]) {
+  typedef float four __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i) {
+    const four v = *reinterpret_cast<const four *>(p + 4 * i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[4 * i + k] = v[k];
+  }
+}
+
+// Rotates the slot's values by the token's angles.
 template <int V, bool INTER>
 __device__ __forceinline__ void rotate(const Slot &sl, const float *cs, float (&x)[2][V]) {
   if constexpr (INTER) {
@@ -156,28 +171,42 @@ __device__ __forceinline__ void rotate(const Slot &sl, const float *cs, float (&
     }
   } else {
     if (!sl.rot[0]) return;
+    float c[V], s[V];
+    load_floats(cs + sl.e[0], c);
+    load_floats(cs + kMaxPairs + sl.e[0], s);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float c = cs[sl.e[0] + i], s = cs[kMaxPairs + sl.e[0] + i];
       const float a = x[0][i], b = x[1][i];
-      x[0][i] = a * c - b * s;
-      x[1][i] = b * c + a * s;
+      x[0][i] = a * c[i] - b * s[i];
+      x[1][i] = b * c[i] + a * s[i];
     }
   }
 }
 
-// Sum over the L lanes of a row (L a power of two up to 32).
-__device__ __forceinline__ float row_sum(float v, int L) {
-  for (int d = 1; d < L; d <<= 1) v += __shfl_xor(v, d);
-  return v;
-}
+// A lane group's rows among nt tokens of `heads` each: every groups-th, from its own.
+struct Walk {
+  int t, h, dt, dh;
+  __device__ __forceinline__ Walk(int group, int groups, int heads)
+      : t(group / heads), h(group - t * heads), dt(groups / heads), dh(groups - dt * heads) {}
+  __device__ __forceinline__ void next(int heads) {
+    t += dt;
+    h += dh;
+    if (h >= heads) {
+      h -= heads;
+      ++t;
+    }
+  }
+};
 
-template <int V>
-__device__ __forceinline__ void load_weight(const void *w, int dt, const Slot &sl, float (&x)[2][V]) {
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[k][i] = sl.has[k] ? gemm::bias_at(w, dt, sl.e[k] + i) : 0.0f;
+// Sum over the L lanes of a row (L a power of two up to 32): in quads, then with the
+// mirrored lane, all on DPP but the last.
+__device__ __forceinline__ float row_sum(float v, int L) {
+  if (L > 1) v += dpp_mov<0xB1>(v);   // quad_perm [1,0,3,2]
+  if (L > 2) v += dpp_mov<0x4E>(v);   // quad_perm [2,3,0,1]
+  if (L > 4) v += dpp_mov<0x141>(v);  // row_half_mirror
+  if (L > 8) v += dpp_mov<0x140>(v);  // row_mirror
+  if (L > 16) v += __shfl_xor(v, 16);
+  return v;
 }
 
 // Where a new token goes: its position and the byte offsets of its rows in the
@@ -224,100 +253,102 @@ __device__ __forceinline__ Place place_of(const Paged &p, int t, int T) {
 
 template <int DT, int V, bool INTER, bool NORM, bool PAGED>
 __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
-  __shared__ float cs[kMaxTB][2 * kMaxPairs];
+  __shared__ __attribute__((aligned(16))) float cs[kMaxTB][2 * kMaxPairs];
+  // Both weights: as registers they would cost more than the rows.
+  __shared__ __attribute__((aligned(16))) float weights[NORM ? 2 : 1][NORM ? kMaxHeadDim : 1];
   __shared__ Place place[PAGED ? kMaxTB : 1];
+  typedef Chunk<DT, V> C;
   constexpr int kSize = DT == NOVA_HIP_DT_F32 ? 4 : 2;
-  const int t0 = blockIdx.x * a.TB, nt = min(a.TB, a.T - t0), pairs = a.R / 2;
+  const int t0 = blockIdx.x * a.TB, nt = min(a.TB, a.T - t0);
+  const int j = threadIdx.x & (a.L - 1), groups = kThreads / a.L;
+  const Slot sl = slot_of<V, INTER>(j, a.D, a.R);
+  const float mean = 1.0f / (float)a.D;
+  // A row's operand (queries, keys, values one behind the other) and head in it.
+  auto part_of = [&](int h, int &head) __attribute__((always_inline)) {
+    const int h1 = a.rows[0].heads, h2 = h1 + a.rows[1].heads;
+    const int part = h < h1 ? 0 : h < h2 ? 1 : 2;
+    head = part == 0 ? h : part == 1 ? h - h1 : h - h2;
+    return part;
+  };
+  typename C::raw raw[kAhead][2] = {};
+  auto fetch = [&](Walk w) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u, w.next(a.heads)) {
+      if (w.t >= nt) continue;
+      int head;
+      const int part = part_of(w.h, head);
+      const Rows &r = part == 0 ? a.rows[0] : part == 1 ? a.rows[1] : a.rows[2];
+      const char *src = r.src + (t0 + w.t) * r.st + head * r.sh;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (sl.has[k])
+          raw[u][k] = __builtin_nontemporal_load(
+              reinterpret_cast<const typename C::raw *>(src + sl.e[k] * kSize));
+    }
+  };
+  Walk w(threadIdx.x / a.L, groups, a.heads);
+  fetch(w);
+  if constexpr (NORM) {
+    static_assert(kThreads == kMaxHeadDim, "a thread to a weight");
+    // (Zeros behind the row, where absent chunks point: only rows that no lane lacks reach 256.)
+    const bool in = (int)threadIdx.x < a.D;
+    weights[0][threadIdx.x] = in && a.rows[0].heads ? gemm::bias_at(a.rows[0].w, a.w_dt, threadIdx.x) : 0.0f;
+    weights[1][threadIdx.x] = in && a.rows[1].heads ? gemm::bias_at(a.rows[1].w, a.w_dt, threadIdx.x) : 0.0f;
+  }
   if constexpr (PAGED) {
-    for (int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < nt; t += kThreads / 64) {
+    for (int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < nt; t += kWaves) {
       const Place p = place_of(a.paged, t0 + t, a.T);
       if ((threadIdx.x & 63) == 0) place[t] = p;
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
-    const int t = i / pairs, k = i - t * pairs;
-    double at;
-    if constexpr (PAGED) at = (double)place[t].position;
-    else at = (double)a.positions[t0 + t];
-    float c, s;
-    angle(at, a.freqs[k], a.scale, a.inverse, c, s);
-    cs[t][k] = c;
-    cs[t][kMaxPairs + k] = s;
-  }
+  angles(cs, nt, a.R / 2, a.freqs, a.scale, a.inverse, [&](int t) {
+    if constexpr (PAGED) return (double)place[t].position;
+    else return (double)a.positions[t0 + t];
+  });
   __syncthreads();
-
-  const int j = threadIdx.x & (a.L - 1), group = threadIdx.x / a.L, groups = kThreads / a.L;
-  const Slot sl = slot_of<V, INTER>(j, a.D, a.R);
-  float w[2][2][V] = {};
-  if constexpr (NORM) {
+  while (__ballot(w.t < nt)) {  // (whole waves: the lanes of a row stay together)
+    Walk now = w;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (a.rows[i].heads) load_weight<V>(a.rows[i].w, a.w_dt, sl, w[i]);
-  }
-  const float mean = 1.0f / (float)a.D;
-  const int ht = groups / a.heads, hr = groups - ht * a.heads;
-  int t = group / a.heads, h = group - t * a.heads;
-  for (; t < nt;) {
-    int part = 0, head = h;
+    for (int u = 0; u < kAhead; ++u, now.next(a.heads)) {
+      if (u && !__ballot(now.t < nt)) break;
+      int head;
+      const int part = part_of(now.h, head), t = min(now.t, nt - 1);
+      float x[2][V];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (part == i && head >= a.rows[i].heads) {
-        head -= a.rows[i].heads;
-        ++part;
+      for (int k = 0; k < 2; ++k) C::widen_to(raw[u][k], x[k]);
+      if constexpr (NORM) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum = __builtin_fmaf(x[k][i], x[k][i], sum);
+        const float r = rsqrtf(__builtin_fmaf(row_sum(sum, a.L), mean, a.eps));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float weight[V];
+          load_floats(&weights[part][0] + sl.e[k], weight);
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[k][i] *= r * weight[i];
+        }
       }
-    const Rows &r0 = a.rows[0], &r1 = a.rows[1], &r2 = a.rows[2];
-    const char *src = part == 0 ? r0.src : part == 1 ? r1.src : r2.src;
-    char *dst = part == 0 ? r0.dst : part == 1 ? r1.dst : r2.dst;
-    const int64_t st = part == 0 ? r0.st : part == 1 ? r1.st : r2.st;
-    const int64_t sh = part == 0 ? r0.sh : part == 1 ? r1.sh : r2.sh;
-    const int64_t dh = part == 0 ? r0.dh : part == 1 ? r1.dh : r2.dh;
-    src += (t0 + t) * st + head * sh;
-    bool write = true;
-    if constexpr (PAGED) {
-      if (part == 0) {
-        write = place[t].position != kNowhere;
-        dst += (t0 + t) * r0.dt + head * dh;
-      } else {
-        const int64_t at = place[t].at[part - 1];
-        write = at >= 0;
-        dst += at + head * dh;
+      if (!PAGED || part < 2) rotate<V, INTER>(sl, cs[t], x);
+      const Rows &r = part == 0 ? a.rows[0] : part == 1 ? a.rows[1] : a.rows[2];
+      int64_t at = (t0 + t) * r.dt;
+      bool write = now.t < nt;
+      if constexpr (PAGED) {
+        if (part) at = part == 1 ? place[t].at[0] : place[t].at[1];
+        write = write && place[t].position != kNowhere && at >= 0;
       }
-    } else {
-      dst += (t0 + t) * (part == 0 ? r0.dt : r1.dt) + head * dh;
+      if (write) {
+        char *dst = r.dst + at + head * r.dh;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (sl.has[k]) C::store(dst + sl.e[k] * kSize, x[k]);
+      }
     }
-    float x[2][V];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (sl.has[k]) load<DT, V>(src + sl.e[k] * kSize, x[k]);
-      else
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[k][i] = 0.0f;
-    }
-    if constexpr (NORM) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum = __builtin_fmaf(x[k][i], x[k][i], sum);
-      const float r = rsqrtf(__builtin_fmaf(row_sum(sum, a.L), mean, a.eps));
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[k][i] *= r * (part == 0 ? w[0][k][i] : w[1][k][i]);
-    }
-    if (!PAGED || part < 2) rotate<V, INTER>(sl, cs[t], x);
-    if (write) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (sl.has[k]) store<DT, V>(dst + sl.e[k] * kSize, x[k]);
-    }
-    t += ht;
-    h += hr;
-    if (h >= a.heads) {
-      h -= a.heads;
-      ++t;
-    }
+    w = now;
+    fetch(w);
   }
 }
 
@@ -334,110 +365,147 @@ struct BackwardArgs {
   const int *positions;
   const float *freqs;
   float scale, eps;
-  int T, D, R, TB, L, NS, w_dt;
+  int T, D, R, TB, L, w_dt;
 };
 
-// Workgroup b < part[0].blocks takes every blocks-th run of TB tokens of the
-// queries, the others the keys'.  A lane keeps its slot's weights and its share
-// of their gradient in registers.
-template <int DT, int V, bool INTER>
-__global__ __launch_bounds__(kThreads) void qk_norm_backward_kernel(BackwardArgs a) {
-  __shared__ float cs[kMaxTB][2 * kMaxPairs];
-  __shared__ float box[kThreads / 64][kMaxHeadDim];
+// A workgroup takes a run of TB tokens, the queries' rows and then the keys' by the same
+// angles, and every gridDim.x-th run on.  A lane keeps its share of the weight's gradient
+// in registers until an operand's rows of a run end, a column's thread the sums of runs.
+// Bound by what is on its way to a CU, so by its waves: chunks of four values to a lane
+// at every type leave room for five waves to a SIMD (8120 tokens of 40 heads of 128 in
+// bf16, 249 MB, cold, with the sums behind: 60 us, 4.1 TB/s, 65536 tokens 4.8; eight: 62 with
+// four waves, 73 with three; runs of four tokens: 67; five waves' 65536 tokens with four 4.0).
+template <int DT, bool INTER>
+__global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardArgs a) {
+  constexpr int V = 4;
+  __shared__ __attribute__((aligned(16))) float cs[kMaxTB][2 * kMaxPairs];
+  __shared__ __attribute__((aligned(16))) float weights[2][kMaxHeadDim];
+  __shared__ float box[kWaves][kMaxHeadDim], total[2][kMaxHeadDim];  // (a column to a thread)
+  typedef Chunk<DT, V> C;
   constexpr int kSize = DT == NOVA_HIP_DT_F32 ? 4 : 2;
-  const int kind = (int)blockIdx.x >= a.part[0].blocks ? 1 : 0;
-  const BackwardArgs::Part &p = a.part[kind];
-  const int block = blockIdx.x - (kind ? a.part[0].blocks : 0);
-  const int pairs = a.R / 2;
-  const int j = threadIdx.x & (a.L - 1), group = threadIdx.x / a.L, groups = kThreads / a.L;
+  const int j = threadIdx.x & (a.L - 1), groups = kThreads / a.L;
   const Slot sl = slot_of<V, INTER>(j, a.D, a.R);
-  float w[2][V], dw[2][V] = {};
-  load_weight<V>(p.w, a.w_dt, sl, w);
   const float mean = 1.0f / (float)a.D;
-  const int ht = groups / p.heads, hr = groups - ht * p.heads;
-  for (int64_t t0 = (int64_t)block * a.TB; t0 < a.T; t0 += (int64_t)p.blocks * a.TB) {
-    const int nt = (int)min((int64_t)a.TB, a.T - t0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
-      const int t = i / pairs, k = i - t * pairs;
-      float c, s;
-      angle((double)a.positions[t0 + t], a.freqs[k], a.scale, true, c, s);
-      cs[t][k] = c;
-      cs[t][kMaxPairs + k] = s;
-    }
-    __syncthreads();
-    int t = group / p.heads, h = group - t * p.heads;
-    while (t < nt) {
-      const char *xp = p.x + (t0 + t) * p.xt + h * p.xh, *gp = p.g + (t0 + t) * p.gt + h * p.gh;
-      float x[2][V], g[2][V];
+  int64_t t0 = 0;
+  int nt = 0;
+  typename C::raw rx[2] = {}, rg[2] = {};
+  auto fetch = [&](const BackwardArgs::Part &p, const Walk &at) __attribute__((always_inline)) {
+    if (at.t >= nt) return;
+    const char *x = p.x + (t0 + at.t) * p.xt + at.h * p.xh;
+    const char *y = p.g + (t0 + at.t) * p.gt + at.h * p.gh;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (sl.has[k]) {
-          load<DT, V>(xp + sl.e[k] * kSize, x[k]);
-          load<DT, V>(gp + sl.e[k] * kSize, g[k]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[k][i] = g[k][i] = 0.0f;
-        }
+    for (int k = 0; k < 2; ++k)
+      if (sl.has[k]) {
+        rx[k] = __builtin_nontemporal_load(reinterpret_cast<const typename C::raw *>(x + sl.e[k] * kSize));
+        rg[k] = __builtin_nontemporal_load(reinterpret_cast<const typename C::raw *>(y + sl.e[k] * kSize));
       }
-      rotate<V, INTER>(sl, cs[t], g);
-      float xx = 0.0f, tx = 0.0f;
+  };
+  // (An operand without heads has its walk behind the last token.)
+  auto walk = [&](int kind) __attribute__((always_inline)) {
+    Walk w(threadIdx.x / a.L, groups, max(a.part[kind].heads, 1));
+    if (a.part[kind].heads == 0) w.t = nt;
+    return w;
+  };
+  const int first = blockIdx.y, last = gridDim.y > 1 ? first : 1;
+  // (Zeros behind the row, where absent chunks point: only rows that no lane lacks reach 256.)
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind)
+    weights[kind][threadIdx.x] = (int)threadIdx.x < a.D && a.part[kind].heads
+                                     ? gemm::bias_at(a.part[kind].w, a.w_dt, threadIdx.x) : 0.0f;
+  total[0][threadIdx.x] = total[1][threadIdx.x] = 0.0f;
+  for (int64_t run = blockIdx.x; run * a.TB < a.T; run += gridDim.x) {
+    t0 = run * a.TB;
+    nt = (int)min((int64_t)a.TB, a.T - t0);
+    Walk at = walk(first);
+    fetch(a.part[first], at);
+    angles(cs, nt, a.R / 2, a.freqs, a.scale, true, [&](int t) { return (double)a.positions[t0 + t]; });
+    __syncthreads();
+#pragma unroll 1
+    for (int kind = first; kind <= last; ++kind) {
+      const BackwardArgs::Part &p = a.part[kind];
+      const float *weight = weights[kind];
+      float dw[2][V] = {};
+      while (__ballot(at.t < nt)) {  // (whole waves: the lanes of a row stay together)
+        float x[2][V], d[2][V];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          C::widen_to(rx[k], x[k]);
+          C::widen_to(rg[k], d[k]);
+        }
+        rotate<V, INTER>(sl, cs[min(at.t, nt - 1)], d);
+        float xx = 0.0f, tx = 0.0f, t[2][V];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          load_floats(weight + sl.e[k], t[k]);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            t[k][i] *= d[k][i];
+            xx = __builtin_fmaf(x[k][i], x[k][i], xx);
+            tx = __builtin_fmaf(t[k][i], x[k][i], tx);
+          }
+        }
+        const float r = rsqrtf(__builtin_fmaf(row_sum(xx, a.L), mean, a.eps));
+        const float m = row_sum(tx, a.L) * mean * r * r;
+        if (at.t < nt) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              const float n = x[k][i] * r;
+              dw[k][i] = __builtin_fmaf(d[k][i], n, dw[k][i]);
+              x[k][i] = __builtin_fmaf(-n, m, r * t[k][i]);
+            }
+            if (sl.has[k]) C::store(p.dx + (t0 + at.t) * p.dt + at.h * p.dh + sl.e[k] * kSize, x[k]);
+          }
+        }
+        at.next(p.heads);
+        fetch(p, at);
+      }
+      if (kind < last) {
+        at = walk(1);
+        fetch(a.part[1], at);
+      }
+      if (p.heads == 0) continue;
+      // The lanes with the same slot, then the waves in order.
+      const int lane = threadIdx.x & 63;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          xx = __builtin_fmaf(x[k][i], x[k][i], xx);
-          tx = __builtin_fmaf(g[k][i] * w[k][i], x[k][i], tx);
+          for (int d = a.L; d < 64; d <<= 1) dw[k][i] += __shfl_xor(dw[k][i], d);
+          if (lane < a.L && sl.has[k]) box[threadIdx.x >> 6][sl.e[k] + i] = dw[k][i];
         }
-      const float r = rsqrtf(__builtin_fmaf(row_sum(xx, a.L), mean, a.eps));
-      const float m = row_sum(tx, a.L) * mean * r * r;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          dw[k][i] = __builtin_fmaf(g[k][i], x[k][i] * r, dw[k][i]);
-          x[k][i] = r * __builtin_fmaf(-x[k][i], m, g[k][i] * w[k][i]);
-        }
-        if (sl.has[k]) store<DT, V>(p.dx + (t0 + t) * p.dt + h * p.dh + sl.e[k] * kSize, x[k]);
-      }
-      t += ht;
-      h += hr;
-      if (h >= p.heads) {
-        h -= p.heads;
-        ++t;
-      }
+      __syncthreads();
+      if ((int)threadIdx.x < a.D)
+        total[kind][threadIdx.x] +=
+            (box[0][threadIdx.x] + box[1][threadIdx.x]) + (box[2][threadIdx.x] + box[3][threadIdx.x]);
+      __syncthreads();
     }
   }
-  // The lanes with the same slot, then the waves in order.
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      for (int d = a.L; d < 64; d <<= 1) dw[k][i] += __shfl_xor(dw[k][i], d);
-      if (lane < a.L && sl.has[k]) box[threadIdx.x >> 6][sl.e[k] + i] = dw[k][i];
-    }
-  __syncthreads();
-  if ((int)threadIdx.x < a.D)
-    p.partial[(int64_t)block * a.D + threadIdx.x] =
-        (box[0][threadIdx.x] + box[1][threadIdx.x]) + (box[2][threadIdx.x] + box[3][threadIdx.x]);
+  if ((int)threadIdx.x >= a.D) return;
+  for (int kind = first; kind <= last; ++kind)
+    if (a.part[kind].heads)
+      a.part[kind].partial[(int64_t)blockIdx.x * a.D + threadIdx.x] = total[kind][threadIdx.x];
 }
 
-// The workgroups' sums of 32 columns: eight rows at a time, then those in order.
-__global__ __launch_bounds__(kThreads) void qk_norm_weight_kernel(BackwardArgs a) {
-  __shared__ float box[8][32];
+// The workgroups' sums of eight columns: every 128th row, then those in order.
+__global__ __launch_bounds__(1024) void qk_norm_weight_kernel(BackwardArgs a) {
+  __shared__ float box[16][8];
   const BackwardArgs::Part &p = a.part[blockIdx.y];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5, d = blockIdx.x * 32 + c;
+  const int c = threadIdx.x & 7, d = blockIdx.x * 8 + c;  // D is a multiple of 8
   float sum = 0.0f;
-  if (d < a.D) {
 #pragma unroll 8
-    for (int i = r; i < p.blocks; i += 8) sum += p.partial[(int64_t)i * a.D + d];
-  }
-  box[r][c] = sum;
+  for (int i = threadIdx.x >> 3; i < p.blocks; i += 128) sum += p.partial[(int64_t)i * a.D + d];
+  // The eight rows of a wave, then the waves.
+  sum += __shfl_xor(sum, 8);
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  if ((threadIdx.x & 63) < 8) box[threadIdx.x >> 6][c] = sum;
   __syncthreads();
-  if (r || d >= a.D) return;
+  if (threadIdx.x >= 8) return;
+  sum = 0.0f;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) sum += box[i][c];
+  for (int i = 0; i < 16; ++i) sum += box[i][c];
   p.dw[d] = sum;
 }
 
@@ -456,9 +524,11 @@ __global__ void rotary_frequencies_kernel(float *freqs, int n, double base, doub
 int chunk_values(int dt, int R, bool interleaved) {
   return dt == NOVA_HIP_DT_F32 || (!interleaved && R % 16) ? 4 : 8;
 }
-void shape(int D, int V, int &NS, int &L) {
-  NS = (D / V + 1) / 2;
-  for (L = 1; L < NS;) L <<= 1;
+// Lanes to a row.
+int lanes_of(int D, int V) {
+  int L = 1;
+  while (L < (D / V + 1) / 2) L <<= 1;
+  return L;
 }
 
 template <int DT, int V, bool INTER>
@@ -473,11 +543,13 @@ void launch_rows(const Args &a, bool norm, bool paged, hipStream_t s) {
   if (norm) hipLaunchKernelGGL((positions_kernel<DT, V, INTER, true, false>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((positions_kernel<DT, V, INTER, false, false>), grid, block, 0, s, a);
 }
-template <int DT, int V, bool INTER>
+template <int DT, bool INTER>
 void launch_back(const BackwardArgs &a, hipStream_t s) {
-  const unsigned grid = (unsigned)(a.part[0].blocks + a.part[1].blocks);
-  if (grid) hipLaunchKernelGGL((qk_norm_backward_kernel<DT, V, INTER>), dim3(grid), dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(qk_norm_weight_kernel, dim3((unsigned)((a.D + 31) / 32), 2), dim3(kThreads), 0, s, a);
+  const unsigned runs = (unsigned)std::max(a.part[0].blocks, a.part[1].blocks);
+  // Few runs: a workgroup for each operand (333 tokens of 24 heads of 80: 8.8 us against 10.6).
+  const dim3 grid(runs, runs <= 512 ? 2 : 1);
+  if (runs) hipLaunchKernelGGL((qk_norm_backward_kernel<DT, INTER>), grid, dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(qk_norm_weight_kernel, dim3((unsigned)a.D / 8, 2), dim3(1024), 0, s, a);
 }
 
 // Calls f<DT, V, INTER>() of a problem.
@@ -502,8 +574,20 @@ void dispatch(int dt, int R, bool interleaved, F f) {
 #undef NOVA_POS_CASE
 }
 
-// Tokens to a workgroup: one while they do not give every CU four, up to eight.
-int tokens_per_block(int64_t T) { return (int)std::min<int64_t>(kMaxTB, std::max<int64_t>(1, T / 1024)); }
+// Tokens to a workgroup, of those that give a lane up to five rows in two: what leaves the
+// fewest lanes idle, and one while there are fewer workgroups than four to a CU.  Cold:
+// 8120 tokens of 40 heads of 128 in bf16 at 1 / 2 / 3 tokens 34.5 / 32.7 / 35.5 us (5.1
+// TB/s, as a copy), 8192 of 12 heads of 64 in f32 at 2 / 5 / 6 / 8 12.5 / 10.3 / 12.5 / 12.2.
+int tokens_per_block(int64_t T, int heads, int L) {
+  const int64_t most = std::min<int64_t>(kMaxTB, T / 1024), lanes = heads * L;
+  int64_t best = 1;
+  double fill = 0.0;
+  for (int64_t n = 1; n <= most && n * lanes <= 5 * kThreads / 2; ++n) {
+    const double f = (double)(n * lanes) / (double)((n * lanes + kThreads - 1) / kThreads);
+    if (f >= fill) fill = f, best = n;
+  }
+  return (int)best;
+}
 
 Rows rows_of(const PositionRows &r, int size) {
   return {static_cast<const char *>(r.src.p), static_cast<char *>(r.dst.p), r.w,
@@ -542,27 +626,32 @@ int32_t launch_positions(const PositionProblem &p, hipStream_t s) {
   a.T = (int)p.T;
   a.D = (int)p.D;
   a.R = (int)p.R;
-  a.TB = pos::tokens_per_block(p.T);
-  // A grid's dimension holds less than 2^32 threads.
-  if ((p.T + a.TB - 1) / a.TB >= 1 << 24)
-    return fail(NOVA_HIP_ERANGE, "%s: %lld tokens exceed 2^27 - 8", p.what, (long long)p.T);
   a.w_dt = p.w_dt;
   a.inverse = p.inverse;
-  pos::shape(a.D, pos::chunk_values(p.dt, a.R, p.interleaved), a.NS, a.L);
+  a.L = pos::lanes_of(a.D, pos::chunk_values(p.dt, a.R, p.interleaved));
+  a.TB = pos::tokens_per_block(p.T, a.heads, a.L);
+  // A grid's dimension holds less than 2^32 threads.
+  if ((p.T + a.TB - 1) / a.TB >= 1 << 24)
+    return fail(NOVA_HIP_ERANGE, "%s: %lld tokens of %d heads exceed 2^24 workgroups", p.what,
+                (long long)p.T, a.heads);
   pos::dispatch(p.dt, a.R, p.interleaved, [&](auto dt, auto v, auto inter) {
     pos::launch_rows<dt.value, v.value, inter.value>(a, p.norm, p.paged != nullptr, s);
   });
   return check_hip(hipGetLastError(), "positions launch");
 }
 
-// Workgroups of the backward pass over `heads` heads of T tokens, of all `all`.
-static int64_t backward_blocks(int64_t T, int64_t heads, int64_t all) {
+// Tokens to a run of the backward pass, and workgroups: up to five to a CU, all with the
+// same number of runs.
+static int backward_run(int64_t T) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(pos::kMaxTB, T / 512));
+}
+static int64_t backward_blocks(int64_t T, int64_t heads) {
   if (T == 0 || heads == 0) return 0;
-  const int64_t TB = pos::tokens_per_block(T);
-  return std::min((T + TB - 1) / TB, std::max<int64_t>(1, 1024 * heads / all));
+  const int64_t runs = (T + backward_run(T) - 1) / backward_run(T), turns = (runs + 1279) / 1280;
+  return (runs + turns - 1) / turns;
 }
 int64_t qk_norm_backward_scratch(int64_t T, int64_t heads, int64_t kv_heads, int64_t D) {
-  return (backward_blocks(T, heads, heads + kv_heads) + backward_blocks(T, kv_heads, heads + kv_heads)) * D;
+  return (backward_blocks(T, heads) + backward_blocks(T, kv_heads)) * D;
 }
 
 int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
@@ -570,10 +659,9 @@ int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
   pos::BackwardArgs a = {};
   const int size = dtype_size(p.dt);
   float *scratch = p.scratch;
-  const int64_t all = p.part[0].heads + p.part[1].heads;
   for (int i = 0; i < 2; ++i) {
     const auto &q = p.part[i];
-    const int64_t blocks = backward_blocks(p.T, q.heads, all);
+    const int64_t blocks = backward_blocks(p.T, q.heads);
     a.part[i] = {static_cast<const char *>(q.x.p), static_cast<const char *>(q.g.p),
                  static_cast<char *>(q.dx.p), q.w, scratch, q.dw,
                  q.x.st * size, q.x.sh * size, q.g.st * size, q.g.sh * size,
@@ -587,12 +675,16 @@ int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
   a.T = (int)p.T;
   a.D = (int)p.D;
   a.R = (int)p.R;
-  a.TB = pos::tokens_per_block(p.T);
   a.w_dt = p.w_dt;
-  pos::shape(a.D, pos::chunk_values(p.dt, a.R, p.interleaved), a.NS, a.L);
-  pos::dispatch(p.dt, a.R, p.interleaved, [&](auto dt, auto v, auto inter) {
-    pos::launch_back<dt.value, v.value, inter.value>(a, s);
-  });
+  a.L = pos::lanes_of(a.D, 4);
+  a.TB = backward_run(p.T);
+  const auto launch = p.dt == NOVA_HIP_DT_F32 ? (p.interleaved ? pos::launch_back<NOVA_HIP_DT_F32, true>
+                                                               : pos::launch_back<NOVA_HIP_DT_F32, false>)
+                      : p.dt == NOVA_HIP_DT_BF16 ? (p.interleaved ? pos::launch_back<NOVA_HIP_DT_BF16, true>
+                                                                  : pos::launch_back<NOVA_HIP_DT_BF16, false>)
+                                                 : (p.interleaved ? pos::launch_back<NOVA_HIP_DT_F16, true>
+                                                                  : pos::launch_back<NOVA_HIP_DT_F16, false>);
+  launch(a, s);
   return check_hip(hipGetLastError(), "qk_norm_rotary_backward launch");
 }
 
