@@ -250,10 +250,9 @@ __device__ __forceinline__ bool find_tile_of_many(const PagedArgs &a, int t, Uni
   u.slot = t * a.splits;
   return u.index >= 0 && u.index < tiles_of(a, u.seq);
 }
-// Their pieces: at most a.splits of them, from the lengths of up to kSummed sequences.
-constexpr int kSummed = 4096;
+// Their pieces: at most a.splits of them (one from 1153 sequences on), from the lengths.
 __device__ __forceinline__ int piece_of_many(const PagedArgs &a) {
-  if (a.splits == 1 || a.B > kSummed) return a.chunk;
+  if (a.splits == 1) return a.chunk;
   float tiles = 0.0f, keys = 0.0f;
   for (int b = threadIdx.x & 63; b < a.B; b += 64) {
     const Seq q = seq_of(a, b);

@@ -283,3 +283,47 @@ def test_tokens_beyond_the_hint_are_left_out(cuda):
         near = (got.double() - out.double()).abs() <= 2.0 ** -6
         assert near[:3].all() and near[7:].all() and (l2[:, :3] - lse[:, :3]).abs().max() < 1e-4
         assert (got[3:7] == 5.0).all() and (l2[:, 3:7] == 5.0).all()
+
+
+@pytest.mark.parametrize("page", [5, 16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_chunks_of_many_long_sequences(cuda, D, page):
+    """More sequences than a wave has lanes, of few tokens over several splits."""
+    seqs = [((0, 5, 1, 7)[i % 4], (2000, 1, 700, 1030, 0, 1500)[i % 6]) for i in range(70)]
+    for causal in (False, True):
+        run(cuda, seqs, 8, 1, D, page=page, causal=causal, pad=2)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_sequences_share_pages(cuda, new):
+    """The same pages in two tables, and the same page twice in one."""
+    lens = [70, 70, 70]
+    c = Cache(cuda, lens, 2, 64, 16, BF)
+    c.table[1] = c.table[0]
+    c.table[2, 1] = c.table[2, 0]
+    k, v = (p.clone() for p in c.packed)
+    for x in (k, v):
+        x[70:140] = x[:70]
+        x[156:172] = x[140:156]
+    q = torch.randn(3 * new, 4, 64, device=cuda).to(BF)
+    out, lse = torch.empty_like(q), torch.empty(4, 3 * new, device=cuda)
+    nh.paged_attention(q, c.k, c.v, offsets([new] * 3, cuda), c.lengths, c.table, out=out, lse=lse)
+    check(out, lse, q, k, v, [new] * 3, lens, True, 64 ** -0.5, new)
+
+
+@pytest.mark.parametrize("count", [3, 90])
+def test_offsets_that_overlap(cuda, count):
+    """Whatever the offsets hold, only the tokens' rows are written, and sequences
+    that are sound and alone with their tokens have their result."""
+    seqs = [(1, 900)] + [(60, 900)] * 2 + [(3, 20)] * (count - 3)
+    q, c, off, out, _ = run(cuda, seqs, 8, 2, 64)
+    T = len(q)
+    wide = torch.full((T + 9, 8, 64), 7.0, dtype=BF, device=cuda)
+    bad = off.clone()
+    bad[2] = 2 ** 31 - 1  # sequence 1 has all tokens from its first, sequence 2 none
+    bad[3] = 1
+    for lens in (c.lengths, c.lengths - 10 ** 9, c.lengths + 10 ** 9):
+        nh.paged_attention(q, c.k, c.v, bad, lens, c.table, out=wide[:T])
+        assert (wide[T:] == 7.0).all()
+    nh.paged_attention(q, c.k, c.v, bad, c.lengths, c.table, out=wide[:T])
+    assert (wide[:1].double() - out[:1].double()).abs().max() <= 2.0 ** -6

@@ -157,6 +157,12 @@ def test_norm_and_backward(cuda, D, R, dt, interleaved):
     norm_case(cuda, 41, 6, 3, D, R, dt, interleaved, weight=dt)
 
 
+@pytest.mark.parametrize("T,H,G", [(12001, 2, 1), (25000, 0, 1), (4095, 1, 1), (4097, 2, 3), (20007, 1, 0)])
+def test_norm_of_many_tokens(cuda, T, H, G):
+    """Runs of up to eight tokens, several to a workgroup of the backward pass."""
+    norm_case(cuda, T, H, G, 40, 24, HF, True)
+
+
 @pytest.mark.parametrize("layout", ["thd", "fused", "htd"])
 @pytest.mark.parametrize("T,H,G", [(1, 1, 1), (1, 40, 8), (7, 0, 2), (7, 3, 0), (1024, 2, 1), (2500, 12, 12),
                                    (9001, 3, 1), (1, 300, 7)])
