@@ -528,7 +528,7 @@ int64_t nova_hip_qk_norm_rotary_backward_scratch(int64_t tokens, int64_t heads, 
  * A paged cache: rows of keys and values in pages, k_pages and v_pages
  * [pages, rows of a page, key heads, D] of dt NOVA_HIP_DT_BF16 or _F16, unit
  * stride on D, any order of the other dims, rows 16-byte aligned, any page size
- * (attention reads keys fastest from pages of a multiple of 8 rows, or of 4 where D
+ * (attention is some 10 % faster on pages of a multiple of 8 rows, or of 4 where D
  * is above 64; it takes tables of up to 2^30 rows and pages of up to
  * 2^30 elements from first to last row).
  * Row i of sequence b is row i % page of page table[b, i / page].

@@ -17,8 +17,10 @@
 // Keys come by DMA into LDS.  Where a page holds whole loads (rows that are a
 // multiple of the 4 or 8 of one instruction) its address is a scalar: a lane looks up
 // each load of a tile, a tile ahead, and a buffer of the load's rows that are there
-// makes the others zero.  Other page sizes go through registers, a row's address per
-// lane.
+// makes the others zero.  Other page sizes: a lane looks up each row, and a load takes
+// its lanes' addresses from those; rows that are not there are a row of zeros (32 heads
+// on 8 of 128, pages of one row against 16: 32 single tokens over 1500 to 8192 rows 117 us
+// against 114, a prompt of 8192 590 against 530; through registers 930 and 1180).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -67,6 +69,9 @@ struct PagedArgs {
   float places;       // workgroups resident at once, to a key head
   bool causal;
 };
+
+// A row behind the last.
+__device__ const __attribute__((aligned(16))) uint32_t kZeros[64] = {};
 
 constexpr float kSlack = 8.0f;  // as in the packed forward
 template <int DT>
@@ -273,7 +278,7 @@ __device__ __forceinline__ float *sums_at(const PagedArgs &a, int kh, int slot) 
 
 // NW waves of 32 rows each.  WHOLE: a load's rows lie in one page.
 template <int DT, int DP, int NW, bool WHOLE>
-__global__ __launch_bounds__(64 * NW, NW == 1 && !WHOLE ? 1 : 2) void attention_paged_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a) {
   constexpr int CH = kPitch<DP>, BN = NW == 1 ? 32 : 64, kTile = BN * CH * 16;
   constexpr int kRows = 64 / CH;               // rows of one DMA instruction
   constexpr int kN = BN / kRows / NW;          // instructions of a wave and tile
@@ -340,27 +345,29 @@ __global__ __launch_bounds__(64 * NW, NW == 1 && !WHOLE ? 1 : 2) void attention_
   auto page_of = [&](int key) __attribute__((always_inline)) {
     return (int)(((double)key + 0.5) * a.per_page);
   };
-  // WHOLE: a lane to each of the next tile's loads finds its page and row there, a
-  // tile ahead of the load itself.
+  // A lane to each of the next tile's loads (WHOLE) or rows finds its page and row there,
+  // a tile ahead of the load itself.
+  constexpr int kStep = WHOLE ? kRows : 1;
+  const int mark = (lane & (BN / kStep - 1)) * kStep;
   int id = 0, at = 0;
   auto look = [&](int t) __attribute__((always_inline)) {
-    const int key = min(from + t * BN + (lane & (BN / kRows - 1)) * kRows, to - 1), pg = page_of(key);
+    const int key = min(from + t * BN + mark, to - 1), pg = page_of(key);
     id = table[pg];
     at = key - pg * a.page;
   };
-  if (WHOLE && to > from) look(0);
+  if (to > from) look(0);
   // The queries are waited for here: at their use in the loop the compiler would
   // wait for every load.
   __builtin_amdgcn_s_waitcnt(0x0F70);
   auto fetch = [&](int t, lds_char *sk, lds_char *sv) __attribute__((always_inline)) {
-    const int k0 = from + t * BN;
+    const int skt = (int)a.skt * 2, svt = (int)a.svt * 2;  // bytes
+    const int pg = min(max(id, 0), a.pages - 1);
+    uint64_t ka = reinterpret_cast<uint64_t>(kp + pg * a.skp) + (uint32_t)(at * skt);
+    uint64_t va = reinterpret_cast<uint64_t>(vp + pg * a.svp) + (uint32_t)(at * svt);
+    const int left = to - (from + t * BN + mark);
     if constexpr (WHOLE) {
-      const int skt = (int)a.skt * 2, svt = (int)a.svt * 2;  // bytes
-      const int pg = min(max(id, 0), a.pages - 1);
-      const uint64_t ka = reinterpret_cast<uint64_t>(kp + pg * a.skp) + (uint32_t)(at * skt);
-      const uint64_t va = reinterpret_cast<uint64_t>(vp + pg * a.svp) + (uint32_t)(at * svt);
       // Rows behind the last read zero.
-      const int n = min(to - k0 - (lane & (BN / kRows - 1)) * kRows, kRows);
+      const int n = min(left, kRows);
       const int kb = max((n - 1) * skt + 2 * a.D, 0), vb = max((n - 1) * svt + 2 * a.D, 0);
       look(t + 1);
       // Ahead of the loads: a wait for it is then none for them.
@@ -385,26 +392,24 @@ __global__ __launch_bounds__(64 * NW, NW == 1 && !WHOLE ? 1 : 2) void attention_
             ch * 8 < a.D ? (uint32_t)(lr * svt + ch * 16) : kOOB, 0, 0, NW == 1 ? 2 : 0);
       }
     } else {
-      typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-      auto rows = [&](const uint16_t *p, int64_t sp, int64_t st, lds_char *tile) __attribute__((always_inline)) {
-        u32x4 x[kN];
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const int r0 = (i * NW + wave) * kRows, lr = lane / CH, key = k0 + r0 + lr;
-          const int ch = (lane & (CH - 1)) ^ swz<CH>(r0 + lr);
-          x[i] = u32x4{0, 0, 0, 0};
-          if (key < to && ch * 8 < a.D) {
-            const int pg = page_of(key), r = key - pg * a.page;
-            const int id = min(max(table[pg], 0), a.pages - 1);
-            x[i] = *reinterpret_cast<const u32x4 *>(p + (id * sp + r * st) + ch * 8);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kN; ++i)
-          *(lds_u32x4 *)(tile + (i * NW + wave) * kRows * CH * 16 + lane * 16) = x[i];
+      const uint64_t zeros = reinterpret_cast<uint64_t>(kZeros);
+      if (left <= 0) ka = va = zeros;
+      look(t + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      auto load = [&](uint64_t p, int r, int ch, lds_char *tile) __attribute__((always_inline)) {
+        const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * r, (int)(uint32_t)p);
+        const uint64_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * r, (int)(p >> 32));
+        typedef const __attribute__((address_space(1))) char global_char;
+        __builtin_amdgcn_global_load_lds(
+            (global_char *)((ch * 8 < a.D ? hi << 32 | lo : zeros) + ch * 16), (lds_void *)tile, 16, 0,
+            NW == 1 ? 2 : 0);
       };
-      rows(kp, a.skp, a.skt, sk);
-      rows(vp, a.svp, a.svt, sv);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int r0 = (i * NW + wave) * kRows, r = r0 + lane / CH, ch = (lane & (CH - 1)) ^ swz<CH>(r);
+        load(ka, r, ch, sk + r0 * CH * 16);
+        load(va, r, ch, sv + r0 * CH * 16);
+      }
     }
   };
 
@@ -487,18 +492,25 @@ __global__ __launch_bounds__(64 * NW, NW == 1 && !WHOLE ? 1 : 2) void attention_
     // A stage is refilled when the reads of it have returned, and read when all
     // but the next stage's loads have landed.  Behind the last tile empty ones are
     // fetched: with branches around the waits the compiler adds stricter ones.
+    constexpr int kInFlight = 2 * kN;
+    auto landed = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_s_waitcnt(0x0F70 | (kInFlight & 15) | ((kInFlight >> 4) << 14));
+    };
     auto turn = [&](int t, lds_char *sk, lds_char *sv, lds_char *nk, lds_char *nv) __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
       __builtin_amdgcn_sched_barrier(0);
       fetch(t + 1, nk, nv);
       __builtin_amdgcn_sched_barrier(0);
-      constexpr int kInFlight = WHOLE ? 2 * kN : 0;
-      __builtin_amdgcn_s_waitcnt(0x0F70 | (kInFlight & 15) | ((kInFlight >> 4) << 14));
+      landed();
       __builtin_amdgcn_sched_barrier(0);
       step(t, sk, sv);
     };
-    if (nt > 0) fetch(0, sk0, sv0);
+    if (nt > 0) {
+      fetch(0, sk0, sv0);
+      __builtin_amdgcn_sched_barrier(0);
+      landed();  // what was looked up, so that the loop need not wait for it
+    }
     for (int t = 0; t < nt; t += 2) {
       turn(t, sk0, sv0, sk1, sv1);
       turn(t + 1, sk1, sv1, sk0, sv0);
