@@ -475,8 +475,8 @@ int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int6
  * of nova.linear's output on their way to an attention call.  No reference
  * counterpart.  For all of them:
  *   rows : [tokens, heads, D], D a multiple of 8 up to 256, unit stride on D,
- *   any order of the other dims, rows 16-byte aligned; dt NOVA_HIP_DT_F32, _BF16
- *   or _F16 (paged calls: 16-bit).
+ *   any order of the other dims, strides below 2^36 bytes, rows 16-byte aligned; dt
+ *   NOVA_HIP_DT_F32, _BF16 or _F16 (paged calls: 16-bit).
  *   freqs : [R / 2] f32, R a multiple of 8 up to D: the first R values of a row
  *   are rotated, the others stay.  With t = position * freqs[i], the pair (a, b)
  *   being values (i, i + R / 2) of the row, or (2 i, 2 i + 1) when interleaved is

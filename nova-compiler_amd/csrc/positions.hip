@@ -28,17 +28,26 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTB = 8;  // tokens whose angles a workgroup holds at once
-// Rows of a lane whose loads are on their way together (append, cold, at 2 / 3: 41.2 / 46.2
+// Rows of a lane whose loads are on their way together (append, cold, at 2 / 3: 41 / 46
 // us).  They and the stores are such that the caches keep nothing for: 33.4 against 36.6.
 constexpr int kAhead = 2;
 constexpr int kMaxPairs = kMaxHeadDim / 2;
 
-// One operand's rows and where they go (strides in bytes).
+// A token's and a head's stride in 16 bytes: two products of 32 bits make a row's place
+// (of 64 they cost the backward pass as much as its arithmetic).
+struct Strides {
+  uint32_t t, h;
+  __device__ __forceinline__ int64_t at(int token, int head) const {
+    return (int64_t)(((uint64_t)(uint32_t)token * t + (uint64_t)(uint32_t)head * h) << 4);
+  }
+};
+
+// One operand's rows and where they go.
 struct Rows {
   const char *src;
   char *dst;
   const void *w;  // the norm's weight
-  int64_t st, sh, dt, dh;
+  Strides from, to;
   int heads;
 };
 
@@ -208,6 +217,15 @@ __device__ __forceinline__ float row_sum(float v, int L) {
   if (L > 16) v += __shfl_xor(v, 16);
   return v;
 }
+__device__ __forceinline__ void row_sums(float &v, float &u, int L) {
+#define NOVA_POS_ADD(c) v += dpp_mov<c>(v), u += dpp_mov<c>(u)
+  if (L > 1) NOVA_POS_ADD(0xB1);
+  if (L > 2) NOVA_POS_ADD(0x4E);
+  if (L > 4) NOVA_POS_ADD(0x141);
+  if (L > 8) NOVA_POS_ADD(0x140);
+#undef NOVA_POS_ADD
+  if (L > 16) v += __shfl_xor(v, 16), u += __shfl_xor(u, 16);
+}
 
 // Where a new token goes: its position and the byte offsets of its rows in the
 // pages, -1 where it is not stored, position kNowhere outside every sequence.
@@ -278,7 +296,7 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
       int head;
       const int part = part_of(w.h, head);
       const Rows &r = part == 0 ? a.rows[0] : part == 1 ? a.rows[1] : a.rows[2];
-      const char *src = r.src + (t0 + w.t) * r.st + head * r.sh;
+      const char *src = r.src + r.from.at(t0 + w.t, head);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         if (sl.has[k])
@@ -334,14 +352,15 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
       }
       if (!PAGED || part < 2) rotate<V, INTER>(sl, cs[t], x);
       const Rows &r = part == 0 ? a.rows[0] : part == 1 ? a.rows[1] : a.rows[2];
-      int64_t at = (t0 + t) * r.dt;
+      int64_t at = r.to.at(t0 + t, head);
       bool write = now.t < nt;
       if constexpr (PAGED) {
-        if (part) at = part == 1 ? place[t].at[0] : place[t].at[1];
-        write = write && place[t].position != kNowhere && at >= 0;
+        const int64_t page = part == 0 ? 0 : part == 1 ? place[t].at[0] : place[t].at[1];
+        at += page;  // (the pages' stride of a token is zero)
+        write = write && place[t].position != kNowhere && page >= 0;
       }
       if (write) {
-        char *dst = r.dst + at + head * r.dh;
+        char *dst = r.dst + at;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
           if (sl.has[k]) C::store(dst + sl.e[k] * kSize, x[k]);
@@ -353,13 +372,13 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
 }
 
 struct BackwardArgs {
-  // Per operand: x, its gradient's source, the gradient (strides in bytes).
+  // Per operand: x, the gradient of its result, its own.
   struct Part {
     const char *x, *g;
     char *dx;
     const void *w;
     float *partial, *dw;  // [blocks][D], [D]
-    int64_t xt, xh, gt, gh, dt, dh;
+    Strides xs, gs, ds;
     int heads, blocks;
   } part[2];
   const int *positions;
@@ -373,8 +392,8 @@ struct BackwardArgs {
 // in registers until an operand's rows of a run end, a column's thread the sums of runs.
 // Bound by what is on its way to a CU, so by its waves: chunks of four values to a lane
 // at every type leave room for five waves to a SIMD (8120 tokens of 40 heads of 128 in
-// bf16, 249 MB, cold, with the sums behind: 60 us, 4.1 TB/s, 65536 tokens 4.8; eight: 62 with
-// four waves, 73 with three; runs of four tokens: 67; five waves' 65536 tokens with four 4.0).
+// bf16, 249 MB, cold, with the sums behind: 59 us, 4.2 TB/s; 65536 tokens 5.1; chunks of
+// eight: 62 with four waves, 73 with three; runs of four tokens: 67).
 template <int DT, bool INTER>
 __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardArgs a) {
   constexpr int V = 4;
@@ -386,13 +405,11 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
   const int j = threadIdx.x & (a.L - 1), groups = kThreads / a.L;
   const Slot sl = slot_of<V, INTER>(j, a.D, a.R);
   const float mean = 1.0f / (float)a.D;
-  int64_t t0 = 0;
-  int nt = 0;
+  int t0 = 0, nt = 0;
   typename C::raw rx[2] = {}, rg[2] = {};
   auto fetch = [&](const BackwardArgs::Part &p, const Walk &at) __attribute__((always_inline)) {
     if (at.t >= nt) return;
-    const char *x = p.x + (t0 + at.t) * p.xt + at.h * p.xh;
-    const char *y = p.g + (t0 + at.t) * p.gt + at.h * p.gh;
+    const char *x = p.x + p.xs.at(t0 + at.t, at.h), *y = p.g + p.gs.at(t0 + at.t, at.h);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (sl.has[k]) {
@@ -413,9 +430,9 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
     weights[kind][threadIdx.x] = (int)threadIdx.x < a.D && a.part[kind].heads
                                      ? gemm::bias_at(a.part[kind].w, a.w_dt, threadIdx.x) : 0.0f;
   total[0][threadIdx.x] = total[1][threadIdx.x] = 0.0f;
-  for (int64_t run = blockIdx.x; run * a.TB < a.T; run += gridDim.x) {
+  for (int run = blockIdx.x; run < (a.T + a.TB - 1) / a.TB; run += gridDim.x) {
     t0 = run * a.TB;
-    nt = (int)min((int64_t)a.TB, a.T - t0);
+    nt = min(a.TB, a.T - t0);
     Walk at = walk(first);
     fetch(a.part[first], at);
     angles(cs, nt, a.R / 2, a.freqs, a.scale, true, [&](int t) { return (double)a.positions[t0 + t]; });
@@ -444,9 +461,10 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
             tx = __builtin_fmaf(t[k][i], x[k][i], tx);
           }
         }
-        const float r = rsqrtf(__builtin_fmaf(row_sum(xx, a.L), mean, a.eps));
-        const float m = row_sum(tx, a.L) * mean * r * r;
+        row_sums(xx, tx, a.L);
+        const float r = rsqrtf(__builtin_fmaf(xx, mean, a.eps)), m = tx * mean * r * r;
         if (at.t < nt) {
+          char *dx = p.dx + p.ds.at(t0 + at.t, at.h);
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
 #pragma unroll
@@ -455,7 +473,7 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
               dw[k][i] = __builtin_fmaf(d[k][i], n, dw[k][i]);
               x[k][i] = __builtin_fmaf(-n, m, r * t[k][i]);
             }
-            if (sl.has[k]) C::store(p.dx + (t0 + at.t) * p.dt + at.h * p.dh + sl.e[k] * kSize, x[k]);
+            if (sl.has[k]) C::store(dx + sl.e[k] * kSize, x[k]);
           }
         }
         at.next(p.heads);
@@ -589,9 +607,13 @@ int tokens_per_block(int64_t T, int heads, int L) {
   return (int)best;
 }
 
-Rows rows_of(const PositionRows &r, int size) {
-  return {static_cast<const char *>(r.src.p), static_cast<char *>(r.dst.p), r.w,
-          r.src.st * size, r.src.sh * size, r.dst.st * size, r.dst.sh * size, (int)r.heads};
+// An operand's strides; false where they do not fit.
+bool strides_of(const AttentionOperand &o, int size, Strides &s) {
+  s = {(uint32_t)(o.st * size / 16), (uint32_t)(o.sh * size / 16)};
+  return o.st * size / 16 == s.t && o.sh * size / 16 == s.h;
+}
+int32_t too_far(const char *what) {
+  return fail(NOVA_HIP_ERANGE, "%s: tokens or heads 2^36 bytes apart", what);
 }
 
 }  // namespace
@@ -609,8 +631,12 @@ int32_t launch_positions(const PositionProblem &p, hipStream_t s) {
   pos::Args a = {};
   const int size = dtype_size(p.dt);
   for (int i = 0; i < 3; ++i) {
-    a.rows[i] = pos::rows_of(p.rows[i], size);
-    a.heads += (int)p.rows[i].heads;
+    const PositionRows &r = p.rows[i];
+    a.heads += (int)r.heads;
+    a.rows[i] = {static_cast<const char *>(r.src.p), static_cast<char *>(r.dst.p), r.w, {}, {}, (int)r.heads};
+    if (p.T == 0 || r.heads == 0) continue;  // (strides of nothing)
+    if (!pos::strides_of(r.src, size, a.rows[i].from) || !pos::strides_of(r.dst, size, a.rows[i].to))
+      return pos::too_far(p.what);
   }
   if (p.T == 0 || a.heads == 0 || p.D == 0) return NOVA_HIP_SUCCESS;
   if (p.paged) {
@@ -663,10 +689,12 @@ int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
     const auto &q = p.part[i];
     const int64_t blocks = backward_blocks(p.T, q.heads);
     a.part[i] = {static_cast<const char *>(q.x.p), static_cast<const char *>(q.g.p),
-                 static_cast<char *>(q.dx.p), q.w, scratch, q.dw,
-                 q.x.st * size, q.x.sh * size, q.g.st * size, q.g.sh * size,
-                 q.dx.st * size, q.dx.sh * size, (int)q.heads, (int)blocks};
+                 static_cast<char *>(q.dx.p), q.w, scratch, q.dw, {}, {}, {}, (int)q.heads, (int)blocks};
     scratch += blocks * p.D;
+    if (blocks == 0) continue;
+    if (!pos::strides_of(q.x, size, a.part[i].xs) || !pos::strides_of(q.g, size, a.part[i].gs) ||
+        !pos::strides_of(q.dx, size, a.part[i].ds))
+      return pos::too_far("qk_norm_rotary_backward");
   }
   a.positions = p.positions;
   a.freqs = p.freqs;

@@ -219,3 +219,13 @@ def test_empty_calls_do_nothing():
     assert app(k=e2, v=e2, q=e, qo=e) == 0
     assert att(q=e, out=e, lse=None) == 0
     assert att(off=at(4, (1,)), lens=d((0,), ptr=0), table=d((0, 8), ptr=0)) == 0    # no sequence
+
+
+@pytest.mark.parametrize("st", [(1 << 35, 64, 1), (256, 1 << 35, 1)])
+def test_rows_too_far_apart(st):
+    """Strides of 2^36 bytes."""
+    assert rot(x=at(20, (2, 4, 64), st), out=at(3, (2, 4, 64)), pos=at(1, (2,))) == ERANGE
+    two = dict(q=at(20, (2, 4, 64), st), k=at(40, (2, 4, 64)), pos=at(60, (2,)))
+    assert norm(qo=at(6, (2, 4, 64)), ko=at(7, (2, 4, 64)), **two) == ERANGE
+    assert back(gq=at(0, (2, 4, 64)), gk=at(1, (2, 4, 64)), dq=at(8, (2, 4, 64)), dk=at(9, (2, 4, 64)),
+                **two) == ERANGE
