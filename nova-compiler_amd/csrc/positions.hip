@@ -10,9 +10,9 @@
 //   dx = r (t - x r^2 mean(t x)),   dw = sum over rows of g x r.
 //
 // All of it is bound by HBM: a row is read and written once.  A workgroup takes one to
-// kMaxTB tokens with all their heads, issues the loads of its rows, works out the tokens'
-// sines and cosines meanwhile, once, into LDS, and ends: angles are taken in 64 bits (in
-// 32 an angle of 10^5 is off by 4e-3).  A row belongs to L = 1 .. 32 neighbouring lanes,
+// kMaxTB tokens with all their heads (see shape_of), issues the loads of its rows, works
+// out the tokens' sines and cosines meanwhile, once, into LDS, and ends: angles are taken
+// in 64 bits (in 32 an angle of 10^5 is off by 4e-3).  A row belongs to L = 1 .. 32 lanes,
 // each with a "slot" of two 16-byte chunks that hold whole pairs, so that the rotation
 // needs no exchange between lanes and the norm log2 L of them.
 #include <hip/hip_runtime.h>
@@ -26,12 +26,45 @@ namespace nova_hip {
 namespace pos {
 namespace {
 
+constexpr int kMaxThreads = 512;  // of a workgroup forward
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTB = 8;  // tokens whose angles a workgroup holds at once
-// Rows of a lane whose loads are on their way together (append, cold, at 2 / 3: 41 / 46
-// us).  They and the stores are such that the caches keep nothing for: 33.4 against 36.6.
+// Rows of a lane whose loads are on their way together (8192 tokens of 8 heads of 64,
+// cold, at 1 / 2: 7.0 / 5.4 us).  They and the stores are such that the caches keep nothing for:
+// 8120 tokens of 40 heads of 128 in 33.4 us against 36.6.
 constexpr int kAhead = 2;
 constexpr int kMaxPairs = kMaxHeadDim / 2;
+
+// n / d for n < 1024 by inverse(d): the product lies above n 2^22 / d by n at most, which is
+// less than 2^22 / d up to d = 4096; beyond, n < d and the product stays below 2^22.
+static_assert(kMaxTB * kMaxPairs <= 1024 && kMaxThreads <= 1024, "what is divided");
+inline uint32_t inverse(int d) { return (1u << 22) / (uint32_t)d + 1; }
+__device__ __forceinline__ int divided(int n, uint32_t inverse) {
+  return (int)(((uint32_t)n * inverse) >> 22);
+}
+
+// A lane group's rows among tokens of `heads` each: every groups-th, from its own.
+struct Steps {
+  int heads, dt, dh;  // a step is of dt tokens and dh heads
+  uint32_t by_heads;
+  Steps() = default;
+  Steps(int groups, int heads)
+      : heads(heads), dt(heads ? groups / heads : 0), dh(heads ? groups % heads : 0),
+        by_heads(heads ? inverse(heads) : 0) {}
+};
+struct Walk {
+  int t, h;
+  __device__ __forceinline__ Walk(int group, const Steps &s)
+      : t(divided(group, s.by_heads)), h(group - t * s.heads) {}
+  __device__ __forceinline__ void next(const Steps &s) {
+    t += s.dt;
+    h += s.dh;
+    if (h >= s.heads) {
+      h -= s.heads;
+      ++t;
+    }
+  }
+};
 
 // A token's and a head's stride in 16 bytes: two products of 32 bits make a row's place
 // (of 64 they cost the backward pass as much as its arithmetic).
@@ -65,7 +98,9 @@ struct Args {
   const int *positions;
   const float *freqs;
   float scale, eps;
-  int T, D, R, TB, L, heads, w_dt;  // heads: of all rows together
+  int T, D, R, TB, L, log_l, w_dt, threads;
+  Steps steps;  // of all rows together
+  uint32_t by_pairs;
   bool inverse;
 };
 
@@ -140,10 +175,10 @@ __device__ __forceinline__ void angle(double position, float freq, float scale, 
 // The angles of tokens 0 .. nt - 1 by a workgroup: cs[t][i] and cs[t][kMaxPairs + i].
 template <typename Position>
 __device__ __forceinline__ void angles(float (&cs)[kMaxTB][2 * kMaxPairs], int nt, int pairs,
-                                       const float *freqs, float scale, bool inverse,
+                                       uint32_t by_pairs, const float *freqs, float scale, bool inverse,
                                        Position position) {
-  for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
-    const int t = i / pairs, k = i - t * pairs;
+  for (int i = threadIdx.x; i < nt * pairs; i += blockDim.x) {
+    const int t = divided(i, by_pairs), k = i - t * pairs;
     float c, s;
     angle(position(t), freqs[k], scale, inverse, c, s);
     cs[t][k] = c;
@@ -191,21 +226,6 @@ __device__ __forceinline__ void rotate(const Slot &sl, const float *cs, float (&
     }
   }
 }
-
-// A lane group's rows among nt tokens of `heads` each: every groups-th, from its own.
-struct Walk {
-  int t, h, dt, dh;
-  __device__ __forceinline__ Walk(int group, int groups, int heads)
-      : t(group / heads), h(group - t * heads), dt(groups / heads), dh(groups - dt * heads) {}
-  __device__ __forceinline__ void next(int heads) {
-    t += dt;
-    h += dh;
-    if (h >= heads) {
-      h -= heads;
-      ++t;
-    }
-  }
-};
 
 // Sum over the L lanes of a row (L a power of two up to 32): in quads, then with the
 // mirrored lane, all on DPP but the last.
@@ -270,7 +290,7 @@ __device__ __forceinline__ Place place_of(const Paged &p, int t, int T) {
 }
 
 template <int DT, int V, bool INTER, bool NORM, bool PAGED>
-__global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
+__global__ __launch_bounds__(kMaxThreads) void positions_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) float cs[kMaxTB][2 * kMaxPairs];
   // Both weights: as registers they would cost more than the rows.
   __shared__ __attribute__((aligned(16))) float weights[NORM ? 2 : 1][NORM ? kMaxHeadDim : 1];
@@ -278,7 +298,7 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
   typedef Chunk<DT, V> C;
   constexpr int kSize = DT == NOVA_HIP_DT_F32 ? 4 : 2;
   const int t0 = blockIdx.x * a.TB, nt = min(a.TB, a.T - t0);
-  const int j = threadIdx.x & (a.L - 1), groups = kThreads / a.L;
+  const int j = threadIdx.x & (a.L - 1);
   const Slot sl = slot_of<V, INTER>(j, a.D, a.R);
   const float mean = 1.0f / (float)a.D;
   // A row's operand (queries, keys, values one behind the other) and head in it.
@@ -291,7 +311,7 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
   typename C::raw raw[kAhead][2] = {};
   auto fetch = [&](Walk w) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u, w.next(a.heads)) {
+    for (int u = 0; u < kAhead; ++u, w.next(a.steps)) {
       if (w.t >= nt) continue;
       int head;
       const int part = part_of(w.h, head);
@@ -304,23 +324,23 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
               reinterpret_cast<const typename C::raw *>(src + sl.e[k] * kSize));
     }
   };
-  Walk w(threadIdx.x / a.L, groups, a.heads);
+  Walk w(threadIdx.x >> a.log_l, a.steps);
   fetch(w);
   if constexpr (NORM) {
-    static_assert(kThreads == kMaxHeadDim, "a thread to a weight");
     // (Zeros behind the row, where absent chunks point: only rows that no lane lacks reach 256.)
-    const bool in = (int)threadIdx.x < a.D;
-    weights[0][threadIdx.x] = in && a.rows[0].heads ? gemm::bias_at(a.rows[0].w, a.w_dt, threadIdx.x) : 0.0f;
-    weights[1][threadIdx.x] = in && a.rows[1].heads ? gemm::bias_at(a.rows[1].w, a.w_dt, threadIdx.x) : 0.0f;
+    for (int d = threadIdx.x; d < kMaxHeadDim; d += blockDim.x) {
+      weights[0][d] = d < a.D && a.rows[0].heads ? gemm::bias_at(a.rows[0].w, a.w_dt, d) : 0.0f;
+      weights[1][d] = d < a.D && a.rows[1].heads ? gemm::bias_at(a.rows[1].w, a.w_dt, d) : 0.0f;
+    }
   }
   if constexpr (PAGED) {
-    for (int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < nt; t += kWaves) {
+    for (int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); t < nt; t += blockDim.x / 64) {
       const Place p = place_of(a.paged, t0 + t, a.T);
       if ((threadIdx.x & 63) == 0) place[t] = p;
     }
     __syncthreads();
   }
-  angles(cs, nt, a.R / 2, a.freqs, a.scale, a.inverse, [&](int t) {
+  angles(cs, nt, a.R / 2, a.by_pairs, a.freqs, a.scale, a.inverse, [&](int t) {
     if constexpr (PAGED) return (double)place[t].position;
     else return (double)a.positions[t0 + t];
   });
@@ -328,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void positions_kernel(Args a) {
   while (__ballot(w.t < nt)) {  // (whole waves: the lanes of a row stay together)
     Walk now = w;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u, now.next(a.heads)) {
+    for (int u = 0; u < kAhead; ++u, now.next(a.steps)) {
       if (u && !__ballot(now.t < nt)) break;
       int head;
       const int part = part_of(now.h, head), t = min(now.t, nt - 1);
@@ -380,11 +400,13 @@ struct BackwardArgs {
     float *partial, *dw;  // [blocks][D], [D]
     Strides xs, gs, ds;
     int heads, blocks;
+    Steps steps;
   } part[2];
   const int *positions;
   const float *freqs;
   float scale, eps;
-  int T, D, R, TB, L, w_dt;
+  int T, D, R, TB, L, log_l, w_dt;
+  uint32_t by_pairs;
 };
 
 // A workgroup takes a run of TB tokens, the queries' rows and then the keys' by the same
@@ -392,7 +414,7 @@ struct BackwardArgs {
 // in registers until an operand's rows of a run end, a column's thread the sums of runs.
 // Bound by what is on its way to a CU, so by its waves: chunks of four values to a lane
 // at every type leave room for five waves to a SIMD (8120 tokens of 40 heads of 128 in
-// bf16, 249 MB, cold, with the sums behind: 59 us, 4.2 TB/s; 65536 tokens 5.1; chunks of
+// bf16, 249 MB, cold, with the sums behind: 58.5 us, 4.3 TB/s; 65536 tokens 5.1; chunks of
 // eight: 62 with four waves, 73 with three; runs of four tokens: 67).
 template <int DT, bool INTER>
 __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardArgs a) {
@@ -402,7 +424,7 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
   __shared__ float box[kWaves][kMaxHeadDim], total[2][kMaxHeadDim];  // (a column to a thread)
   typedef Chunk<DT, V> C;
   constexpr int kSize = DT == NOVA_HIP_DT_F32 ? 4 : 2;
-  const int j = threadIdx.x & (a.L - 1), groups = kThreads / a.L;
+  const int j = threadIdx.x & (a.L - 1);
   const Slot sl = slot_of<V, INTER>(j, a.D, a.R);
   const float mean = 1.0f / (float)a.D;
   int t0 = 0, nt = 0;
@@ -419,7 +441,7 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
   };
   // (An operand without heads has its walk behind the last token.)
   auto walk = [&](int kind) __attribute__((always_inline)) {
-    Walk w(threadIdx.x / a.L, groups, max(a.part[kind].heads, 1));
+    Walk w(threadIdx.x >> a.log_l, a.part[kind].steps);
     if (a.part[kind].heads == 0) w.t = nt;
     return w;
   };
@@ -435,7 +457,7 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
     nt = min(a.TB, a.T - t0);
     Walk at = walk(first);
     fetch(a.part[first], at);
-    angles(cs, nt, a.R / 2, a.freqs, a.scale, true, [&](int t) { return (double)a.positions[t0 + t]; });
+    angles(cs, nt, a.R / 2, a.by_pairs, a.freqs, a.scale, true, [&](int t) { return (double)a.positions[t0 + t]; });
     __syncthreads();
 #pragma unroll 1
     for (int kind = first; kind <= last; ++kind) {
@@ -476,7 +498,7 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
             if (sl.has[k]) C::store(dx + sl.e[k] * kSize, x[k]);
           }
         }
-        at.next(p.heads);
+        at.next(p.steps);
         fetch(p, at);
       }
       if (kind < last) {
@@ -551,7 +573,7 @@ int lanes_of(int D, int V) {
 
 template <int DT, int V, bool INTER>
 void launch_rows(const Args &a, bool norm, bool paged, hipStream_t s) {
-  const dim3 grid((unsigned)((a.T + a.TB - 1) / a.TB)), block(kThreads);
+  const dim3 grid((unsigned)((a.T + a.TB - 1) / a.TB)), block((unsigned)a.threads);
   if constexpr (DT != NOVA_HIP_DT_F32) {
     if (paged) {
       hipLaunchKernelGGL((positions_kernel<DT, V, INTER, false, true>), grid, block, 0, s, a);
@@ -592,19 +614,25 @@ void dispatch(int dt, int R, bool interleaved, F f) {
 #undef NOVA_POS_CASE
 }
 
-// Tokens to a workgroup, of those that give a lane up to five rows in two: what leaves the
-// fewest lanes idle, and one while there are fewer workgroups than four to a CU.  Cold:
-// 8120 tokens of 40 heads of 128 in bf16 at 1 / 2 / 3 tokens 34.5 / 32.7 / 35.5 us (5.1
-// TB/s, as a copy), 8192 of 12 heads of 64 in f32 at 2 / 5 / 6 / 8 12.5 / 10.3 / 12.5 / 12.2.
-int tokens_per_block(int64_t T, int heads, int L) {
-  const int64_t most = std::min<int64_t>(kMaxTB, T / 1024), lanes = heads * L;
-  int64_t best = 1;
+// Tokens and threads of a workgroup.  Few tokens: one, a thread to each of its lanes (32
+// tokens of 40 heads of 128 normed: 3.9 us, with 256 threads 4.6).  Else up to two rows to a
+// lane of 256 threads at most, what leaves the fewest lanes idle: short workgroups keep
+// what the chip works on at a time together (8120 tokens of 40 heads of 128, cold, one
+// token to 192 threads 30.5 us, 5.4 TB/s; two to 256 32.5, to 384 38.6; 8192 of 12 heads of
+// 64 in f32, four to 192 9.6, six to 256 12.5).
+void shape_of(int64_t T, int heads, int L, int &TB, int &threads) {
+  const int64_t lanes = heads * L;
+  TB = 1;
+  threads = (int)std::min<int64_t>(kMaxThreads, (lanes + 63) / 64 * 64);
+  if (T < 1024) return;
+  const int64_t most = std::min<int64_t>(kMaxTB, T / 1024);
   double fill = 0.0;
-  for (int64_t n = 1; n <= most && n * lanes <= 5 * kThreads / 2; ++n) {
-    const double f = (double)(n * lanes) / (double)((n * lanes + kThreads - 1) / kThreads);
-    if (f >= fill) fill = f, best = n;
+  for (int64_t n = 1; n == 1 || (n <= most && n * lanes <= 512); ++n) {
+    const int64_t rows = (n * lanes + 255) / 256;
+    const int64_t t = ((n * lanes + rows - 1) / rows + 63) / 64 * 64;
+    const double f = (double)(n * lanes) / (double)(rows * t);
+    if (f >= fill) fill = f, TB = (int)n, threads = (int)t;
   }
-  return (int)best;
 }
 
 // An operand's strides; false where they do not fit.
@@ -630,15 +658,16 @@ int32_t launch_rotary_frequencies(float *freqs, int64_t n, double base, double f
 int32_t launch_positions(const PositionProblem &p, hipStream_t s) {
   pos::Args a = {};
   const int size = dtype_size(p.dt);
+  int heads = 0;
   for (int i = 0; i < 3; ++i) {
     const PositionRows &r = p.rows[i];
-    a.heads += (int)r.heads;
+    heads += (int)r.heads;
     a.rows[i] = {static_cast<const char *>(r.src.p), static_cast<char *>(r.dst.p), r.w, {}, {}, (int)r.heads};
     if (p.T == 0 || r.heads == 0) continue;  // (strides of nothing)
     if (!pos::strides_of(r.src, size, a.rows[i].from) || !pos::strides_of(r.dst, size, a.rows[i].to))
       return pos::too_far(p.what);
   }
-  if (p.T == 0 || a.heads == 0 || p.D == 0) return NOVA_HIP_SUCCESS;
+  if (p.T == 0 || heads == 0 || p.D == 0) return NOVA_HIP_SUCCESS;
   if (p.paged) {
     const PagedCache &c = *p.paged;
     a.paged = {c.offsets, c.lengths, c.table, {c.k.sp * size, c.v.sp * size},
@@ -655,11 +684,14 @@ int32_t launch_positions(const PositionProblem &p, hipStream_t s) {
   a.w_dt = p.w_dt;
   a.inverse = p.inverse;
   a.L = pos::lanes_of(a.D, pos::chunk_values(p.dt, a.R, p.interleaved));
-  a.TB = pos::tokens_per_block(p.T, a.heads, a.L);
+  a.log_l = __builtin_ctz(a.L);
+  pos::shape_of(p.T, heads, a.L, a.TB, a.threads);
+  a.steps = pos::Steps(a.threads / a.L, heads);
+  a.by_pairs = a.R ? pos::inverse(a.R / 2) : 0;
   // A grid's dimension holds less than 2^32 threads.
   if ((p.T + a.TB - 1) / a.TB >= 1 << 24)
     return fail(NOVA_HIP_ERANGE, "%s: %lld tokens of %d heads exceed 2^24 workgroups", p.what,
-                (long long)p.T, a.heads);
+                (long long)p.T, heads);
   pos::dispatch(p.dt, a.R, p.interleaved, [&](auto dt, auto v, auto inter) {
     pos::launch_rows<dt.value, v.value, inter.value>(a, p.norm, p.paged != nullptr, s);
   });
@@ -684,12 +716,18 @@ int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
   if (p.D == 0) return NOVA_HIP_SUCCESS;
   pos::BackwardArgs a = {};
   const int size = dtype_size(p.dt);
+  a.D = (int)p.D;
+  a.R = (int)p.R;
+  a.L = pos::lanes_of(a.D, 4);
+  a.log_l = __builtin_ctz(a.L);
+  a.by_pairs = a.R ? pos::inverse(a.R / 2) : 0;
   float *scratch = p.scratch;
   for (int i = 0; i < 2; ++i) {
     const auto &q = p.part[i];
     const int64_t blocks = backward_blocks(p.T, q.heads);
     a.part[i] = {static_cast<const char *>(q.x.p), static_cast<const char *>(q.g.p),
-                 static_cast<char *>(q.dx.p), q.w, scratch, q.dw, {}, {}, {}, (int)q.heads, (int)blocks};
+                 static_cast<char *>(q.dx.p), q.w, scratch, q.dw, {}, {}, {}, (int)q.heads, (int)blocks,
+                 pos::Steps(pos::kThreads / a.L, (int)q.heads)};
     scratch += blocks * p.D;
     if (blocks == 0) continue;
     if (!pos::strides_of(q.x, size, a.part[i].xs) || !pos::strides_of(q.g, size, a.part[i].gs) ||
@@ -701,10 +739,7 @@ int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
   a.scale = p.scale;
   a.eps = p.eps;
   a.T = (int)p.T;
-  a.D = (int)p.D;
-  a.R = (int)p.R;
   a.w_dt = p.w_dt;
-  a.L = pos::lanes_of(a.D, 4);
   a.TB = backward_run(p.T);
   const auto launch = p.dt == NOVA_HIP_DT_F32 ? (p.interleaved ? pos::launch_back<NOVA_HIP_DT_F32, true>
                                                                : pos::launch_back<NOVA_HIP_DT_F32, false>)
