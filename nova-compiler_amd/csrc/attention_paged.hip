@@ -210,7 +210,8 @@ __device__ __forceinline__ bool find_split(const Work &w, int t, Unit &u) {
 // S(x) <= t, found bit by bit.
 __device__ __forceinline__ bool find_unit(const PagedArgs &a, const Work &w, int t, Unit &u) {
   const int len = min(w.piece, w.q.len), longest = wave_max_int(w.tiles > 0 ? len : 0);
-  const int d = (int)fminf((float)(longest - min(len, longest)) * (float)a.group.d * (1.0f / kBM), 1e7f);
+  const float behind = (float)(longest - min(len, longest)) * (float)a.group.d * (1.0f / kBM);
+  const int d = (int)fminf(behind, 1e7f);
   auto below = [&](int x) __attribute__((always_inline)) {
     return wave_sum_int(w.n * min(max(x - d, 0), w.tiles));
   };

@@ -121,6 +121,9 @@ struct Chunk {
       else x[i] = widen<DT>(i & 1 ? r[i / 2] >> 16 : r[i / 2] & 0xffffu);
     }
   }
+  static __device__ __forceinline__ raw load(const char *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const raw *>(p));
+  }
   static __device__ __forceinline__ void store(char *p, const float (&x)[V]) {
     raw r;
     if constexpr (DT == NOVA_HIP_DT_F32) {
@@ -320,8 +323,7 @@ __global__ __launch_bounds__(kMaxThreads) void positions_kernel(Args a) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         if (sl.has[k])
-          raw[u][k] = __builtin_nontemporal_load(
-              reinterpret_cast<const typename C::raw *>(src + sl.e[k] * kSize));
+          raw[u][k] = C::load(src + sl.e[k] * kSize);
     }
   };
   Walk w(threadIdx.x >> a.log_l, a.steps);
@@ -435,8 +437,8 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (sl.has[k]) {
-        rx[k] = __builtin_nontemporal_load(reinterpret_cast<const typename C::raw *>(x + sl.e[k] * kSize));
-        rg[k] = __builtin_nontemporal_load(reinterpret_cast<const typename C::raw *>(y + sl.e[k] * kSize));
+        rx[k] = C::load(x + sl.e[k] * kSize);
+        rg[k] = C::load(y + sl.e[k] * kSize);
       }
   };
   // (An operand without heads has its walk behind the last token.)
@@ -457,7 +459,8 @@ __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardA
     nt = min(a.TB, a.T - t0);
     Walk at = walk(first);
     fetch(a.part[first], at);
-    angles(cs, nt, a.R / 2, a.by_pairs, a.freqs, a.scale, true, [&](int t) { return (double)a.positions[t0 + t]; });
+    angles(cs, nt, a.R / 2, a.by_pairs, a.freqs, a.scale, true,
+           [&](int t) { return (double)a.positions[t0 + t]; });
     __syncthreads();
 #pragma unroll 1
     for (int kind = first; kind <= last; ++kind) {
@@ -583,12 +586,15 @@ void launch_rows(const Args &a, bool norm, bool paged, hipStream_t s) {
   if (norm) hipLaunchKernelGGL((positions_kernel<DT, V, INTER, true, false>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((positions_kernel<DT, V, INTER, false, false>), grid, block, 0, s, a);
 }
-template <int DT, bool INTER>
-void launch_back(const BackwardArgs &a, hipStream_t s) {
+template <int DT>
+void launch_back(const BackwardArgs &a, bool interleaved, hipStream_t s) {
   const unsigned runs = (unsigned)std::max(a.part[0].blocks, a.part[1].blocks);
   // Few runs: a workgroup for each operand (333 tokens of 24 heads of 80: 8.8 us against 10.6).
   const dim3 grid(runs, runs <= 512 ? 2 : 1);
-  if (runs) hipLaunchKernelGGL((qk_norm_backward_kernel<DT, INTER>), grid, dim3(kThreads), 0, s, a);
+  if (runs && interleaved)
+    hipLaunchKernelGGL((qk_norm_backward_kernel<DT, true>), grid, dim3(kThreads), 0, s, a);
+  else if (runs)
+    hipLaunchKernelGGL((qk_norm_backward_kernel<DT, false>), grid, dim3(kThreads), 0, s, a);
   hipLaunchKernelGGL(qk_norm_weight_kernel, dim3((unsigned)a.D / 8, 2), dim3(1024), 0, s, a);
 }
 
@@ -662,7 +668,8 @@ int32_t launch_positions(const PositionProblem &p, hipStream_t s) {
   for (int i = 0; i < 3; ++i) {
     const PositionRows &r = p.rows[i];
     heads += (int)r.heads;
-    a.rows[i] = {static_cast<const char *>(r.src.p), static_cast<char *>(r.dst.p), r.w, {}, {}, (int)r.heads};
+    a.rows[i] = {static_cast<const char *>(r.src.p), static_cast<char *>(r.dst.p), r.w, {}, {},
+                 (int)r.heads};
     if (p.T == 0 || r.heads == 0) continue;  // (strides of nothing)
     if (!pos::strides_of(r.src, size, a.rows[i].from) || !pos::strides_of(r.dst, size, a.rows[i].to))
       return pos::too_far(p.what);
@@ -741,13 +748,9 @@ int32_t launch_qk_norm_backward(const QkNormBackwardProblem &p, hipStream_t s) {
   a.T = (int)p.T;
   a.w_dt = p.w_dt;
   a.TB = backward_run(p.T);
-  const auto launch = p.dt == NOVA_HIP_DT_F32 ? (p.interleaved ? pos::launch_back<NOVA_HIP_DT_F32, true>
-                                                               : pos::launch_back<NOVA_HIP_DT_F32, false>)
-                      : p.dt == NOVA_HIP_DT_BF16 ? (p.interleaved ? pos::launch_back<NOVA_HIP_DT_BF16, true>
-                                                                  : pos::launch_back<NOVA_HIP_DT_BF16, false>)
-                                                 : (p.interleaved ? pos::launch_back<NOVA_HIP_DT_F16, true>
-                                                                  : pos::launch_back<NOVA_HIP_DT_F16, false>);
-  launch(a, s);
+  if (p.dt == NOVA_HIP_DT_F32) pos::launch_back<NOVA_HIP_DT_F32>(a, p.interleaved, s);
+  else if (p.dt == NOVA_HIP_DT_BF16) pos::launch_back<NOVA_HIP_DT_BF16>(a, p.interleaved, s);
+  else pos::launch_back<NOVA_HIP_DT_F16>(a, p.interleaved, s);
   return check_hip(hipGetLastError(), "qk_norm_rotary_backward launch");
 }
 

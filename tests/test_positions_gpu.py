@@ -157,6 +157,14 @@ def test_norm_and_backward(cuda, D, R, dt, interleaved):
     norm_case(cuda, 41, 6, 3, D, R, dt, interleaved, weight=dt)
 
 
+@pytest.mark.parametrize("T,H,G,D", [(1023, 70, 3, 256), (1100, 40, 8, 256), (1500, 33, 1, 96), (2500, 5, 0, 8),
+                                     (8300, 17, 4, 64), (1024, 1, 1, 248), (1, 600, 1, 128)])
+def test_norm_of_many_heads(cuda, T, H, G, D):
+    """Workgroups of every shape: more rows to a token than threads, and fewer."""
+    norm_case(cuda, T, H, G, D, D, BF, False)
+    norm_case(cuda, min(T, 1500), H, G, D, 8, F32, True, layout="htd")
+
+
 @pytest.mark.parametrize("T,H,G", [(12001, 2, 1), (25000, 0, 1), (4095, 1, 1), (4097, 2, 3), (20007, 1, 0)])
 def test_norm_of_many_tokens(cuda, T, H, G):
     """Runs of up to eight tokens, several to a workgroup of the backward pass."""
