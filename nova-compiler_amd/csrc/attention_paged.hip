@@ -125,7 +125,9 @@ __device__ __forceinline__ int lanes_below(int v) {
 // The work is cut so that it fills the chip's places for workgroups and no place is
 // left with a long remainder.  With fewer tiles than places, a sequence's keys into as
 // many splits as fill the places once; with more, only where its tiles see kLong times
-// the keys that a place has in the mean (one token over a long cache among prompts).
+// the keys that a place has in the mean (one token over a long cache among prompts; at
+// 1.0 / 1.3 / 1.6 / 2.0 a step of 3751 tokens takes 247 / 247 / 242 / 241 us, a prompt of
+// 4096 beside one token over 131072 rows 260 / 265 / 274 / 319).
 constexpr float kLong = 2.0f;
 constexpr int kBM = 128;
 
@@ -384,7 +386,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a
         const int l = i * NW + wave, r0 = l * kRows;
         const __amdgpu_buffer_rsrc_t rk = buffer(ka, kb, l), rv = buffer(va, vb, l);
         const int lr = lane / CH, ch = (lane & (CH - 1)) ^ swz<CH>(r0 + lr);
-        // Single tokens: read once by the whole chip, see attention_decode.hip.
+        // Single tokens: read once by the whole chip (116 us against 125 where the caches
+        // keep them).
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
             rk, (lds_void *)(sk + r0 * CH * 16), 16,
             ch * 8 < a.D ? (uint32_t)(lr * skt + ch * 16) : kOOB, 0, 0, NW == 1 ? 2 : 0);
@@ -785,9 +788,11 @@ int32_t launch_paged_d(const PagedArgs &a, bool narrow, hipStream_t s) {
   if (narrow)
     hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((unsigned)(a.T * a.heads)), dim3(256), 0, s, a);
   else {
-    // Groups where tiles are so few that they may have eight splits and more.
+    // Groups where tiles are so few, and keys so many, that a tile may have eight splits and
+    // more (one group against four, heads of 128: 16 tokens over 32768 rows 44.7 us against
+    // 38.7, a step of 3751 tokens 238 against 245; 300 over 1000, heads of 64, 12.7 against 14.7).
     const dim3 grid((unsigned)a.kv_heads, (unsigned)a.split_tiles, DP / 32);
-    if (a.split_tiles * 8 <= a.places)
+    if (a.split_tiles * 8 <= a.places && a.cap >= 8 * a.least)
       hipLaunchKernelGGL((paged_join_tile_kernel<DT, DP, 4>), grid, dim3(8 * kBM), 0, s, a);
     else
       hipLaunchKernelGGL((paged_join_tile_kernel<DT, DP, 1>), grid, dim3(2 * kBM), 0, s, a);
@@ -812,10 +817,14 @@ Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D, i
              int64_t max_queries) {
   Plan p = {};
   const int64_t group = heads / kv_heads;
+  // Single tokens in the chunks' form: those 32 128 us, one over 8192 rows 20 against 15.
   p.narrow = max_queries * group <= 32 && B <= 0xffff;
   p.chunk = std::max<int64_t>(rows, 1);
   // Workgroups resident at once, by LDS (a wave's 32 or 16 KB) and registers; single
-  // tokens: as many as it takes to fill the memory's pipes.
+  // tokens: as many as it takes to fill the memory's pipes (512 / 768 / 1024: 32 tokens over
+  // 1500 to 8192 rows 123 / 116 / 116 us, 8 over 8192 55 / 52 / 56; chunks, 256 / 512 / 768:
+  // 512 tokens over 8192 rows 105 / 90 / 100).  Least keys of a piece of 128 instead of 256
+  // and 32 instead of 64: within 1 us either way.
   p.places = p.narrow ? (D <= 64 ? 1536 : 768) : (D <= 64 ? 768 : 512);
   p.least = p.narrow ? 64 : 256;
   const int64_t most = (rows + p.least - 1) / p.least, mine = (p.places + kv_heads - 1) / kv_heads;
