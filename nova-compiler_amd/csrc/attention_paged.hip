@@ -29,11 +29,13 @@
 #include <algorithm>
 
 #include "attention.h"
+#include "paged_work.h"
 #include "wave.h"
 
 namespace nova_hip {
 namespace attn {
 namespace {
+using namespace paged;
 
 // n / d for n < 2^31: the upper bits of n m, m the least number above 2^(31 + l) / d.
 struct Divider {
@@ -125,19 +127,6 @@ __device__ __forceinline__ int lanes_below(int v) {
   return x - v;
 }
 
-// The work is cut so that it fills the chip's places for workgroups and no place is
-// left with a long remainder.  With fewer tiles than places, a sequence's keys into as
-// many splits as fill the places once; with more, only where its tiles see kLong times
-// the keys that a place has in the mean (one token over a long cache among prompts; at
-// 1.0 / 1.3 / 1.6 / 2.0 a step of 3751 tokens takes 247 / 247 / 242 / 241 us, a prompt of
-// 4096 beside one token over 131072 rows 260 / 265 / 274 / 319).
-constexpr float kLong = 2.0f;
-constexpr int kBM = 128;
-
-// Keys that the tiles of a sequence see in the mean, or more.
-__device__ __forceinline__ float mean_keys(const PagedArgs &a, const Seq &q) {
-  return a.causal ? fmaxf(0.5f * (float)q.len, (float)q.len - 0.5f * (float)q.n) : (float)q.len;
-}
 __device__ __forceinline__ int tiles_of(const PagedArgs &a, const Seq &q) {
   return (q.n * (int)a.group.d + kBM - 1) / kBM;
 }
@@ -159,26 +148,18 @@ __device__ __forceinline__ Work work_of(const PagedArgs &a, int BM) {
   w.base = 0;
   if (a.slots == 0) return w;
   const float tiles = (float)w.tiles, len = (float)w.q.len;
-  const float all = wave_sum(tiles);
-  float c = wave_sum(tiles * mean_keys(a, w.q)) / a.places;
-  if (all >= a.places) {
-    c *= kLong;
-  } else {
-    for (int i = 0; i < 8; ++i) {
-      const float units = wave_sum(tiles * ceilf(len * __builtin_amdgcn_rcpf(fmaxf(c, 1.0f))));
-      if (units <= a.places) break;
-      c *= fmaxf(1.02f, units * __builtin_amdgcn_rcpf(a.places));
-    }
-  }
-  c = fmaxf(c, (float)a.least);
-  const float n = fmaxf(1.0f, ceilf(len * __builtin_amdgcn_rcpf(c)));
-  // As many slots as the host counted on, or no splits.
+  const float all = wave_sum(tiles), mean = wave_sum(tiles * mean_keys(w.q.n, w.q.len, a.causal)) / a.places;
+  const float c = piece_keys(all, mean, a.places, (float)a.least, (float)a.slots,
+                             [&](float keys, bool split) __attribute__((always_inline)) {
+                               const float n = splits_at(len, keys);
+                               return wave_sum(split && n <= 1.0f ? 0.0f : tiles * n);
+                             });
+  const float n = splits_at(len, c);
+  // No more slots than there are, whatever the rounding.
   const float mine = n > 1.0f ? tiles * n : 0.0f;
   if (!(wave_sum(mine) <= (float)a.slots)) return w;
   w.n = (int)n;
-  // n of them hold the sequence: what the quotient is off by is less than the margin.
-  if (n > 1.0f)
-    w.piece = ((int)(len * __builtin_amdgcn_rcpf(n)) + 2 + (w.q.len >> 20) + 63) / 64 * 64;
+  if (n > 1.0f) w.piece = piece_of(w.q.len, n);
   w.base = lanes_below((int)mine);
   return w;
 }
@@ -268,7 +249,7 @@ __device__ __forceinline__ int piece_of_many(const PagedArgs &a) {
   for (int b = threadIdx.x & 63; b < a.B; b += 64) {
     const Seq q = seq_of(a, b);
     tiles += (float)tiles_of(a, q);
-    keys += (float)tiles_of(a, q) * mean_keys(a, q);
+    keys += (float)tiles_of(a, q) * mean_keys(q.n, q.len, a.causal);
   }
   const float c = wave_sum(keys) / a.places * (wave_sum(tiles) >= a.places ? kLong : 1.25f);
   return __builtin_amdgcn_readfirstlane(max(a.chunk, ((int)fminf(c, (float)a.cap) + 63) / 64 * 64));
@@ -810,60 +791,13 @@ int32_t launch_paged(const PagedArgs &a, bool narrow, hipStream_t s) {
   return launch_paged_d<DT, 128>(a, narrow, s);
 }
 
-// The form of a call, its tiles of rows per key head (up to 64 sequences: with their
-// splits), its splits and slots.
-struct Plan {
-  bool narrow;
-  int64_t tiles, chunk, splits, slots, least, places;
-};
-Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D, int64_t rows,
-             int64_t max_queries) {
-  Plan p = {};
-  const int64_t group = heads / kv_heads;
-  // Single tokens in the chunks' form: those 32 128 us, one over 8192 rows 20 against 15.
-  p.narrow = max_queries * group <= 32 && B <= 0xffff;
-  p.chunk = std::max<int64_t>(rows, 1);
-  // Workgroups resident at once, by LDS (a wave's 32 or 16 KB) and registers; single
-  // tokens: as many as it takes to fill the memory's pipes (512 / 768 / 1024: 32 tokens over
-  // 1500 to 8192 rows 123 / 116 / 116 us, 8 over 8192 55 / 52 / 56; chunks, 256 / 512 / 768:
-  // 512 tokens over 8192 rows 105 / 90 / 100).  Least keys of a piece of 128 instead of 256
-  // and 32 instead of 64: within 1 us either way.
-  p.places = p.narrow ? (D <= 64 ? 1536 : 768) : (D <= 64 ? 768 : 512);
-  p.least = p.narrow ? 64 : 256;
-  const int64_t most = (rows + p.least - 1) / p.least, mine = (p.places + kv_heads - 1) / kv_heads;
-  // Work::n: fewer tiles than places have as many units as places at most; with more
-  // tiles, those that are split have less than 4 / kLong units to a place.
-  auto room = [&](int64_t tiles) { return std::min(tiles * most, tiles < mine ? mine : 2 * mine); };
-  if (p.narrow && B <= 64 && B * kv_heads * most > p.places) {
-    p.slots = room(B);
-    p.tiles = B + p.slots;
-  } else if (p.narrow) {
-    // As for the padded cache (attention_decode.hip).
-    const int64_t all = B * rows * kv_heads;
-    const int64_t keys = std::max(std::min<int64_t>(512, all / 2048), std::min<int64_t>(2048, all / 8192));
-    p.chunk = std::max<int64_t>(64, (std::max(keys, rows / 32768) + 63) / 64 * 64);
-  } else if (B <= 64) {
-    p.tiles = std::min(T * group, T * group / kBM + B);
-    if (most > 1) p.slots = room(p.tiles);
-    p.tiles += p.slots;
-  } else {
-    p.tiles = T * group / kBM + B;
-    const int64_t splits =
-        std::max<int64_t>(1, std::min(3 * p.places / (2 * p.tiles * kv_heads), rows / 512));
-    p.chunk = std::max<int64_t>(64, ((rows + splits - 1) / splits + 63) / 64 * 64);
-  }
-  p.splits = std::max<int64_t>(1, (rows + p.chunk - 1) / p.chunk);
-  if (!p.narrow && p.splits > 1) p.slots = p.tiles * p.splits;
-  return p;
-}
-
 }  // namespace
 }  // namespace attn
 
 int64_t paged_attention_scratch(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t D,
                                 int64_t rows, int64_t max_queries) {
-  const attn::Plan p = attn::plan_of(T, B, heads, kv_heads, D, rows, max_queries);
-  if (!p.narrow) return kv_heads * p.slots * attn::kBM * ((D + 31) / 32 * 32 + 2);
+  const attn::paged::Plan p = attn::paged::plan_of(T, B, heads, kv_heads, D, rows, max_queries);
+  if (!p.narrow) return kv_heads * p.slots * attn::paged::kBM * ((D + 31) / 32 * 32 + 2);
   const int64_t sums = p.slots ? kv_heads * p.slots * 32 : p.splits > 1 ? T * heads * p.splits : 0;
   return sums ? sums * (D + 2) + (2 * T * heads + 3) / 4 * 4 : 0;
 }
@@ -897,7 +831,7 @@ int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
   a.pages = (int)c.pages;
   a.width = (int)c.width;
   a.cap = (int)(c.width * c.page);
-  const attn::Plan plan = attn::plan_of(p.T, c.B, p.heads, c.kv_heads, c.D, a.cap, p.max_queries);
+  const attn::paged::Plan plan = attn::paged::plan_of(p.T, c.B, p.heads, c.kv_heads, c.D, a.cap, p.max_queries);
   // Rows are counted in 32 bits, a grid's dimension holds less than 2^32 threads.
   if (p.T * p.heads >= (1LL << 31) - (1 << 20) || plan.tiles * c.kv_heads >= 1 << 24 ||
       (plan.narrow && (plan.splits > 1 || plan.slots > 0) && p.T * p.heads >= 1 << 24))
