@@ -21,10 +21,12 @@ constexpr int kBM = 128;  // (token, head of the group) rows of a chunk's tile
 // The work is cut so that it fills the chip's places for workgroups and no place is
 // left with a long remainder.  With fewer tiles than places, a sequence's keys into as
 // many splits as fill the places once; with more, only where its tiles see kLong times
-// the keys that a place has in the mean (one token over a long cache among prompts; at
-// 1.0 / 1.3 / 1.6 / 2.0 a step of 3751 tokens takes 247 / 247 / 242 / 241 us, a prompt of
-// 4096 beside one token over 131072 rows 260 / 265 / 274 / 319).
-constexpr float kLong = 2.0f;
+// the keys that a place has in the mean (one token over a long cache among prompts).  20
+// drawn steps of 1.05 to 4 tiles to a place, heads of 64 and 128, at 1.0 / 1.3 / 1.6 / 2.0
+// take 2.3 / 1.5 / 2.5 / 7.9 % longer than the best of the four in the mean, 18 / 17 / 12 /
+// 29 % at most; a step of 3751 tokens 241 / 246 / 240 / 236 us, a prompt of 4096 beside one
+// token over 131072 rows 237 / 246 / 257 / 310.
+constexpr float kLong = 1.6f;
 // Filling the places once ends with the longest piece; pieces of kLong times the mean on
 // more units than places end, longest first, by the mean and a piece: 1 + kLong.
 constexpr float kFill = 1.0f + kLong;
@@ -55,22 +57,20 @@ NOVA_BOTH int piece_of(int len, float n) {
 // few units above them; where only pieces past kFill times its start would fill them, the
 // tiles are cut as where there are more.  Room is then found by longer pieces: the units of
 // split sequences are sum tiles ceil(len / c) < 2 sum tiles len / c, and a mean is half of
-// len or more, so they are less than 4 places mean / c.  That is 2 places at kLong, the room
-// for more tiles than places, and the places, the least room there is, at 4 times the mean.
+// len or more, so they are less than 4 places mean / c.  That is the places, the least room
+// there is, at 4 times the mean.
 // (13 chunks of 128 tokens over 8192 rows beside one token over 131072, 16 heads in groups
 // of 4 of 128: 208 us, 3090 where a batch whose search ends above its room is not split.)
 template <typename Units>
 NOVA_BOTH float piece_keys(float all, float mean, float places, float least, float room, Units units) {
-  const float longer = fmaxf(kLong * mean, least);
-  if (all >= places) return longer;
   float c = fmaxf(mean, 1.0f);
-  const float end = kFill * c;
+  const float end = all < places ? kFill * c : 0.0f;
   for (int i = 0; i < 8 && c <= end; ++i) {
     const float n = units(c, false);
     if (n <= places) return fmaxf(c, least);
     c *= fmaxf(1.02f, n * reciprocal(places));
   }
-  c = c > end ? longer : fmaxf(c, least);
+  c = fmaxf(c > end ? kLong * mean : c, least);
   for (int i = 0; i < 32 && units(c, true) > room; ++i) c *= 1.05f;
   return c;
 }
@@ -96,8 +96,8 @@ inline Plan plan_of(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64
   p.places = p.narrow ? (D <= 64 ? 1536 : 768) : (D <= 64 ? 768 : 512);
   p.least = p.narrow ? 64 : 256;
   const int64_t most = (rows + p.least - 1) / p.least, mine = (p.places + kv_heads - 1) / kv_heads;
-  // What piece_keys allots: fewer tiles than places as many units as places at most, or in
-  // split sequences; more tiles less than twice as many in split sequences.
+  // For the units of split sequences (see piece_keys): the places, or twice those where
+  // there may be more tiles than places.
   auto room = [&](int64_t tiles) { return std::min(tiles * most, tiles < mine ? mine : 2 * mine); };
   if (p.narrow && B <= 64 && B * kv_heads * most > p.places) {
     p.slots = room(B);

@@ -95,6 +95,14 @@ def test_batches_that_missed_their_room(cut):
     assert longest <= 2.0 * mean
 
 
+def test_a_long_sequence_among_more_tiles_than_places(cut):
+    """No piece past 1.6 times what a place has in the mean, and its rounding."""
+    for new, lens, heads, kv_heads in (([4096, 1], [4096, 131072], 32, 8), ([2048, 2048, 64], [2048, 2048, 16384], 32, 8),
+                                       ([8192] * 3 + [1], [8192] * 3 + [65536], 12, 12)):
+        longest, mean, _ = cut(new, lens, heads, kv_heads, 128)
+        assert longest <= 1.6 * mean + 64 + 2
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_any_batch(cut, seed):
     rng = random.Random(seed)
