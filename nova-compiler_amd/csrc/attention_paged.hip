@@ -65,7 +65,7 @@ struct PagedArgs {
   int64_t skp, skt, skh, svp, svt, svh, stb, slse;
   double per_page;  // 1 / page
   Divider group;    // query heads to a key head
-  int T, B, heads, kv_heads, D, page, pages, width, cap;  // cap: rows of a sequence
+  int T, B, heads, kv_heads, D, page, pages, cap;  // cap: rows of a sequence
   int tiles;          // per key head; up to 64 sequences: with their splits
   int split_tiles;    // those that may have several
   int splits, chunk;  // chunk: what `splits` cover all rows with, at least 1
@@ -242,16 +242,15 @@ __device__ __forceinline__ bool find_tile_of_many(const PagedArgs &a, int t, Uni
   u.slot = t * a.splits;
   return u.index >= 0 && u.index < tiles_of(a, u.seq);
 }
-// Their pieces: at most a.splits of them (one from 1153 sequences on), from the lengths.
+// Their pieces: at most a.splits of them, from the lengths.
 __device__ __forceinline__ int piece_of_many(const PagedArgs &a) {
   if (a.splits == 1) return a.chunk;
-  float tiles = 0.0f, keys = 0.0f;
+  float keys = 0.0f;
   for (int b = threadIdx.x & 63; b < a.B; b += 64) {
     const Seq q = seq_of(a, b);
-    tiles += (float)tiles_of(a, q);
     keys += (float)tiles_of(a, q) * mean_keys(q.n, q.len, a.causal);
   }
-  const float c = wave_sum(keys) / a.places * (wave_sum(tiles) >= a.places ? kLong : 1.25f);
+  const float c = 1.25f * wave_sum(keys) / a.places;
   return __builtin_amdgcn_readfirstlane(max(a.chunk, ((int)fminf(c, (float)a.cap) + 63) / 64 * 64));
 }
 
@@ -829,7 +828,6 @@ int32_t launch_paged_attention(const PagedAttentionProblem &p, hipStream_t s) {
   a.D = (int)c.D;
   a.page = (int)c.page;
   a.pages = (int)c.pages;
-  a.width = (int)c.width;
   a.cap = (int)(c.width * c.page);
   const attn::paged::Plan plan = attn::paged::plan_of(p.T, c.B, p.heads, c.kv_heads, c.D, a.cap, p.max_queries);
   // Rows are counted in 32 bits, a grid's dimension holds less than 2^32 threads.
