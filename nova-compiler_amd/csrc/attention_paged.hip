@@ -148,13 +148,14 @@ __device__ __forceinline__ Work work_of(const PagedArgs &a, int BM) {
   w.base = 0;
   if (a.slots == 0) return w;
   const float tiles = (float)w.tiles, len = (float)w.q.len;
+  const float counted = counted_keys(w.q.n, w.q.len, a.causal);
   const float all = wave_sum(tiles), mean = wave_sum(tiles * mean_keys(w.q.n, w.q.len, a.causal)) / a.places;
   const float c = piece_keys(all, mean, a.places, (float)a.least, (float)a.slots,
                              [&](float keys, bool split) __attribute__((always_inline)) {
-                               const float n = splits_at(len, keys);
+                               const float n = splits_at(len, counted, keys);
                                return wave_sum(split && n <= 1.0f ? 0.0f : tiles * n);
                              });
-  const float n = splits_at(len, c);
+  const float n = splits_at(len, counted, c);
   // No more slots than there are, whatever the rounding.
   const float mine = n > 1.0f ? tiles * n : 0.0f;
   if (!(wave_sum(mine) <= (float)a.slots)) return w;

@@ -24,12 +24,13 @@ constexpr int kBM = 128;  // (token, head of the group) rows of a chunk's tile
 // the keys that a place has in the mean (one token over a long cache among prompts).  20
 // drawn steps of 1.05 to 4 tiles to a place, heads of 64 and 128, at 1.0 / 1.3 / 1.6 / 2.0
 // take 2.3 / 1.5 / 2.5 / 7.9 % longer than the best of the four in the mean, 18 / 17 / 12 /
-// 29 % at most; a step of 3751 tokens 241 / 246 / 240 / 236 us, a prompt of 4096 beside one
-// token over 131072 rows 237 / 246 / 257 / 310.
+// 29 % at most; with what counted_keys leaves whole 1.6 against 2.0: 4 % less in the mean, 19 %
+// less to 8 % more.  A step of 3751 tokens 236 us at either, a prompt of 4096 beside one token
+// over 131072 rows 255 against 304.
 constexpr float kLong = 1.6f;
-// Filling the places once ends with the longest piece; pieces of kLong times the mean on
-// more units than places end, longest first, by the mean and a piece: 1 + kLong.
-constexpr float kFill = 1.0f + kLong;
+// Filling the places once ends with the longest piece.  A causal prompt alone, whose tiles
+// see half of it in the mean, finds its tiles whole at less than 3 times that.
+constexpr float kFill = 3.0f;
 
 NOVA_BOTH float reciprocal(float x) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -44,9 +45,19 @@ NOVA_BOTH float mean_keys(int n, int len, bool causal) {
   return causal ? fmaxf(0.5f * (float)len, (float)len - 0.5f * (float)n) : (float)len;
 }
 
-// Splits of a sequence of len rows at c keys to a piece, and the rows of a piece: what
-// the quotient is off by is less than the margin, so that n of them hold the sequence.
-NOVA_BOTH float splits_at(float len, float c) { return fmaxf(1.0f, ceilf(len * reciprocal(c))); }
+// What counts of them against a piece, at least 3/4 of the rows: the last tiles of a causal
+// prompt see all of it, but run beside its first ones, which leave them the CU.  A prompt
+// alone, or several of a length, are so never cut where tiles are as many as places (8192
+// tokens of 12 heads of 64: 153 us, counted in full, and cut, 168).
+NOVA_BOTH float counted_keys(int n, int len, bool causal) {
+  return fmaxf(mean_keys(n, len, causal), 0.75f * (float)len);
+}
+
+// Splits at c keys to a piece of a sequence of len rows, `counted` of them, and the rows of a
+// piece: what the quotient is off by is less than the margin, so that n of them hold it.
+NOVA_BOTH float splits_at(float len, float counted, float c) {
+  return counted > c ? fmaxf(1.0f, ceilf(len * reciprocal(c))) : 1.0f;
+}
 NOVA_BOTH int piece_of(int len, float n) {
   return ((int)((float)len * reciprocal(n)) + 2 + (len >> 20) + 63) / 64 * 64;
 }

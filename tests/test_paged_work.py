@@ -21,10 +21,13 @@ extern "C" void cut(long T, int B, const int *n, const int *len, long heads, lon
   float all = 0.0f, keys = 0.0f;
   auto tiles = [&](int b) { return p.narrow ? (float)(n[b] > 0) : (float)((n[b] * group + kBM - 1) / kBM); };
   for (int b = 0; b < B; ++b) all += tiles(b), keys += tiles(b) * mean_keys(n[b], len[b], causal != 0);
+  auto splits_of = [&](int b, float c) {
+    return splits_at((float)len[b], counted_keys(n[b], len[b], causal != 0), c);
+  };
   auto units = [&](float c, bool split) {
     float sum = 0.0f;
     for (int b = 0; b < B; ++b) {
-      const float k = splits_at((float)len[b], c);
+      const float k = splits_of(b, c);
       sum += split && k <= 1.0f ? 0.0f : tiles(b) * k;
     }
     return sum;
@@ -33,7 +36,7 @@ extern "C" void cut(long T, int B, const int *n, const int *len, long heads, lon
   sizes[0] = p.narrow, sizes[1] = p.tiles, sizes[2] = p.slots, sizes[3] = p.least;
   found[0] = units(c, false), found[1] = units(c, true), found[2] = keys / places;
   for (int b = 0; b < B; ++b) {
-    const float k = splits_at((float)len[b], c);
+    const float k = splits_of(b, c);
     splits[b] = (int)k;
     piece[b] = k > 1.0f ? piece_of(len[b], k) : len[b];
   }
@@ -101,6 +104,19 @@ def test_a_long_sequence_among_more_tiles_than_places(cut):
                                        ([8192] * 3 + [1], [8192] * 3 + [65536], 12, 12)):
         longest, mean, _ = cut(new, lens, heads, kv_heads, 128)
         assert longest <= 1.6 * mean + 64 + 2
+
+
+@pytest.mark.parametrize("heads,kv_heads,D,places", [(32, 8, 128, 64), (12, 12, 64, 64), (6, 6, 64, 128),
+                                                     (64, 8, 128, 64), (9, 3, 80, 171)])
+def test_plain_prompts_stay_whole(cut, heads, kv_heads, D, places):
+    """Prompts of one length and as many tiles as places, or more: no unit but their tiles."""
+    for count in (1, 2, 3, 5):
+        for more in range(3, 400, 7):
+            tokens = ((-(-places // count) - 1) * 128 + more) // (heads // kv_heads) + 1
+            tiles = count * -(-tokens * (heads // kv_heads) // 128)
+            assert tiles >= places
+            found = cut([tokens] * count, [tokens] * count, heads, kv_heads, D)
+            assert found is None or found[2] == tiles  # (None: no room for splits at all)
 
 
 @pytest.mark.parametrize("seed", range(8))
