@@ -489,7 +489,8 @@ int64_t nova_hip_attention_decode_scratch(int64_t sequences, int64_t cache, int6
 /* freqs[i] = base^(-2 i / R), R = 2 (size of freqs, at most 128), for contexts
  * `factor` times longer than the model's: with original = 0 all divided by
  * factor; with original the context it was trained on, those that turn `high`
- * times over it stay, those that turn `low` times are divided by factor, with
+ * times over it stay, those that turn `low` times are divided by factor (low and high
+ * belong to the model as base and factor do: with others its positions are wrong), with
  *   keep = clamp((original freqs[i] / 2 pi - low) / (high - low), 0, 1):
  *   freqs[i] (keep + (1 - keep) / factor).
  * Computed in 64 bits.  factor = 1 changes nothing. */
@@ -529,8 +530,8 @@ int64_t nova_hip_qk_norm_rotary_backward_scratch(int64_t tokens, int64_t heads, 
  * [pages, rows of a page, key heads, D] of dt NOVA_HIP_DT_BF16 or _F16, unit
  * stride on D, any order of the other dims, rows 16-byte aligned, any page size
  * (attention is some 10 % faster on pages of a multiple of 8 rows, or of 4 where D
- * is above 64; it takes tables of up to 2^30 rows and pages of up to
- * 2^30 elements from first to last row).
+ * is above 64; it takes tables of up to 2^30 rows, and pages whose rows are up to 2^23
+ * elements apart and up to 2^30 from first to last).
  * Row i of sequence b is row i % page of page table[b, i / page].
  *   offsets : [sequences + 1] i32, not decreasing: the new tokens of sequence b
  *   are the packed rows [offsets[b], offsets[b + 1]);
@@ -556,8 +557,14 @@ int32_t _mlir_ciface_nova_hip_paged_append(
 /* Attention of the new tokens over their sequences' rows, as
  * _mlir_ciface_nova_hip_attention has it (causal: a token sees the rows up to its
  * own position; groups, types, roundings, empty rows and near masked infinities
- * the same).  Lengths are cut to what the table holds, entries of the table to the
- * pages that there are; rows behind a length are not read.
+ * the same).  Lengths are cut to what the table holds (positions then count from the
+ * cut length), entries of the table to the pages that there are; rows behind a length are
+ * not read.  f16 weights are held times 2^7, as there, also where a sequence has one new
+ * token (_mlir_ciface_nova_hip_attention_decode: times 2^15).
+ *   Up to 64 sequences the work is shared out by the lengths.  With more, one with a far
+ * longer cache than the others can hold up a call: where max_queries G is more than 32
+ * its keys are mostly not split, and where none has, the splits, and scratch, follow the
+ * table's width.  Such a sequence is better given to a call of its own.
  *   q, out : [tokens, heads, D], D a multiple of 8 up to 128; lse : [heads,
  *   tokens] f32 or NULL; rows outside every sequence are left as they were.
  *   max_queries : no sequence has more new tokens (0: not known); tokens beyond it

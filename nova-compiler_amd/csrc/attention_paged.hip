@@ -8,22 +8,29 @@
 // sum and the LDS tiles are those of the packed forward (attention.hip).
 //
 // Two forms.  Chunks: four waves of 32 rows share tiles of 64 keys; bound by the products
-// and the softmax between them (32 heads on 8 of 128 in bf16: a prompt of 8192 530 us, 1.04
-// PFLOP/s; 512 tokens over 8192 rows 90, 740 TFLOP/s; the matrix cores are busy for 43 % of
-// a step of 3751 tokens).  Up to 32 rows per sequence (single tokens): a wave per split of
-// the keys, tiles of 32, without a barrier; bound by HBM (32 tokens over 1500 to 8192 rows
-// 108 to 116 us, 5.3 TB/s; 8 over 131072 6.2).  Either cuts the keys of a tile of rows into
-// pieces where there are few tiles (see work_of); a tile whose rows see at most one writes
-// its result, the others' sums go to the caller's scratch, where a second kernel adds them
-// in order.
+// and the softmax between them (32 heads on 8 of 128 in bf16: a prompt of 8192 530 to 565 us,
+// 0.97 to 1.04 PFLOP/s; 512 tokens over 8192 rows 88 to 91, 730 to 760 TFLOP/s; the matrix
+// cores are busy for 43 % of a step of 3751 tokens).  Up to 32 rows per sequence (single
+// tokens): a wave per split of the keys, tiles of 32, without a barrier; bound by HBM (32
+// tokens over 1500 to 8192 rows 108 us, 5.5 TB/s; 8 over 131072 6.5).  Either cuts the keys of
+// a tile of rows into pieces where there are few tiles (see work_of); a tile whose rows see
+// at most one writes its result, the others' sums go to the caller's scratch, where a second
+// kernel adds them in order.
+//
+// Up to 64 sequences a workgroup reads all lengths and takes its unit of work from them.
+// With more the host provides for splits by the sizes alone: none for chunks where tiles
+// times key heads are more than 3/4 of the places, so that one workgroup to a key head walks
+// the longest sequence (a prompt of 4096 beside one token over 131072 rows 257 us, with 70
+// single tokens more 3060), and for single tokens as many as the table's width asks for.
 //
 // Keys come by DMA into LDS.  Where a page holds whole loads (rows that are a
 // multiple of the 4 or 8 of one instruction) its address is a scalar: a lane looks up
 // each load of a tile, a tile ahead, and a buffer of the load's rows that are there
 // makes the others zero.  Other page sizes: a lane looks up each row, and a load takes
 // its lanes' addresses from those; rows that are not there are a row of zeros (32 heads
-// on 8 of 128, pages of one row against 16: 32 single tokens over 1500 to 8192 rows 117 us
-// against 114, a prompt of 8192 590 against 530; through registers 930 and 1180).
+// on 8 of 128, pages of one row against 16: 32 single tokens over 1500 to 8192 rows 115 us
+// against 107, a prompt of 8192 620 to 627 against 558 to 563; through registers 930 and
+// 1180).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -79,6 +86,9 @@ struct PagedArgs {
 __device__ const __attribute__((aligned(16))) uint32_t kZeros[64] = {};
 
 constexpr float kSlack = 8.0f;  // as in the packed forward
+// So are f16 weights taken times 2^7, in both forms (the padded single-token form, without
+// the slack, 2^15): one that rounds to zero is under 2^-32 of the largest in its piece, and
+// 2^20 keys of such weights together under half a step of an f16 result.
 template <int DT>
 constexpr float kUp = DT == NOVA_HIP_DT_F16 ? 7.0f : 0.0f;
 
@@ -450,7 +460,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_paged_kernel(PagedArgs a
     for (int i = 0; i < BN / 32; ++i)
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
-        // Weights round to the operands' type, as in the packed forward.
+        // Weights round to the operands' type, as in the packed forward: a result is 2.0e-3
+        // to 2.4e-3 off in bf16 (2-norm, relative), 1.7e-3 of it by its own rounding.
         const u32x4 pf = pack_frag<DT>(s[i], kk);
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)

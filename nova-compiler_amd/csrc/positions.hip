@@ -29,9 +29,11 @@ namespace {
 constexpr int kMaxThreads = 512;  // of a workgroup forward
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTB = 8;  // tokens whose angles a workgroup holds at once
-// Rows of a lane whose loads are on their way together (8192 tokens of 8 heads of 64,
-// cold, at 1 / 2: 7.0 / 5.4 us).  They and the stores are such that the caches keep nothing for:
-// 8120 tokens of 40 heads of 128 in 33.4 us against 36.6.
+// Rows of a lane whose loads are on their way together (1 / 2, cold: 8120 tokens of 32 + 8
+// heads of 128 normed 32.8 / 33.8 us, into the cache 37.4 / 37.2; 8192 of 12 heads of 64 in
+// f32, 32 values rotated, warm, 10.4 / 9.6).  They and the stores are such that the caches
+// keep nothing for: 8120 tokens of 40 heads of 128, cold, in 30.0 us against 34.7, where they
+// still lie in a cache 30.4 against 27.1.
 constexpr int kAhead = 2;
 constexpr int kMaxPairs = kMaxHeadDim / 2;
 
@@ -416,8 +418,11 @@ struct BackwardArgs {
 // in registers until an operand's rows of a run end, a column's thread the sums of runs.
 // Bound by what is on its way to a CU, so by its waves: chunks of four values to a lane
 // at every type leave room for five waves to a SIMD (8120 tokens of 40 heads of 128 in
-// bf16, 249 MB, cold, with the sums behind: 58.5 us, 4.3 TB/s; 65536 tokens 5.1; chunks of
-// eight: 62 with four waves, 73 with three; runs of four tokens: 67).
+// bf16, 249 MB, cold, with the sums behind: 57.3 us, 4.3 TB/s, vector units 63 % busy; 65536
+// tokens 5.1; chunks of eight: 62 with four waves, 73 with three; runs of four tokens: 67).
+// In f32, 499 MB, vector units are 30 % busy and HBM is the bound (105 us warm, 4.8 TB/s).
+// Five waves cost 4 registers to scratch in f32 and 2 in bf16 interleaved: the latter takes
+// as long as bf16 in halves, which has none there (kernel alone 50.0 and 50.4 us).
 template <int DT, bool INTER>
 __global__ __launch_bounds__(kThreads, 5) void qk_norm_backward_kernel(BackwardArgs a) {
   constexpr int V = 4;

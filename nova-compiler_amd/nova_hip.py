@@ -710,7 +710,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, 
     """base^(-2 i / dim) [dim / 2] f32 on the GPU, for contexts ``factor`` times
     longer than the model's: all divided by it, or, with ``original`` the context
     it was trained on, only those that turn few times over that (divided in full
-    at ``low`` turns, kept from ``high`` on)."""
+    at ``low`` turns, kept from ``high`` on).  Both are the model's, as ``base`` and
+    ``factor`` are: pass those it was trained with, often 1 and 4; the defaults are no
+    model's in particular."""
     torch = _torch()
     if freqs is None:
         if dim % 2:
@@ -821,7 +823,8 @@ def paged_attention(q, k_pages, v_pages, offsets, lengths, table, *, causal: boo
     their sequences in the pages, described as for ``paged_append``; causal: a
     token sees the rows up to its own position.  ``max_queries`` says that no
     sequence has more new tokens (1: single tokens); a view of the table's first
-    columns that none is longer.  Returns out; ``lse`` [heads, tokens] f32 is
+    columns that none is longer.  Of more than 64 sequences one with a far longer cache
+    than the others is better given to a call of its own.  Returns out; ``lse`` [heads, tokens] f32 is
     written when given."""
     torch = _torch()
     f32, i32, dt, dev = torch.float32, torch.int32, q.dtype, q.get_device()
