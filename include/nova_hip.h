@@ -561,10 +561,10 @@ int32_t _mlir_ciface_nova_hip_paged_append(
  * cut length), entries of the table to the pages that there are; rows behind a length are
  * not read.  f16 weights are held times 2^7, as there, also where a sequence has one new
  * token (_mlir_ciface_nova_hip_attention_decode: times 2^15).
- *   Up to 64 sequences the work is shared out by the lengths.  With more, one with a far
- * longer cache than the others can hold up a call: where max_queries G is more than 32
- * its keys are mostly not split, and where none has, the splits, and scratch, follow the
- * table's width.  Such a sequence is better given to a call of its own.
+ *   Up to 64 sequences the work is shared out by the lengths.  With more, one with a
+ * far longer cache than the others can hold up a call and is better given to a call of
+ * its own: where max_queries times G is more than 32 its keys are mostly not split, else
+ * the splits, and the scratch, follow the table's width.
  *   q, out : [tokens, heads, D], D a multiple of 8 up to 128; lse : [heads,
  *   tokens] f32 or NULL; rows outside every sequence are left as they were.
  *   max_queries : no sequence has more new tokens (0: not known); tokens beyond it
